@@ -295,6 +295,105 @@ typedef struct rgp_rnn_scan {
 rgp_status rgp_rnn_scan_forward(rgp_handle h, const rgp_rnn_scan* a);
 rgp_status rgp_rnn_scan_backward(rgp_handle h, const rgp_rnn_scan* a);
 
+/* ---- sequence operators of the state-space encoder cell -----------------------------------------------------------------------
+ * The recognition networks of autoreg/rnn_encoder.py:21-150 get one more cell: a linear recurrence whose step size and input / output
+ * maps depend on the data, behind a short causal convolution and a root-mean-square norm.  It has no counterpart in the reference.
+ * What differs from the calls above: they take four storage types, the stream they are enqueued on as an argument (they run inside the
+ * caller's autograd graph and may be captured), and their work buffer from the caller (two graphs or streams then share nothing);
+ * they allocate nothing, never synchronise and use no atomics, so results do not depend on timing.
+ *   dtype  RGP_F64 / RGP_F32 / RGP_BF16 / RGP_F16: type of the activations and their gradients.  Parameters, states, sums and
+ *          parameter gradients ("acc" below) are double for RGP_F64 and float for the others.
+ *   Rows   off == NULL: n_seq sequences of T steps (rows = T * n_seq); step t of sequence s is at base + t * st + s * sb (strides in
+ *          ELEMENTS, features contiguous), outputs are contiguous [T][n_seq][features].  off != NULL: packed rows, sequence s is rows
+ *          off[s] .. off[s+1] (device int64[n_seq + 1], increasing, off[0] = 0, off[n_seq] = rows; lengths of 0 are allowed), step t
+ *          at base + (off[s] + t) * st, outputs contiguous [rows][features].  max_len: the longest sequence (a hint for the split
+ *          over time; any value is safe).  reverse != 0 walks every sequence from its last step to its first. */
+enum { RGP_F64 = 0, RGP_F32 = 1, RGP_BF16 = 2, RGP_F16 = 3 };
+
+/* Selective state-space scan.  Per step, channel d < D, state n < N, group g = d / (D / G) of B and C:
+ *     dt = softplus(delta + bias);  s[n] = exp(dt A[d][n]) s[n] + dt u B[g][n];  p = sum_n C[g][n] s[n] + skip[d] u;
+ *     y = p * z * sigmoid(z)   (y = p without z)
+ * u, delta, z, gy [..][D]; B, C [..][G][N]; A [D][N]; skip, bias [D] (NULL = 0); init, last [n_seq][D][N] acc (NULL: zero / not wanted).
+ * states: rgp_ssm_scan_states_bytes(a) bytes, written by the forward call when not NULL and read by the backward call.
+ * Backward: gy = dL/dy -> gu, gdelta, gz [..][D], gB, gC [..][G][N] (dtype, contiguous), gA [D][N], gskip, gbias [D] (acc; the last
+ * two, and gz, may be NULL where skip, bias, z are).  N <= 64.  work: rgp_ssm_scan_workspace(a, backward) bytes, 16-byte aligned. */
+typedef struct rgp_ssm_scan {
+  int32_t dtype, n_seq, D, N, G, reverse;
+  int64_t T, rows, max_len;
+  const int64_t* off;
+  const void *u, *delta, *z, *B, *C;
+  int64_t u_st, u_sb, delta_st, delta_sb, z_st, z_sb, B_st, B_sb, C_st, C_sb, gy_st, gy_sb;
+  const void *A, *skip, *bias, *init;
+  void *y, *last, *states;
+  const void* gy;
+  void *gu, *gdelta, *gz, *gB, *gC, *gA, *gskip, *gbias;
+  void* work;
+  int64_t work_bytes;
+} rgp_ssm_scan;
+int64_t    rgp_ssm_scan_states_bytes(const rgp_ssm_scan* a);      /* -1: an argument the operator does not take */
+int64_t    rgp_ssm_scan_workspace(const rgp_ssm_scan* a, int backward);
+rgp_status rgp_ssm_scan_forward(rgp_handle h, void* stream, const rgp_ssm_scan* a);
+rgp_status rgp_ssm_scan_backward(rgp_handle h, void* stream, const rgp_ssm_scan* a);
+/* One step of n_seq sequences (rows = n_seq, T = 1, off = NULL; u_sb.. are the strides of the batch): init = last is the state, updated
+ * in place; y [n_seq][D]. */
+rgp_status rgp_ssm_scan_step(rgp_handle h, void* stream, const rgp_ssm_scan* a);
+
+/* Short causal convolution, one filter of W taps per channel, 2 <= W <= 8:
+ *     v_t = pre * sigmoid(pre),  pre = bias + sum_{j < W} w[d][j] x_{t - W + 1 + j}
+ * x, gv [..][D]; w [D][W], bias [D] (NULL = 0) acc; init, last [n_seq][W - 1][D] dtype: the W - 1 inputs before the first step (NULL =
+ * zeros) and before the next one, oldest first.  Backward: gv = dL/dv -> gx [..][D] dtype contiguous, gw [D][W], gbias [D] acc. */
+typedef struct rgp_ssm_conv {
+  int32_t dtype, n_seq, D, W, reverse, reserved;
+  int64_t T, rows, max_len;
+  const int64_t* off;
+  const void* x;
+  int64_t x_st, x_sb, gv_st, gv_sb;
+  const void *w, *bias, *init;
+  void *v, *last;
+  const void* gv;
+  void *gx, *gw, *gbias;
+  void* work;
+  int64_t work_bytes;
+} rgp_ssm_conv;
+int64_t    rgp_ssm_conv_workspace(const rgp_ssm_conv* a, int backward);
+rgp_status rgp_ssm_conv_forward(rgp_handle h, void* stream, const rgp_ssm_conv* a);
+rgp_status rgp_ssm_conv_backward(rgp_handle h, void* stream, const rgp_ssm_conv* a);
+/* One step of n_seq sequences: init = last is the state, updated in place; v [n_seq][D]. */
+rgp_status rgp_ssm_conv_step(rgp_handle h, void* stream, const rgp_ssm_conv* a);
+
+/* Root-mean-square norm of x + residual over the last dimension, per row:
+ *     hid = x + residual;  y = hid * r * w,  r = (mean(hid^2) + eps)^(-1/2)
+ * x, residual (NULL = 0), y, hid [rows][C] dtype (row strides in elements; y, hid contiguous; hid NULL iff residual is), w [C] acc,
+ * rstd [rows] acc (NULL: not wanted; the backward call reads it).  Backward: gy, ghid (NULL = 0) -> gx [rows][C] (the gradient of x and
+ * of residual alike), gw [C] acc; x and residual are the forward call's (or x = hid and no residual: the same up to hid's rounding). */
+typedef struct rgp_rms_norm {
+  int32_t dtype, reserved;
+  int64_t rows, C;
+  double eps;
+  const void *x, *residual;
+  int64_t x_st, residual_st, gy_st, ghid_st;
+  const void* w;
+  void *y, *hid, *rstd;
+  const void *gy, *ghid;
+  void *gx, *gw;
+  void* work;
+  int64_t work_bytes;
+} rgp_rms_norm;
+int64_t    rgp_rms_norm_workspace(const rgp_rms_norm* a, int backward);
+rgp_status rgp_rms_norm_forward(rgp_handle h, void* stream, const rgp_rms_norm* a);
+rgp_status rgp_rms_norm_backward(rgp_handle h, void* stream, const rgp_rms_norm* a);
+
+/* Global norm of n gradient tensors (host arrays ptr / numel / dtype of device pointers, element counts and types) and their clipping.
+ * rgp_grad_sumsq: sumsq[0] = sum of all squares, in double whatever the types (a squared bf16 or float value never overflows there).
+ * rgp_grad_clip: norm[0] = sqrt(sumsq[0]); every tensor is multiplied by max_norm / (norm + 1e-6) where that is below 1; otherwise, and
+ * where the norm is not finite, the tensors stay as they are.  sumsq and norm may be the same address.  Between the two calls a
+ * data-parallel caller adds the sums of the other ranks.  work: rgp_grad_workspace bytes.  The tensors must not overlap. */
+int64_t    rgp_grad_workspace(int n, const int64_t* numel, const int32_t* dtype);
+rgp_status rgp_grad_sumsq(rgp_handle h, void* stream, int n, void* const* ptr, const int64_t* numel, const int32_t* dtype, double* sumsq,
+                          void* work, int64_t work_bytes);
+rgp_status rgp_grad_clip(rgp_handle h, void* stream, int n, void* const* ptr, const int64_t* numel, const int32_t* dtype,
+                         const double* sumsq, double max_norm, double* norm);
+
 /* ---- optimiser step on device (the outer SVI loop's Adam; positive parameters live in softplus space) -------- */
 /* x, m, v: n doubles of optimiser-space parameter and Adam moments; g: gradient w.r.t. the CONSTRAINED value p;
  * positive[i] != 0 -> p = softplus(x) and the chain factor 1-exp(-p) is applied (paramz Logexp).  The new constrained

@@ -54,6 +54,31 @@ class RnnScan(C.Structure):
                 ('g_out', c_dp), ('dgi', c_dp), ('dgh', c_dp)]
 
 
+DT_F64, DT_F32, DT_BF16, DT_F16 = 0, 1, 2, 3                                  # RGP_F64 ..
+
+
+class SsmScan(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ('dtype', 'n_seq', 'D', 'N', 'G', 'reverse')] + \
+               [(n, C.c_int64) for n in ('T', 'rows', 'max_len')] + \
+               [(n, c_dp) for n in ('off', 'u', 'delta', 'z', 'B', 'C')] + \
+               [(n, C.c_int64) for n in ('u_st', 'u_sb', 'delta_st', 'delta_sb', 'z_st', 'z_sb', 'B_st', 'B_sb', 'C_st', 'C_sb', 'gy_st', 'gy_sb')] + \
+               [(n, c_dp) for n in ('A', 'skip', 'bias', 'init', 'y', 'last', 'states', 'gy', 'gu', 'gdelta', 'gz', 'gB', 'gC', 'gA', 'gskip',
+                                    'gbias', 'work')] + [('work_bytes', C.c_int64)]
+
+
+class SsmConv(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ('dtype', 'n_seq', 'D', 'W', 'reverse', 'reserved')] + \
+               [(n, C.c_int64) for n in ('T', 'rows', 'max_len')] + [('off', c_dp), ('x', c_dp)] + \
+               [(n, C.c_int64) for n in ('x_st', 'x_sb', 'gv_st', 'gv_sb')] + \
+               [(n, c_dp) for n in ('w', 'bias', 'init', 'v', 'last', 'gv', 'gx', 'gw', 'gbias', 'work')] + [('work_bytes', C.c_int64)]
+
+
+class RmsNorm(C.Structure):
+    _fields_ = [('dtype', C.c_int32), ('reserved', C.c_int32), ('rows', C.c_int64), ('C', C.c_int64), ('eps', C.c_double),
+                ('x', c_dp), ('residual', c_dp)] + [(n, C.c_int64) for n in ('x_st', 'residual_st', 'gy_st', 'ghid_st')] + \
+               [(n, c_dp) for n in ('w', 'y', 'hid', 'rstd', 'gy', 'ghid', 'gx', 'gw', 'work')] + [('work_bytes', C.c_int64)]
+
+
 # every symbol include/rgp_hip.h declares: name -> (restype, argtypes)
 SYMBOLS = {
     'rgp_create': (C.c_int, [C.POINTER(C.c_void_p), C.c_int, C.c_void_p]),
@@ -92,6 +117,23 @@ SYMBOLS = {
     'rgp_mlp_scan_backward': (C.c_int, [C.c_void_p, C.POINTER(MlpScan)]),
     'rgp_rnn_scan_forward': (C.c_int, [C.c_void_p, C.POINTER(RnnScan)]),
     'rgp_rnn_scan_backward': (C.c_int, [C.c_void_p, C.POINTER(RnnScan)]),
+    'rgp_ssm_scan_states_bytes': (C.c_int64, [C.POINTER(SsmScan)]),
+    'rgp_ssm_scan_workspace': (C.c_int64, [C.POINTER(SsmScan), C.c_int]),
+    'rgp_ssm_scan_forward': (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(SsmScan)]),
+    'rgp_ssm_scan_backward': (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(SsmScan)]),
+    'rgp_ssm_scan_step': (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(SsmScan)]),
+    'rgp_ssm_conv_workspace': (C.c_int64, [C.POINTER(SsmConv), C.c_int]),
+    'rgp_ssm_conv_forward': (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(SsmConv)]),
+    'rgp_ssm_conv_backward': (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(SsmConv)]),
+    'rgp_ssm_conv_step': (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(SsmConv)]),
+    'rgp_rms_norm_workspace': (C.c_int64, [C.POINTER(RmsNorm), C.c_int]),
+    'rgp_rms_norm_forward': (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(RmsNorm)]),
+    'rgp_rms_norm_backward': (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(RmsNorm)]),
+    'rgp_grad_workspace': (C.c_int64, [C.c_int, C.POINTER(C.c_int64), C.POINTER(C.c_int32)]),
+    'rgp_grad_sumsq': (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_int64), C.POINTER(C.c_int32), c_dp,
+                                 C.c_void_p, C.c_int64]),
+    'rgp_grad_clip': (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_int64), C.POINTER(C.c_int32), c_dp,
+                                C.c_double, c_dp]),
 }
 PREPARE_CHAIN_ONLY, PREPARE_ROWS_ONLY, PREPARE_ROWS_EARLY = 1, 2, 4          # rgp_layer_in.reserved for rgp_layer_prepare
 

@@ -1,0 +1,505 @@
+// rgp_norm.hip -- root-mean-square norm of x + residual and its gradient; global norm of many gradient tensors and their clipping.
+// All of it is bound by memory: every kernel reads its operands once, 16 bytes a lane, and keeps a row in registers between the sum of
+// squares and the product.
+#include "rgp_seq.h"
+
+struct NormDev {
+  rgp_rms_norm a;
+  int wx, wr, wgy, wgh, wout;
+  void* part;
+};
+
+// sum over the TPR threads of a row; TPR <= 64: lanes of one wave, else the whole workgroup of TPR threads
+template <int TPR, typename A>
+static __device__ __forceinline__ A row_sum(A v, A* sh) {
+  if constexpr (TPR <= 64) {
+    return seq_sum_wide<TPR>(v);
+  } else {
+    v = seq_sum_wide<64>(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    A s = (A)0;
+#pragma unroll
+    for (int i = 0; i < TPR / 64; ++i) s += sh[i];
+    return s;
+  }
+}
+
+// TPR threads a row, NE vectors of V elements each; rows TPR * NE * V >= C.  hid is rounded to its type where it is written; the norm
+// uses the sum before that rounding.
+template <typename T, int TPR, int NE>
+static __global__ void __launch_bounds__(256) rms_fwd_kernel(NormDev d) {
+  typedef typename SeqAcc<T>::type A;
+  constexpr int V = SeqVec<T>::V, RPB = 256 / TPR;
+  __shared__ A sh[4];
+  const rgp_rms_norm& a = d.a;
+  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  const int l = threadIdx.x % TPR;
+  if (TPR <= 64 && row >= a.rows) return;
+  A h[NE][V], q = (A)0;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const int64_t c = (int64_t)(l + i * TPR) * V;
+    const int n = a.C - c < V ? (a.C - c < 0 ? 0 : (int)(a.C - c)) : V;
+    const SeqVec<T> x = seq_load((const T*)a.x + row * a.x_st + c, n, d.wx);
+    SeqVec<T> r = seq_load((const T*)a.x, 0, false);
+    if (a.residual) r = seq_load((const T*)a.residual + row * a.residual_st + c, n, d.wr);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      h[i][j] = (A)x.e[j] + (A)r.e[j];
+      q += h[i][j] * h[i][j];
+    }
+  }
+  q = row_sum<TPR>(q, sh);
+  const A rs = seq_rsqrt(q / (A)a.C + (A)a.eps);
+  if (a.rstd && l == 0) ((A*)a.rstd)[row] = rs;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const int64_t c = (int64_t)(l + i * TPR) * V;
+    const int n = a.C - c < V ? (a.C - c < 0 ? 0 : (int)(a.C - c)) : V;
+    if (n > 0) {
+      SeqVec<T> y, o;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        o.e[j] = (T)h[i][j];
+        y.e[j] = (T)(h[i][j] * rs * (j < n ? ((const A*)a.w)[c + j] : (A)0));
+      }
+      seq_store((T*)a.y + row * a.C + c, y, n, d.wout);
+      if (a.hid) seq_store((T*)a.hid + row * a.C + c, o, n, d.wout);
+    }
+  }
+}
+// rows longer than a workgroup's registers: the sum of squares, then the row once more
+template <typename T>
+static __global__ void __launch_bounds__(256) rms_fwd_long_kernel(NormDev d) {
+  typedef typename SeqAcc<T>::type A;
+  constexpr int V = SeqVec<T>::V;
+  __shared__ A sh[4];
+  const rgp_rms_norm& a = d.a;
+  const int64_t row = blockIdx.x;
+  A q = (A)0, rs = (A)0;
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int64_t c = (int64_t)threadIdx.x * V; c < a.C; c += 256 * V) {
+      const int n = a.C - c < V ? (int)(a.C - c) : V;
+      const SeqVec<T> x = seq_load((const T*)a.x + row * a.x_st + c, n, d.wx);
+      SeqVec<T> r = seq_load((const T*)a.x, 0, false), y, o;
+      if (a.residual) r = seq_load((const T*)a.residual + row * a.residual_st + c, n, d.wr);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const A h = (A)x.e[j] + (A)r.e[j];
+        if (pass == 0) q += h * h;
+        o.e[j] = (T)h;
+        y.e[j] = (T)(h * rs * (j < n ? ((const A*)a.w)[c + j] : (A)0));
+      }
+      if (pass == 1) {
+        seq_store((T*)a.y + row * a.C + c, y, n, d.wout);
+        if (a.hid) seq_store((T*)a.hid + row * a.C + c, o, n, d.wout);
+      }
+    }
+    if (pass == 0) {
+      q = row_sum<256>(q, sh);
+      rs = seq_rsqrt(q / (A)a.C + (A)a.eps);
+      if (a.rstd && threadIdx.x == 0) ((A*)a.rstd)[row] = rs;
+    }
+  }
+}
+
+// gx = ghid + r (gy w - hid r^2 mean(gy w hid)); gw = sum over rows of gy hid r.  hid is x + residual again, before its rounding to a 16-bit
+// storage type: gw is a sum over many rows in 32 bits, and that rounding (2^-9 relative) would be its largest error by far.  A workgroup takes every nblk-th group of
+// rows, sums gw in registers and adds its row groups through LDS; the workgroups' sums are added in a fixed order afterwards.
+template <typename T, int TPR, int NE>
+static __global__ void __launch_bounds__(256) rms_bwd_kernel(NormDev d) {
+  typedef typename SeqAcc<T>::type A;
+  constexpr int V = SeqVec<T>::V, RPB = 256 / TPR;
+  __shared__ A sh[4];
+  __shared__ A acc[256 * V];
+  const rgp_rms_norm& a = d.a;
+  const int l = threadIdx.x % TPR, rg = threadIdx.x / TPR;
+  A gw[NE][V], w[NE][V];
+#pragma unroll
+  for (int i = 0; i < NE; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int64_t c = (int64_t)(l + i * TPR) * V + j;
+      gw[i][j] = (A)0;
+      w[i][j] = c < a.C ? ((const A*)a.w)[c] : (A)0;
+    }
+  const A inv = (A)1 / (A)a.C;
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t row = r0 + rg;
+    const bool live = row < a.rows;
+    const int64_t rr = live ? row : 0;
+    SeqVec<T> x[NE], r[NE], g[NE], gh[NE];
+    const A rs = live ? ((const A*)a.rstd)[rr] : (A)0;
+    A q = (A)0;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int64_t c = (int64_t)(l + i * TPR) * V;
+      const int n = !live || a.C - c < 0 ? 0 : (a.C - c < V ? (int)(a.C - c) : V);
+      x[i] = seq_load((const T*)a.x + rr * a.x_st + c, n, d.wx);
+      if (a.residual) r[i] = seq_load((const T*)a.residual + rr * a.residual_st + c, n, d.wr);
+      g[i] = seq_load((const T*)a.gy + rr * a.gy_st + c, n, d.wgy);
+      if (a.ghid) gh[i] = seq_load((const T*)a.ghid + rr * a.ghid_st + c, n, d.wgh);
+    }
+    A hid[NE][V];
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        hid[i][j] = (A)x[i].e[j] + (a.residual ? (A)r[i].e[j] : (A)0);
+        q += (A)g[i].e[j] * w[i][j] * hid[i][j];
+      }
+    q = row_sum<TPR>(q, sh) * inv * rs * rs;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int64_t c = (int64_t)(l + i * TPR) * V;
+      const int n = !live || a.C - c < 0 ? 0 : (a.C - c < V ? (int)(a.C - c) : V);
+      SeqVec<T> o;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const A gy = (A)g[i].e[j], h = hid[i][j];
+        A v = rs * (gy * w[i][j] - h * q);
+        if (a.ghid) v += (A)gh[i].e[j];
+        o.e[j] = (T)v;
+        if (n > 0) gw[i][j] += gy * h * rs;
+      }
+      if (n > 0) seq_store((T*)a.gx + rr * a.C + c, o, n, d.wout);
+    }
+  }
+  A* const part = (A*)d.part + (int64_t)blockIdx.x * a.C;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[threadIdx.x * V + j] = gw[i][j];
+    __syncthreads();
+    for (int e = threadIdx.x; e < TPR * V; e += 256) {
+      A v = (A)0;
+#pragma unroll
+      for (int q = 0; q < RPB; ++q) v += acc[q * TPR * V + e];
+      const int64_t c = (int64_t)i * TPR * V + e;
+      if (c < a.C) part[c] = v;
+    }
+  }
+}
+// rows longer than a workgroup's registers: gw goes through memory, one row of the partial sums per workgroup
+template <typename T>
+static __global__ void __launch_bounds__(256) rms_bwd_long_kernel(NormDev d) {
+  typedef typename SeqAcc<T>::type A;
+  constexpr int V = SeqVec<T>::V;
+  __shared__ A sh[4];
+  const rgp_rms_norm& a = d.a;
+  A* const part = (A*)d.part + (int64_t)blockIdx.x * a.C;
+  for (int64_t c = threadIdx.x; c < a.C; c += 256) part[c] = (A)0;
+  __syncthreads();
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const A rs = ((const A*)a.rstd)[row];
+    A q = (A)0;
+    for (int pass = 0; pass < 2; ++pass) {
+      for (int64_t c = (int64_t)threadIdx.x * V; c < a.C; c += 256 * V) {
+        const int n = a.C - c < V ? (int)(a.C - c) : V;
+        const SeqVec<T> x = seq_load((const T*)a.x + row * a.x_st + c, n, d.wx);
+        const SeqVec<T> g = seq_load((const T*)a.gy + row * a.gy_st + c, n, d.wgy);
+        SeqVec<T> r = seq_load((const T*)a.x, 0, false), gh = r, o;
+        if (a.residual) r = seq_load((const T*)a.residual + row * a.residual_st + c, n, d.wr);
+        if (pass == 1 && a.ghid) gh = seq_load((const T*)a.ghid + row * a.ghid_st + c, n, d.wgh);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const A w = j < n ? ((const A*)a.w)[c + j] : (A)0, gy = (A)g.e[j], h = (A)x.e[j] + (A)r.e[j];
+          if (pass == 0) {
+            q += gy * w * h;
+          } else {
+            o.e[j] = (T)((A)gh.e[j] + rs * (gy * w - h * q));
+            if (j < n) part[c + j] += gy * h * rs;
+          }
+        }
+        if (pass == 1) seq_store((T*)a.gx + row * a.C + c, o, n, d.wout);
+      }
+      if (pass == 0) q = row_sum<256>(q, sh) / (A)a.C * rs * rs;
+    }
+  }
+}
+
+// threads a row and vectors a thread: the fewest lanes left idle, at most 8 vectors (a row then needs 64 arithmetic registers of operands)
+struct RmsShape { int tpr, ne; };
+static RmsShape rms_shape(int64_t C, int V) {
+  const int64_t nv = (C + V - 1) / V;
+  const int tprs[4] = {8, 16, 64, 256}, nes[4] = {1, 2, 4, 8};
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 4; ++j)
+      if ((int64_t)tprs[i] * nes[j] >= nv && (j < 2 || i == 3 || (i < 3 && j == 2 && (int64_t)tprs[i] * 4 >= nv))) return RmsShape{tprs[i], nes[j]};
+  return RmsShape{0, 0};
+}
+static int64_t rms_blocks(const rgp_rms_norm* a, RmsShape s) {
+  const int64_t rpb = s.tpr ? 256 / s.tpr : 1, want = (a->rows + rpb - 1) / rpb;
+  return want < 1024 ? (want < 1 ? 1 : want) : 1024;
+}
+static const char* rms_bad(const rgp_rms_norm* a) {
+  if (!a) return "null arguments";
+  if (a->dtype < 0 || a->dtype > 3) return "dtype must be RGP_F64, RGP_F32, RGP_BF16 or RGP_F16";
+  if (a->rows < 0 || a->C < 1) return "empty rows";
+  if (!(a->eps > 0.0)) return "eps must be positive";
+  return nullptr;
+}
+extern "C" int64_t rgp_rms_norm_workspace(const rgp_rms_norm* a, int backward) {
+  if (rms_bad(a)) return -1;
+  if (!backward) return 0;
+  return rms_blocks(a, rms_shape(a->C, 16 / seq_dtype_bytes(a->dtype))) * a->C * (a->dtype == RGP_F64 ? 8 : 4);
+}
+template <typename T, int TPR, int NE>
+static hipError_t rms_go(const NormDev& d, bool back, int64_t blocks, hipStream_t s) {
+  if (back) hipLaunchKernelGGL((rms_bwd_kernel<T, TPR, NE>), dim3((unsigned)blocks), dim3(256), 0, s, d);
+  else hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, NE>), dim3((unsigned)((d.a.rows + 256 / TPR - 1) / (256 / TPR))), dim3(256), 0, s, d);
+  return hipGetLastError();
+}
+template <typename T, int TPR>
+static hipError_t rms_ne(const NormDev& d, int ne, bool back, int64_t blocks, hipStream_t s) {
+  switch (ne) {
+    case 1: return rms_go<T, TPR, 1>(d, back, blocks, s);
+    case 2: return rms_go<T, TPR, 2>(d, back, blocks, s);
+    case 4: return rms_go<T, TPR, 4>(d, back, blocks, s);
+    default:
+      if constexpr (TPR == 256) return rms_go<T, TPR, 8>(d, back, blocks, s);
+      return hipErrorInvalidValue;
+  }
+}
+template <typename T>
+static hipError_t rms_pick(const NormDev& d, RmsShape sh, bool back, int64_t blocks, hipStream_t s) {
+  switch (sh.tpr) {
+    case 8: return rms_ne<T, 8>(d, sh.ne, back, blocks, s);
+    case 16: return rms_ne<T, 16>(d, sh.ne, back, blocks, s);
+    case 64: return rms_ne<T, 64>(d, sh.ne, back, blocks, s);
+    case 256: return rms_ne<T, 256>(d, sh.ne, back, blocks, s);
+    default:
+      if (back) hipLaunchKernelGGL(rms_bwd_long_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, d);
+      else hipLaunchKernelGGL(rms_fwd_long_kernel<T>, dim3((unsigned)d.a.rows), dim3(256), 0, s, d);
+      return hipGetLastError();
+  }
+}
+static rgp_status rms_run(rgp_handle h, hipStream_t s, const rgp_rms_norm* a, bool back) {
+  const std::string name = back ? "rms norm backward: " : "rms norm: ";
+  if (const char* bad = rms_bad(a)) return rgp_fail(h, RGP_ERR_BAD_ARG, name + bad);
+  if (!a->w || (back && !a->gw) || (a->rows > 0 && (!a->x || (!back && !a->y) || (back && (!a->gy || !a->gx || !a->rstd)))))
+    return rgp_fail(h, RGP_ERR_BAD_ARG, name + "a required buffer is null");
+  if (!back && a->rows > 0 && (a->residual != nullptr) != (a->hid != nullptr)) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "residual and hid go together");
+  if (a->rows > 2147483647) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "more than 2^31 - 1 rows");
+  const int e = seq_dtype_bytes(a->dtype), V = 16 / e;
+  const RmsShape sh = rms_shape(a->C, V);
+  const int64_t blocks = rms_blocks(a, sh);
+  if (!back && (double)a->rows * (sh.tpr ? sh.tpr : 256) > 4294967040.0) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "more than 2^32 work items");
+  if (back && (rgp_rms_norm_workspace(a, 1) > a->work_bytes || !a->work || ((uintptr_t)a->work & 15)))
+    return rgp_fail(h, RGP_ERR_WORKSPACE, name + "work buffer too small or not 16-byte aligned");
+  NormDev d{};
+  d.a = *a;
+  d.wx = seq_aligned(a->x, a->x_st, 0, e);
+  d.wr = a->residual && seq_aligned(a->residual, a->residual_st, 0, e);
+  d.wgy = back && seq_aligned(a->gy, a->gy_st, 0, e);
+  d.wgh = back && a->ghid && seq_aligned(a->ghid, a->ghid_st, 0, e);
+  d.wout = a->C % V == 0 && (back ? seq_aligned(a->gx, 0, 0, e) : seq_aligned(a->y, 0, 0, e) && (!a->hid || seq_aligned(a->hid, 0, 0, e)));
+  d.part = a->work;
+  if (!back && a->rows == 0) return RGP_OK;
+  hipError_t err = a->dtype == RGP_F64 ? rms_pick<double>(d, sh, back, blocks, s) : a->dtype == RGP_F32 ? rms_pick<float>(d, sh, back, blocks, s)
+                 : a->dtype == RGP_BF16 ? rms_pick<__bf16>(d, sh, back, blocks, s) : rms_pick<_Float16>(d, sh, back, blocks, s);
+  if (err != hipSuccess) return rgp_fail(h, RGP_ERR_HIP, name + hipGetErrorString(err));
+  if (!back) return RGP_OK;
+  const int acc = a->dtype == RGP_F64 ? RGP_F64 : RGP_F32;
+  return seq_reduce(h, s, acc, acc, d.part, blocks, a->C, a->C, a->gw);
+}
+extern "C" rgp_status rgp_rms_norm_forward(rgp_handle h, void* stream, const rgp_rms_norm* a) {
+  SEQ_ENTRY(h, "rms norm", { return rms_run(h, (hipStream_t)stream, a, false); })
+}
+extern "C" rgp_status rgp_rms_norm_backward(rgp_handle h, void* stream, const rgp_rms_norm* a) {
+  SEQ_ENTRY(h, "rms norm", { return rms_run(h, (hipStream_t)stream, a, true); })
+}
+
+// ---- global gradient norm and clipping ---------------------------------------------------------------------------------------------------------
+// The tensors of a launch travel in the kernel's arguments (GT of them), so nothing is uploaded and a captured launch keeps its table.
+// A workgroup takes one piece of GP bytes of one tensor; its sum of squares, in double, goes to its own place, and the pieces are added in
+// a fixed order.
+#define GT 128
+#define GP 65536
+struct GradTable {
+  void* p[GT];
+  int64_t n[GT];
+  int first[GT + 1];             // first piece of each tensor, counted inside the launch
+  uint8_t dt[GT];
+  int count;
+};
+static inline int64_t grad_pieces(int64_t n, int dt) { return (n * seq_dtype_bytes(dt) + GP - 1) / GP; }
+
+static __device__ __forceinline__ int grad_find(const GradTable& t, int piece) {
+  int lo = 0, hi = t.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.first[mid] <= piece) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+// calls f(pointer, n, wide) for the elements of one piece: single elements up to a 16-byte boundary, vectors, single elements
+template <typename T, typename F>
+static __device__ __forceinline__ void grad_walk(T* p, int64_t n, F f) {
+  constexpr int V = SeqVec<T>::V;
+  int64_t head = (int64_t)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(T);
+  if (head > n) head = n;
+  const int64_t nv = (n - head) / V, tail = n - head - nv * V;
+  if ((int64_t)threadIdx.x < head) f(p + threadIdx.x, 1, false);
+  T* const q = p + head;
+  for (int64_t v = threadIdx.x; v < nv; v += 256) f(q + v * V, V, true);
+  if ((int64_t)threadIdx.x < tail) f(q + nv * V + threadIdx.x, 1, false);
+}
+template <typename T>
+static __device__ __forceinline__ double grad_sum(T* p, int64_t n) {
+  double s = 0.0;
+  grad_walk(p, n, [&](T* q, int k, bool wide) {
+    const SeqVec<T> v = seq_load((const T*)q, k, wide);
+#pragma unroll
+    for (int i = 0; i < SeqVec<T>::V; ++i) {
+      const double x = (double)(typename SeqAcc<T>::type)v.e[i];
+      s = fma(x, x, s);
+    }
+  });
+  return s;
+}
+static __global__ void __launch_bounds__(256) grad_sumsq_kernel(GradTable t, double* part) {
+  __shared__ double sh[16];
+  const int i = grad_find(t, blockIdx.x);
+  const int es = t.dt[i] == RGP_F64 ? 8 : t.dt[i] == RGP_F32 ? 4 : 2;
+  const int64_t per = GP / es, o = (int64_t)((int)blockIdx.x - t.first[i]) * per, n = t.n[i] - o < per ? t.n[i] - o : per;
+  double s;
+  switch (t.dt[i]) {
+    case RGP_F64: s = grad_sum((double*)t.p[i] + o, n); break;
+    case RGP_F32: s = grad_sum((float*)t.p[i] + o, n); break;
+    case RGP_BF16: s = grad_sum((__bf16*)t.p[i] + o, n); break;
+    default: s = grad_sum((_Float16*)t.p[i] + o, n); break;
+  }
+  s = block_sum(s, sh);
+  if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
+static __global__ void __launch_bounds__(1024) grad_total_kernel(const double* part, int64_t n, double* out) {
+  __shared__ double sh[16];
+  double s0 = 0.0, s1 = 0.0, s2 = 0.0, s3 = 0.0;
+  int64_t i = threadIdx.x;
+  for (; i + 1024 * 3 < n; i += 4096) {
+    s0 += part[i];
+    s1 += part[i + 1024];
+    s2 += part[i + 2048];
+    s3 += part[i + 1024 * 3];
+  }
+  for (; i < n; i += 1024) s0 += part[i];
+  const double s = block_sum((s0 + s1) + (s2 + s3), sh);
+  if (threadIdx.x == 0) out[0] = s;
+}
+template <typename T>
+static __device__ __forceinline__ void grad_scale(T* p, int64_t n, double c) {
+  typedef typename SeqAcc<T>::type A;
+  const A f = (A)c;
+  grad_walk(p, n, [&](T* q, int k, bool wide) {
+    SeqVec<T> v = seq_load((const T*)q, k, wide);
+#pragma unroll
+    for (int i = 0; i < SeqVec<T>::V; ++i) v.e[i] = (T)((A)v.e[i] * f);
+    seq_store(q, v, k, wide);
+  });
+}
+static __global__ void __launch_bounds__(256) grad_clip_kernel(GradTable t, const double* sumsq, double max_norm) {
+  const double norm = sqrt(sumsq[0]), c = max_norm / (norm + 1e-6);
+  if (!(c < 1.0) || !(norm < 1.7976931348623157e308)) return;           // nothing to clip, or a norm that is no number
+  const int i = grad_find(t, blockIdx.x);
+  const int es = t.dt[i] == RGP_F64 ? 8 : t.dt[i] == RGP_F32 ? 4 : 2;
+  const int64_t per = GP / es, o = (int64_t)((int)blockIdx.x - t.first[i]) * per, n = t.n[i] - o < per ? t.n[i] - o : per;
+  switch (t.dt[i]) {
+    case RGP_F64: grad_scale((double*)t.p[i] + o, n, c); break;
+    case RGP_F32: grad_scale((float*)t.p[i] + o, n, c); break;
+    case RGP_BF16: grad_scale((__bf16*)t.p[i] + o, n, c); break;
+    default: grad_scale((_Float16*)t.p[i] + o, n, c); break;
+  }
+}
+static __global__ void grad_norm_kernel(const double* sumsq, double* norm) { norm[0] = sqrt(sumsq[0]); }
+
+static const char* grad_bad(int n, const int64_t* numel, const int32_t* dtype) {
+  if (n < 0 || (n > 0 && (!numel || !dtype))) return "null arguments";
+  for (int i = 0; i < n; ++i) {
+    if (numel[i] < 0) return "a negative element count";
+    if (dtype[i] < 0 || dtype[i] > 3) return "dtype must be RGP_F64, RGP_F32, RGP_BF16 or RGP_F16";
+  }
+  return nullptr;
+}
+extern "C" int64_t rgp_grad_workspace(int n, const int64_t* numel, const int32_t* dtype) {
+  if (grad_bad(n, numel, dtype)) return -1;
+  int64_t p = 0;
+  for (int i = 0; i < n; ++i) p += grad_pieces(numel[i], dtype[i]);
+  return (p < 1 ? 1 : p) * (int64_t)sizeof(double);
+}
+// calls f(table, pieces, first piece of the launch) for groups of up to GT tensors
+template <typename F>
+static rgp_status grad_tables(rgp_handle h, int n, void* const* ptr, const int64_t* numel, const int32_t* dtype, F f) {
+  GradTable t;
+  t.count = 0;
+  int64_t pieces = 0, before = 0;
+  auto flush = [&]() -> rgp_status {
+    if (!t.count) return RGP_OK;
+    t.first[t.count] = (int)pieces;
+    const rgp_status st = f(t, (unsigned)pieces, before);
+    before += pieces;
+    pieces = 0;
+    t.count = 0;
+    return st;
+  };
+  for (int i = 0; i < n; ++i) {
+    if (numel[i] == 0) continue;
+    const int64_t add = grad_pieces(numel[i], dtype[i]);
+    if (add > 8000000) return rgp_fail(h, RGP_ERR_BAD_ARG, "gradient norm: a tensor of more than 500 GB");
+    if (t.count == GT || pieces + add > 8000000) {
+      const rgp_status st = flush();
+      if (st) return st;
+    }
+    t.p[t.count] = ptr[i];
+    t.n[t.count] = numel[i];
+    t.dt[t.count] = (uint8_t)dtype[i];
+    t.first[t.count++] = (int)pieces;
+    pieces += add;
+  }
+  return flush();
+}
+static rgp_status grad_check(rgp_handle h, int n, void* const* ptr, const int64_t* numel, const int32_t* dtype) {
+  if (const char* bad = grad_bad(n, numel, dtype)) return rgp_fail(h, RGP_ERR_BAD_ARG, std::string("gradient norm: ") + bad);
+  if (n > 0 && !ptr) return rgp_fail(h, RGP_ERR_BAD_ARG, "gradient norm: null arguments");
+  for (int i = 0; i < n; ++i)
+    if (numel[i] > 0 && (!ptr[i] || (uintptr_t)ptr[i] % seq_dtype_bytes(dtype[i]))) return rgp_fail(h, RGP_ERR_BAD_ARG, "gradient norm: a null or misaligned tensor");
+  return RGP_OK;
+}
+extern "C" rgp_status rgp_grad_sumsq(rgp_handle h, void* stream, int n, void* const* ptr, const int64_t* numel, const int32_t* dtype,
+                                     double* sumsq, void* work, int64_t work_bytes) {
+  SEQ_ENTRY(h, "gradient norm", {
+    rgp_status st = grad_check(h, n, ptr, numel, dtype);
+    if (st) return st;
+    if (!sumsq || !work || ((uintptr_t)work & 7) || rgp_grad_workspace(n, numel, dtype) > work_bytes)
+      return rgp_fail(h, RGP_ERR_WORKSPACE, "gradient norm: work buffer too small");
+    const hipStream_t s = (hipStream_t)stream;
+    int64_t total = 0;
+    st = grad_tables(h, n, ptr, numel, dtype, [&](const GradTable& t, unsigned pieces, int64_t before) {
+      hipLaunchKernelGGL(grad_sumsq_kernel, dim3(pieces), dim3(256), 0, s, t, (double*)work + before);
+      total = before + pieces;
+      return seq_launched(h, "gradient norm");
+    });
+    if (st) return st;
+    hipLaunchKernelGGL(grad_total_kernel, dim3(1), dim3(1024), 0, s, (const double*)work, total, sumsq);
+    return seq_launched(h, "gradient norm");
+  })
+}
+extern "C" rgp_status rgp_grad_clip(rgp_handle h, void* stream, int n, void* const* ptr, const int64_t* numel, const int32_t* dtype,
+                                    const double* sumsq, double max_norm, double* norm) {
+  SEQ_ENTRY(h, "gradient clip", {
+    rgp_status st = grad_check(h, n, ptr, numel, dtype);
+    if (st) return st;
+    if (!sumsq || !norm || !(max_norm > 0.0)) return rgp_fail(h, RGP_ERR_BAD_ARG, "gradient clip: sumsq, norm and a positive max_norm are required");
+    const hipStream_t s = (hipStream_t)stream;
+    st = grad_tables(h, n, ptr, numel, dtype, [&](const GradTable& t, unsigned pieces, int64_t) {
+      hipLaunchKernelGGL(grad_clip_kernel, dim3(pieces), dim3(256), 0, s, t, sumsq, max_norm);
+      return seq_launched(h, "gradient clip");
+    });
+    if (st) return st;
+    hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(1), 0, s, sumsq, norm);
+    return seq_launched(h, "gradient clip");
+  })
+}
