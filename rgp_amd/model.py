@@ -566,7 +566,31 @@ class DeepAutoreg(object):
         self._adam = dict(m=torch.zeros_like(self.param_array), v=torch.zeros_like(self.param_array),
                           t_glob=0, t_loc=np.zeros(self.nSeq, dtype=np.int64))
 
-    def svi_step(self, seqs, lr=1e-2, allreduce=None, qU_ratio=None, update=True, lazy_elbo=False, next_seqs=None):
+    def _clip_gradients(self, replicated, local, max_grad_norm, allreduce):
+        """Clips the gradients of one step, in place, to a global norm of ``max_grad_norm`` (seq_ops.clip_grad_norm): ``replicated`` tensors
+        are the same on every rank and count once, the squares of ``local`` ones are summed over the ranks.  The norm stays on the device
+        as ``last_grad_norm``."""
+        from . import seq_ops
+        with torch.cuda.stream(self.handle.stream):           # where the gradients are written and the update reads them
+            total = None
+            if allreduce is not None:
+                total = seq_ops.grad_sumsq(self.handle, local).view(1)
+                allreduce(total)
+                total = total + seq_ops.grad_sumsq(self.handle, replicated)
+            self.last_grad_norm = seq_ops.clip_grad_norm(self.handle, list(replicated) + list(local), max_grad_norm, sumsq=total)
+
+    last_grad_norm = None
+
+    def _touched_ranges(self, seqs):
+        """Contiguous index ranges [(start, stop)] of the sequences of a minibatch, in the order given."""
+        if isinstance(seqs, slice):
+            r = range(*seqs.indices(self.nSeq))
+            return [(r.start, r.stop)] if len(r) else []
+        if seqs is None:
+            return [(0, self.nSeq)]
+        return [(int(s), int(s) + 1) for s in seqs]
+
+    def svi_step(self, seqs, lr=1e-2, allreduce=None, qU_ratio=None, update=True, lazy_elbo=False, next_seqs=None, max_grad_norm=None):
         """One SVI step on the sequences ``seqs`` (slice of contiguous indices or index list): ELBO + gradients,
         optional all-reduce of the global bucket (data-parallel), one Adam update of the global parameters and of the
         touched sequences' latent parameters.  Returns the device ELBO scalar (pre-update).
@@ -574,6 +598,10 @@ class DeepAutoreg(object):
         lazy_elbo=True (pipelined steps only): the ELBO is summed on the library's side stream and the main stream does not
         wait for the last layer's M x M algebra, so the next step's row work starts earlier; the returned tensor may only be
         read after ``handle.join()`` / a device synchronisation.
+
+        max_grad_norm: clip the step's gradients (``grad_array``: globals, and the latents of the touched sequences of all ranks) to this
+        global norm before the update; the norm before clipping is left in ``last_grad_norm`` (device scalar).  Every gradient is needed
+        before the first update then, so such a step is not pipelined.
 
         next_seqs (pipelined steps only): the minibatch of the FOLLOWING step when the data streamer already knows it.  If it
         shares no sequence with ``seqs`` its row terms are computed while this step still runs (RGP_PREPARE_ROWS_EARLY), so the
@@ -584,7 +612,7 @@ class DeepAutoreg(object):
         if self._adam is None:
             self._init_adam()
         ad, h = self._adam, self.handle
-        pipelined = update and self.svi and self.pipeline and len(self.layers) <= 3 and type(self).evaluate is DeepAutoreg.evaluate \
+        pipelined = max_grad_norm is None and update and self.svi and self.pipeline and len(self.layers) <= 3 and type(self).evaluate is DeepAutoreg.evaluate \
             and not (allreduce is not None and self.single_bucket)
         if pipelined:
             try:
@@ -601,18 +629,19 @@ class DeepAutoreg(object):
                 elbo = self.grad_array[self.elbo_slot]
             if not update:              # debugging / kernel ablations only
                 return elbo
-            ad['t_glob'] += 1
             G = self.n_global
+            if max_grad_norm is not None:
+                local, end = [], -1
+                for r0, r1 in sorted(self._touched_ranges(seqs)):
+                    if max(r0, end) < r1:                       # a sequence that is named twice counts once
+                        a, b = int(self.seq_loc_off[max(r0, end)]), int(self.seq_loc_off[r1])
+                        local += [self.grad_array[base + a:base + b] for base in (self.loc0, self.loc0 + self.n_local)]
+                        end = r1
+                self._clip_gradients([self.grad_array[:G]], local, max_grad_norm, allreduce)
+            ad['t_glob'] += 1
             h.adam_step(self.opt_array[:G], self.param_array[:G], self.grad_array[:G], ad['m'][:G], ad['v'][:G],
                         self.positive[:G], lr, ad['t_glob'])
-        if isinstance(seqs, slice):
-            r = range(*seqs.indices(self.nSeq))
-            ranges = [(r.start, r.stop)] if len(r) else []
-        elif seqs is None:
-            ranges = [(0, self.nSeq)]
-        else:
-            ranges = [(int(s), int(s) + 1) for s in seqs]
-        for (r0, r1) in ranges:
+        for (r0, r1) in self._touched_ranges(seqs):
             ad['t_loc'][r0:r1] += 1
             # one launch per run of sequences with the same step count (the bias correction depends on it)
             s0 = r0
@@ -850,11 +879,15 @@ class DeepAutoreg_rnn(_EncoderParamsMixin, DeepAutoreg):
     """autoreg.DeepAutoreg_rnn (model.py:284-629): q(X) of every hidden layer is produced by a recurrent encoder from the
     raw sequences (equal lengths, stacked to (T, batch, D_y + D_u) as at model.py:429), so the latents are NOT free
     parameters; the trainable parameters are the GP globals and the encoder weights.  The GP layers run through
-    librgp_hip.so exactly as in DeepAutoreg (latents with one row per raw time step); the encoder is PyTorch-ROCm fp64."""
+    librgp_hip.so exactly as in DeepAutoreg (latents with one row per raw time step); the encoder is PyTorch-ROCm fp64.
+
+    rnn_type 'ssm' (no counterpart in the reference): the encoder layers are state-space blocks (rnn_encoder.MeanVarSSM), which parallelise
+    over time and can go on from a state one observation at a time (``online_state`` / ``encode_online``).  rnn_compute_dtype (such encoders
+    only): the type of their activations -- torch.float64, float32, bfloat16 or float16; parameters and q(X) stay fp64."""
 
     def __init__(self, wins, Y, U=None, U_win=1, nDims=None, num_inducing=10, kernels=None, rnn_type='rnn',
                  rnn_hidden_dims=None, rnn_bidirectional=False, inference_method='svi', mb_inf_tot_data_size=None,
-                 device=None, seed=0, Zs=None, **kw):
+                 device=None, seed=0, Zs=None, rnn_compute_dtype=None, **kw):
         from .rnn_encoder import SeqEncoder
         Ys = [Y] if isinstance(Y, np.ndarray) else list(Y)
         Us = None if U is None else ([U] if isinstance(U, np.ndarray) else list(U))
@@ -866,7 +899,7 @@ class DeepAutoreg_rnn(_EncoderParamsMixin, DeepAutoreg):
         in_dims = list(self.nDims[:-1])
         in_dims[0] += (Us[0].shape[1] if Us is not None else 0)              # encode_include_input (model.py:409-412)
         hid = rnn_hidden_dims[0] if rnn_hidden_dims is not None else 10
-        self.encoder = SeqEncoder(in_dims, self.nDims[1:], hid, rnn_type, rnn_bidirectional).to(self.device)
+        self.encoder = SeqEncoder(in_dims, self.nDims[1:], hid, rnn_type, rnn_bidirectional, rnn_compute_dtype).to(self.device)
         for lay in self.encoder.layers:                                      # GRU time loops run as device scans
             lay.handle = self.handle
         raw = np.stack([np.hstack([y, u]) if Us is not None else y for y, u in zip(Ys, Us or Ys)], axis=1)
@@ -912,14 +945,29 @@ class DeepAutoreg_rnn(_EncoderParamsMixin, DeepAutoreg):
     def encoder_grad_vector(self):
         return torch.cat([p.grad.reshape(-1) for p in self.encoder.parameters()])
 
-    def svi_step(self, seqs, lr=1e-2, allreduce=None, qU_ratio=None, update=True):
+    @torch.no_grad()
+    def online_state(self, seqs=None):
+        """The 'ssm' encoder's state behind the last observation of the sequences ``seqs`` (None: all), for ``encode_online``."""
+        idx = slice(None) if seqs is None else (seqs if isinstance(seqs, slice) else torch.as_tensor(list(seqs), device=self.device))
+        return self.encoder(self.enc_input[:, idx, :], return_state=True)[2]
+
+    @torch.no_grad()
+    def encode_online(self, rows, state):
+        """q(X) for one new observation of every sequence: rows (batch, D_y + D_u) in the order of the constructor's data, state from
+        ``online_state`` or ``encoder.initial_state(batch)``, updated in place.  Returns (means, variances), one (batch, H) pair per hidden
+        layer, lowest first -- the row that ``encode`` would give with the observation appended."""
+        rows = torch.as_tensor(rows, dtype=torch.float64, device=self.device)
+        return self.encoder.step(rows, state)
+
+    def svi_step(self, seqs, lr=1e-2, allreduce=None, qU_ratio=None, update=True, max_grad_norm=None):
         """One SVI step: ELBO + gradients, optional all-reduce (global GP bucket and encoder-weight gradients, both
-        replicated parameters), Adam on the GP globals (device kernel) and on the encoder weights (torch.optim.Adam)."""
+        replicated parameters), Adam on the GP globals (device kernel) and on the encoder weights (torch.optim.Adam).
+        max_grad_norm: clip the gradients of the GP globals and the encoder weights to this global norm before the update."""
         if self._adam is None:
             self._init_adam()
             self._enc_opt = torch.optim.Adam(self.encoder.parameters(), lr=lr, maximize=True)
         ad, h = self._adam, self.handle
-        carry = allreduce is None and update        # single process: the next step's chains start right after the update
+        carry = allreduce is None and update and max_grad_norm is None        # single process: the next step's chains start right after the update
         self._use_chains = carry
         try:
             elbo = self.evaluate(seqs, qU_ratio=qU_ratio)
@@ -936,6 +984,9 @@ class DeepAutoreg_rnn(_EncoderParamsMixin, DeepAutoreg):
             elbo = self.grad_array[self.elbo_slot]
         if not update:
             return elbo
+        if max_grad_norm is not None:
+            self._clip_gradients([self.grad_array[:self.n_global]] + [p.grad for p in self.encoder.parameters() if p.grad is not None], [],
+                                 max_grad_norm, None)            # all of them replicated, and reduced already
         ad['t_glob'] += 1
         G = self.n_global
         h.adam_step(self.opt_array[:G], self.param_array[:G], self.grad_array[:G], ad['m'][:G], ad['v'][:G],
@@ -1033,17 +1084,17 @@ class DeepAutoreg_mlp(_EncoderParamsMixin, DeepAutoreg):
     def encoder_grad_vector(self):
         return torch.cat([(p.grad if p.grad is not None else torch.zeros_like(p)).reshape(-1) for p in self.encoder.parameters()])
 
-    def svi_step(self, seqs, lr=1e-2, allreduce=None, qU_ratio=None, update=True):
+    def svi_step(self, seqs, lr=1e-2, allreduce=None, qU_ratio=None, update=True, max_grad_norm=None):
         """One SVI step: ELBO + gradients, optional all-reduce of the replicated parameters' gradients (GP globals and MLP
         weights; the per-sequence latent parameters stay local), Adam on the GP globals (device kernel) and torch Adam on
-        the recursion parameters."""
+        the recursion parameters.  max_grad_norm: clip all of the step's gradients to this global norm before the update."""
         from .mlp_encoder import RowAdam
         if self._adam is None:
             self._init_adam()
         if self._enc_opt is None:
             self._enc_opt = RowAdam(self.encoder)
         ad, h = self._adam, self.handle
-        carry = allreduce is None and update        # single process: the next step's chains start right after the update
+        carry = allreduce is None and update and max_grad_norm is None        # single process: the next step's chains start right after the update
         self._use_chains = carry
         try:
             elbo = self.evaluate(seqs, qU_ratio=qU_ratio)
@@ -1056,6 +1107,11 @@ class DeepAutoreg_mlp(_EncoderParamsMixin, DeepAutoreg):
             elbo = self.grad_array[self.elbo_slot]
         if not update:
             return elbo
+        if max_grad_norm is not None:
+            mine = set(id(p) for p in self.encoder.per_sequence_parameters())
+            have = [p for p in self.encoder.parameters() if p.grad is not None]
+            self._clip_gradients([self.grad_array[:self.n_global]] + [p.grad for p in have if id(p) not in mine],
+                                 [p.grad for p in have if id(p) in mine], max_grad_norm, allreduce)
         ad['t_glob'] += 1
         G = self.n_global
         h.adam_step(self.opt_array[:G], self.param_array[:G], self.grad_array[:G], ad['m'][:G], ad['v'][:G],

@@ -12,7 +12,9 @@ The time loop of every layer (Elman/tanh RNN, LSTM or GRU cell) runs as a per-se
 time steps, the heads and every weight gradient stay (batched) torch GEMMs, only the strictly sequential recurrence moves --
 the per-time-step kernel launches of the fp64 torch GRU were 95 % of a config-3 SVI step.  The parameters remain those of the
 nn.RNN / nn.LSTM / nn.GRU module, so the torch path (hidden width beyond the scan's limit, no handle) and the scan are
-interchangeable and are compared in tests/test_gpu_rnn.py."""
+interchangeable and are compared in tests/test_gpu_rnn.py.
+
+rnn_type 'ssm' replaces the cell by a state-space block (MeanVarSSM) on the sequence operators of rgp_amd/seq_ops.py."""
 import torch
 import torch.nn as nn
 
@@ -131,22 +133,181 @@ class MeanVarRNN(nn.Module):
         return self.linear_mean(out), self.soft_plus(self.linear_var(out))
 
 
-class SeqEncoder(nn.Module):
-    """Stack of MeanVarRNN layers, lower hidden layer first (rnn_encoder.py:86-150)."""
+class _SsmBlock(nn.Module):
+    """One direction of a state-space layer, on the sequence operators of librgp_hip.so (rgp_amd/seq_ops.py):
 
-    def __init__(self, input_dims, output_dims, hidden_dim, rnn_type='rnn', bidirectional=False):
+        h = W_in x + b;   n = rms_norm(h);   [c | z] = W_uz n;   u = silu(causal convolution of c)
+        [r | B | C] = W_x u;   delta = W_dt r;   y = selective scan(u, delta, A, B, C, D, z);   n' = rms_norm(W_out y + h)
+
+    Parameters are kept in fp64 with the model's other parameters; the activations have the type of x, and the operators' parameters its
+    arithmetic type."""
+
+    N, W = 16, 4                                    # states per channel, taps of the convolution
+
+    def __init__(self, input_dim, hidden_dim, reverse):
+        nn.Module.__init__(self)
+        E, N, W = hidden_dim, self.N, self.W
+        R = (E + 15) // 16
+        self.E, self.R, self.reverse = E, R, reverse
+        self.inp = nn.Linear(input_dim, hidden_dim)
+        self.norm_in = nn.Parameter(torch.ones(hidden_dim))
+        self.uz = nn.Linear(hidden_dim, 2 * E, bias=False)
+        self.conv_weight = nn.Parameter((torch.rand(E, W) * 2 - 1) / W ** 0.5)
+        self.conv_bias = nn.Parameter((torch.rand(E) * 2 - 1) / W ** 0.5)
+        self.maps = nn.Linear(E, R + 2 * N, bias=False)
+        self.dt = nn.Parameter((torch.rand(E, R) * 2 - 1) / R ** 0.5)
+        step = torch.exp(torch.rand(E) * 4.60517 - 6.90776)                     # softplus(dt_bias) between 1e-3 and 1e-1
+        self.dt_bias = nn.Parameter(step + torch.log(-torch.expm1(-step)))
+        self.A_log = nn.Parameter(torch.log(torch.arange(1, N + 1, dtype=torch.float64)).repeat(E, 1))
+        self.skip = nn.Parameter(torch.ones(E))
+        self.out = nn.Linear(E, hidden_dim, bias=False)
+        self.norm_out = nn.Parameter(torch.ones(hidden_dim))
+
+    @staticmethod
+    def _linear(x, W, b=None):
+        W, b = W.to(x.dtype), None if b is None else b.to(x.dtype)
+        if b is not None and x.dim() == 3 and x.dtype == torch.float64 and x.shape[0] * x.shape[1] >= 1024:
+            return tall_linear(x, W, b)                                          # split-K weight gradients
+        return nn.functional.linear(x, W, b)
+
+    def _parts(self, handle, x):
+        from . import seq_ops
+        p = (lambda t: t) if x.dtype == torch.float64 else (lambda t: t.float())
+        h = self._linear(x, self.inp.weight, self.inp.bias)
+        c, z = self._linear(seq_ops.rms_norm(handle, h, p(self.norm_in)), self.uz.weight).split(self.E, dim=-1)
+        return p, h, c, z
+
+    def _maps(self, u):
+        r, B, Cm = self._linear(u, self.maps.weight).split((self.R, self.N, self.N), dim=-1)
+        return self._linear(r, self.dt), B, Cm
+
+    def _finish(self, handle, p, y, h):
+        from . import seq_ops
+        return seq_ops.rms_norm(handle, self._linear(y, self.out.weight), p(self.norm_out), residual=h)[0]
+
+    def forward(self, handle, x, state=None, return_state=False):
+        from . import seq_ops
+        p, h, c, z = self._parts(handle, x)
+        conv, scan = state if state is not None else (None, None)
+        u = seq_ops.ssm_conv(handle, c, p(self.conv_weight), p(self.conv_bias), init=conv, reverse=self.reverse, return_state=return_state)
+        u, conv = u if return_state else (u, None)
+        delta, B, Cm = self._maps(u)
+        y = seq_ops.ssm_scan(handle, u, delta, -torch.exp(p(self.A_log)), B, Cm, D=p(self.skip), z=z, delta_bias=p(self.dt_bias), init=scan,
+                             reverse=self.reverse, return_state=return_state)
+        y, scan = y if return_state else (y, None)
+        n = self._finish(handle, p, y, h)
+        return (n, (conv, scan)) if return_state else n
+
+    def step(self, handle, x, state):
+        from . import seq_ops
+        p, h, c, z = self._parts(handle, x)
+        u = seq_ops.ssm_conv_step(handle, c, p(self.conv_weight), p(self.conv_bias), state[0])
+        delta, B, Cm = self._maps(u)
+        y = seq_ops.ssm_scan_step(handle, u, delta, -torch.exp(p(self.A_log)), B, Cm, p(self.skip), state[1], z=z, delta_bias=p(self.dt_bias))
+        return self._finish(handle, p, y, h)
+
+    def initial_state(self, batch, dtype, device):
+        acc = torch.float64 if dtype == torch.float64 else torch.float32
+        return (torch.zeros(batch, self.W - 1, self.E, dtype=dtype, device=device), torch.zeros(batch, self.E, self.N, dtype=acc, device=device))
+
+
+class MeanVarSSM(nn.Module):
+    """State-space encoder layer with the heads of MeanVarRNN.  Its recurrence is linear in the state, so it is split over time as well as
+    over sequences and channels (any hidden width, any length), and it can go on from a state.  It needs the model's handle: there is no
+    other path.  compute_dtype: the type of the activations inside; input, heads' output and parameters are fp64."""
+
+    handle = None
+
+    def __init__(self, input_dim, output_dim, hidden_dim, bidirectional=False, compute_dtype=None):
+        nn.Module.__init__(self)
+        self.compute_dtype = torch.float64 if compute_dtype is None else compute_dtype
+        if self.compute_dtype not in (torch.float64, torch.float32, torch.bfloat16, torch.float16):
+            raise ValueError('rnn_compute_dtype must be torch.float64, float32, bfloat16 or float16')
+        self.blocks = nn.ModuleList([_SsmBlock(input_dim, hidden_dim, r) for r in ((False, True) if bidirectional else (False,))])
+        self.linear_mean = nn.Linear(hidden_dim * len(self.blocks), output_dim)
+        self.linear_var = nn.Linear(hidden_dim * len(self.blocks), output_dim)
+        self.soft_plus = nn.Softplus()
+
+    def _heads(self, n):
+        n = n.double()
+        lin = _SsmBlock._linear
+        return lin(n, self.linear_mean.weight, self.linear_mean.bias), self.soft_plus(lin(n, self.linear_var.weight, self.linear_var.bias))
+
+    def _need(self, online):
+        if self.handle is None:
+            raise RuntimeError("the 'ssm' encoder runs on librgp_hip.so: set .handle (DeepAutoreg_rnn does)")
+        if online and len(self.blocks) > 1:
+            raise ValueError('a bidirectional encoder reads every sequence to its end: it has no online state')
+
+    def forward(self, x, state=None, return_state=False):                       # x: (seq_len, batch, input_dim)
+        self._need(state is not None or return_state)
+        x = x.to(self.compute_dtype)
+        if return_state:
+            n, state = self.blocks[0](self.handle, x, state, True)
+            return self._heads(n) + (state,)
+        ns = [b(self.handle, x, state) for b in self.blocks]
+        return self._heads(ns[0] if len(ns) == 1 else torch.cat(ns, dim=2))
+
+    def step(self, x, state):                                                   # x: (batch, input_dim); state updated in place
+        self._need(True)
+        return self._heads(self.blocks[0].step(self.handle, x.to(self.compute_dtype), state))
+
+    def initial_state(self, batch):
+        self._need(True)
+        return self.blocks[0].initial_state(batch, self.compute_dtype, self.linear_mean.weight.device)
+
+
+class SeqEncoder(nn.Module):
+    """Stack of MeanVarRNN layers, lower hidden layer first (rnn_encoder.py:86-150); rnn_type 'ssm': of MeanVarSSM layers."""
+
+    def __init__(self, input_dims, output_dims, hidden_dim, rnn_type='rnn', bidirectional=False, compute_dtype=None):
         nn.Module.__init__(self)
         assert len(input_dims) == len(output_dims)
+        if compute_dtype is not None and rnn_type != 'ssm':
+            raise ValueError("rnn_compute_dtype is for rnn_type 'ssm': the other cells compute in fp64")
         self.layers = nn.ModuleList()
         for l, (din, dout) in enumerate(zip(input_dims, output_dims)):
-            self.layers.append(MeanVarRNN(din if l == 0 else 2 * din, dout, hidden_dim, rnn_type, bidirectional))
+            d = din if l == 0 else 2 * din
+            self.layers.append(MeanVarSSM(d, dout, hidden_dim, bidirectional, compute_dtype) if rnn_type == 'ssm' else
+                               MeanVarRNN(d, dout, hidden_dim, rnn_type, bidirectional))
         self.double()
 
-    def forward(self, x0):
-        means, variances = [], []
+    def forward(self, x0, state=None, return_state=False):
+        """(means, variances) of every layer, (seq_len, batch, H) each.  'ssm' layers: state (a list with one entry per layer, from
+        ``initial_state`` or an earlier call) continues sequences; return_state=True also returns the state behind the last step."""
+        online = state is not None or return_state
+        if online:
+            self._need_ssm()
+        means, variances, states = [], [], []
         m, v = x0, None
         for l, layer in enumerate(self.layers):
-            m, v = layer(m if l == 0 else torch.cat((m, v), dim=2))
+            x = m if l == 0 else torch.cat((m, v), dim=2)
+            if return_state:
+                m, v, st = layer(x, None if state is None else state[l], True)
+                states.append(st)
+            else:
+                m, v = layer(x, state[l]) if online else layer(x)
+            means.append(m)
+            variances.append(v)
+        return (means, variances, states) if return_state else (means, variances)
+
+    def _need_ssm(self):
+        if not all(isinstance(layer, MeanVarSSM) for layer in self.layers):
+            raise ValueError("only rnn_type 'ssm' encoders go on from a state")
+
+    def initial_state(self, batch):
+        """The state before the first observation of ``batch`` sequences."""
+        self._need_ssm()
+        return [layer.initial_state(batch) for layer in self.layers]
+
+    def step(self, x, state):
+        """One observation of every sequence: x (batch, input_dim) -> (means, variances) of every layer, (batch, H) each; state is updated
+        in place."""
+        self._need_ssm()
+        means, variances = [], []
+        m, v = x, None
+        for l, layer in enumerate(self.layers):
+            m, v = layer.step(m if l == 0 else torch.cat((m, v), dim=1), state[l])
             means.append(m)
             variances.append(v)
         return means, variances
