@@ -5,7 +5,7 @@
 
 struct NormDev {
   rgp_rms_norm a;
-  int wx, wr, wgy, wgh, wout;
+  int wide;
   void* part;
 };
 
@@ -26,75 +26,94 @@ static __device__ __forceinline__ A row_sum(A v, A* sh) {
   }
 }
 
-// TPR threads a row, NE vectors of V elements each; rows TPR * NE * V >= C.  hid is rounded to its type where it is written; the norm
-// uses the sum before that rounding.
-template <typename T, int TPR, int NE>
+// TPR threads a row, NE vectors of V elements each (V = 1 where alignment or an odd width forbids 16 bytes); rows of TPR * NE * V >= C
+// elements.  A workgroup takes every gridDim-th group of rows and keeps w; the next rows are loaded while these are normed.  hid is rounded
+// to its type where it is written; the norm uses the sum before that rounding.
+template <typename T, int TPR, int NE, int V>
 static __global__ void __launch_bounds__(256) rms_fwd_kernel(NormDev d) {
   typedef typename SeqAcc<T>::type A;
-  constexpr int V = SeqVec<T>::V, RPB = 256 / TPR;
+  typedef SeqVec<T, V> Vec;
+  constexpr int RPB = 256 / TPR;
   __shared__ A sh[4];
   const rgp_rms_norm& a = d.a;
-  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
-  const int l = threadIdx.x % TPR;
-  if (TPR <= 64 && row >= a.rows) return;
-  A h[NE][V], q = (A)0;
+  const int l = threadIdx.x % TPR, rg = threadIdx.x / TPR;
+  A w[NE][V];
+  int64_t col[NE];
+  bool in[NE];
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
     const int64_t c = (int64_t)(l + i * TPR) * V;
-    const int n = a.C - c < V ? (a.C - c < 0 ? 0 : (int)(a.C - c)) : V;
-    const SeqVec<T> x = seq_load((const T*)a.x + row * a.x_st + c, n, d.wx);
-    SeqVec<T> r = seq_load((const T*)a.x, 0, false);
-    if (a.residual) r = seq_load((const T*)a.residual + row * a.residual_st + c, n, d.wr);
+    in[i] = c < a.C;
+    col[i] = in[i] ? c : 0;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      h[i][j] = (A)x.e[j] + (A)r.e[j];
-      q += h[i][j] * h[i][j];
-    }
+    for (int j = 0; j < V; ++j) w[i][j] = in[i] ? ((const A*)a.w)[c + j] : (A)0;
   }
-  q = row_sum<TPR>(q, sh);
-  const A rs = seq_rsqrt(q / (A)a.C + (A)a.eps);
-  if (a.rstd && l == 0) ((A*)a.rstd)[row] = rs;
+  Vec x[NE], r[NE];
+  auto fetch = [&](int64_t row) {                    // rows behind the last one read the last one
+    const int64_t rr = row < a.rows ? row : a.rows - 1;
 #pragma unroll
-  for (int i = 0; i < NE; ++i) {
-    const int64_t c = (int64_t)(l + i * TPR) * V;
-    const int n = a.C - c < V ? (a.C - c < 0 ? 0 : (int)(a.C - c)) : V;
-    if (n > 0) {
-      SeqVec<T> y, o;
+    for (int i = 0; i < NE; ++i) {
+      x[i] = *(const Vec*)((const T*)a.x + rr * a.x_st + col[i]);
+      if (a.residual) r[i] = *(const Vec*)((const T*)a.residual + rr * a.residual_st + col[i]);
+    }
+  };
+  int64_t r0 = (int64_t)blockIdx.x * RPB;
+  if (r0 < a.rows) fetch(r0 + rg);
+  for (; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t row = r0 + rg;
+    A h[NE][V], q = (A)0;
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        o.e[j] = (T)h[i][j];
-        y.e[j] = (T)(h[i][j] * rs * (j < n ? ((const A*)a.w)[c + j] : (A)0));
+        h[i][j] = (A)x[i].e[j] + (a.residual ? (A)r[i].e[j] : (A)0);
+        q += in[i] ? h[i][j] * h[i][j] : (A)0;
       }
-      seq_store((T*)a.y + row * a.C + c, y, n, d.wout);
-      if (a.hid) seq_store((T*)a.hid + row * a.C + c, o, n, d.wout);
+    if (r0 + (int64_t)gridDim.x * RPB < a.rows) fetch(row + (int64_t)gridDim.x * RPB);
+    q = row_sum<TPR>(q, sh);
+    const A rs = seq_rsqrt(q / (A)a.C + (A)a.eps);
+    if (row < a.rows) {
+      if (a.rstd && l == 0) ((A*)a.rstd)[row] = rs;
+#pragma unroll
+      for (int i = 0; i < NE; ++i) {
+        if (in[i]) {
+          Vec y, o;
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            o.e[j] = (T)h[i][j];
+            y.e[j] = (T)(h[i][j] * rs * w[i][j]);
+          }
+          *(Vec*)((T*)a.y + row * a.C + col[i]) = y;
+          if (a.hid) *(Vec*)((T*)a.hid + row * a.C + col[i]) = o;
+        }
+      }
     }
   }
 }
 // rows longer than a workgroup's registers: the sum of squares, then the row once more
-template <typename T>
+template <typename T, int V>
 static __global__ void __launch_bounds__(256) rms_fwd_long_kernel(NormDev d) {
   typedef typename SeqAcc<T>::type A;
-  constexpr int V = SeqVec<T>::V;
+  typedef SeqVec<T, V> Vec;
   __shared__ A sh[4];
   const rgp_rms_norm& a = d.a;
   const int64_t row = blockIdx.x;
   A q = (A)0, rs = (A)0;
   for (int pass = 0; pass < 2; ++pass) {
     for (int64_t c = (int64_t)threadIdx.x * V; c < a.C; c += 256 * V) {
-      const int n = a.C - c < V ? (int)(a.C - c) : V;
-      const SeqVec<T> x = seq_load((const T*)a.x + row * a.x_st + c, n, d.wx);
-      SeqVec<T> r = seq_load((const T*)a.x, 0, false), y, o;
-      if (a.residual) r = seq_load((const T*)a.residual + row * a.residual_st + c, n, d.wr);
+      const Vec x = *(const Vec*)((const T*)a.x + row * a.x_st + c);
+      Vec r, y, o;
+      if (a.residual) r = *(const Vec*)((const T*)a.residual + row * a.residual_st + c);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const A h = (A)x.e[j] + (A)r.e[j];
+        const A h = (A)x.e[j] + (a.residual ? (A)r.e[j] : (A)0);
         if (pass == 0) q += h * h;
         o.e[j] = (T)h;
-        y.e[j] = (T)(h * rs * (j < n ? ((const A*)a.w)[c + j] : (A)0));
+        y.e[j] = (T)(h * rs * ((const A*)a.w)[c + j]);
       }
       if (pass == 1) {
-        seq_store((T*)a.y + row * a.C + c, y, n, d.wout);
-        if (a.hid) seq_store((T*)a.hid + row * a.C + c, o, n, d.wout);
+        *(Vec*)((T*)a.y + row * a.C + c) = y;
+        if (a.hid) *(Vec*)((T*)a.hid + row * a.C + c) = o;
       }
     }
     if (pass == 0) {
@@ -106,65 +125,69 @@ static __global__ void __launch_bounds__(256) rms_fwd_long_kernel(NormDev d) {
 }
 
 // gx = ghid + r (gy w - hid r^2 mean(gy w hid)); gw = sum over rows of gy hid r.  hid is x + residual again, before its rounding to a 16-bit
-// storage type: gw is a sum over many rows in 32 bits, and that rounding (2^-9 relative) would be its largest error by far.  A workgroup takes every nblk-th group of
-// rows, sums gw in registers and adds its row groups through LDS; the workgroups' sums are added in a fixed order afterwards.
-template <typename T, int TPR, int NE>
+// storage type: gw is a sum over many rows in 32 bits, and that rounding (2^-9 relative) would be its largest error by far.  A workgroup
+// takes every gridDim-th group of rows, sums gw in registers and adds its row groups through LDS; the workgroups' sums are added in a fixed
+// order afterwards.
+template <typename T, int TPR, int NE, int V>
 static __global__ void __launch_bounds__(256) rms_bwd_kernel(NormDev d) {
   typedef typename SeqAcc<T>::type A;
-  constexpr int V = SeqVec<T>::V, RPB = 256 / TPR;
+  typedef SeqVec<T, V> Vec;
+  constexpr int RPB = 256 / TPR;
   __shared__ A sh[4];
   __shared__ A acc[256 * V];
   const rgp_rms_norm& a = d.a;
   const int l = threadIdx.x % TPR, rg = threadIdx.x / TPR;
   A gw[NE][V], w[NE][V];
+  int64_t col[NE];
+  bool in[NE];
 #pragma unroll
-  for (int i = 0; i < NE; ++i)
+  for (int i = 0; i < NE; ++i) {
+    const int64_t c = (int64_t)(l + i * TPR) * V;
+    in[i] = c < a.C;
+    col[i] = in[i] ? c : 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int64_t c = (int64_t)(l + i * TPR) * V + j;
       gw[i][j] = (A)0;
-      w[i][j] = c < a.C ? ((const A*)a.w)[c] : (A)0;
+      w[i][j] = in[i] ? ((const A*)a.w)[c + j] : (A)0;
     }
+  }
   const A inv = (A)1 / (A)a.C;
   for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
     const int64_t row = r0 + rg;
     const bool live = row < a.rows;
-    const int64_t rr = live ? row : 0;
-    SeqVec<T> x[NE], r[NE], g[NE], gh[NE];
-    const A rs = live ? ((const A*)a.rstd)[rr] : (A)0;
-    A q = (A)0;
+    const int64_t rr = live ? row : a.rows - 1;
+    Vec x[NE], r[NE], g[NE], gh[NE];
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      const int64_t c = (int64_t)(l + i * TPR) * V;
-      const int n = !live || a.C - c < 0 ? 0 : (a.C - c < V ? (int)(a.C - c) : V);
-      x[i] = seq_load((const T*)a.x + rr * a.x_st + c, n, d.wx);
-      if (a.residual) r[i] = seq_load((const T*)a.residual + rr * a.residual_st + c, n, d.wr);
-      g[i] = seq_load((const T*)a.gy + rr * a.gy_st + c, n, d.wgy);
-      if (a.ghid) gh[i] = seq_load((const T*)a.ghid + rr * a.ghid_st + c, n, d.wgh);
+      x[i] = *(const Vec*)((const T*)a.x + rr * a.x_st + col[i]);
+      if (a.residual) r[i] = *(const Vec*)((const T*)a.residual + rr * a.residual_st + col[i]);
+      g[i] = *(const Vec*)((const T*)a.gy + rr * a.gy_st + col[i]);
+      if (a.ghid) gh[i] = *(const Vec*)((const T*)a.ghid + rr * a.ghid_st + col[i]);
     }
-    A hid[NE][V];
+    const A rs = ((const A*)a.rstd)[rr];
+    A hid[NE][V], q = (A)0;
 #pragma unroll
     for (int i = 0; i < NE; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         hid[i][j] = (A)x[i].e[j] + (a.residual ? (A)r[i].e[j] : (A)0);
-        q += (A)g[i].e[j] * w[i][j] * hid[i][j];
+        q += in[i] ? (A)g[i].e[j] * w[i][j] * hid[i][j] : (A)0;
       }
     q = row_sum<TPR>(q, sh) * inv * rs * rs;
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      const int64_t c = (int64_t)(l + i * TPR) * V;
-      const int n = !live || a.C - c < 0 ? 0 : (a.C - c < V ? (int)(a.C - c) : V);
-      SeqVec<T> o;
+      if (in[i] && live) {
+        Vec o;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const A gy = (A)g[i].e[j], h = hid[i][j];
-        A v = rs * (gy * w[i][j] - h * q);
-        if (a.ghid) v += (A)gh[i].e[j];
-        o.e[j] = (T)v;
-        if (n > 0) gw[i][j] += gy * h * rs;
+        for (int j = 0; j < V; ++j) {
+          const A gy = (A)g[i].e[j], h = hid[i][j];
+          A v = rs * (gy * w[i][j] - h * q);
+          if (a.ghid) v += (A)gh[i].e[j];
+          o.e[j] = (T)v;
+          gw[i][j] += gy * h * rs;
+        }
+        *(Vec*)((T*)a.gx + rr * a.C + col[i]) = o;
       }
-      if (n > 0) seq_store((T*)a.gx + rr * a.C + c, o, n, d.wout);
     }
   }
   A* const part = (A*)d.part + (int64_t)blockIdx.x * a.C;
@@ -184,57 +207,66 @@ static __global__ void __launch_bounds__(256) rms_bwd_kernel(NormDev d) {
   }
 }
 // rows longer than a workgroup's registers: gw goes through memory, one row of the partial sums per workgroup
-template <typename T>
+template <typename T, int V>
 static __global__ void __launch_bounds__(256) rms_bwd_long_kernel(NormDev d) {
   typedef typename SeqAcc<T>::type A;
-  constexpr int V = SeqVec<T>::V;
+  typedef SeqVec<T, V> Vec;
   __shared__ A sh[4];
   const rgp_rms_norm& a = d.a;
   A* const part = (A*)d.part + (int64_t)blockIdx.x * a.C;
-  for (int64_t c = threadIdx.x; c < a.C; c += 256) part[c] = (A)0;
-  __syncthreads();
+  for (int64_t c = (int64_t)threadIdx.x * V; c < a.C; c += 256 * V)      // the elements that this thread adds to below
+#pragma unroll
+    for (int j = 0; j < V; ++j) part[c + j] = (A)0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const A rs = ((const A*)a.rstd)[row];
     A q = (A)0;
     for (int pass = 0; pass < 2; ++pass) {
       for (int64_t c = (int64_t)threadIdx.x * V; c < a.C; c += 256 * V) {
-        const int n = a.C - c < V ? (int)(a.C - c) : V;
-        const SeqVec<T> x = seq_load((const T*)a.x + row * a.x_st + c, n, d.wx);
-        const SeqVec<T> g = seq_load((const T*)a.gy + row * a.gy_st + c, n, d.wgy);
-        SeqVec<T> r = seq_load((const T*)a.x, 0, false), gh = r, o;
-        if (a.residual) r = seq_load((const T*)a.residual + row * a.residual_st + c, n, d.wr);
-        if (pass == 1 && a.ghid) gh = seq_load((const T*)a.ghid + row * a.ghid_st + c, n, d.wgh);
+        const Vec x = *(const Vec*)((const T*)a.x + row * a.x_st + c);
+        const Vec g = *(const Vec*)((const T*)a.gy + row * a.gy_st + c);
+        Vec r, gh, o;
+        if (a.residual) r = *(const Vec*)((const T*)a.residual + row * a.residual_st + c);
+        if (pass == 1 && a.ghid) gh = *(const Vec*)((const T*)a.ghid + row * a.ghid_st + c);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          const A w = j < n ? ((const A*)a.w)[c + j] : (A)0, gy = (A)g.e[j], h = (A)x.e[j] + (A)r.e[j];
+          const A w = ((const A*)a.w)[c + j], gy = (A)g.e[j], h = (A)x.e[j] + (a.residual ? (A)r.e[j] : (A)0);
           if (pass == 0) {
             q += gy * w * h;
           } else {
-            o.e[j] = (T)((A)gh.e[j] + rs * (gy * w - h * q));
-            if (j < n) part[c + j] += gy * h * rs;
+            o.e[j] = (T)((a.ghid ? (A)gh.e[j] : (A)0) + rs * (gy * w - h * q));
+            part[c + j] += gy * h * rs;
           }
         }
-        if (pass == 1) seq_store((T*)a.gx + row * a.C + c, o, n, d.wout);
+        if (pass == 1) *(Vec*)((T*)a.gx + row * a.C + c) = o;
       }
       if (pass == 0) q = row_sum<256>(q, sh) / (A)a.C * rs * rs;
     }
   }
 }
 
-// threads a row and vectors a thread: the fewest lanes left idle, at most 8 vectors (a row then needs 64 arithmetic registers of operands)
+// Threads a row and vectors a thread: of the shapes that hold a row, the one that leaves the fewest lanes idle, and of those the one with the
+// fewest threads a row -- unless the rows are few, where more threads a row finish it sooner.
 struct RmsShape { int tpr, ne; };
-static RmsShape rms_shape(int64_t C, int V) {
+static RmsShape rms_shape(int64_t C, int V, int64_t rows) {
   const int64_t nv = (C + V - 1) / V;
-  const int tprs[4] = {8, 16, 64, 256}, nes[4] = {1, 2, 4, 8};
+  static const int tprs[4] = {8, 16, 64, 256}, nes[5] = {1, 2, 3, 4, 8};
+  RmsShape best{0, 0};
   for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j)
-      if ((int64_t)tprs[i] * nes[j] >= nv && (j < 2 || i == 3 || (i < 3 && j == 2 && (int64_t)tprs[i] * 4 >= nv))) return RmsShape{tprs[i], nes[j]};
-  return RmsShape{0, 0};
+    for (int j = 0; j < 5; ++j) {
+      const int64_t hold = (int64_t)tprs[i] * nes[j];
+      if (hold < nv || (nes[j] == 8 && tprs[i] < 256)) continue;
+      const bool few = rows * tprs[i] <= 65536;                          // fewer threads than the card has lanes: the wider shape is free
+      if (!best.tpr || hold < (int64_t)best.tpr * best.ne || (few && tprs[i] > best.tpr && hold <= 2 * (int64_t)best.tpr * best.ne))
+        best = RmsShape{tprs[i], nes[j]};
+    }
+  return best;
 }
-static int64_t rms_blocks(const rgp_rms_norm* a, RmsShape s) {
+static int64_t rms_blocks(const rgp_rms_norm* a, RmsShape s, int most) {
   const int64_t rpb = s.tpr ? 256 / s.tpr : 1, want = (a->rows + rpb - 1) / rpb;
-  return want < 1024 ? (want < 1 ? 1 : want) : 1024;
+  return want < most ? (want < 1 ? 1 : want) : most;
 }
+#define RMS_FWD_BLOCKS 2048
+#define RMS_BWD_BLOCKS 512
 static const char* rms_bad(const rgp_rms_norm* a) {
   if (!a) return "null arguments";
   if (a->dtype < 0 || a->dtype > 3) return "dtype must be RGP_F64, RGP_F32, RGP_BF16 or RGP_F16";
@@ -245,37 +277,44 @@ static const char* rms_bad(const rgp_rms_norm* a) {
 extern "C" int64_t rgp_rms_norm_workspace(const rgp_rms_norm* a, int backward) {
   if (rms_bad(a)) return -1;
   if (!backward) return 0;
-  return rms_blocks(a, rms_shape(a->C, 16 / seq_dtype_bytes(a->dtype))) * a->C * (a->dtype == RGP_F64 ? 8 : 4);
+  const int64_t one = rms_blocks(a, rms_shape(a->C, 1, a->rows), RMS_BWD_BLOCKS);
+  const int64_t wide = rms_blocks(a, rms_shape(a->C, 16 / seq_dtype_bytes(a->dtype), a->rows), RMS_BWD_BLOCKS);
+  return (one > wide ? one : wide) * a->C * (a->dtype == RGP_F64 ? 8 : 4);
 }
-template <typename T, int TPR, int NE>
+template <typename T, int TPR, int NE, int V>
 static hipError_t rms_go(const NormDev& d, bool back, int64_t blocks, hipStream_t s) {
-  if (back) hipLaunchKernelGGL((rms_bwd_kernel<T, TPR, NE>), dim3((unsigned)blocks), dim3(256), 0, s, d);
-  else hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, NE>), dim3((unsigned)((d.a.rows + 256 / TPR - 1) / (256 / TPR))), dim3(256), 0, s, d);
+  if (back) hipLaunchKernelGGL((rms_bwd_kernel<T, TPR, NE, V>), dim3((unsigned)blocks), dim3(256), 0, s, d);
+  else hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, NE, V>), dim3((unsigned)blocks), dim3(256), 0, s, d);
   return hipGetLastError();
 }
-template <typename T, int TPR>
+template <typename T, int TPR, int V>
 static hipError_t rms_ne(const NormDev& d, int ne, bool back, int64_t blocks, hipStream_t s) {
   switch (ne) {
-    case 1: return rms_go<T, TPR, 1>(d, back, blocks, s);
-    case 2: return rms_go<T, TPR, 2>(d, back, blocks, s);
-    case 4: return rms_go<T, TPR, 4>(d, back, blocks, s);
+    case 1: return rms_go<T, TPR, 1, V>(d, back, blocks, s);
+    case 2: return rms_go<T, TPR, 2, V>(d, back, blocks, s);
+    case 3: return rms_go<T, TPR, 3, V>(d, back, blocks, s);
+    case 4: return rms_go<T, TPR, 4, V>(d, back, blocks, s);
     default:
-      if constexpr (TPR == 256) return rms_go<T, TPR, 8>(d, back, blocks, s);
+      if constexpr (TPR == 256) return rms_go<T, TPR, 8, V>(d, back, blocks, s);
       return hipErrorInvalidValue;
+  }
+}
+template <typename T, int V>
+static hipError_t rms_shaped(const NormDev& d, RmsShape sh, bool back, int64_t blocks, hipStream_t s) {
+  switch (sh.tpr) {
+    case 8: return rms_ne<T, 8, V>(d, sh.ne, back, blocks, s);
+    case 16: return rms_ne<T, 16, V>(d, sh.ne, back, blocks, s);
+    case 64: return rms_ne<T, 64, V>(d, sh.ne, back, blocks, s);
+    case 256: return rms_ne<T, 256, V>(d, sh.ne, back, blocks, s);
+    default:
+      if (back) hipLaunchKernelGGL((rms_bwd_long_kernel<T, V>), dim3((unsigned)blocks), dim3(256), 0, s, d);
+      else hipLaunchKernelGGL((rms_fwd_long_kernel<T, V>), dim3((unsigned)d.a.rows), dim3(256), 0, s, d);
+      return hipGetLastError();
   }
 }
 template <typename T>
 static hipError_t rms_pick(const NormDev& d, RmsShape sh, bool back, int64_t blocks, hipStream_t s) {
-  switch (sh.tpr) {
-    case 8: return rms_ne<T, 8>(d, sh.ne, back, blocks, s);
-    case 16: return rms_ne<T, 16>(d, sh.ne, back, blocks, s);
-    case 64: return rms_ne<T, 64>(d, sh.ne, back, blocks, s);
-    case 256: return rms_ne<T, 256>(d, sh.ne, back, blocks, s);
-    default:
-      if (back) hipLaunchKernelGGL(rms_bwd_long_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, d);
-      else hipLaunchKernelGGL(rms_fwd_long_kernel<T>, dim3((unsigned)d.a.rows), dim3(256), 0, s, d);
-      return hipGetLastError();
-  }
+  return d.wide ? rms_shaped<T, 16 / (int)sizeof(T)>(d, sh, back, blocks, s) : rms_shaped<T, 1>(d, sh, back, blocks, s);
 }
 static rgp_status rms_run(rgp_handle h, hipStream_t s, const rgp_rms_norm* a, bool back) {
   const std::string name = back ? "rms norm backward: " : "rms norm: ";
@@ -283,20 +322,17 @@ static rgp_status rms_run(rgp_handle h, hipStream_t s, const rgp_rms_norm* a, bo
   if (!a->w || (back && !a->gw) || (a->rows > 0 && (!a->x || (!back && !a->y) || (back && (!a->gy || !a->gx || !a->rstd)))))
     return rgp_fail(h, RGP_ERR_BAD_ARG, name + "a required buffer is null");
   if (!back && a->rows > 0 && (a->residual != nullptr) != (a->hid != nullptr)) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "residual and hid go together");
-  if (a->rows > 2147483647) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "more than 2^31 - 1 rows");
+  if (a->rows > 16777215) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "more than 2^24 - 1 rows");
   const int e = seq_dtype_bytes(a->dtype), V = 16 / e;
-  const RmsShape sh = rms_shape(a->C, V);
-  const int64_t blocks = rms_blocks(a, sh);
-  if (!back && (double)a->rows * (sh.tpr ? sh.tpr : 256) > 4294967040.0) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "more than 2^32 work items");
-  if (back && (rgp_rms_norm_workspace(a, 1) > a->work_bytes || !a->work || ((uintptr_t)a->work & 15)))
-    return rgp_fail(h, RGP_ERR_WORKSPACE, name + "work buffer too small or not 16-byte aligned");
   NormDev d{};
   d.a = *a;
-  d.wx = seq_aligned(a->x, a->x_st, 0, e);
-  d.wr = a->residual && seq_aligned(a->residual, a->residual_st, 0, e);
-  d.wgy = back && seq_aligned(a->gy, a->gy_st, 0, e);
-  d.wgh = back && a->ghid && seq_aligned(a->ghid, a->ghid_st, 0, e);
-  d.wout = a->C % V == 0 && (back ? seq_aligned(a->gx, 0, 0, e) : seq_aligned(a->y, 0, 0, e) && (!a->hid || seq_aligned(a->hid, 0, 0, e)));
+  d.wide = a->C % V == 0 && seq_aligned(a->x, a->x_st, 0, e) && (!a->residual || seq_aligned(a->residual, a->residual_st, 0, e));
+  if (back) d.wide = d.wide && seq_aligned(a->gy, a->gy_st, 0, e) && (!a->ghid || seq_aligned(a->ghid, a->ghid_st, 0, e)) && seq_aligned(a->gx, 0, 0, e);
+  else d.wide = d.wide && seq_aligned(a->y, 0, 0, e) && (!a->hid || seq_aligned(a->hid, 0, 0, e));
+  const RmsShape sh = rms_shape(a->C, d.wide ? V : 1, a->rows);
+  const int64_t blocks = rms_blocks(a, sh, back ? RMS_BWD_BLOCKS : RMS_FWD_BLOCKS);
+  if (back && (rgp_rms_norm_workspace(a, 1) > a->work_bytes || !a->work || ((uintptr_t)a->work & 15)))
+    return rgp_fail(h, RGP_ERR_WORKSPACE, name + "work buffer too small or not 16-byte aligned");
   d.part = a->work;
   if (!back && a->rows == 0) return RGP_OK;
   hipError_t err = a->dtype == RGP_F64 ? rms_pick<double>(d, sh, back, blocks, s) : a->dtype == RGP_F32 ? rms_pick<float>(d, sh, back, blocks, s)
@@ -304,7 +340,9 @@ static rgp_status rms_run(rgp_handle h, hipStream_t s, const rgp_rms_norm* a, bo
   if (err != hipSuccess) return rgp_fail(h, RGP_ERR_HIP, name + hipGetErrorString(err));
   if (!back) return RGP_OK;
   const int acc = a->dtype == RGP_F64 ? RGP_F64 : RGP_F32;
-  return seq_reduce(h, s, acc, acc, d.part, blocks, a->C, a->C, a->gw);
+  SeqSums sums;
+  sums.add(d.part, blocks, a->C, a->C, a->gw, acc);
+  return sums.run(h, s, acc);
 }
 extern "C" rgp_status rgp_rms_norm_forward(rgp_handle h, void* stream, const rgp_rms_norm* a) {
   SEQ_ENTRY(h, "rms norm", { return rms_run(h, (hipStream_t)stream, a, false); })
@@ -401,12 +439,13 @@ static __device__ __forceinline__ void grad_scale(T* p, int64_t n, double c) {
     seq_store(q, v, k, wide);
   });
 }
+// walks tensors and pieces from the last to the first: what the norm read last is still in the memory-side cache
 static __global__ void __launch_bounds__(256) grad_clip_kernel(GradTable t, const double* sumsq, double max_norm) {
   const double norm = sqrt(sumsq[0]), c = max_norm / (norm + 1e-6);
   if (!(c < 1.0) || !(norm < 1.7976931348623157e308)) return;           // nothing to clip, or a norm that is no number
   const int i = grad_find(t, blockIdx.x);
   const int es = t.dt[i] == RGP_F64 ? 8 : t.dt[i] == RGP_F32 ? 4 : 2;
-  const int64_t per = GP / es, o = (int64_t)((int)blockIdx.x - t.first[i]) * per, n = t.n[i] - o < per ? t.n[i] - o : per;
+  const int64_t per = GP / es, o = (int64_t)(t.first[i + 1] - 1 - (int)blockIdx.x) * per, n = t.n[i] - o < per ? t.n[i] - o : per;
   switch (t.dt[i]) {
     case RGP_F64: grad_scale((double*)t.p[i] + o, n, c); break;
     case RGP_F32: grad_scale((float*)t.p[i] + o, n, c); break;
@@ -430,36 +469,33 @@ extern "C" int64_t rgp_grad_workspace(int n, const int64_t* numel, const int32_t
   for (int i = 0; i < n; ++i) p += grad_pieces(numel[i], dtype[i]);
   return (p < 1 ? 1 : p) * (int64_t)sizeof(double);
 }
-// calls f(table, pieces, first piece of the launch) for groups of up to GT tensors
+// calls f(table, pieces, pieces before) for groups of up to GT tensors; back: from the last tensor to the first
 template <typename F>
-static rgp_status grad_tables(rgp_handle h, int n, void* const* ptr, const int64_t* numel, const int32_t* dtype, F f) {
+static rgp_status grad_tables(rgp_handle h, int n, void* const* ptr, const int64_t* numel, const int32_t* dtype, bool back, F f) {
   GradTable t;
-  t.count = 0;
-  int64_t pieces = 0, before = 0;
-  auto flush = [&]() -> rgp_status {
-    if (!t.count) return RGP_OK;
+  int64_t before = 0;
+  for (int k = 0; k < n;) {                              // a group: the next GT tensors that have elements, fewer where the grid would grow too long
+    int64_t pieces = 0;
+    t.count = 0;
+    for (; k < n && t.count < GT; ++k) {
+      const int i = back ? n - 1 - k : k;
+      if (numel[i] == 0) continue;
+      const int64_t add = grad_pieces(numel[i], dtype[i]);
+      if (add > 8000000) return rgp_fail(h, RGP_ERR_BAD_ARG, "gradient norm: a tensor of more than 500 GB");
+      if (pieces + add > 8000000) break;
+      t.p[t.count] = ptr[i];
+      t.n[t.count] = numel[i];
+      t.dt[t.count] = (uint8_t)dtype[i];
+      t.first[t.count++] = (int)pieces;
+      pieces += add;
+    }
+    if (!t.count) continue;
     t.first[t.count] = (int)pieces;
     const rgp_status st = f(t, (unsigned)pieces, before);
+    if (st) return st;
     before += pieces;
-    pieces = 0;
-    t.count = 0;
-    return st;
-  };
-  for (int i = 0; i < n; ++i) {
-    if (numel[i] == 0) continue;
-    const int64_t add = grad_pieces(numel[i], dtype[i]);
-    if (add > 8000000) return rgp_fail(h, RGP_ERR_BAD_ARG, "gradient norm: a tensor of more than 500 GB");
-    if (t.count == GT || pieces + add > 8000000) {
-      const rgp_status st = flush();
-      if (st) return st;
-    }
-    t.p[t.count] = ptr[i];
-    t.n[t.count] = numel[i];
-    t.dt[t.count] = (uint8_t)dtype[i];
-    t.first[t.count++] = (int)pieces;
-    pieces += add;
   }
-  return flush();
+  return RGP_OK;
 }
 static rgp_status grad_check(rgp_handle h, int n, void* const* ptr, const int64_t* numel, const int32_t* dtype) {
   if (const char* bad = grad_bad(n, numel, dtype)) return rgp_fail(h, RGP_ERR_BAD_ARG, std::string("gradient norm: ") + bad);
@@ -477,7 +513,7 @@ extern "C" rgp_status rgp_grad_sumsq(rgp_handle h, void* stream, int n, void* co
       return rgp_fail(h, RGP_ERR_WORKSPACE, "gradient norm: work buffer too small");
     const hipStream_t s = (hipStream_t)stream;
     int64_t total = 0;
-    st = grad_tables(h, n, ptr, numel, dtype, [&](const GradTable& t, unsigned pieces, int64_t before) {
+    st = grad_tables(h, n, ptr, numel, dtype, false, [&](const GradTable& t, unsigned pieces, int64_t before) {
       hipLaunchKernelGGL(grad_sumsq_kernel, dim3(pieces), dim3(256), 0, s, t, (double*)work + before);
       total = before + pieces;
       return seq_launched(h, "gradient norm");
@@ -494,7 +530,7 @@ extern "C" rgp_status rgp_grad_clip(rgp_handle h, void* stream, int n, void* con
     if (st) return st;
     if (!sumsq || !norm || !(max_norm > 0.0)) return rgp_fail(h, RGP_ERR_BAD_ARG, "gradient clip: sumsq, norm and a positive max_norm are required");
     const hipStream_t s = (hipStream_t)stream;
-    st = grad_tables(h, n, ptr, numel, dtype, [&](const GradTable& t, unsigned pieces, int64_t) {
+    st = grad_tables(h, n, ptr, numel, dtype, true, [&](const GradTable& t, unsigned pieces, int64_t) {
       hipLaunchKernelGGL(grad_clip_kernel, dim3(pieces), dim3(256), 0, s, t, sumsq, max_norm);
       return seq_launched(h, "gradient clip");
     });

@@ -12,9 +12,9 @@
 template <typename T> struct SeqAcc { typedef float type; };
 template <> struct SeqAcc<double> { typedef double type; };
 
-template <typename T>
-struct alignas(16) SeqVec {
-  static constexpr int V = 16 / (int)sizeof(T);
+template <typename T, int W = 16 / (int)sizeof(T)>
+struct alignas(W * sizeof(T)) SeqVec {
+  static constexpr int V = W;
   T e[V];
 };
 
@@ -130,26 +130,20 @@ static __device__ __forceinline__ float seq_log1p01(float e) {
 }
 static __device__ __forceinline__ double seq_log1p01(double e) { return log1p(e); }
 
-// softplus(x) and the sigmoid (its derivative)
+// softplus(x) and the sigmoid (its derivative); NaN passes through both
 template <typename A>
 static __device__ __forceinline__ A seq_softplus(A x, A& sig) {
   const A e = seq_exp_neg(x), big = seq_rcp((A)1 + e);
   sig = x >= (A)0 ? big : e * big;
-  if (x != x) sig = x;
-  const A m = x > (A)0 ? x : (A)0;
-  return x != x ? x : m + seq_log1p01(e);
+  return (x > (A)0 ? x : (A)0) + seq_log1p01(e);
 }
-// sigmoid and 1 - sigmoid, each with its own relative accuracy
+// the sigmoid, off by at most |x| half steps relative to its value (what the argument of the exponential rounds by)
 template <typename A>
-static __device__ __forceinline__ A seq_sigmoid(A x, A& comp) {
-  const A e = seq_exp_neg(x), big = seq_rcp((A)1 + e), small = e * big;
-  comp = x >= (A)0 ? small : big;
-  return x >= (A)0 ? big : (x != x ? x : small);
-}
+static __device__ __forceinline__ A seq_sigmoid(A x) { return seq_rcp((A)1 + seq_exp(-x)); }
 
 // ---- rows of sequences --------------------------------------------------------------------------------------------------------------
 // off == nullptr: n_seq sequences of T steps, step t of sequence s at base + s * sb + t * st; otherwise packed rows, step t of sequence s
-// at base + (off[s] + t) * st.  Sequences are cut into blocks of L steps that never cross a sequence; block j of sequence i is number
+// at base + (off[s] + t) * st.  Sequences are cut into blocks of L = 2^lg steps that never cross a sequence; block j of sequence i is number
 // i * ceil(T / L) + j, or floor(off[i] / L) + i + j for packed rows: those numbers are increasing, distinct and below rows / L + n_seq
 // without a table of block counts (some stay empty).  Offsets are clamped to the rows there are, so a wrong table cannot make a kernel
 // touch memory outside its tensors.
@@ -162,40 +156,40 @@ struct SeqBlock {
   int64_t start, len, seq, j;      // first row (packed) or seq * T, steps of the sequence, sequence, block
   bool ok;
 };
-static __host__ __device__ inline int64_t seq_blocks(const SeqGeo& g, int64_t L) {
-  return g.off ? g.rows / L + g.n_seq : (int64_t)g.n_seq * ((g.T + L - 1) / L);
+static __host__ __device__ inline int64_t seq_blocks(const SeqGeo& g, int lg) {
+  return g.off ? (g.rows >> lg) + g.n_seq : (int64_t)g.n_seq * ((g.T + ((int64_t)1 << lg) - 1) >> lg);
 }
 static __device__ __forceinline__ int64_t seq_off(const SeqGeo& g, int64_t i) {
   int64_t v = g.off[i];
   v = v < 0 ? 0 : v;
   return v > g.rows ? g.rows : v;
 }
-static __device__ __forceinline__ SeqBlock seq_find(const SeqGeo& g, int64_t slot, int64_t L) {
+static __device__ __forceinline__ SeqBlock seq_find(const SeqGeo& g, uint32_t slot, int lg) {       // slot < 2^32, host-checked
   SeqBlock b;
   if (!g.off) {
-    const int64_t per = (g.T + L - 1) / L;
-    b.seq = per > 0 ? slot / per : 0;
-    b.j = slot - b.seq * per;
+    const uint32_t per = (uint32_t)((g.T + ((int64_t)1 << lg) - 1) >> lg), q = slot / per;
+    b.seq = q;
+    b.j = slot - q * per;
     b.start = b.seq * g.T;
     b.len = g.T;
     b.ok = b.seq < g.n_seq;
     return b;
   }
-  int64_t lo = 0, hi = g.n_seq - 1;                     // the last i with off[i] / L + i <= slot
+  int lo = 0, hi = g.n_seq - 1;                         // the last i with floor(off[i] / L) + i <= slot
   while (lo < hi) {
-    const int64_t mid = (lo + hi + 1) >> 1;
-    if (seq_off(g, mid) / L + mid <= slot) lo = mid; else hi = mid - 1;
+    const int mid = (int)(((unsigned)lo + (unsigned)hi + 1) >> 1);
+    if ((seq_off(g, mid) >> lg) + mid <= (int64_t)slot) lo = mid; else hi = mid - 1;
   }
   b.seq = lo;
   b.start = seq_off(g, lo);
   const int64_t end = seq_off(g, lo + 1);
   b.len = end > b.start ? end - b.start : 0;
-  b.j = slot - (b.start / L + lo);
-  b.ok = b.j >= 0 && b.j * L < b.len;
+  b.j = (int64_t)slot - ((b.start >> lg) + lo);
+  b.ok = b.j >= 0 && (b.j << lg) < b.len;
   return b;
 }
-static __device__ __forceinline__ int64_t seq_slot0(const SeqGeo& g, int64_t seq, int64_t start, int64_t L) {
-  return g.off ? start / L + seq : seq * ((g.T + L - 1) / L);
+static __device__ __forceinline__ int64_t seq_slot0(const SeqGeo& g, int64_t seq, int64_t start, int lg) {
+  return g.off ? (start >> lg) + seq : seq * ((g.T + ((int64_t)1 << lg) - 1) >> lg);
 }
 struct SeqStride { int64_t st, sb; };
 template <typename T>
@@ -208,8 +202,15 @@ static __device__ __forceinline__ int64_t seq_row_index(const SeqGeo& g, const S
   return g.off ? b.start + r : r * g.n_seq + b.seq;
 }
 
-// out[i] = sum over p of part[p * stride + i], i < n, added in a fixed order (no atomics: results do not depend on timing)
-rgp_status seq_reduce(rgp_handle h, hipStream_t s, int dtype_acc, int dtype_out, const void* part, int64_t P, int64_t stride, int64_t n, void* out);
+// out[i] = sum over p < P of part[p * stride + i], i < n, rounded to type dt; up to five such sums in one launch, each in a fixed order (no
+// atomics: results do not depend on timing).  turn > 1: the partials are [turn][n / turn], out is [n / turn][turn].
+struct SeqSum { const void* part; int64_t P, stride, n; void* out; int dt, turn, block0; };
+struct SeqSums {
+  SeqSum job[5];
+  int count = 0, blocks = 0;
+  void add(const void* part, int64_t P, int64_t stride, int64_t n, void* out, int dt, int turn = 1);
+  rgp_status run(rgp_handle h, hipStream_t s, int acc);
+};
 
 // the current device is the handle's for the length of a call
 struct SeqDevice {
@@ -237,7 +238,7 @@ static inline rgp_status seq_launched(rgp_handle h, const char* what) {
   return e == hipSuccess ? RGP_OK : rgp_fail(h, RGP_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
 }
 static inline int seq_dtype_bytes(int dt) { return dt == RGP_F64 ? 8 : dt == RGP_F32 ? 4 : 2; }
-static inline bool seq_aligned(const void* p, int64_t st, int64_t sb, int elem) {
-  const int v = 16 / elem;
-  return ((uintptr_t)p & 15) == 0 && st % v == 0 && sb % v == 0;
+static inline bool seq_aligned(const void* p, int64_t st, int64_t sb, int elem, int v = 0) {        // for vectors of v elements (0: 16 bytes)
+  if (!v) v = 16 / elem;
+  return (uintptr_t)p % (v * elem) == 0 && st % v == 0 && sb % v == 0;
 }

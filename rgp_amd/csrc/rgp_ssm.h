@@ -5,19 +5,26 @@
 
 #define SSM_R 4                      // states per lane
 
-// Steps between the states that a training forward pass leaves for the backward pass, and the steps the backward kernel holds in
-// registers.  Their bytes per (row, channel) are N * sizeof(acc) / CK: 4 at N = 16 for 32-bit states, against 6 to 14 that the activations
-// cost; 8 steps for 64-bit ones, whose registers are twice as wide.
-template <typename A> struct SsmCk { static constexpr int n = 16; };
-template <> struct SsmCk<double> { static constexpr int n = 8; };
+// Steps between the states that a training forward pass leaves for the backward pass, and the steps whose states and decays the backward
+// kernel holds in registers.  At N = 16 their bytes per (row, channel) are 8 in 32 bits; 16 steps would halve that but need 64 registers
+// more, and the kernel is bound by the latency of one wave per SIMD then.
+#define SSM_CK_LG 3
+#define SSM_CK (1 << SSM_CK_LG)
+// A step behind the end of a block has dt = u = gp = 0 and changes nothing: its decay is exp(0 A) = 1.  For that A must be finite:
+// minus infinity (forget everything) is held as the lowest finite value, whose product with any dt of a real step still decays to 0.
+template <typename A> static __device__ __forceinline__ A ssm_finite(A a) {
+  const A low = sizeof(A) == 4 ? (A)-3.0e38f : (A)-1.0e308;
+  return a < low ? low : a;
+}
 
 struct SsmDev {
   rgp_ssm_scan a;
   SeqGeo g;
-  int64_t L;                         // steps per block of the time split
+  int lg;                            // the time split has blocks of L = 2^lg steps
+  int64_t L;
   int64_t nslot;                     // blocks
   int Dg, ncb;                       // channels per group, channel blocks per group
-  int wu, wd, wz, wgy, wout;         // 16-byte accesses possible: u, delta, z, gy, outputs
+  int wide;                          // every activation in 16-byte vectors: aligned, and Dg a multiple of a vector
   void* part;                        // state (forward) or adjoint (backward) that every block starts from [nslot][D][N]
   void* sumdt;                       // sum of dt over a block [nslot][D]
   void *pA, *pD, *pBC;               // partial sums of the backward pass: [nslot][D][N], [nslot][2][D], [ncb][rows][2][G][N]

@@ -3,82 +3,123 @@
 #include "rgp_ssm.h"
 
 // ---- sums of partial results in a fixed order -----------------------------------------------------------------------------------------
-// 64 outputs a workgroup, 4 threads for each: thread q adds partials q, q + 4, ..., four at a time into separate sums so that the loads
-// overlap; the order depends on P alone.
-template <typename A, typename O>
-static __global__ void __launch_bounds__(256) seq_reduce_kernel(const A* part, int64_t P, int64_t stride, int64_t n, O* out) {
-  __shared__ A sh[4][64];
-  const int64_t i = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-  const int q = threadIdx.x >> 6;
-  A s0 = (A)0, s1 = (A)0, s2 = (A)0, s3 = (A)0;
-  if (i < n) {
-    int64_t p = q;
-    for (; p + 12 < P; p += 16) {
-      s0 += part[p * stride + i];
-      s1 += part[(p + 4) * stride + i];
-      s2 += part[(p + 8) * stride + i];
-      s3 += part[(p + 12) * stride + i];
+// A workgroup forms 64 outputs of one of up to five sums, 16 threads for each: thread q adds partials q, q + 16, ... in eight interleaved
+// sums (that many loads are in flight), then the 16 are added in LDS.  The order depends on the count of partials alone.
+template <typename A>
+static __global__ void __launch_bounds__(1024) seq_sums_kernel(SeqSums g) {
+  __shared__ A sh[16][64];
+  int k = 0;
+  while (k + 1 < g.count && (int)blockIdx.x >= g.job[k + 1].block0) ++k;
+  const SeqSum& j = g.job[k];
+  const int l = threadIdx.x & 63, q = threadIdx.x >> 6;
+  const int64_t i = (int64_t)((int)blockIdx.x - j.block0) * 64 + l;
+  const A* const part = (const A*)j.part;
+  A v8[8] = {};
+  if (i < j.n) {
+    const A* p = part + q * j.stride + i;
+    int64_t left = j.P > q ? (j.P - q + 15) / 16 : 0;
+    for (; left >= 8; left -= 8, p += 128 * j.stride) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v8[u] += p[u * 16 * j.stride];
     }
-    for (; p < P; p += 4) s0 += part[p * stride + i];
+#pragma unroll
+    for (int u = 0; u < 7; ++u)
+      if (u < left) v8[u] += p[u * 16 * j.stride];
   }
-  sh[q][threadIdx.x & 63] = (s0 + s1) + (s2 + s3);
+  sh[q][l] = ((v8[0] + v8[1]) + (v8[2] + v8[3])) + ((v8[4] + v8[5]) + (v8[6] + v8[7]));
   __syncthreads();
-  if (q == 0 && i < n) {
-    const int l = threadIdx.x;
-    out[i] = (O)((sh[0][l] + sh[1][l]) + (sh[2][l] + sh[3][l]));
+  if (q == 0 && i < j.n) {
+    A v = sh[0][l];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) v += sh[r][l];
+    const int64_t o = j.turn > 1 ? (i % (j.n / j.turn)) * j.turn + i / (j.n / j.turn) : i;
+    switch (j.dt) {
+      case RGP_F64: ((double*)j.out)[o] = (double)v; break;
+      case RGP_F32: ((float*)j.out)[o] = (float)v; break;
+      case RGP_BF16: ((__bf16*)j.out)[o] = (__bf16)(float)v; break;
+      default: ((_Float16*)j.out)[o] = (_Float16)(float)v; break;
+    }
   }
 }
-template <typename A, typename O>
-static rgp_status reduce_go(rgp_handle h, hipStream_t s, const void* part, int64_t P, int64_t stride, int64_t n, void* out) {
-  if (n < 1) return RGP_OK;
-  hipLaunchKernelGGL((seq_reduce_kernel<A, O>), dim3((unsigned)((n + 63) / 64)), dim3(256), 0, s, (const A*)part, P, stride, n, (O*)out);
-  return seq_launched(h, "sum of partial results");
+void SeqSums::add(const void* part, int64_t P, int64_t stride, int64_t n, void* out, int dt, int turn) {
+  if (!out || n < 1) return;
+  SeqSum& j = job[count++];
+  j.part = part; j.P = P; j.stride = stride; j.n = n; j.out = out; j.dt = dt; j.turn = turn; j.block0 = blocks;
+  blocks += (int)((n + 63) / 64);
 }
-rgp_status seq_reduce(rgp_handle h, hipStream_t s, int acc, int dt, const void* part, int64_t P, int64_t stride, int64_t n, void* out) {
-  if (acc == RGP_F64) return reduce_go<double, double>(h, s, part, P, stride, n, out);
-  if (dt == RGP_F32) return reduce_go<float, float>(h, s, part, P, stride, n, out);
-  if (dt == RGP_BF16) return reduce_go<float, __bf16>(h, s, part, P, stride, n, out);
-  return reduce_go<float, _Float16>(h, s, part, P, stride, n, out);
+rgp_status SeqSums::run(rgp_handle h, hipStream_t s, int acc) {
+  if (!count) return RGP_OK;
+  if (acc == RGP_F64) hipLaunchKernelGGL(seq_sums_kernel<double>, dim3(blocks), dim3(1024), 0, s, *this);
+  else hipLaunchKernelGGL(seq_sums_kernel<float>, dim3(blocks), dim3(1024), 0, s, *this);
+  return seq_launched(h, "sum of partial results");
 }
 
 // ---- joining the blocks of the time split -----------------------------------------------------------------------------------------------
-// part[block] holds what a block adds to the state that enters it; a thread walks one (sequence, channel, state) over the blocks and
-// leaves the entering state there.  A whole block multiplies it by exp(A sum dt): the decays of a diagonal recurrence commute.
-// back: the same for the adjoint, from the last block to the first.
-template <typename A>
-static __global__ void __launch_bounds__(256) ssm_join_kernel(SsmDev d, int back) {
+// part[block] holds what a block adds to the state that enters it, and is left holding that entering state.  A whole block multiplies the
+// state by exp(A sum dt): the decays of a diagonal recurrence commute.  back: the same for the adjoint, from the last block to the first.
+// 64 lanes take neighbouring (channel, state) pairs of one sequence, Q threads a pair: each walks its part of the blocks twice, first for
+// what that stretch does as a whole, then with the state that enters it (Q = 1: once).  The walk waits for memory, JOIN_U blocks at a time;
+// with Q = 16 for 1024 blocks of 8 sequences it takes 21 us where one thread a pair took 479, but 98 instead of 15 for many short sequences.
+#define JOIN_U 8
+template <typename A, int Q>
+static __global__ void __launch_bounds__(Q == 1 ? 256 : Q * 64) ssm_join_kernel(SsmDev d, int back) {
+  __shared__ A shP[Q][64], shH[Q][64];
   const rgp_ssm_scan& a = d.a;
-  const int64_t DN = (int64_t)a.D * a.N, idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t seq = idx / DN, dn = idx - seq * DN, ch = dn / a.N;
-  if (seq >= a.n_seq) return;
+  const int l = threadIdx.x & 63, q = Q == 1 ? 0 : threadIdx.x >> 6, wide = Q == 1 ? 256 : 64;
+  const int64_t DN = (int64_t)a.D * a.N, per = (DN + wide - 1) / wide, seq = blockIdx.x / per;
+  const int64_t dn = (blockIdx.x - seq * per) * wide + (Q == 1 ? threadIdx.x : l);
+  const bool ok = dn < DN;
   int64_t start = seq * d.g.T, len = d.g.T;
   if (d.g.off) {
     start = seq_off(d.g, seq);
     const int64_t end = seq_off(d.g, seq + 1);
     len = end > start ? end - start : 0;
   }
-  const int64_t nb = (len + d.L - 1) / d.L, slot0 = seq_slot0(d.g, seq, start, d.L);
-  const A Av = ((const A*)a.A)[dn];
-  A* const part = (A*)d.part + slot0 * DN + dn;
+  const int64_t nb = (len + d.L - 1) >> d.lg, slot0 = seq_slot0(d.g, seq, start, d.lg);
+  const int64_t each = (nb + Q - 1) / Q, j0 = q * each < nb ? q * each : nb, j1 = !ok ? j0 : (j0 + each < nb ? j0 + each : nb);
+  const int64_t at0 = ok ? dn : 0, ch = at0 / a.N;
+  const A Av = ssm_finite(((const A*)a.A)[at0]);
+  A* const part = (A*)d.part + slot0 * DN + at0;
   const A* const sum = (const A*)d.sumdt + slot0 * a.D + ch;
-  A s = !back && a.init ? ((const A*)a.init)[seq * DN + dn] : (A)0;
-  constexpr int U = 8;
-  for (int64_t j = 0; j < nb; j += U) {
-    A p[U], q[U];
+  A P = (A)1, H = (A)0, s = (A)0;
+  if (Q == 1) s = !back && a.init && ok ? ((const A*)a.init)[seq * DN + dn] : (A)0;
+  for (int pass = Q == 1 ? 1 : 0; pass < 2; ++pass) {
+    for (int64_t j = j0; j < j1; j += JOIN_U) {
+      A p[JOIN_U], e[JOIN_U];
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int64_t jj = j + i < nb ? j + i : nb - 1, at = back ? nb - 1 - jj : jj;
-      p[i] = part[at * DN];
-      q[i] = seq_exp(Av * sum[at * a.D]);
-    }
+      for (int i = 0; i < JOIN_U; ++i) {                  // the block that nothing follows has left no sums: what is read there goes unused
+        const int64_t jj = j + i < j1 ? j + i : j, at = back ? nb - 1 - jj : jj;
+        p[i] = part[at * DN];
+        e[i] = seq_exp(Av * sum[at * a.D]);
+      }
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      if (j + i < nb) {
-        part[(back ? nb - 1 - (j + i) : j + i) * DN] = s;
-        s = q[i] * s + p[i];
+      for (int i = 0; i < JOIN_U; ++i) {
+        if (j + i < j1) {
+          if (pass == 0) {
+            P *= e[i];
+            H = e[i] * H + p[i];
+          } else {
+            part[(back ? nb - 1 - (j + i) : j + i) * DN] = s;
+            s = e[i] * s + p[i];
+          }
+        }
       }
     }
+    if (pass == 0) {
+      shP[q][l] = P;
+      shH[q][l] = H;
+      __syncthreads();                                    // also: every block's sums are read before the states replace them
+      s = !back && a.init && ok ? ((const A*)a.init)[seq * DN + dn] : (A)0;
+      for (int r = 0; r < q; ++r) s = shP[r][l] * s + shH[r][l];
+    }
   }
+}
+
+template <typename A>
+static void join_launch(const SsmDev& d, int Q, unsigned grid, int back, hipStream_t s) {
+  if (Q == 1) hipLaunchKernelGGL((ssm_join_kernel<A, 1>), dim3(grid), dim3(256), 0, s, d, back);
+  else if (Q == 4) hipLaunchKernelGGL((ssm_join_kernel<A, 4>), dim3(grid), dim3(256), 0, s, d, back);
+  else hipLaunchKernelGGL((ssm_join_kernel<A, 16>), dim3(grid), dim3(1024), 0, s, d, back);
 }
 
 // ---- host side of the scan --------------------------------------------------------------------------------------------------------------
@@ -94,7 +135,7 @@ static const char* scan_bad(const rgp_ssm_scan* a) {
 
 struct ScanPlan {
   SsmDev d;
-  int K, CH, acc;
+  int K, CH, acc, Q;               // Q: threads that walk the blocks of one state in the join
   bool split;
   int64_t part_bytes, sum_bytes, pA_bytes, pD_bytes, pBC_bytes, bytes;
 };
@@ -112,23 +153,28 @@ static void scan_plan(const rgp_ssm_scan* a, bool back, ScanPlan& p) {
   if (p.K == 4 && (d.Dg + 15) / 16 * 16 < (d.Dg + 63) / 64 * 64) p.CH = 16;
   d.ncb = (d.Dg + p.CH - 1) / p.CH;
   const int64_t longest = a->off ? (a->max_len > 0 && a->max_len < a->rows ? a->max_len : a->rows) : a->T;
-  // Split over time where whole sequences would leave most of the card's 1024 SIMDs without a wave: a split walks every step twice.
-  const int64_t waves = (int64_t)a->n_seq * a->G * d.ncb * (p.CH * p.K / 64);
-  const double mean = (double)a->rows / a->n_seq;
-  int64_t L = 0;
-  const double want = 2048.0;
-  if (longest >= 256) {
-    const double one = (double)longest + (double)waves * mean / 2048.0;           // steps of the longest sequence, and of the whole work
-    int64_t l = (int64_t)(waves * mean / want);
-    l = (l + 63) / 64 * 64;
-    if (l < 64) l = 64;
-    const double two = 1.8 * ((double)l + (double)waves * mean / 2048.0) + 100.0;
-    if (two < one) L = l;
-  }
-  p.split = L > 0;
-  d.L = p.split ? L : (a->off ? (a->rows + 63) / 64 * 64 : (a->T + 63) / 64 * 64);
-  if (d.L < 64) d.L = 64;
-  d.nslot = seq_blocks(d.g, d.L);
+  // Split over time.  In units of the time in which a SIMD with several waves walks one wave's step: unsplit, the whole work spread over
+  // 1024 SIMDs, but no less than the longest sequence at twice that time (a lone wave waits for its own results); split, about 1.65 times
+  // the work (the state's part of it is done twice), the two walks over one block, and the join.  Blocks of 64 steps, of 32 where that
+  // leaves most SIMDs idle, longer ones where the waves get many: shorter blocks balance ragged lengths, longer ones leave the join (and
+  // the sums of the backward pass) less to read.
+  const double waves = (double)a->G * d.ncb * (p.CH * p.K / 64.0), work = waves * a->rows / 1024.0, most = back ? 12288.0 : 24576.0;
+  auto count = [&](int g) { return waves * ((double)(a->rows >> g) + a->n_seq); };
+  int lg = count(6) < 1024.0 ? 5 : 6;
+  while (lg < 20 && count(lg) > most) ++lg;
+  const double one = work > 2.0 * longest ? work : 2.0 * longest, two = 1.65 * (work + 2.0 * ((int64_t)1 << lg)) + 130.0;
+  if (!(two < one)) lg = 0;
+#ifdef SSM_TUNE
+  if (getenv("SSM_LG")) lg = atoi(getenv("SSM_LG"));
+#endif
+  p.split = lg > 0;
+  if (!p.split)
+    for (lg = 6; ((int64_t)1 << lg) < (a->off ? a->rows : a->T); ++lg) {}
+  d.lg = lg;
+  d.L = (int64_t)1 << lg;
+  const int64_t deep = (longest + d.L - 1) >> d.lg;
+  p.Q = deep <= 8 ? 1 : deep <= 128 ? 4 : 16;
+  d.nslot = seq_blocks(d.g, d.lg);
   const int64_t DN = (int64_t)a->D * a->N;
   p.part_bytes = p.split ? up256(d.nslot * DN * p.acc) : 0;
   p.sum_bytes = p.split ? up256(d.nslot * a->D * p.acc) : 0;
@@ -147,8 +193,7 @@ extern "C" int64_t rgp_ssm_scan_workspace(const rgp_ssm_scan* a, int backward) {
 extern "C" int64_t rgp_ssm_scan_states_bytes(const rgp_ssm_scan* a) {
   if (scan_bad(a)) return -1;
   const SeqGeo g{a->off, a->T, a->rows, a->n_seq, a->reverse};
-  const int ck = a->dtype == RGP_F64 ? SsmCk<double>::n : SsmCk<float>::n;
-  return seq_blocks(g, ck) * a->D * a->N * (a->dtype == RGP_F64 ? 8 : 4);
+  return seq_blocks(g, SSM_CK_LG) * a->D * a->N * (a->dtype == RGP_F64 ? 8 : 4);
 }
 
 static rgp_status scan_run(rgp_handle h, hipStream_t s, const rgp_ssm_scan* a, bool back) {
@@ -165,13 +210,10 @@ static rgp_status scan_run(rgp_handle h, hipStream_t s, const rgp_ssm_scan* a, b
   if (p.bytes > a->work_bytes || (p.bytes && !a->work) || ((uintptr_t)a->work & 15))
     return rgp_fail(h, RGP_ERR_WORKSPACE, std::string(what) + "work buffer too small or not 16-byte aligned");
   const int e = seq_dtype_bytes(a->dtype), V = 16 / e;
-  const bool groups = a->G == 1 || d.Dg % V == 0;
-  d.wu = groups && seq_aligned(a->u, a->u_st, a->u_sb, e);
-  d.wd = groups && seq_aligned(a->delta, a->delta_st, a->delta_sb, e);
-  d.wz = groups && a->z && seq_aligned(a->z, a->z_st, a->z_sb, e);
-  d.wgy = groups && back && seq_aligned(a->gy, a->gy_st, a->gy_sb, e);
-  d.wout = groups && a->D % V == 0 && (back ? seq_aligned(a->gu, 0, 0, e) && seq_aligned(a->gdelta, 0, 0, e) && (!a->z || seq_aligned(a->gz, 0, 0, e))
-                                             : seq_aligned(a->y, 0, 0, e));
+  d.wide = d.Dg % V == 0 && seq_aligned(a->u, a->u_st, a->u_sb, e) && seq_aligned(a->delta, a->delta_st, a->delta_sb, e) &&
+           (!a->z || seq_aligned(a->z, a->z_st, a->z_sb, e));
+  if (back) d.wide = d.wide && seq_aligned(a->gy, a->gy_st, a->gy_sb, e) && seq_aligned(a->gu, 0, 0, e) && seq_aligned(a->gdelta, 0, 0, e) && (!a->z || seq_aligned(a->gz, 0, 0, e));
+  else d.wide = d.wide && seq_aligned(a->y, 0, 0, e);
   char* w = (char*)a->work;
   auto take = [&](int64_t bytes) { void* r = bytes ? (void*)w : nullptr; w += bytes; return r; };
   d.part = take(p.part_bytes);
@@ -179,17 +221,17 @@ static rgp_status scan_run(rgp_handle h, hipStream_t s, const rgp_ssm_scan* a, b
   d.pA = take(p.pA_bytes);
   d.pD = take(p.pD_bytes);
   d.pBC = take(p.pBC_bytes);
-  if ((double)d.nslot * a->G * d.ncb * p.CH * p.K > 4294967295.0 || (double)a->n_seq * a->D * a->N > 1.0e12)
-    return rgp_fail(h, RGP_ERR_BAD_ARG, std::string(what) + "more than 2^32 work items");
   const int64_t DN = (int64_t)a->D * a->N;
-  const unsigned join = (unsigned)((a->n_seq * DN + 255) / 256);
+  const int64_t join = (int64_t)a->n_seq * (p.Q == 1 ? (DN + 255) / 256 : (DN + 63) / 64);
+  if ((double)d.nslot * p.CH * p.K > 4294967295.0 || (int64_t)a->G * d.ncb > 65535 || seq_blocks(d.g, SSM_CK_LG) > 4294967295 || (double)join * 1024 > 4294967295.0)
+    return rgp_fail(h, RGP_ERR_BAD_ARG, std::string(what) + "more than 2^32 work items");
   hipError_t err = hipSuccess;
   if (d.nslot > 0) {
     if (p.split) {
       err = back ? ssm_bwd_launch(d, p.K, p.CH, 1, s) : ssm_fwd_launch(d, p.K, p.CH, 1, s);
       if (err == hipSuccess) {
-        if (p.acc == 8) hipLaunchKernelGGL(ssm_join_kernel<double>, dim3(join), dim3(256), 0, s, d, back ? 1 : 0);
-        else hipLaunchKernelGGL(ssm_join_kernel<float>, dim3(join), dim3(256), 0, s, d, back ? 1 : 0);
+        if (p.acc == 8) join_launch<double>(d, p.Q, (unsigned)join, back ? 1 : 0, s);
+        else join_launch<float>(d, p.Q, (unsigned)join, back ? 1 : 0, s);
         err = hipGetLastError();
       }
     }
@@ -198,15 +240,16 @@ static rgp_status scan_run(rgp_handle h, hipStream_t s, const rgp_ssm_scan* a, b
   }
   if (!back) return RGP_OK;
   const int acc = a->dtype == RGP_F64 ? RGP_F64 : RGP_F32;
-  rgp_status st = seq_reduce(h, s, acc, acc, d.pA, d.nslot, DN, DN, a->gA);
-  if (!st && a->gskip) st = seq_reduce(h, s, acc, acc, d.pD, d.nslot, 2 * (int64_t)a->D, a->D, a->gskip);
-  if (!st && a->gbias) st = seq_reduce(h, s, acc, acc, (char*)d.pD + (int64_t)a->D * p.acc, d.nslot, 2 * (int64_t)a->D, a->D, a->gbias);
-  if (!st && d.ncb > 1) {
+  SeqSums sums;
+  sums.add(d.pA, d.nslot, DN, DN, a->gA, acc);
+  sums.add(d.pD, d.nslot, 2 * (int64_t)a->D, a->D, a->gskip, acc);
+  sums.add((char*)d.pD + (int64_t)a->D * p.acc, d.nslot, 2 * (int64_t)a->D, a->D, a->gbias, acc);
+  if (d.ncb > 1) {
     const int64_t n = a->rows * a->G * a->N;
-    st = seq_reduce(h, s, acc, a->dtype, d.pBC, d.ncb, 2 * n, n, a->gB);
-    if (!st) st = seq_reduce(h, s, acc, a->dtype, (char*)d.pBC + n * p.acc, d.ncb, 2 * n, n, a->gC);
+    sums.add(d.pBC, d.ncb, 2 * n, n, a->gB, a->dtype);
+    sums.add((char*)d.pBC + n * p.acc, d.ncb, 2 * n, n, a->gC, a->dtype);
   }
-  return st;
+  return sums.run(h, s, acc);
 }
 extern "C" rgp_status rgp_ssm_scan_forward(rgp_handle h, void* stream, const rgp_ssm_scan* a) {
   SEQ_ENTRY(h, "ssm scan", { return scan_run(h, (hipStream_t)stream, a, false); })
@@ -218,13 +261,13 @@ extern "C" rgp_status rgp_ssm_scan_backward(rgp_handle h, void* stream, const rg
 // ---- one step -----------------------------------------------------------------------------------------------------------------------------
 // Bound by reading and writing the state: K lanes a channel, 16 bytes of state a lane (32 in fp64), as in the kernels over time.
 template <typename T, int K>
-static __global__ void __launch_bounds__(256) ssm_step_kernel(rgp_ssm_scan a, int Dg) {
+static __global__ void __launch_bounds__(256) ssm_step_kernel(rgp_ssm_scan a, int Dg, int whole) {
   typedef typename SeqAcc<T>::type A;
   constexpr int R = SSM_R;
-  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) / K;
+  const uint32_t e = (blockIdx.x * 256u + threadIdx.x) / K;              // host-checked: below 2^32
   const int k = threadIdx.x % K, N = a.N;
-  const bool live = e < (int64_t)a.n_seq * a.D;
-  const int64_t row = live ? e / a.D : 0;
+  const bool live = e < (uint32_t)a.n_seq * (uint32_t)a.D;
+  const int64_t row = live ? e / (uint32_t)a.D : 0;
   const int ch = live ? (int)(e - row * a.D) : 0, grp = ch / Dg;
   A sig;
   const A u = (A)((const T*)a.u)[row * a.u_sb + ch];
@@ -236,27 +279,44 @@ static __global__ void __launch_bounds__(256) ssm_step_kernel(rgp_ssm_scan a, in
     const A* const Ar = (const A*)a.A + (int64_t)ch * N + k * R;
     const T* const B = (const T*)a.B + row * a.B_sb + (int64_t)grp * N + k * R;
     const T* const C = (const T*)a.C + row * a.C_sb + (int64_t)grp * N + k * R;
-    A s[R];
+    struct alignas(16) Quad { A v[R]; };
+    Quad s, Aq, Bq, Cq;
+    if (whole) {
+      s = *(const Quad*)st;
+      Aq = *(const Quad*)Ar;
 #pragma unroll
-    for (int r = 0; r < R; ++r) s[r] = k * R + r < N ? st[r] : (A)0;
+      for (int r = 0; r < R; ++r) {
+        Bq.v[r] = (A)B[r];
+        Cq.v[r] = (A)C[r];
+      }
+    } else {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (k * R + r < N) {
-        s[r] = seq_exp(dt * Ar[r]) * s[r] + w * (A)B[r];
-        acc += s[r] * (A)C[r];
+      for (int r = 0; r < R; ++r) {
+        const bool in = k * R + r < N;
+        s.v[r] = in ? st[r] : (A)0;
+        Aq.v[r] = in ? Ar[r] : (A)0;
+        Bq.v[r] = in ? (A)B[r] : (A)0;
+        Cq.v[r] = in ? (A)C[r] : (A)0;
       }
     }
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (k * R + r < N) st[r] = s[r];
+    for (int r = 0; r < R; ++r) {
+      s.v[r] = seq_exp(dt * Aq.v[r]) * s.v[r] + w * Bq.v[r];
+      acc += s.v[r] * Cq.v[r];
+    }
+    if (whole) *(Quad*)st = s;
+    else {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (k * R + r < N) st[r] = s.v[r];
+    }
   }
   acc = seq_sum<K>(acc);
   if (live && k == 0) {
     A y = acc + (a.skip ? ((const A*)a.skip)[ch] : (A)0) * u;
     if (a.z) {
-      A comp;
       const A z = (A)((const T*)a.z)[row * a.z_sb + ch];
-      y *= z * seq_sigmoid(z, comp);
+      y *= z * seq_sigmoid(z);
     }
     ((T*)a.y)[row * a.D + ch] = (T)y;
   }
@@ -266,12 +326,13 @@ static hipError_t step_pick(const rgp_ssm_scan& a, hipStream_t s) {
   const int K = a.N <= 4 ? 1 : a.N <= 8 ? 2 : a.N <= 16 ? 4 : a.N <= 32 ? 8 : 16;
   const unsigned grid = (unsigned)(((int64_t)a.n_seq * a.D * K + 255) / 256);
   const int Dg = a.D / a.G;
+  const int whole = a.N == SSM_R * K && ((uintptr_t)a.last & 15) == 0 && ((uintptr_t)a.A & 15) == 0;
   switch (K) {
-    case 1: hipLaunchKernelGGL((ssm_step_kernel<T, 1>), dim3(grid), dim3(256), 0, s, a, Dg); break;
-    case 2: hipLaunchKernelGGL((ssm_step_kernel<T, 2>), dim3(grid), dim3(256), 0, s, a, Dg); break;
-    case 4: hipLaunchKernelGGL((ssm_step_kernel<T, 4>), dim3(grid), dim3(256), 0, s, a, Dg); break;
-    case 8: hipLaunchKernelGGL((ssm_step_kernel<T, 8>), dim3(grid), dim3(256), 0, s, a, Dg); break;
-    default: hipLaunchKernelGGL((ssm_step_kernel<T, 16>), dim3(grid), dim3(256), 0, s, a, Dg); break;
+    case 1: hipLaunchKernelGGL((ssm_step_kernel<T, 1>), dim3(grid), dim3(256), 0, s, a, Dg, whole); break;
+    case 2: hipLaunchKernelGGL((ssm_step_kernel<T, 2>), dim3(grid), dim3(256), 0, s, a, Dg, whole); break;
+    case 4: hipLaunchKernelGGL((ssm_step_kernel<T, 4>), dim3(grid), dim3(256), 0, s, a, Dg, whole); break;
+    case 8: hipLaunchKernelGGL((ssm_step_kernel<T, 8>), dim3(grid), dim3(256), 0, s, a, Dg, whole); break;
+    default: hipLaunchKernelGGL((ssm_step_kernel<T, 16>), dim3(grid), dim3(256), 0, s, a, Dg, whole); break;
   }
   return hipGetLastError();
 }
@@ -291,73 +352,79 @@ extern "C" rgp_status rgp_ssm_scan_step(rgp_handle h, void* stream, const rgp_ss
 }
 
 // ---- short causal convolution ---------------------------------------------------------------------------------------------------------------
-// v_t = silu(bias + sum_j w_j x_{t-W+1+j}) reads x once and writes v once: bound by memory.  A thread holds V channels (16 bytes) and walks a
+// v_t = silu(bias + sum_j w_j x_{t-W+1+j}) reads x once and writes v once: bound by memory.  A thread holds V = 4 channels (2 in fp64) and walks a
 // run of CONV_RUN steps with the last W - 1 inputs in registers; the W - 1 rows before a run are read again (from cache).
-#define CONV_RUN 16
-#define CONV_FLY 8
+#define CONV_FLY 4
+#define CONV_V(bytes) ((bytes) == 8 ? 2 : 4)
 struct ConvDev {
   rgp_ssm_conv a;
   SeqGeo g;
   int64_t nrun, nvec;
-  int wx, wgv, wout, lanes;        // 16-byte accesses; vectors side by side in a workgroup (backward)
+  int lg;                          // a run has 2^lg steps
+  int wide, same, lanes;           // vector accesses; a wave's lanes are in one run; vectors side by side in a workgroup (backward)
   void* part;
 };
 
-// x at step t of the sequence, in walking order; before the first step the state, behind the last one zero
-template <typename T, int W>
-static __device__ __forceinline__ SeqVec<T> conv_x(const ConvDev& d, const SeqBlock& b, int64_t t, int64_t c, int n) {
+// x at step t of the sequence, in walking order; before the first step the state
+template <typename T, int W, int V>
+static __device__ __forceinline__ SeqVec<T, V> conv_x(const ConvDev& d, const SeqBlock& b, int64_t t, int64_t c) {
   const rgp_ssm_conv& a = d.a;
-  if (t < 0) {
-    SeqVec<T> z = seq_load((const T*)a.x, 0, false);
-    if (!a.init) return z;
-    return seq_load((const T*)a.init + ((b.seq * (W - 1) + W - 1 + t) * a.D + c), n, false);
-  }
-  return seq_load(seq_row((const T*)a.x, d.g, b, SeqStride{a.x_st, a.x_sb}, t) + c, n, d.wx);
+  if (t >= 0) return *(const SeqVec<T, V>*)(seq_row((const T*)a.x, d.g, b, SeqStride{a.x_st, a.x_sb}, t) + c);
+  SeqVec<T, V> z;
+#pragma unroll
+  for (int i = 0; i < V; ++i) z.e[i] = a.init ? ((const T*)a.init)[(b.seq * (W - 1) + W - 1 + t) * a.D + c + i] : (T)0;
+  return z;
 }
 
-template <typename T, int W>
+template <typename T, int W, int V>
 static __global__ void __launch_bounds__(256) conv_fwd_kernel(ConvDev d) {
   typedef typename SeqAcc<T>::type A;
-  constexpr int V = SeqVec<T>::V;
+  typedef SeqVec<T, V> Vec;
   const rgp_ssm_conv& a = d.a;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x, run = idx / d.nvec, c = (idx - run * d.nvec) * V;
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x, run = idx / (uint32_t)d.nvec;
+  const int64_t c = (int64_t)(idx - run * (uint32_t)d.nvec) * V;
   if (run >= d.nrun) return;
-  const SeqBlock b = seq_find(d.g, run, CONV_RUN);
+  const SeqBlock b = seq_find(d.g, d.same ? (uint32_t)__builtin_amdgcn_readfirstlane(run) : run, d.lg);
   if (!b.ok) return;
-  const int n = a.D - c < V ? (int)(a.D - c) : V;
-  const int64_t t0 = b.j * CONV_RUN;
-  const int nt = b.len - t0 < CONV_RUN ? (int)(b.len - t0) : CONV_RUN;
-  A w[W][V], bias[V];
+  const int64_t t0 = b.j << d.lg;
+  const int L = 1 << d.lg, nt = b.len - t0 < L ? (int)(b.len - t0) : L;
+  A w[W][V], bias[V], x[W][V];                     // x: the window, in the arithmetic type
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    bias[i] = a.bias && i < n ? ((const A*)a.bias)[c + i] : (A)0;
+    bias[i] = a.bias ? ((const A*)a.bias)[c + i] : (A)0;
 #pragma unroll
-    for (int j = 0; j < W; ++j) w[j][i] = i < n ? ((const A*)a.w)[(c + i) * W + j] : (A)0;
+    for (int j = 0; j < W; ++j) w[j][i] = ((const A*)a.w)[(c + i) * W + j];
   }
-  A x[W][V];                                       // the window, in the arithmetic type
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) {
-    const SeqVec<T> r = conv_x<T, W>(d, b, t0 - (W - 1) + j, c, n);
+    const Vec r = conv_x<T, W, V>(d, b, t0 - (W - 1) + j, c);
 #pragma unroll
     for (int i = 0; i < V; ++i) x[j][i] = (A)r.e[i];
   }
+  const T* px = seq_row((const T*)a.x, d.g, b, SeqStride{a.x_st, a.x_sb}, t0) + c;
+  T* pv = (T*)a.v + seq_row_index(d.g, b, t0) * a.D + c;
+  const int64_t sx = d.g.reverse ? -a.x_st : a.x_st, vrow = (d.g.off ? 1 : (int64_t)a.n_seq) * a.D, sv = d.g.reverse ? -vrow : vrow;
   for (int tb = 0; tb < nt; tb += CONV_FLY) {
-    SeqVec<T> r[CONV_FLY];                         // this many rows are in flight at once
+    Vec r[CONV_FLY];                               // this many rows are in flight at once; behind the end the last row again
 #pragma unroll
-    for (int k = 0; k < CONV_FLY; ++k) r[k] = conv_x<T, W>(d, b, t0 + (tb + k < nt ? tb + k : nt - 1), c, n);
+    for (int k = 0; k < CONV_FLY; ++k) {
+      r[k] = *(const Vec*)px;
+      px += tb + k + 1 < nt ? sx : 0;
+    }
 #pragma unroll
     for (int k = 0; k < CONV_FLY; ++k) {
       if (tb + k < nt) {
-        SeqVec<T> o;
+        Vec o;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           x[W - 1][i] = (A)r[k].e[i];
-          A p = bias[i], comp;
+          A p = bias[i];
 #pragma unroll
           for (int j = 0; j < W; ++j) p += w[j][i] * x[j][i];
-          o.e[i] = (T)(p * seq_sigmoid(p, comp));
+          o.e[i] = (T)(p * seq_sigmoid(p));
         }
-        seq_store((T*)a.v + seq_row_index(d.g, b, t0 + tb + k) * a.D + c, o, n, d.wout);
+        *(Vec*)pv = o;
+        pv += sv;
 #pragma unroll
         for (int j = 0; j < W - 1; ++j)
 #pragma unroll
@@ -367,9 +434,8 @@ static __global__ void __launch_bounds__(256) conv_fwd_kernel(ConvDev d) {
   }
 }
 // the W - 1 inputs before the step behind the last one
-template <typename T, int W>
+template <typename T, int W, int V>
 static __global__ void __launch_bounds__(256) conv_last_kernel(ConvDev d) {
-  constexpr int V = SeqVec<T>::V;
   const rgp_ssm_conv& a = d.a;
   const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x, seq = idx / d.nvec, c = (idx - seq * d.nvec) * V;
   if (seq >= a.n_seq) return;
@@ -382,48 +448,46 @@ static __global__ void __launch_bounds__(256) conv_last_kernel(ConvDev d) {
     const int64_t end = seq_off(d.g, seq + 1);
     b.len = end > b.start ? end - b.start : 0;
   }
-  const int n = a.D - c < V ? (int)(a.D - c) : V;
-  SeqVec<T> x[W - 1];                              // all read before any is written: last may be init
 #pragma unroll
-  for (int j = 0; j < W - 1; ++j) x[j] = conv_x<T, W>(d, b, b.len - (W - 1) + j, c, n);
+  for (int j = 0; j < W - 1; ++j) {
+    const SeqVec<T, V> x = conv_x<T, W, V>(d, b, b.len - (W - 1) + j, c);
 #pragma unroll
-  for (int j = 0; j < W - 1; ++j) seq_store((T*)a.last + (seq * (W - 1) + j) * a.D + c, x[j], n, false);
+    for (int i = 0; i < V; ++i) ((T*)a.last)[(seq * (W - 1) + j) * a.D + c + i] = x.e[i];
+  }
 }
 
 // Backward: gp = gv silu'(pre), gx_t = sum_j w_j gp_{t+W-1-j}, gw_j = sum_t gp_t x_{t-W+1+j}, gbias = sum gp.  pre is formed again from x
-// (one more read would cost more than W multiply-adds).  A thread walks its run and W - 1 steps behind it; the parameter sums of the
+// (one more read would cost more than W multiply-adds).  A thread walks its runs and W - 1 steps behind each; the parameter sums of the
 // threads with the same channels go through LDS, then from all workgroups through `part`.
-template <typename T, int W>
+template <typename T, int W, int V>
 static __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvDev d) {
   typedef typename SeqAcc<T>::type A;
-  constexpr int V = SeqVec<T>::V;
+  typedef SeqVec<T, V> Vec;
   __shared__ A sh[256 * V];
   const rgp_ssm_conv& a = d.a;
   const int lane = threadIdx.x % d.lanes, rl = threadIdx.x / d.lanes, nr = 256 / d.lanes;
-  const int64_t nvb = (d.nvec + d.lanes - 1) / d.lanes;                  // workgroups side by side over the channels
-  const int64_t rb = blockIdx.x / nvb, vb = blockIdx.x - rb * nvb, nrb = gridDim.x / nvb;
-  const int64_t vec = vb * d.lanes + lane, c = vec * V;
-  const int n = vec < d.nvec ? (a.D - c < V ? (int)(a.D - c) : V) : 0;
+  const int64_t vec = (int64_t)blockIdx.y * d.lanes + lane, c = vec * V;
+  const bool live = vec < d.nvec;
   A w[W][V], bias[V], gw[W][V], gb[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    bias[i] = a.bias && i < n ? ((const A*)a.bias)[c + i] : (A)0;
+    bias[i] = a.bias && live ? ((const A*)a.bias)[c + i] : (A)0;
     gb[i] = (A)0;
 #pragma unroll
     for (int j = 0; j < W; ++j) {
-      w[j][i] = i < n ? ((const A*)a.w)[(c + i) * W + j] : (A)0;
+      w[j][i] = live ? ((const A*)a.w)[(c + i) * W + j] : (A)0;
       gw[j][i] = (A)0;
     }
   }
-  if (n > 0)
-    for (int64_t run = rb * nr + rl; run < d.nrun; run += nrb * nr) {
-      const SeqBlock b = seq_find(d.g, run, CONV_RUN);
+  if (live)
+    for (int64_t run = (int64_t)blockIdx.x * nr + rl; run < d.nrun; run += (int64_t)gridDim.x * nr) {
+      const SeqBlock b = seq_find(d.g, d.lanes == 64 ? (uint32_t)__builtin_amdgcn_readfirstlane((int)run) : (uint32_t)run, d.lg);
       if (!b.ok) continue;
-      const int64_t t0 = b.j * CONV_RUN, t1 = t0 + CONV_RUN < b.len ? t0 + CONV_RUN : b.len;
+      const int64_t t0 = b.j << d.lg, L = (int64_t)1 << d.lg, t1 = t0 + L < b.len ? t0 + L : b.len;
       A x[W][V], gp[W][V];
 #pragma unroll
       for (int j = 0; j < W; ++j) {
-        const SeqVec<T> r = conv_x<T, W>(d, b, t0 - (W - 1) + (j < W - 1 ? j : 0), c, n);
+        const Vec r = conv_x<T, W, V>(d, b, t0 - (W - 1) + (j < W - 1 ? j : 0), c);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           x[j][i] = (A)r.e[i];
@@ -431,44 +495,50 @@ static __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvDev d) {
         }
       }
       const int nt = (int)(t1 - t0) + W - 1;                             // gp of step t0 + k; gx of step t0 + k - W + 1 is then complete
+      const int in = (int)(t1 - t0), have = b.len - t0 < nt ? (int)(b.len - t0) : nt;
+      const T* px = seq_row((const T*)a.x, d.g, b, SeqStride{a.x_st, a.x_sb}, t0) + c;
+      const T* pg = seq_row((const T*)a.gv, d.g, b, SeqStride{a.gv_st, a.gv_sb}, t0) + c;
+      T* po = (T*)a.gx + seq_row_index(d.g, b, t0) * a.D + c;
+      const int64_t orow = (d.g.off ? 1 : (int64_t)a.n_seq) * a.D;
+      const int64_t sx = d.g.reverse ? -a.x_st : a.x_st, sg = d.g.reverse ? -a.gv_st : a.gv_st, so = d.g.reverse ? -orow : orow;
       for (int kb = 0; kb < nt; kb += CONV_FLY) {
-        SeqVec<T> rx[CONV_FLY], rg[CONV_FLY];
+        Vec rx[CONV_FLY], rg[CONV_FLY];
 #pragma unroll
         for (int k = 0; k < CONV_FLY; ++k) {
-          const int64_t t = t0 + kb + k < b.len ? t0 + kb + k : b.len - 1;
-          rx[k] = conv_x<T, W>(d, b, t, c, n);
-          rg[k] = seq_load(seq_row((const T*)a.gv, d.g, b, SeqStride{a.gv_st, a.gv_sb}, t) + c, n, d.wgv);
+          rx[k] = *(const Vec*)px;                                       // behind the end the last row again
+          rg[k] = *(const Vec*)pg;
+          px += kb + k + 1 < have ? sx : 0;
+          pg += kb + k + 1 < have ? sg : 0;
         }
 #pragma unroll
         for (int k = 0; k < CONV_FLY; ++k) {
           if (kb + k < nt) {
-            const int64_t t = t0 + kb + k;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
               x[W - 1][i] = (A)rx[k].e[i];
-              A p = bias[i], comp;
+              A p = bias[i];
 #pragma unroll
               for (int j = 0; j < W; ++j) p += w[j][i] * x[j][i];
-              const A sg = seq_sigmoid(p, comp);
-              const A q = t < b.len ? (A)rg[k].e[i] * (sg + p * sg * comp) : (A)0;
+              const A sg = seq_sigmoid(p);
+              const A q = kb + k < have ? (A)rg[k].e[i] * (sg + p * sg * ((A)1 - sg)) : (A)0;
               gp[W - 1][i] = q;
-              if (t < t1) {
+              if (kb + k < in) {
                 gb[i] += q;
 #pragma unroll
                 for (int j = 0; j < W; ++j) gw[j][i] += q * x[j][i];
               }
             }
-            const int64_t to = t - (W - 1);
-            if (to >= t0) {
-              SeqVec<T> o;
+            if (kb + k >= W - 1) {
+              Vec o;
 #pragma unroll
               for (int i = 0; i < V; ++i) {
                 A v = (A)0;
 #pragma unroll
-                for (int j = 0; j < W; ++j) v += w[W - 1 - j][i] * gp[j][i];      // gp[j] is step to + j, whose tap W - 1 - j reads x_to
+                for (int j = 0; j < W; ++j) v += w[W - 1 - j][i] * gp[j][i];      // gp[j] is j steps on, and its tap W - 1 - j reads this x
                 o.e[i] = (T)v;
               }
-              seq_store((T*)a.gx + seq_row_index(d.g, b, to) * a.D + c, o, n, d.wout);
+              *(Vec*)po = o;
+              po += so;
             }
 #pragma unroll
             for (int j = 0; j < W - 1; ++j)
@@ -481,7 +551,7 @@ static __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvDev d) {
         }
       }
     }
-  A* const part = (A*)d.part + rb * (W + 1) * a.D;                       // [W][D] taps, then [D] bias
+  A* const part = (A*)d.part + (int64_t)blockIdx.x * (W + 1) * a.D;      // [W][D] taps, then [D] bias
 #pragma unroll
   for (int j = 0; j <= W; ++j) {
 #pragma unroll
@@ -490,61 +560,42 @@ static __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvDev d) {
     for (int e = threadIdx.x; e < d.lanes * V; e += 256) {
       A v = (A)0;
       for (int q = 0; q < nr; ++q) v += sh[q * d.lanes * V + e];
-      const int64_t ch = vb * d.lanes * V + e;
+      const int64_t ch = (int64_t)blockIdx.y * d.lanes * V + e;
       if (ch < a.D) part[j * a.D + ch] = v;
     }
     __syncthreads();
   }
 }
-// gw [D][W] and gbias [D] from part [P][W + 1][D]
-template <typename A>
-static __global__ void __launch_bounds__(256) conv_sum_kernel(const A* part, int64_t P, int D, int W, A* gw, A* gbias) {
-  __shared__ A sh[4][64];
-  const int64_t n = (int64_t)(W + 1) * D, i = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-  const int q = threadIdx.x >> 6;
-  A s0 = (A)0, s1 = (A)0;
-  if (i < n) {
-    int64_t p = q;
-    for (; p + 4 < P; p += 8) {
-      s0 += part[p * n + i];
-      s1 += part[(p + 4) * n + i];
-    }
-    for (; p < P; p += 4) s0 += part[p * n + i];
-  }
-  sh[q][threadIdx.x & 63] = s0 + s1;
-  __syncthreads();
-  if (q == 0 && i < n) {
-    const A v = (sh[0][threadIdx.x] + sh[1][threadIdx.x]) + (sh[2][threadIdx.x] + sh[3][threadIdx.x]);
-    const int64_t j = i / D, ch = i - j * D;
-    if (j < W) gw[ch * W + j] = v;
-    else if (gbias) gbias[ch] = v;
-  }
-}
 
-template <typename T, int W>
+template <typename T, int W, int V>
 static __global__ void __launch_bounds__(256) conv_step_kernel(ConvDev d) {
   typedef typename SeqAcc<T>::type A;
-  constexpr int V = SeqVec<T>::V;
+  typedef SeqVec<T, V> Vec;
   const rgp_ssm_conv& a = d.a;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x, seq = idx / d.nvec, c = (idx - seq * d.nvec) * V;
-  if (seq >= a.n_seq) return;
-  const int n = a.D - c < V ? (int)(a.D - c) : V;
-  T* const st = (T*)a.last + seq * (W - 1) * a.D + c;
-  SeqVec<T> x[W];
+  const uint32_t idx = blockIdx.x * 256u + threadIdx.x, seq = idx / (uint32_t)d.nvec;
+  const int64_t c = (int64_t)(idx - seq * (uint32_t)d.nvec) * V;
+  if (seq >= (uint32_t)a.n_seq) return;
+  T* const st = (T*)a.last + (int64_t)seq * (W - 1) * a.D + c;
+  Vec x[W];
 #pragma unroll
-  for (int j = 0; j < W - 1; ++j) x[j] = seq_load((const T*)st + (int64_t)j * a.D, n, d.wout);
-  x[W - 1] = seq_load((const T*)a.x + seq * a.x_sb + c, n, d.wx);
-  SeqVec<T> o;
+  for (int j = 0; j < W - 1; ++j) x[j] = *(const Vec*)(st + (int64_t)j * a.D);
+  x[W - 1] = *(const Vec*)((const T*)a.x + seq * a.x_sb + c);
+  A w[V][W];
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[i][j] = ((const A*)a.w)[(c + i) * W + j];
+  Vec o;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    A p = a.bias && i < n ? ((const A*)a.bias)[c + i] : (A)0, comp;
+    A p = a.bias ? ((const A*)a.bias)[c + i] : (A)0;
 #pragma unroll
-    for (int j = 0; j < W; ++j) p += (i < n ? ((const A*)a.w)[(c + i) * W + j] : (A)0) * (A)x[j].e[i];
-    o.e[i] = (T)(p * seq_sigmoid(p, comp));
+    for (int j = 0; j < W; ++j) p += w[i][j] * (A)x[j].e[i];
+    o.e[i] = (T)(p * seq_sigmoid(p));
   }
-  seq_store((T*)a.v + seq * a.D + c, o, n, d.wgv);
+  *(Vec*)((T*)a.v + (int64_t)seq * a.D + c) = o;
 #pragma unroll
-  for (int j = 0; j < W - 1; ++j) seq_store(st + (int64_t)j * a.D, x[j + 1], n, d.wout);
+  for (int j = 0; j < W - 1; ++j) *(Vec*)(st + (int64_t)j * a.D) = x[j + 1];
 }
 
 static const char* conv_bad(const rgp_ssm_conv* a) {
@@ -555,54 +606,65 @@ static const char* conv_bad(const rgp_ssm_conv* a) {
   if (!a->off && (a->T < 1 || a->T * a->n_seq != a->rows)) return "rows must be T * n_seq, T >= 1";
   return nullptr;
 }
-static void conv_plan(const rgp_ssm_conv* a, ConvDev& d, int64_t& grid, int64_t& nrb) {
+static void conv_plan(const rgp_ssm_conv* a, bool wide, ConvDev& d, int64_t& nrb, int64_t& nvb) {
   d = ConvDev{};
   d.a = *a;
   d.g = SeqGeo{a->off, a->T, a->rows, a->n_seq, a->reverse};
-  const int V = 16 / seq_dtype_bytes(a->dtype);
+  d.wide = wide;
+  const int V = wide ? CONV_V(seq_dtype_bytes(a->dtype)) : 1;
   d.nvec = (a->D + V - 1) / V;
-  d.nrun = seq_blocks(d.g, CONV_RUN);
+  d.same = d.nvec % 64 == 0;
+  // runs of 16 steps (the W - 1 rows before a run come from cache) unless that leaves fewer than four waves a SIMD
+  for (d.lg = 4; d.lg > 3 && seq_blocks(d.g, d.lg) * d.nvec < 262144; --d.lg) {}
+  d.nrun = seq_blocks(d.g, d.lg);
   d.lanes = 1;
   while (d.lanes < 64 && d.lanes < d.nvec) d.lanes *= 2;
-  const int64_t nvb = (d.nvec + d.lanes - 1) / d.lanes, nr = 256 / d.lanes;
+  nvb = (d.nvec + d.lanes - 1) / d.lanes;
+  const int64_t nr = 256 / d.lanes, most = nvb > 2048 ? 1 : 2048 / nvb;  // eight workgroups a CU; more only lengthens the sum over them
   nrb = (d.nrun + nr - 1) / nr;
-  const int64_t most = nvb > 2048 ? 1 : 2048 / nvb;                      // eight workgroups a CU; more only lengthens the sum over them
   if (nrb > most) nrb = most;
   if (nrb < 1) nrb = 1;
-  grid = nrb * nvb;
 }
 extern "C" int64_t rgp_ssm_conv_workspace(const rgp_ssm_conv* a, int backward) {
   if (conv_bad(a)) return -1;
   if (!backward) return 0;
-  ConvDev d;
-  int64_t grid, nrb;
-  conv_plan(a, d, grid, nrb);
-  return nrb * (a->W + 1) * a->D * (a->dtype == RGP_F64 ? 8 : 4);
+  int64_t most = 0;
+  for (int wide = 0; wide < 2; ++wide) {
+    ConvDev d;
+    int64_t nrb, nvb;
+    conv_plan(a, wide != 0, d, nrb, nvb);
+    most = nrb > most ? nrb : most;
+  }
+  return most * (a->W + 1) * a->D * (a->dtype == RGP_F64 ? 8 : 4);
 }
 
 enum { CONV_FWD, CONV_LAST, CONV_BWD, CONV_STEP };
-template <typename T, int W>
-static hipError_t conv_go(const ConvDev& d, int what, int64_t grid, hipStream_t s) {
-  if (grid < 1) return hipSuccess;
-  if (what == CONV_FWD) hipLaunchKernelGGL((conv_fwd_kernel<T, W>), dim3((unsigned)grid), dim3(256), 0, s, d);
-  else if (what == CONV_LAST) hipLaunchKernelGGL((conv_last_kernel<T, W>), dim3((unsigned)grid), dim3(256), 0, s, d);
-  else if (what == CONV_BWD) hipLaunchKernelGGL((conv_bwd_kernel<T, W>), dim3((unsigned)grid), dim3(256), 0, s, d);
-  else hipLaunchKernelGGL((conv_step_kernel<T, W>), dim3((unsigned)grid), dim3(256), 0, s, d);
+template <typename T, int W, int V>
+static hipError_t conv_go(const ConvDev& d, int what, dim3 grid, hipStream_t s) {
+  if (grid.x < 1) return hipSuccess;
+  if (what == CONV_FWD) hipLaunchKernelGGL((conv_fwd_kernel<T, W, V>), grid, dim3(256), 0, s, d);
+  else if (what == CONV_LAST) hipLaunchKernelGGL((conv_last_kernel<T, W, V>), grid, dim3(256), 0, s, d);
+  else if (what == CONV_BWD) hipLaunchKernelGGL((conv_bwd_kernel<T, W, V>), grid, dim3(256), 0, s, d);
+  else hipLaunchKernelGGL((conv_step_kernel<T, W, V>), grid, dim3(256), 0, s, d);
   return hipGetLastError();
 }
+template <typename T, int W>
+static hipError_t conv_wide(const ConvDev& d, int what, dim3 grid, hipStream_t s) {
+  return d.wide ? conv_go<T, W, CONV_V((int)sizeof(T))>(d, what, grid, s) : conv_go<T, W, 1>(d, what, grid, s);
+}
 template <typename T>
-static hipError_t conv_taps(const ConvDev& d, int what, int64_t grid, hipStream_t s) {
+static hipError_t conv_taps(const ConvDev& d, int what, dim3 grid, hipStream_t s) {
   switch (d.a.W) {
-    case 2: return conv_go<T, 2>(d, what, grid, s);
-    case 3: return conv_go<T, 3>(d, what, grid, s);
-    case 4: return conv_go<T, 4>(d, what, grid, s);
-    case 5: return conv_go<T, 5>(d, what, grid, s);
-    case 6: return conv_go<T, 6>(d, what, grid, s);
-    case 7: return conv_go<T, 7>(d, what, grid, s);
-    default: return conv_go<T, 8>(d, what, grid, s);
+    case 2: return conv_wide<T, 2>(d, what, grid, s);
+    case 3: return conv_wide<T, 3>(d, what, grid, s);
+    case 4: return conv_wide<T, 4>(d, what, grid, s);
+    case 5: return conv_wide<T, 5>(d, what, grid, s);
+    case 6: return conv_wide<T, 6>(d, what, grid, s);
+    case 7: return conv_wide<T, 7>(d, what, grid, s);
+    default: return conv_wide<T, 8>(d, what, grid, s);
   }
 }
-static hipError_t conv_launch(const ConvDev& d, int what, int64_t grid, hipStream_t s) {
+static hipError_t conv_launch(const ConvDev& d, int what, dim3 grid, hipStream_t s) {
   switch (d.a.dtype) {
     case RGP_F64: return conv_taps<double>(d, what, grid, s);
     case RGP_F32: return conv_taps<float>(d, what, grid, s);
@@ -613,44 +675,43 @@ static hipError_t conv_launch(const ConvDev& d, int what, int64_t grid, hipStrea
 static rgp_status conv_run(rgp_handle h, hipStream_t s, const rgp_ssm_conv* a, int what) {
   const std::string name = what == CONV_BWD ? "ssm conv backward: " : what == CONV_STEP ? "ssm conv step: " : "ssm conv forward: ";
   if (const char* bad = conv_bad(a)) return rgp_fail(h, RGP_ERR_BAD_ARG, name + bad);
-  const bool some = a->rows > 0;
+  const bool some = a->rows > 0;                       // without rows the activations may have no memory
   if (!a->w || (some && !a->x)) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "x and w are required");
+  if (what == CONV_BWD && (!a->gw || (some && (!a->gv || !a->gx)))) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "gv, gx and gw are required");
+  if (what == CONV_STEP && (a->off || a->T != 1)) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "one row per sequence (T = 1, no offsets)");
+  if (what == CONV_STEP && (!a->v || !a->last || a->init != a->last)) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "v and the state (init = last) are required");
+  if (what == CONV_FWD && some && !a->v) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "v is required");
+  if (what == CONV_FWD && a->last && a->last == a->init) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "last must not be init");
+  const int e = seq_dtype_bytes(a->dtype), V = CONV_V(e);
+  const int64_t st = what == CONV_STEP ? 0 : a->x_st;
+  bool wide = a->D % V == 0 && seq_aligned(a->x, st, a->x_sb, e, V);
+  if (what == CONV_BWD) wide = wide && seq_aligned(a->gv, a->gv_st, a->gv_sb, e, V) && seq_aligned(a->gx, 0, 0, e, V);
+  else wide = wide && seq_aligned(a->v, 0, 0, e, V) && (what != CONV_STEP || seq_aligned(a->last, 0, 0, e, V));
   ConvDev d;
-  int64_t grid, nrb;
-  conv_plan(a, d, grid, nrb);
-  const int e = seq_dtype_bytes(a->dtype), V = 16 / e;
-  if ((double)d.nrun * d.nvec > 4294967295.0 || (double)a->n_seq * d.nvec > 4294967295.0 || (double)grid * 256 > 4294967295.0)
-    return rgp_fail(h, RGP_ERR_BAD_ARG, name + "more than 2^32 work items");
-  d.wx = seq_aligned(a->x, a->x_st, a->x_sb, e);
+  int64_t nrb, nvb;
+  conv_plan(a, wide, d, nrb, nvb);
   const int64_t seqs = ((int64_t)a->n_seq * d.nvec + 255) / 256;
+  if ((double)d.nrun * d.nvec > 4294967295.0 - 256.0 || (double)a->n_seq * d.nvec > 4294967295.0 - 256.0 || nvb > 65535 || (double)nrb * 256 > 4294967295.0)
+    return rgp_fail(h, RGP_ERR_BAD_ARG, name + "more than 2^32 work items");
   hipError_t err = hipSuccess;
   if (what == CONV_BWD) {
-    if (!a->gw || (some && (!a->gv || !a->gx))) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "gv, gx and gw are required");
     if (rgp_ssm_conv_workspace(a, 1) > a->work_bytes || !a->work || ((uintptr_t)a->work & 15))
       return rgp_fail(h, RGP_ERR_WORKSPACE, name + "work buffer too small or not 16-byte aligned");
-    d.wgv = seq_aligned(a->gv, a->gv_st, a->gv_sb, e);
-    d.wout = a->D % V == 0 && seq_aligned(a->gx, 0, 0, e);
     d.part = a->work;
-    err = conv_launch(d, CONV_BWD, grid, s);
+    err = conv_launch(d, CONV_BWD, dim3((unsigned)nrb, (unsigned)nvb), s);
     if (err == hipSuccess) {
-      const unsigned sg = (unsigned)(((int64_t)(a->W + 1) * a->D + 63) / 64);
-      if (a->dtype == RGP_F64) hipLaunchKernelGGL(conv_sum_kernel<double>, dim3(sg), dim3(256), 0, s, (const double*)d.part, nrb, a->D, a->W, (double*)a->gw, (double*)a->gbias);
-      else hipLaunchKernelGGL(conv_sum_kernel<float>, dim3(sg), dim3(256), 0, s, (const float*)d.part, nrb, a->D, a->W, (float*)a->gw, (float*)a->gbias);
-      err = hipGetLastError();
+      const int acc = a->dtype == RGP_F64 ? RGP_F64 : RGP_F32;
+      const int64_t n = (int64_t)a->W * a->D, per = n + a->D;
+      SeqSums sums;
+      sums.add(d.part, nrb, per, n, a->gw, acc, a->W);
+      sums.add((char*)d.part + n * (acc == RGP_F64 ? 8 : 4), nrb, per, a->D, a->gbias, acc);
+      return sums.run(h, s, acc);
     }
   } else if (what == CONV_STEP) {
-    if (a->off || a->T != 1) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "one row per sequence (T = 1, no offsets)");
-    if (!a->v || !a->last || a->init != a->last) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "v and the state (init = last) are required");
-    d.wx = seq_aligned(a->x, 0, a->x_sb, e);
-    d.wout = a->D % V == 0 && seq_aligned(a->last, 0, 0, e);
-    d.wgv = a->D % V == 0 && seq_aligned(a->v, 0, 0, e);
-    err = conv_launch(d, CONV_STEP, seqs, s);
+    err = conv_launch(d, CONV_STEP, dim3((unsigned)seqs), s);
   } else {
-    if (some && !a->v) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "v is required");
-    if (a->last && a->last == a->init) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "last must not be init");
-    d.wout = a->D % V == 0 && seq_aligned(a->v, 0, 0, e);
-    err = conv_launch(d, CONV_FWD, (d.nrun * d.nvec + 255) / 256, s);
-    if (err == hipSuccess && a->last) err = conv_launch(d, CONV_LAST, seqs, s);
+    err = conv_launch(d, CONV_FWD, dim3((unsigned)((d.nrun * d.nvec + 255) / 256)), s);
+    if (err == hipSuccess && a->last) err = conv_launch(d, CONV_LAST, dim3((unsigned)seqs), s);
   }
   return err == hipSuccess ? RGP_OK : rgp_fail(h, RGP_ERR_HIP, name + hipGetErrorString(err));
 }

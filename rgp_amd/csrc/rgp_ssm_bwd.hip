@@ -3,32 +3,34 @@
 // the gradients are
 //     gu = dt sum_n lam B + skip gp;   gdelta = sigmoid(delta + bias) (u sum_n lam B + sum_n lam a s_{t-1} A);
 //     gB[n] = sum_d lam dt u;  gC[n] = sum_d gp s;  gA[n] = sum_t lam a s_{t-1} dt;  gskip = sum_t gp u;  gz = gy p silu'(z).
-// The work is laid out as in the forward pass.  A tile is CK steps: it starts from a state that the forward pass left every CK steps, keeps
-// the tile's states and decays in registers, then walks back.  Running the recurrence backwards instead (s_{t-1} = (s_t - dt u B) / a) would
+// The work is laid out as in the forward pass.  A tile is walked in pieces of CK steps: each starts from a state that the
+// forward pass left there, keeps the piece's states and decays in registers, then walks back.  Running the recurrence backwards instead (s_{t-1} = (s_t - dt u B) / a) would
 // lose everything for small a.  The sums over channels in gB and gC fold 2 SSM_R values over the wave's channels with half-wave and
 // 16-lane register swaps, then over the waves through LDS; what crosses workgroups is written once and summed in a fixed order.
 #include "rgp_ssm.h"
 
-template <typename T, int K, int CH, int MODE>
-static __global__ void __launch_bounds__(CH* K) ssm_bwd_kernel(SsmDev d) {
+template <typename T, int K, int CH, int MODE, int V>
+static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2) ssm_bwd_kernel(SsmDev d) {
   typedef typename SeqAcc<T>::type A;
-  constexpr int THREADS = CH * K, V = SeqVec<T>::V, NV = CH / V, CK = SsmCk<A>::n, TL = CK, NP = SSM_R * K, R = SSM_R, WAVES = THREADS / 64;
-  constexpr int ITEMS = TL * NV, NI = (ITEMS + THREADS - 1) / THREADS, NB = (TL * NP + THREADS - 1) / THREADS;
+  typedef SeqVec<T, V> Vec;
+  constexpr int THREADS = CH * K, NV = CH / V, RPI = THREADS / NV, CK = SSM_CK, TL = sizeof(T) == 8 ? 8 : sizeof(T) == 4 || K > 4 ? 16 : 32, SUB = TL / CK, NP = SSM_R * K, R = SSM_R, WAVES = THREADS / 64;
+  constexpr int NI = RPI >= TL ? 1 : TL / RPI, NB = (TL * NP + THREADS - 1) / THREADS;
   struct alignas(4 * sizeof(A)) Four { A x, y, z, w; };
   struct alignas(16) Quad { A v[R]; };
-  __shared__ Four pl[TL][CH];                          // in: dt, u, gp; out: sum lam B, sum lam a s A, sum C s
+  __shared__ Four pl[TL][CH];                          // in: dt, u, gp, sigmoid(delta + bias); out: gu, gdelta, p
+  __shared__ A zf[MODE == 0 ? TL : 1][CH];              // gy silu'(z)
   __shared__ Quad Bl[MODE == 0 ? TL : 1][K];
   __shared__ Quad Cl[TL][K];
   __shared__ A red[MODE == 0 ? WAVES : 1][MODE == 0 ? TL : 1][2 * NP];
   const rgp_ssm_scan& a = d.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t nchb = (int64_t)a.G * d.ncb;
-  const int64_t slot = blockIdx.x / nchb;
-  const int cb = (int)(blockIdx.x - slot * nchb), grp = cb / d.ncb, cig = cb - grp * d.ncb, c0 = cig * CH;
-  const SeqBlock b = seq_find(d.g, slot, d.L);
+  const int64_t slot = blockIdx.x;
+  const int grp = (int)blockIdx.y / d.ncb, cig = (int)blockIdx.y - grp * d.ncb, c0 = cig * CH;
+  const SeqBlock b = seq_find(d.g, blockIdx.x, d.lg);
   const int N = a.N, chn = d.Dg - c0 < CH ? d.Dg - c0 : CH, ch0 = grp * d.Dg + c0;
-  const int ev = tid % NV, et = tid / NV, eval = chn - ev * V < 0 ? 0 : (chn - ev * V < V ? chn - ev * V : V);
-  const int ech = ch0 + ev * V;
+  const int ev = tid % NV, et = tid / NV;               // roles as in the forward kernel
+  const bool here = ev * V < chn && et < TL;
+  const int ech = ch0 + (ev * V < chn ? ev * V : 0);
   const int ch = tid / K, k = tid % K;
   const bool live = ch < chn;
   if (!b.ok) {                                        // an empty block still owns a row of the partial sums
@@ -43,83 +45,68 @@ static __global__ void __launch_bounds__(CH* K) ssm_bwd_kernel(SsmDev d) {
     }
     return;
   }
+  if (MODE == 1 && b.j == 0) return;                              // nothing precedes the first block of a sequence
   const int64_t t0 = b.j * d.L, t1 = t0 + d.L < b.len ? t0 + d.L : b.len;
-  A bias[V], skip[V], gD[V], gbias[V];
+  A bias[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    bias[i] = a.bias && i < eval ? ((const A*)a.bias)[ech + i] : (A)0;
-    skip[i] = MODE == 0 && a.skip && i < eval ? ((const A*)a.skip)[ech + i] : (A)0;
-    gD[i] = gbias[i] = (A)0;
-  }
+  for (int i = 0; i < V; ++i) bias[i] = a.bias ? ((const A*)a.bias)[ech + i] : (A)0;
+  const A skip = MODE == 0 && a.skip && live ? ((const A*)a.skip)[ch0 + ch] : (A)0;
+  A gD = (A)0, gbias = (A)0;
   A Ar[R], carry[R], gA[R], sum = (A)0;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const bool ok = live && k * R + r < N;
-    Ar[r] = ok ? ((const A*)a.A)[(int64_t)(ch0 + ch) * N + k * R + r] : (A)0;
+    Ar[r] = ok ? ssm_finite(((const A*)a.A)[(int64_t)(ch0 + ch) * N + k * R + r]) : (A)0;
     carry[r] = MODE == 0 && d.part && ok ? ((const A*)d.part)[(slot * a.D + ch0 + ch) * N + k * R + r] : (A)0;
     gA[r] = (A)0;
   }
-  const A* const ckpt = MODE == 0 ? (const A*)a.states + (seq_slot0(d.g, b.seq, b.start, CK) * a.D + ch0 + ch) * N + k * R : nullptr;
+  const A* const ckpt = MODE == 0 ? (const A*)a.states + (seq_slot0(d.g, b.seq, b.start, SSM_CK_LG) * a.D + ch0 + ch) * N + k * R : nullptr;
   const SeqStride su{a.u_st, a.u_sb}, sd{a.delta_st, a.delta_sb}, sz{a.z_st, a.z_sb}, sB{a.B_st, a.B_sb}, sC{a.C_st, a.C_sb}, sg{a.gy_st, a.gy_sb};
   auto decay = [&](A dt, int r) {
     return sizeof(A) == 4 ? (A)seq_exp2((float)(dt * (Ar[r] * (A)1.44269504088896341))) : seq_exp(dt * Ar[r]);
   };
 
-  SeqVec<T> ru[NI], rd[NI], rz[NI], rg[NI];
+  Vec ru[NI], rd[NI], rz[NI], rg[NI];
   T rB[NB], rC[NB];
-  A rs[R];
   auto fetch = [&](int64_t tt) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int tl = et + i * (THREADS / NV);
-      const int n = tl < TL && tt + tl < t1 ? eval : 0;
-      const int64_t t = n ? tt + tl : t0;
-      if (MODE == 0) ru[i] = seq_load(seq_row((const T*)a.u, d.g, b, su, t) + ech, n, d.wu);
-      rd[i] = seq_load(seq_row((const T*)a.delta, d.g, b, sd, t) + ech, n, d.wd);
-      rg[i] = seq_load(seq_row((const T*)a.gy, d.g, b, sg, t) + ech, n, d.wgy);
-      if (a.z) rz[i] = seq_load(seq_row((const T*)a.z, d.g, b, sz, t) + ech, n, d.wz);
+      const int64_t at = tt + et + i * RPI, t = at < t1 ? at : t1 - 1;
+      if (MODE == 0) ru[i] = *(const Vec*)(seq_row((const T*)a.u, d.g, b, su, t) + ech);
+      rd[i] = *(const Vec*)(seq_row((const T*)a.delta, d.g, b, sd, t) + ech);
+      rg[i] = *(const Vec*)(seq_row((const T*)a.gy, d.g, b, sg, t) + ech);
+      if (a.z) rz[i] = *(const Vec*)(seq_row((const T*)a.z, d.g, b, sz, t) + ech);
     }
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      const int e = tid + i * THREADS, tl = e / NP, n = e % NP;
-      const bool ok = tl < TL && n < N && tt + tl < t1;
-      const int64_t t = ok ? tt + tl : t0;
-      if (MODE == 0) rB[i] = ok ? seq_row((const T*)a.B, d.g, b, sB, t)[(int64_t)grp * N + n] : (T)0;
-      rC[i] = ok ? seq_row((const T*)a.C, d.g, b, sC, t)[(int64_t)grp * N + n] : (T)0;
-    }
-    if (MODE == 0) {
-#pragma unroll
-      for (int r = 0; r < R; ++r) rs[r] = live && k * R + r < N ? ckpt[tt / CK * ((int64_t)a.D * N) + r] : (A)0;
+      const int e = tid + i * THREADS, n = e % NP < N ? e % NP : 0;
+      const int64_t at = tt + e / NP, t = at < t1 ? at : t1 - 1;
+      if (MODE == 0) rB[i] = seq_row((const T*)a.B, d.g, b, sB, t)[(int64_t)grp * N + n];
+      rC[i] = seq_row((const T*)a.C, d.g, b, sC, t)[(int64_t)grp * N + n];
     }
   };
   const int64_t last = t0 + (t1 - t0 - 1) / TL * TL;
   fetch(last);
   for (int64_t tt = last; tt >= t0; tt -= TL) {
     const int nt = t1 - tt < TL ? (int)(t1 - tt) : TL;
-    SeqVec<T> cu[NI], cz[NI], cg[NI];
-    A sig[NI][V], dts[NI][V];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int tl = et + i * (THREADS / NV);
-      cu[i] = ru[i];
-      cz[i] = rz[i];
-      cg[i] = rg[i];
-      if (tl < TL) {
+      const int tl = et + i * RPI;
+      if (et < TL) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           Four p;
-          p.x = dts[i][j] = seq_softplus((A)rd[i].e[j] + bias[j], sig[i][j]);
-          p.y = MODE == 0 ? (A)ru[i].e[j] : (A)0;
-          p.z = (A)rg[i].e[j];
-          p.w = (A)0;
+          const A dt = seq_softplus((A)rd[i].e[j] + bias[j], p.w);
+          const bool ok = tl < nt && ev * V < chn;             // all lanes' values are folded below
+          p.x = ok ? dt : (A)0;
+          p.y = MODE == 0 && ok ? (A)ru[i].e[j] : (A)0;
+          A gp = (A)rg[i].e[j];
           if (a.z) {
-            A comp;
-            const A z = (A)rz[i].e[j];
-            p.z *= z * seq_sigmoid(z, comp);
+            const A z = (A)rz[i].e[j], q = gp * seq_sigmoid(z);
+            if (MODE == 0) zf[tl][ev * V + j] = q + (gp - q) * (z * seq_sigmoid(z));
+            gp = z * q;
           }
-          if (MODE == 0) {
-            gD[j] += p.z * p.y;
-          }
+          p.z = ok ? gp : (A)0;
           pl[tl][ev * V + j] = p;
         }
       }
@@ -127,87 +114,98 @@ static __global__ void __launch_bounds__(CH* K) ssm_bwd_kernel(SsmDev d) {
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       const int e = tid + i * THREADS, tl = e / NP, n = e % NP;
-      if (tl < TL) {
-        if (MODE == 0) Bl[tl][n / R].v[n % R] = (A)rB[i];
-        Cl[tl][n / R].v[n % R] = (A)rC[i];
+      if (TL * NP % THREADS == 0 || tl < TL) {
+        const bool ok = n < N && tl < nt;
+        if (MODE == 0) Bl[tl][n / R].v[n % R] = ok ? (A)rB[i] : (A)0;
+        Cl[tl][n / R].v[n % R] = ok ? (A)rC[i] : (A)0;
       }
-    }
-    A s0[R];
-    if (MODE == 0) {
-#pragma unroll
-      for (int r = 0; r < R; ++r) s0[r] = rs[r];
     }
     __syncthreads();
     if (tt > t0) fetch(tt - TL);
     if (MODE == 1) {
 #pragma unroll
-      for (int t = TL - 1; t >= 0; --t) {
-        if (t < nt) {
-          const Four p = pl[t][ch];
-          const Quad C = Cl[t][k];
-          sum += p.x;
+      for (int t = TL - 1; t >= 0; --t) {                         // steps behind the end change nothing
+        const Four p = pl[t][ch];
+        const Quad C = Cl[t][k];
+        sum += p.x;
 #pragma unroll
-          for (int r = 0; r < R; ++r) carry[r] = (C.v[r] * p.z + carry[r]) * decay(p.x, r);
-        }
+        for (int r = 0; r < R; ++r) carry[r] = (C.v[r] * p.z + carry[r]) * decay(p.x, r);
       }
     } else {
-      A s[TL][R], e[TL][R];
+#pragma unroll 1
+      for (int sub = SUB - 1; sub >= 0; --sub) {
+        const int tb = sub * CK;
+        if (tb >= nt) continue;
+        A s0[R], s[CK][R], e[CK][R];
 #pragma unroll
-      for (int t = 0; t < TL; ++t) {
-        if (t < nt) {
-          const Four p = pl[t][ch];
-          const Quad B = Bl[t][k];
+        for (int r = 0; r < R; ++r) s0[r] = live && k * R + r < N ? ckpt[((tt + tb) / CK) * ((int64_t)a.D * N) + r] : (A)0;
+        // operands of a step are read from LDS while the step before is computed
+        Four p = pl[tb][ch];
+        Quad B = Bl[tb][k], C;
+#pragma unroll
+        for (int i = 0; i < CK; ++i) {
+          const int tn = tb + (i + 1 < CK ? i + 1 : i);
+          const Four pn = pl[tn][ch];
+          const Quad Bn = Bl[tn][k];
           const A w = p.x * p.y;
 #pragma unroll
           for (int r = 0; r < R; ++r) {
-            e[t][r] = decay(p.x, r);
-            s[t][r] = e[t][r] * (t ? s[t ? t - 1 : 0][r] : s0[r]) + w * B.v[r];
+            e[i][r] = decay(p.x, r);
+            s[i][r] = e[i][r] * (i ? s[i ? i - 1 : 0][r] : s0[r]) + w * B.v[r];
           }
+          p = pn;
+          B = Bn;
+          if (i + 1 == CK) C = Cl[tb + CK - 1][k];
         }
-      }
 #pragma unroll
-      for (int t = TL - 1; t >= 0; --t) {
-        if (t < nt) {
-          const Four p = pl[t][ch];
-          const Quad B = Bl[t][k], C = Cl[t][k];
+        for (int i = CK - 1; i >= 0; --i) {
+          const int t = tb + i, tn = t - (i ? 1 : 0);
+          const Four pn = pl[tn][ch];
+          const Quad Bn = Bl[tn][k], Cn = Cl[tn][k];
           const A w = p.x * p.y;
           A g1 = (A)0, g2 = (A)0, yd = (A)0, vB[R], vC[R];
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             const A lam = C.v[r] * p.z + carry[r];
-            vC[r] = p.z * s[t][r];
+            vC[r] = p.z * s[i][r];
             vB[r] = lam * w;
             g1 += lam * B.v[r];
-            yd += C.v[r] * s[t][r];
-            carry[r] = lam * e[t][r];
-            const A q = carry[r] * (t ? s[t ? t - 1 : 0][r] : s0[r]);
+            yd += C.v[r] * s[i][r];
+            carry[r] = lam * e[i][r];
+            const A q = carry[r] * (i ? s[i ? i - 1 : 0][r] : s0[r]);
             g2 += q * Ar[r];
             gA[r] += q * p.x;
           }
           g1 = seq_sum<K>(g1);
           g2 = seq_sum<K>(g2);
           yd = seq_sum<K>(yd);
-          if (k == 0) {
-            Four o;
-            o.x = g1; o.y = g2; o.z = yd; o.w = (A)0;
-            pl[t][ch] = o;
-          }
+          Four o;                                                 // the same in all K lanes
+          o.x = p.x * g1 + skip * p.z;
+          o.y = (p.y * g1 + g2) * p.w;
+          o.z = yd + skip * p.y;
+          o.w = (A)0;
+          gD += p.z * p.y;
+          gbias += t < nt ? o.y : (A)0;
+          if (k == 0) pl[t][ch] = o;
           // over the wave's channels: lane bit 5 selects gB / gC, bit 4 and bit 3 the state
           const bool b3 = (lane & 8) != 0;
           A f0 = seq_fold<true>(vB[0], vC[0]), f1 = seq_fold<true>(vB[1], vC[1]), f2 = seq_fold<true>(vB[2], vC[2]), f3 = seq_fold<true>(vB[3], vC[3]);
           f0 = seq_fold<false>(f0, f2);
           f1 = seq_fold<false>(f1, f3);
-          A* const o = &red[wave][t][(lane >> 5) * NP + k * R + ((lane >> 4) & 1) * 2];
+          A* const f_to = &red[wave][t][(lane >> 5) * NP + k * R + ((lane >> 4) & 1) * 2];
           if constexpr (K == 16) {
-            o[0] = f0;
-            o[1] = f1;
+            f_to[0] = f0;
+            f_to[1] = f1;
           } else {
             A f = seq_fold8(f0, f1, b3);
             if constexpr (K <= 4) f += seq_xor4(f);
             if constexpr (K <= 2) f += seq_dpp<0x4E>(f);
             if constexpr (K == 1) f += seq_dpp<0xB1>(f);
-            if ((lane & 7) == k) o[b3] = f;
+            if ((lane & 7) == k) f_to[b3] = f;
           }
+          p = pn;
+          B = Bn;
+          C = Cn;
         }
       }
     }
@@ -215,29 +213,20 @@ static __global__ void __launch_bounds__(CH* K) ssm_bwd_kernel(SsmDev d) {
     if (MODE == 0) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int tl = et + i * (THREADS / NV);
-        if (tl < nt && eval > 0) {
-          SeqVec<T> ou, od, oz;
+        const int tl = et + i * RPI;
+        if (here && tl < nt) {
+          Vec ou, od, oz;
 #pragma unroll
           for (int j = 0; j < V; ++j) {
             const Four p = pl[tl][ev * V + j];
-            const A u = (A)cu[i].e[j], gy = (A)cg[i].e[j];
-            A gp = gy;
-            if (a.z) {
-              A comp;
-              const A z = (A)cz[i].e[j], sg_ = seq_sigmoid(z, comp);
-              gp = gy * (z * sg_);
-              oz.e[j] = (T)(gy * (p.z + skip[j] * u) * (sg_ + z * sg_ * comp));
-            }
-            ou.e[j] = (T)(dts[i][j] * p.x + skip[j] * gp);
-            const A graw = (u * p.x + p.y) * sig[i][j];
-            gbias[j] += graw;
-            od.e[j] = (T)graw;
+            ou.e[j] = (T)p.x;
+            od.e[j] = (T)p.y;
+            if (a.z) oz.e[j] = (T)(zf[tl][ev * V + j] * p.z);
           }
           const int64_t o = seq_row_index(d.g, b, tt + tl) * a.D + ech;
-          seq_store((T*)a.gu + o, ou, eval, d.wout);
-          seq_store((T*)a.gdelta + o, od, eval, d.wout);
-          if (a.z) seq_store((T*)a.gz + o, oz, eval, d.wout);
+          *(Vec*)((T*)a.gu + o) = ou;
+          *(Vec*)((T*)a.gdelta + o) = od;
+          if (a.z) *(Vec*)((T*)a.gz + o) = oz;
         }
       }
       for (int e = tid; e < nt * 2 * NP; e += THREADS) {
@@ -272,31 +261,20 @@ static __global__ void __launch_bounds__(CH* K) ssm_bwd_kernel(SsmDev d) {
     for (int r = 0; r < R; ++r)
       if (k * R + r < N) ((A*)d.pA)[(slot * a.D + ch0 + ch) * N + k * R + r] = gA[r];
   }
-  // gskip and gbias: the threads that share a vector of channels, through the tile's LDS; only threads below QR saw a row of the tile
-  constexpr int QR = THREADS / NV < TL ? THREADS / NV : TL;
-  A* const buf = (A*)&pl[0][0];
-  static_assert(QR * CH <= TL * CH * 4, "one value per contributing thread and channel of a vector");
-#pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    if (et < QR) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) buf[et * CH + ev * V + j] = which ? gbias[j] : gD[j];
-    }
-    __syncthreads();
-    if (tid < chn) {
-      A v = (A)0;
-      for (int q = 0; q < QR; ++q) v += buf[q * CH + tid];
-      ((A*)d.pD)[(slot * 2 + which) * a.D + ch0 + tid] = v;
-    }
-    __syncthreads();
+  if (live && k == 0) {
+    ((A*)d.pD)[slot * 2 * a.D + ch0 + ch] = gD;
+    ((A*)d.pD)[(slot * 2 + 1) * a.D + ch0 + ch] = gbias;
   }
 }
 
 template <typename T, int K, int CH>
 static hipError_t go(const SsmDev& d, int mode, hipStream_t s) {
-  const int64_t grid = d.nslot * d.a.G * d.ncb;
-  if (mode == 0) hipLaunchKernelGGL((ssm_bwd_kernel<T, K, CH, 0>), dim3((unsigned)grid), dim3(CH * K), 0, s, d);
-  else hipLaunchKernelGGL((ssm_bwd_kernel<T, K, CH, 1>), dim3((unsigned)grid), dim3(CH * K), 0, s, d);
+  constexpr int V = 16 / (int)sizeof(T);
+  const dim3 g((unsigned)d.nslot, (unsigned)(d.a.G * d.ncb)), t(CH * K);
+  if (mode == 0 && d.wide) hipLaunchKernelGGL((ssm_bwd_kernel<T, K, CH, 0, V>), g, t, 0, s, d);
+  else if (mode == 0) hipLaunchKernelGGL((ssm_bwd_kernel<T, K, CH, 0, 1>), g, t, 0, s, d);
+  else if (d.wide) hipLaunchKernelGGL((ssm_bwd_kernel<T, K, CH, 1, V>), g, t, 0, s, d);
+  else hipLaunchKernelGGL((ssm_bwd_kernel<T, K, CH, 1, 1>), g, t, 0, s, d);
   return hipGetLastError();
 }
 template <typename T>

@@ -2,15 +2,16 @@
 //     dt = softplus(delta + bias);  s[n] = exp(dt A[n]) s[n] + dt u B[n];  y = (sum_n C[n] s[n] + skip u) silu(z).
 // K lanes hold one channel's states, SSM_R each; a workgroup holds CH channels of one group of B / C and walks its block of time in tiles
 // of TL steps.  What is elementwise over (step, channel) -- softplus, silu, the loads and stores, 16 bytes a lane -- runs with the lanes
-// over the tile's elements; between them the recurrence reads (dt, dt u) and the rows of B and C from LDS and leaves y there.  The next
+// over the tile's elements (a vector of 16 bytes each, or single elements where alignment or an odd width forbids that); between them the recurrence reads (dt, dt u) and the rows of B and C from LDS and leaves y there.  The next
 // tile's loads are in flight while a tile is walked.
 #include "rgp_ssm.h"
 
-template <typename T, int K, int CH, int MODE>
+template <typename T, int K, int CH, int MODE, int V>
 static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
   typedef typename SeqAcc<T>::type A;
-  constexpr int THREADS = CH * K, V = SeqVec<T>::V, NV = CH / V, TL = sizeof(A) == 8 ? 16 : 32, NP = SSM_R * K, R = SSM_R;
-  constexpr int ITEMS = TL * NV, NI = (ITEMS + THREADS - 1) / THREADS, NB = (TL * NP + THREADS - 1) / THREADS, CK = SsmCk<A>::n;
+  typedef SeqVec<T, V> Vec;
+  constexpr int THREADS = CH * K, NV = CH / V, TL = sizeof(A) == 8 ? 16 : 32, NP = SSM_R * K, R = SSM_R, RPI = THREADS / NV;
+  constexpr int NI = RPI >= TL ? 1 : TL / RPI, NB = (TL * NP + THREADS - 1) / THREADS, CK = SSM_CK;
   struct alignas(2 * sizeof(A)) Pair { A dt, w; };
   struct alignas(16) Quad { A v[R]; };
   __shared__ Pair pl[TL][CH];
@@ -18,10 +19,9 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
   __shared__ Quad Cl[MODE == 0 ? TL : 1][K];
   const rgp_ssm_scan& a = d.a;
   const int tid = threadIdx.x;
-  const int64_t nchb = (int64_t)a.G * d.ncb;
-  const int64_t slot = blockIdx.x / nchb;
-  const int cb = (int)(blockIdx.x - slot * nchb), grp = cb / d.ncb, c0 = (cb - grp * d.ncb) * CH;      // first channel, inside the group
-  const SeqBlock b = seq_find(d.g, slot, d.L);
+  const int64_t slot = blockIdx.x;
+  const int grp = (int)blockIdx.y / d.ncb, c0 = ((int)blockIdx.y - grp * d.ncb) * CH;       // group, first channel inside the group
+  const SeqBlock b = seq_find(d.g, blockIdx.x, d.lg);
   if (!b.ok) {
     if (MODE == 0 && a.last && b.len == 0 && b.j == 0) {         // a sequence without steps hands its state on
       const int c = c0 + (int)threadIdx.x / K, n0 = (int)threadIdx.x % K * R;
@@ -33,18 +33,21 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
     }
     return;
   }
+  if (MODE == 1 && (b.j + 1) * d.L >= b.len) return;              // nothing follows the last block of a sequence
   const int64_t t0 = b.j * d.L, t1 = t0 + d.L < b.len ? t0 + d.L : b.len;
   const int N = a.N, chn = d.Dg - c0 < CH ? d.Dg - c0 : CH;      // channels of this block
   const int ch0 = grp * d.Dg + c0;                               // first channel
 
-  // elementwise role: vector v of the rows tid / NV, tid / NV + THREADS / NV, ...
-  const int ev = tid % NV, et = tid / NV, eval = chn - ev * V < 0 ? 0 : (chn - ev * V < V ? chn - ev * V : V);
-  const int ech = ch0 + ev * V;
+  // Elementwise role: vector ev of the rows et, et + RPI, ... of a tile.  Rows behind the end and channels behind the last one read the
+  // last row and the first channel there are, and count as zero.
+  const int ev = tid % NV, et = tid / NV;
+  const bool here = ev * V < chn && et < TL;
+  const int ech = ch0 + (ev * V < chn ? ev * V : 0);
   A bias[V], skip[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    bias[i] = a.bias && i < eval ? ((const A*)a.bias)[ech + i] : (A)0;
-    skip[i] = MODE == 0 && a.skip && i < eval ? ((const A*)a.skip)[ech + i] : (A)0;
+    bias[i] = a.bias ? ((const A*)a.bias)[ech + i] : (A)0;
+    skip[i] = MODE == 0 && a.skip ? ((const A*)a.skip)[ech + i] : (A)0;
   }
   // recurrence role: states k R .. k R + R - 1 of channel ch
   const int ch = tid / K, k = tid % K;
@@ -55,53 +58,51 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
     const bool ok = live && k * R + r < N;
     Ar[r] = ok ? ((const A*)a.A)[(int64_t)(ch0 + ch) * N + k * R + r] : (A)0;
     if (sizeof(A) == 4) Ar[r] *= (A)1.44269504088896341;          // exp(dt A) = 2^(dt A log2 e)
+    Ar[r] = ssm_finite(Ar[r]);
     s[r] = (A)0;
     if (MODE == 0 && ok) {
       if (d.part) s[r] = ((const A*)d.part)[(slot * a.D + ch0 + ch) * N + k * R + r];
       else if (a.init) s[r] = ((const A*)a.init)[(b.seq * a.D + ch0 + ch) * N + k * R + r];
     }
   }
-  A* const ckpt = MODE == 0 && a.states ? (A*)a.states + ((seq_slot0(d.g, b.seq, b.start, CK)) * a.D + ch0 + ch) * N + k * R : nullptr;
+  A* const ckpt = MODE == 0 && a.states ? (A*)a.states + ((seq_slot0(d.g, b.seq, b.start, SSM_CK_LG)) * a.D + ch0 + ch) * N + k * R : nullptr;
   const SeqStride su{a.u_st, a.u_sb}, sd{a.delta_st, a.delta_sb}, sz{a.z_st, a.z_sb}, sB{a.B_st, a.B_sb}, sC{a.C_st, a.C_sb};
 
-  SeqVec<T> ru[NI], rd[NI], rz[NI];
+  Vec ru[NI], rd[NI], rz[NI];
   T rB[NB], rC[NB];
   auto fetch = [&](int64_t tt) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int tl = et + i * (THREADS / NV);
-      const int n = tl < TL && tt + tl < t1 ? eval : 0;
-      const int64_t t = n ? tt + tl : t0;                        // an address inside the block even where nothing is read
-      ru[i] = seq_load(seq_row((const T*)a.u, d.g, b, su, t) + ech, n, d.wu);
-      rd[i] = seq_load(seq_row((const T*)a.delta, d.g, b, sd, t) + ech, n, d.wd);
-      if (MODE == 0 && a.z) rz[i] = seq_load(seq_row((const T*)a.z, d.g, b, sz, t) + ech, n, d.wz);
+      const int64_t at = tt + et + i * RPI, t = at < t1 ? at : t1 - 1;
+      ru[i] = *(const Vec*)(seq_row((const T*)a.u, d.g, b, su, t) + ech);
+      rd[i] = *(const Vec*)(seq_row((const T*)a.delta, d.g, b, sd, t) + ech);
+      if (MODE == 0 && a.z) rz[i] = *(const Vec*)(seq_row((const T*)a.z, d.g, b, sz, t) + ech);
     }
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      const int e = tid + i * THREADS, tl = e / NP, n = e % NP;
-      const bool ok = tl < TL && n < N && tt + tl < t1;
-      const int64_t t = ok ? tt + tl : t0;
-      rB[i] = ok ? seq_row((const T*)a.B, d.g, b, sB, t)[(int64_t)grp * N + n] : (T)0;
-      if (MODE == 0) rC[i] = ok ? seq_row((const T*)a.C, d.g, b, sC, t)[(int64_t)grp * N + n] : (T)0;
+      const int e = tid + i * THREADS, n = e % NP < N ? e % NP : 0;
+      const int64_t at = tt + e / NP, t = at < t1 ? at : t1 - 1;
+      rB[i] = seq_row((const T*)a.B, d.g, b, sB, t)[(int64_t)grp * N + n];
+      if (MODE == 0) rC[i] = seq_row((const T*)a.C, d.g, b, sC, t)[(int64_t)grp * N + n];
     }
   };
   fetch(t0);
   for (int64_t tt = t0; tt < t1; tt += TL) {
     const int nt = t1 - tt < TL ? (int)(t1 - tt) : TL;
-    SeqVec<T> cu[NI], cz[NI];
+    Vec cu[NI], cz[NI];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int tl = et + i * (THREADS / NV);
+      const int tl = et + i * RPI;
       cu[i] = ru[i];
       if (MODE == 0) cz[i] = rz[i];
-      if (tl < TL) {
+      if (et < TL) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           A sig;
           const A dt = seq_softplus((A)rd[i].e[j] + bias[j], sig);
           Pair p;
-          p.dt = dt;
-          p.w = dt * (A)ru[i].e[j];
+          p.dt = tl < nt ? dt : (A)0;
+          p.w = tl < nt ? dt * (A)ru[i].e[j] : (A)0;
           pl[tl][ev * V + j] = p;
         }
       }
@@ -109,9 +110,10 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       const int e = tid + i * THREADS, tl = e / NP, n = e % NP;
-      if (tl < TL) {
-        Bl[tl][n / R].v[n % R] = (A)rB[i];
-        if (MODE == 0) Cl[tl][n / R].v[n % R] = (A)rC[i];
+      if (TL * NP % THREADS == 0 || tl < TL) {
+        const bool ok = n < N && tl < nt;
+        Bl[tl][n / R].v[n % R] = ok ? (A)rB[i] : (A)0;
+        if (MODE == 0) Cl[tl][n / R].v[n % R] = ok ? (A)rC[i] : (A)0;
       }
     }
     __syncthreads();
@@ -119,28 +121,31 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
     for (int tb = 0; tb < nt; tb += CK) {
       if (MODE == 0 && ckpt && live) {
         A* const c = ckpt + (tt + tb) / CK * ((int64_t)a.D * N);
+        if (N == NP) {
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-          if (k * R + r < N) c[r] = s[r];
+          for (int r = 0; r < R; ++r) c[r] = s[r];
+        } else {
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            if (k * R + r < N) c[r] = s[r];
+        }
       }
 #pragma unroll
       for (int i = 0; i < CK; ++i) {
-        const int t = tb + i;
-        if (t < nt) {
-          const Pair p = pl[t][ch];
-          const Quad B = Bl[t][k];
-          A acc = (A)0;
-          if (MODE == 1) sum += p.dt;
+        const int t = tb + i;                                     // steps behind the end change nothing
+        const Pair p = pl[t][ch];
+        const Quad B = Bl[t][k];
+        A acc = (A)0;
+        if (MODE == 1) sum += p.dt;
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            const A e = sizeof(A) == 4 ? (A)seq_exp2((float)(p.dt * Ar[r])) : seq_exp(p.dt * Ar[r]);
-            s[r] = e * s[r] + p.w * B.v[r];
-            if (MODE == 0) acc += s[r] * Cl[t][k].v[r];
-          }
-          if (MODE == 0) {
-            acc = seq_sum<K>(acc);
-            if (k == 0) pl[t][ch].dt = acc;
-          }
+        for (int r = 0; r < R; ++r) {
+          const A e = sizeof(A) == 4 ? (A)seq_exp2((float)(p.dt * Ar[r])) : seq_exp(p.dt * Ar[r]);
+          s[r] = e * s[r] + p.w * B.v[r];
+          if (MODE == 0) acc += s[r] * Cl[t][k].v[r];
+        }
+        if (MODE == 0) {
+          acc = seq_sum<K>(acc);
+          if (k == 0) pl[t][ch].dt = acc;
         }
       }
     }
@@ -148,20 +153,19 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
     if (MODE == 0) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int tl = et + i * (THREADS / NV);
-        if (tl < nt && eval > 0) {
-          SeqVec<T> o;
+        const int tl = et + i * RPI;
+        if (here && tl < nt) {
+          Vec o;
 #pragma unroll
           for (int j = 0; j < V; ++j) {
             A y = pl[tl][ev * V + j].dt + skip[j] * (A)cu[i].e[j];
             if (a.z) {
-              A comp;
               const A z = (A)cz[i].e[j];
-              y *= z * seq_sigmoid(z, comp);
+              y *= z * seq_sigmoid(z);
             }
             o.e[j] = (T)y;
           }
-          seq_store((T*)a.y + seq_row_index(d.g, b, tt + tl) * a.D + ech, o, eval, d.wout);
+          *(Vec*)((T*)a.y + seq_row_index(d.g, b, tt + tl) * a.D + ech) = o;
         }
       }
     }
@@ -181,9 +185,12 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
 
 template <typename T, int K, int CH>
 static hipError_t go(const SsmDev& d, int mode, hipStream_t s) {
-  const int64_t grid = d.nslot * d.a.G * d.ncb;
-  if (mode == 0) hipLaunchKernelGGL((ssm_fwd_kernel<T, K, CH, 0>), dim3((unsigned)grid), dim3(CH * K), 0, s, d);
-  else hipLaunchKernelGGL((ssm_fwd_kernel<T, K, CH, 1>), dim3((unsigned)grid), dim3(CH * K), 0, s, d);
+  constexpr int V = 16 / (int)sizeof(T);
+  const dim3 g((unsigned)d.nslot, (unsigned)(d.a.G * d.ncb)), t(CH * K);
+  if (mode == 0 && d.wide) hipLaunchKernelGGL((ssm_fwd_kernel<T, K, CH, 0, V>), g, t, 0, s, d);
+  else if (mode == 0) hipLaunchKernelGGL((ssm_fwd_kernel<T, K, CH, 0, 1>), g, t, 0, s, d);
+  else if (d.wide) hipLaunchKernelGGL((ssm_fwd_kernel<T, K, CH, 1, V>), g, t, 0, s, d);
+  else hipLaunchKernelGGL((ssm_fwd_kernel<T, K, CH, 1, 1>), g, t, 0, s, d);
   return hipGetLastError();
 }
 template <typename T>
