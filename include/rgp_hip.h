@@ -385,14 +385,15 @@ rgp_status rgp_rms_norm_backward(rgp_handle h, void* stream, const rgp_rms_norm*
 
 /* Global norm of n gradient tensors (host arrays ptr / numel / dtype of device pointers, element counts and types) and their clipping.
  * rgp_grad_sumsq: sumsq[0] = sum of all squares, in double whatever the types (a squared bf16 or float value never overflows there).
- * rgp_grad_clip: norm[0] = sqrt(sumsq[0]); every tensor is multiplied by max_norm / (norm + 1e-6) where that is below 1; otherwise, and
- * where the norm is not finite, the tensors stay as they are.  sumsq and norm may be the same address.  Between the two calls a
- * data-parallel caller adds the sums of the other ranks.  work: rgp_grad_workspace bytes.  The tensors must not overlap. */
+ * rgp_grad_clip: norm[0] = sqrt(sumsq[0]), or without sumsq (NULL) that of the tensors themselves; every tensor is multiplied by
+ * max_norm / (norm + 1e-6) where that is below 1; otherwise, and where the norm is not finite, the tensors stay as they are.  norm must not
+ * be sumsq.  Between the two calls a data-parallel caller adds the sums of the other ranks.  work: rgp_grad_workspace bytes (NULL where
+ * sumsq is given).  The tensors must not overlap. */
 int64_t    rgp_grad_workspace(int n, const int64_t* numel, const int32_t* dtype);
 rgp_status rgp_grad_sumsq(rgp_handle h, void* stream, int n, void* const* ptr, const int64_t* numel, const int32_t* dtype, double* sumsq,
                           void* work, int64_t work_bytes);
 rgp_status rgp_grad_clip(rgp_handle h, void* stream, int n, void* const* ptr, const int64_t* numel, const int32_t* dtype,
-                         const double* sumsq, double max_norm, double* norm);
+                         const double* sumsq, double max_norm, double* norm, void* work, int64_t work_bytes);
 
 /* ---- optimiser step on device (the outer SVI loop's Adam; positive parameters live in softplus space) -------- */
 /* x, m, v: n doubles of optimiser-space parameter and Adam moments; g: gradient w.r.t. the CONSTRAINED value p;

@@ -117,23 +117,21 @@ SYMBOLS = {
     'rgp_mlp_scan_backward': (C.c_int, [C.c_void_p, C.POINTER(MlpScan)]),
     'rgp_rnn_scan_forward': (C.c_int, [C.c_void_p, C.POINTER(RnnScan)]),
     'rgp_rnn_scan_backward': (C.c_int, [C.c_void_p, C.POINTER(RnnScan)]),
-    'rgp_ssm_scan_states_bytes': (C.c_int64, [C.POINTER(SsmScan)]),
-    'rgp_ssm_scan_workspace': (C.c_int64, [C.POINTER(SsmScan), C.c_int]),
-    'rgp_ssm_scan_forward': (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(SsmScan)]),
-    'rgp_ssm_scan_backward': (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(SsmScan)]),
-    'rgp_ssm_scan_step': (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(SsmScan)]),
-    'rgp_ssm_conv_workspace': (C.c_int64, [C.POINTER(SsmConv), C.c_int]),
-    'rgp_ssm_conv_forward': (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(SsmConv)]),
-    'rgp_ssm_conv_backward': (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(SsmConv)]),
-    'rgp_ssm_conv_step': (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(SsmConv)]),
-    'rgp_rms_norm_workspace': (C.c_int64, [C.POINTER(RmsNorm), C.c_int]),
-    'rgp_rms_norm_forward': (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(RmsNorm)]),
-    'rgp_rms_norm_backward': (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(RmsNorm)]),
-    'rgp_grad_workspace': (C.c_int64, [C.c_int, C.POINTER(C.c_int64), C.POINTER(C.c_int32)]),
-    'rgp_grad_sumsq': (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_int64), C.POINTER(C.c_int32), c_dp,
-                                 C.c_void_p, C.c_int64]),
-    'rgp_grad_clip': (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_int64), C.POINTER(C.c_int32), c_dp,
-                                C.c_double, c_dp]),
+    'rgp_ssm_scan_states_bytes': (C.c_int64, [C.c_void_p]),
+    'rgp_ssm_scan_workspace': (C.c_int64, [C.c_void_p, C.c_int]),
+    'rgp_ssm_scan_forward': (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    'rgp_ssm_scan_backward': (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    'rgp_ssm_scan_step': (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    'rgp_ssm_conv_workspace': (C.c_int64, [C.c_void_p, C.c_int]),
+    'rgp_ssm_conv_forward': (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    'rgp_ssm_conv_backward': (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    'rgp_ssm_conv_step': (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    'rgp_rms_norm_workspace': (C.c_int64, [C.c_void_p, C.c_int]),
+    'rgp_rms_norm_forward': (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    'rgp_rms_norm_backward': (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    'rgp_grad_workspace': (C.c_int64, [C.c_int, C.c_void_p, C.c_void_p]),
+    'rgp_grad_sumsq': (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, c_dp, C.c_void_p, C.c_int64]),
+    'rgp_grad_clip': (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, c_dp, C.c_double, c_dp, C.c_void_p, C.c_int64]),
 }
 PREPARE_CHAIN_ONLY, PREPARE_ROWS_ONLY, PREPARE_ROWS_EARLY = 1, 2, 4          # rgp_layer_in.reserved for rgp_layer_prepare
 

@@ -353,18 +353,24 @@ extern "C" rgp_status rgp_rms_norm_backward(rgp_handle h, void* stream, const rg
 
 // ---- global gradient norm and clipping ---------------------------------------------------------------------------------------------------------
 // The tensors of a launch travel in the kernel's arguments (GT of them), so nothing is uploaded and a captured launch keeps its table.
-// A workgroup takes one piece of GP bytes of one tensor; its sum of squares, in double, goes to its own place, and the pieces are added in
-// a fixed order.
+// A workgroup takes one piece of one tensor -- 64 KB, or 8 KB where all of them are little and a longer walk would only add latency; its sum
+// of squares, in double, goes to its own place, and the places are added in a fixed order: by a workgroup of their own, or, up to GFEW of
+// them, by every workgroup of the clipping (which saves a launch where launches are what counts).
 #define GT 128
-#define GP 65536
+#define GFEW 1024
 struct GradTable {
   void* p[GT];
   int64_t n[GT];
   int first[GT + 1];             // first piece of each tensor, counted inside the launch
   uint8_t dt[GT];
-  int count;
+  int count, bytes;              // tensors, bytes of a piece
 };
-static inline int64_t grad_pieces(int64_t n, int dt) { return (n * seq_dtype_bytes(dt) + GP - 1) / GP; }
+static inline int grad_piece_bytes(int n, const int64_t* numel, const int32_t* dtype) {
+  int64_t all = 0;
+  for (int i = 0; i < n; ++i) all += numel[i] * seq_dtype_bytes(dtype[i]);
+  return all <= (4 << 20) ? 8192 : 65536;
+}
+static inline int64_t grad_pieces(int64_t n, int dt, int bytes) { return (n * seq_dtype_bytes(dt) + bytes - 1) / bytes; }
 
 static __device__ __forceinline__ int grad_find(const GradTable& t, int piece) {
   int lo = 0, hi = t.count - 1;
@@ -403,7 +409,7 @@ static __global__ void __launch_bounds__(256) grad_sumsq_kernel(GradTable t, dou
   __shared__ double sh[16];
   const int i = grad_find(t, blockIdx.x);
   const int es = t.dt[i] == RGP_F64 ? 8 : t.dt[i] == RGP_F32 ? 4 : 2;
-  const int64_t per = GP / es, o = (int64_t)((int)blockIdx.x - t.first[i]) * per, n = t.n[i] - o < per ? t.n[i] - o : per;
+  const int64_t per = t.bytes / es, o = (int64_t)((int)blockIdx.x - t.first[i]) * per, n = t.n[i] - o < per ? t.n[i] - o : per;
   double s;
   switch (t.dt[i]) {
     case RGP_F64: s = grad_sum((double*)t.p[i] + o, n); break;
@@ -414,18 +420,22 @@ static __global__ void __launch_bounds__(256) grad_sumsq_kernel(GradTable t, dou
   s = block_sum(s, sh);
   if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
-static __global__ void __launch_bounds__(1024) grad_total_kernel(const double* part, int64_t n, double* out) {
-  __shared__ double sh[16];
+static __device__ __forceinline__ double grad_add(const double* part, int64_t n, double* sh) {
+  const int step = blockDim.x;
   double s0 = 0.0, s1 = 0.0, s2 = 0.0, s3 = 0.0;
   int64_t i = threadIdx.x;
-  for (; i + 1024 * 3 < n; i += 4096) {
+  for (; i + 3 * step < n; i += 4 * step) {
     s0 += part[i];
-    s1 += part[i + 1024];
-    s2 += part[i + 2048];
-    s3 += part[i + 1024 * 3];
+    s1 += part[i + step];
+    s2 += part[i + 2 * step];
+    s3 += part[i + 3 * step];
   }
-  for (; i < n; i += 1024) s0 += part[i];
-  const double s = block_sum((s0 + s1) + (s2 + s3), sh);
+  for (; i < n; i += step) s0 += part[i];
+  return block_sum((s0 + s1) + (s2 + s3), sh);
+}
+static __global__ void __launch_bounds__(1024) grad_total_kernel(const double* part, int64_t n, double* out) {
+  __shared__ double sh[16];
+  const double s = grad_add(part, n, sh);
   if (threadIdx.x == 0) out[0] = s;
 }
 template <typename T>
@@ -439,13 +449,16 @@ static __device__ __forceinline__ void grad_scale(T* p, int64_t n, double c) {
     seq_store(q, v, k, wide);
   });
 }
-// walks tensors and pieces from the last to the first: what the norm read last is still in the memory-side cache
-static __global__ void __launch_bounds__(256) grad_clip_kernel(GradTable t, const double* sumsq, double max_norm) {
-  const double norm = sqrt(sumsq[0]), c = max_norm / (norm + 1e-6);
-  if (!(c < 1.0) || !(norm < 1.7976931348623157e308)) return;           // nothing to clip, or a norm that is no number
+// sum: nsum places to add (1: the sum itself).  Walks tensors and pieces from the last to the first: what the norm read last is still in the
+// memory-side cache.  The first workgroup of the launch that says so writes the norm.
+static __global__ void __launch_bounds__(256) grad_clip_kernel(GradTable t, const double* sum, int nsum, double max_norm, double* norm_out) {
+  __shared__ double sh[16];
+  const double norm = sqrt(nsum == 1 ? sum[0] : grad_add(sum, nsum, sh)), c = max_norm / (norm + 1e-6);
+  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = norm;
+  if (t.count == 0 || !(c < 1.0) || !(norm < 1.7976931348623157e308)) return;           // nothing to clip, or a norm that is no number
   const int i = grad_find(t, blockIdx.x);
   const int es = t.dt[i] == RGP_F64 ? 8 : t.dt[i] == RGP_F32 ? 4 : 2;
-  const int64_t per = GP / es, o = (int64_t)(t.first[i + 1] - 1 - (int)blockIdx.x) * per, n = t.n[i] - o < per ? t.n[i] - o : per;
+  const int64_t per = t.bytes / es, o = (int64_t)(t.first[i + 1] - 1 - (int)blockIdx.x) * per, n = t.n[i] - o < per ? t.n[i] - o : per;
   switch (t.dt[i]) {
     case RGP_F64: grad_scale((double*)t.p[i] + o, n, c); break;
     case RGP_F32: grad_scale((float*)t.p[i] + o, n, c); break;
@@ -453,7 +466,6 @@ static __global__ void __launch_bounds__(256) grad_clip_kernel(GradTable t, cons
     default: grad_scale((_Float16*)t.p[i] + o, n, c); break;
   }
 }
-static __global__ void grad_norm_kernel(const double* sumsq, double* norm) { norm[0] = sqrt(sumsq[0]); }
 
 static const char* grad_bad(int n, const int64_t* numel, const int32_t* dtype) {
   if (n < 0 || (n > 0 && (!numel || !dtype))) return "null arguments";
@@ -465,14 +477,16 @@ static const char* grad_bad(int n, const int64_t* numel, const int32_t* dtype) {
 }
 extern "C" int64_t rgp_grad_workspace(int n, const int64_t* numel, const int32_t* dtype) {
   if (grad_bad(n, numel, dtype)) return -1;
+  const int bytes = grad_piece_bytes(n, numel, dtype);
   int64_t p = 0;
-  for (int i = 0; i < n; ++i) p += grad_pieces(numel[i], dtype[i]);
+  for (int i = 0; i < n; ++i) p += grad_pieces(numel[i], dtype[i], bytes);
   return (p < 1 ? 1 : p) * (int64_t)sizeof(double);
 }
 // calls f(table, pieces, pieces before) for groups of up to GT tensors; back: from the last tensor to the first
 template <typename F>
 static rgp_status grad_tables(rgp_handle h, int n, void* const* ptr, const int64_t* numel, const int32_t* dtype, bool back, F f) {
   GradTable t;
+  t.bytes = grad_piece_bytes(n, numel, dtype);
   int64_t before = 0;
   for (int k = 0; k < n;) {                              // a group: the next GT tensors that have elements, fewer where the grid would grow too long
     int64_t pieces = 0;
@@ -480,7 +494,7 @@ static rgp_status grad_tables(rgp_handle h, int n, void* const* ptr, const int64
     for (; k < n && t.count < GT; ++k) {
       const int i = back ? n - 1 - k : k;
       if (numel[i] == 0) continue;
-      const int64_t add = grad_pieces(numel[i], dtype[i]);
+      const int64_t add = grad_pieces(numel[i], dtype[i], t.bytes);
       if (add > 8000000) return rgp_fail(h, RGP_ERR_BAD_ARG, "gradient norm: a tensor of more than 500 GB");
       if (pieces + add > 8000000) break;
       t.p[t.count] = ptr[i];
@@ -504,38 +518,61 @@ static rgp_status grad_check(rgp_handle h, int n, void* const* ptr, const int64_
     if (numel[i] > 0 && (!ptr[i] || (uintptr_t)ptr[i] % seq_dtype_bytes(dtype[i]))) return rgp_fail(h, RGP_ERR_BAD_ARG, "gradient norm: a null or misaligned tensor");
   return RGP_OK;
 }
+// the pieces' sums in `work`; their number
+static rgp_status grad_sums(rgp_handle h, hipStream_t s, int n, void* const* ptr, const int64_t* numel, const int32_t* dtype, void* work,
+                            int64_t work_bytes, int64_t& total) {
+  if (!work || ((uintptr_t)work & 7) || rgp_grad_workspace(n, numel, dtype) > work_bytes)
+    return rgp_fail(h, RGP_ERR_WORKSPACE, "gradient norm: work buffer too small");
+  total = 0;
+  return grad_tables(h, n, ptr, numel, dtype, false, [&](const GradTable& t, unsigned pieces, int64_t before) {
+    hipLaunchKernelGGL(grad_sumsq_kernel, dim3(pieces), dim3(256), 0, s, t, (double*)work + before);
+    total = before + pieces;
+    return seq_launched(h, "gradient norm");
+  });
+}
 extern "C" rgp_status rgp_grad_sumsq(rgp_handle h, void* stream, int n, void* const* ptr, const int64_t* numel, const int32_t* dtype,
                                      double* sumsq, void* work, int64_t work_bytes) {
   SEQ_ENTRY(h, "gradient norm", {
     rgp_status st = grad_check(h, n, ptr, numel, dtype);
     if (st) return st;
-    if (!sumsq || !work || ((uintptr_t)work & 7) || rgp_grad_workspace(n, numel, dtype) > work_bytes)
-      return rgp_fail(h, RGP_ERR_WORKSPACE, "gradient norm: work buffer too small");
-    const hipStream_t s = (hipStream_t)stream;
+    if (!sumsq) return rgp_fail(h, RGP_ERR_BAD_ARG, "gradient norm: sumsq is required");
     int64_t total = 0;
-    st = grad_tables(h, n, ptr, numel, dtype, false, [&](const GradTable& t, unsigned pieces, int64_t before) {
-      hipLaunchKernelGGL(grad_sumsq_kernel, dim3(pieces), dim3(256), 0, s, t, (double*)work + before);
-      total = before + pieces;
-      return seq_launched(h, "gradient norm");
-    });
+    st = grad_sums(h, (hipStream_t)stream, n, ptr, numel, dtype, work, work_bytes, total);
     if (st) return st;
-    hipLaunchKernelGGL(grad_total_kernel, dim3(1), dim3(1024), 0, s, (const double*)work, total, sumsq);
+    hipLaunchKernelGGL(grad_total_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, (const double*)work, total, sumsq);
     return seq_launched(h, "gradient norm");
   })
 }
 extern "C" rgp_status rgp_grad_clip(rgp_handle h, void* stream, int n, void* const* ptr, const int64_t* numel, const int32_t* dtype,
-                                    const double* sumsq, double max_norm, double* norm) {
+                                    const double* sumsq, double max_norm, double* norm, void* work, int64_t work_bytes) {
   SEQ_ENTRY(h, "gradient clip", {
     rgp_status st = grad_check(h, n, ptr, numel, dtype);
     if (st) return st;
-    if (!sumsq || !norm || !(max_norm > 0.0)) return rgp_fail(h, RGP_ERR_BAD_ARG, "gradient clip: sumsq, norm and a positive max_norm are required");
+    if (!norm || norm == sumsq || !(max_norm > 0.0)) return rgp_fail(h, RGP_ERR_BAD_ARG, "gradient clip: norm, apart from sumsq, and a positive max_norm are required");
     const hipStream_t s = (hipStream_t)stream;
+    const double* sum = sumsq;
+    int64_t nsum = 1;
+    if (!sumsq) {
+      st = grad_sums(h, s, n, ptr, numel, dtype, work, work_bytes, nsum);
+      if (st) return st;
+      sum = (const double*)work;
+      if (nsum > GFEW || nsum == 0) {                    // into the first place, which only this workgroup reads
+        hipLaunchKernelGGL(grad_total_kernel, dim3(1), dim3(1024), 0, s, (const double*)work, nsum, (double*)work);
+        nsum = 1;
+        st = seq_launched(h, "gradient clip");
+        if (st) return st;
+      }
+    }
+    bool first = true;
     st = grad_tables(h, n, ptr, numel, dtype, true, [&](const GradTable& t, unsigned pieces, int64_t) {
-      hipLaunchKernelGGL(grad_clip_kernel, dim3(pieces), dim3(256), 0, s, t, sumsq, max_norm);
+      hipLaunchKernelGGL(grad_clip_kernel, dim3(pieces), dim3(256), 0, s, t, sum, (int)nsum, max_norm, first ? norm : nullptr);
+      first = false;
       return seq_launched(h, "gradient clip");
     });
-    if (st) return st;
-    hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(1), 0, s, sumsq, norm);
+    if (st || !first) return st;
+    GradTable none;                                      // no elements at all: the norm alone
+    none.count = 0;
+    hipLaunchKernelGGL(grad_clip_kernel, dim3(1), dim3(256), 0, s, none, sum, (int)nsum, max_norm, norm);
     return seq_launched(h, "gradient clip");
   })
 }

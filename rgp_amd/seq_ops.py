@@ -13,9 +13,9 @@ stream of the handle's device, allocates through torch (so it can be captured in
 same bits every time.  Wrong arguments raise RgpError (RGP_ERR_BAD_ARG) before anything is launched.
 
 A captured backward pass needs leaves that no eager graph holds at that time: take the gradients with torch.autograd.grad inside the
-captured region, on a forward pass of the same region."""
-import ctypes as C
+captured region, on a forward pass of the same region.  There are no second derivatives: a backward pass with create_graph=True is refused."""
 import math
+import struct
 
 import torch
 
@@ -34,21 +34,37 @@ def _acc(dtype):
 
 
 def _stream(handle):
-    return C.c_void_p(torch.cuda.current_stream(handle.device).cuda_stream)
+    return torch._C._cuda_getCurrentRawStream(handle.device.index)
 
 
-def _call(handle, fn, a):
-    st = fn(handle.h, _stream(handle), C.byref(a))
+# The argument structs of include/rgp_hip.h as one pack each (a ctypes struct costs several microseconds to fill, as much as a short kernel
+# runs); the last two fields, work and work_bytes, are packed apart because their size is asked for with the others.
+_SCAN, _CONV, _RMS = struct.Struct('@6i3q6Q12q16Q'), struct.Struct('@6i3q2Q4q9Q'), struct.Struct('@2i2qd2Q4q8Q')
+_WORK, _NO_WORK = struct.Struct('@Qq'), b'\0' * 16
+
+
+def _call(handle, fn, head, tail=_NO_WORK):
+    st = fn(handle.h, _stream(handle), head + tail)
     if st != 0:
         handle._check(st)
 
 
-def _work(handle, nbytes):
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=handle.device)
+def _new_work(handle, query, head, backward):
+    """The work buffer of a call and its fields of the struct."""
+    n = query(head + _NO_WORK, backward)
+    if n <= 0:
+        return None, _NO_WORK
+    w = torch.empty(n, dtype=torch.uint8, device=handle.device)
+    return w, _WORK.pack(w.data_ptr(), n)
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
+
+
+def _once():
+    if torch.is_grad_enabled():
+        raise RuntimeError('the sequence operators have no second derivatives (create_graph=True)')
 
 
 def _overlaps(t):
@@ -78,28 +94,27 @@ class SeqTable(object):
         self.off = torch.tensor(off, dtype=torch.int64).to(handle.device)
 
 
-def _rows(name, t, like=None, lead=None, tail=1):
-    """Leading shape of an activation after its checks."""
+def _rows(name, t, like, lead):
+    """Checks an activation's type, place and leading shape."""
     if not isinstance(t, torch.Tensor):
         _bad('%s must be a device tensor' % name)
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+    if t.dtype is not like.dtype or t.device != like.device:
         _bad('%s is %s on %s, %s on %s expected' % (name, t.dtype, t.device, like.dtype, like.device))
-    if lead is not None and tuple(t.shape[:len(lead)]) != tuple(lead):
+    if t.shape[:len(lead)] != lead:
         _bad('%s has shape %s, leading dimensions %s expected' % (name, tuple(t.shape), tuple(lead)))
-    return t
 
 
 def _inner(t, dims):
     """The tensor with its last ``dims`` dimensions contiguous (a copy only where they are not)."""
-    want = 1
+    shape, stride, want = t.shape, t.stride(), 1
     for i in range(1, dims + 1):
-        if t.shape[-i] > 1 and t.stride(-i) != want:
+        if stride[-i] != want and shape[-i] > 1:
             return t.contiguous()
-        want *= t.shape[-i]
+        want *= shape[-i]
     return t
 
 
-def _geometry(handle, x, seqs, what):
+def _geometry(handle, x, seqs, what, step=False):
     """(lead, n_seq, T, rows, max_len, off) of a (T, batch, D) or packed (rows, D) activation."""
     if not isinstance(x, torch.Tensor):
         _bad('%s must be a device tensor' % what)
@@ -107,25 +122,30 @@ def _geometry(handle, x, seqs, what):
         _bad('%s must be float64, float32, bfloat16 or float16, not %s' % (what, x.dtype))
     if x.device != handle.device:
         _bad('%s is on %s, the handle on %s' % (what, x.device, handle.device))
+    if step:                                     # (batch, D): one row of every sequence
+        if x.numel() == 0:
+            _bad('%s is empty: shape %s' % (what, tuple(x.shape)))
+        return x.shape[:1], x.shape[0], 1, x.shape[0], 1, None
     if seqs is None:
         if x.dim() != 3:
             _bad('%s must be (T, batch, features); packed rows need a SeqTable' % what)
         T, n = x.shape[0], x.shape[1]
         if T < 1 or n < 1 or x.shape[2] < 1:
             _bad('%s is empty: shape %s' % (what, tuple(x.shape)))
-        return (T, n), n, T, T * n, T, None
+        return x.shape[:2], n, T, T * n, T, None
     if x.dim() != 2 or x.shape[1] < 1:
         _bad('%s must be packed rows (rows, features) with a SeqTable' % what)
     if seqs.device != x.device:
         _bad('the sequence table is on %s, %s on %s' % (seqs.device, what, x.device))
     if seqs.rows != x.shape[0]:
         _bad('%s has %d rows, the sequence table %d' % (what, x.shape[0], seqs.rows))
-    return (x.shape[0],), seqs.n_seq, 0, seqs.rows, seqs.max_len, seqs.off
+    return x.shape[:1], seqs.n_seq, 0, seqs.rows, seqs.max_len, seqs.off
 
 
 def _strides(t, packed):
     """Element strides of (step, sequence)."""
-    return (t.stride(0), 0) if packed else (t.stride(0), t.stride(1))
+    st = t.stride()
+    return (st[0], 0) if packed else (st[0], st[1])
 
 
 def _param(name, t, shape, x, optional=False):
@@ -135,16 +155,16 @@ def _param(name, t, shape, x, optional=False):
         _bad('%s is required' % name)
     if not isinstance(t, torch.Tensor) or t.device != x.device:
         _bad('%s must be a tensor on %s' % (name, x.device))
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         _bad('%s has shape %s, %s expected' % (name, tuple(t.shape), tuple(shape)))
-    if t.dtype != _acc(x.dtype):
+    if t.dtype is not _acc(x.dtype):
         _bad('%s is %s: parameters and states are %s for %s activations' % (name, t.dtype, _acc(x.dtype), x.dtype))
     return t if t.is_contiguous() else t.contiguous()
 
 
 def _state(name, t, shape, dtype, x):
     """A state that is updated in place."""
-    if not isinstance(t, torch.Tensor) or t.device != x.device or tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.device != x.device or t.shape != shape or t.dtype is not dtype or not t.is_contiguous():
         _bad('%s must be a contiguous %s tensor of shape %s on %s' % (name, dtype, tuple(shape), x.device))
     if t.requires_grad:
         _bad('%s is updated in place and takes no gradient' % name)
@@ -157,24 +177,24 @@ def _no_grad_state(name, t):
 
 
 # ---------------------------------------------------------------------------------------------------------------------- convolution
-def _conv_args(x, w, bias, geo, reverse):
-    lead, n_seq, T, rows, max_len, off = geo
-    a = _lib.SsmConv()
-    a.dtype, a.n_seq, a.D, a.W, a.reverse = _DTYPES[x.dtype], n_seq, x.shape[-1], w.shape[1], 1 if reverse else 0
-    a.T, a.rows, a.max_len, a.off = T, rows, max_len, _ptr(off)
-    a.x, a.w, a.bias = x.data_ptr(), w.data_ptr(), _ptr(bias)
-    a.x_st, a.x_sb = _strides(x, off is not None)
-    return a
+def _conv_head(x, w, bias, geo, reverse, init=0, v=0, last=0, gv=0, gv_st=(0, 0), gx=0, gw=0, gb=0):
+    _, n_seq, T, rows, max_len, off = geo
+    st = _strides(x, off is not None)
+    return _CONV.pack(_DTYPES[x.dtype], n_seq, x.shape[-1], w.shape[1], reverse, 0, T, rows, max_len, _ptr(off), x.data_ptr(), st[0], st[1], gv_st[0],
+                      gv_st[1], w.data_ptr(), _ptr(bias), init, v, last, gv, gx, gw, gb)
+
+
+def _conv_forward(handle, x, w, bias, init, geo, reverse, want_last):
+    v = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    last = torch.empty(geo[1], w.shape[1] - 1, x.shape[-1], dtype=x.dtype, device=x.device) if want_last else None
+    _call(handle, handle.lib.rgp_ssm_conv_forward, _conv_head(x, w, bias, geo, reverse, _ptr(init), v.data_ptr(), _ptr(last)))
+    return v, last
 
 
 class _ConvFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, handle, x, w, bias, init, geo, reverse, want_last):
-        v = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        last = torch.empty(geo[1], w.shape[1] - 1, x.shape[-1], dtype=x.dtype, device=x.device) if want_last else None
-        a = _conv_args(x, w, bias, geo, reverse)
-        a.init, a.v, a.last = _ptr(init), v.data_ptr(), _ptr(last)
-        _call(handle, handle.lib.rgp_ssm_conv_forward, a)
+        v, last = _conv_forward(handle, x, w, bias, init, geo, reverse, want_last)
         ctx.handle, ctx.geo, ctx.reverse = handle, geo, reverse
         ctx.save_for_backward(x, w, bias, init)
         ctx.set_materialize_grads(False)
@@ -183,22 +203,28 @@ class _ConvFn(torch.autograd.Function):
         return v, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gv, _):
+        _once()
         if gv is None:
             return (None,) * 8
         x, w, bias, init = ctx.saved_tensors
         handle = ctx.handle
         gv = _inner(gv, 1)
-        a = _conv_args(x, w, bias, ctx.geo, ctx.reverse)
-        a.gv_st, a.gv_sb = _strides(gv, ctx.geo[5] is not None)
-        gx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        gw = torch.empty_like(w)
+        gx, gw = torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty_like(w)
         gb = torch.empty_like(bias) if bias is not None else None
-        work = _work(handle, handle.lib.rgp_ssm_conv_workspace(C.byref(a), 1))
-        a.init, a.gv, a.gx, a.gw, a.gbias, a.work, a.work_bytes = _ptr(init), gv.data_ptr(), gx.data_ptr(), gw.data_ptr(), _ptr(gb), work.data_ptr(), work.numel()
-        _call(handle, handle.lib.rgp_ssm_conv_backward, a)
+        head = _conv_head(x, w, bias, ctx.geo, ctx.reverse, _ptr(init), 0, 0, gv.data_ptr(), _strides(gv, ctx.geo[5] is not None), gx.data_ptr(),
+                          gw.data_ptr(), _ptr(gb))
+        work, tail = _new_work(handle, handle.lib.rgp_ssm_conv_workspace, head, 1)
+        _call(handle, handle.lib.rgp_ssm_conv_backward, head, tail)
         return None, gx, gw, gb, None, None, None, None
+
+
+def _wants_grad(*ts):
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def ssm_conv(handle, x, weight, bias=None, seqs=None, init=None, reverse=False, return_state=False):
@@ -215,10 +241,12 @@ def ssm_conv(handle, x, weight, bias=None, seqs=None, init=None, reverse=False, 
     b = _param('bias', bias, (D,), x, optional=True)
     if init is not None:
         _no_grad_state('init', init)
-        if tuple(init.shape) != (geo[1], w.shape[1] - 1, D) or init.dtype != x.dtype or init.device != x.device:
+        if init.shape != (geo[1], w.shape[1] - 1, D) or init.dtype is not x.dtype or init.device != x.device:
             _bad('init must be %s of shape %s on %s' % (x.dtype, (geo[1], w.shape[1] - 1, D), x.device))
         init = init.contiguous()
-    v, last = _ConvFn.apply(handle, _inner(x, 1), w, b, init, geo, bool(reverse), bool(return_state))
+    x = _inner(x, 1)
+    run = _ConvFn.apply if _wants_grad(x, w, b) else _conv_forward
+    v, last = run(handle, x, w, b, init, geo, bool(reverse), bool(return_state))
     return (v, last) if return_state else v
 
 
@@ -226,50 +254,50 @@ def ssm_conv_step(handle, x, weight, bias, state):
     """One step of ``ssm_conv``: x (batch, D), state (batch, W - 1, D) of x's type, updated in place.  No gradients."""
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         _bad('x must be (batch, D)')
-    x3 = x.detach().unsqueeze(0)
-    geo = _geometry(handle, x3, None, 'x')
+    geo = _geometry(handle, x, None, 'x', step=True)
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not 2 <= weight.shape[1] <= 8:
         _bad('weight must be (D, W) with 2 to 8 taps')
     D = x.shape[1]
     w, b = _param('weight', weight, (D, weight.shape[1]), x), _param('bias', bias, (D,), x, optional=True)
     _state('state', state, (x.shape[0], weight.shape[1] - 1, D), x.dtype, x)
-    x3 = _inner(x3, 1)
-    v = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    a = _conv_args(x3, w, b, geo, False)
-    a.init = a.last = state.data_ptr()
-    a.v = v.data_ptr()
-    _call(handle, handle.lib.rgp_ssm_conv_step, a)
+    x = _inner(x, 1)
+    v, st = torch.empty(x.shape, dtype=x.dtype, device=x.device), state.data_ptr()
+    _call(handle, handle.lib.rgp_ssm_conv_step, _CONV.pack(_DTYPES[x.dtype], x.shape[0], D, w.shape[1], 0, 0, 1, x.shape[0], 1, 0, x.data_ptr(), 0,
+                                                          x.stride(0), 0, 0, w.data_ptr(), _ptr(b), st, v.data_ptr(), st, 0, 0, 0, 0))
     return v
 
 
 # ---------------------------------------------------------------------------------------------------------------------- scan
-def _scan_args(u, delta, A, B, Cm, skip, z, bias, geo, reverse):
-    lead, n_seq, T, rows, max_len, off = geo
+def _scan_head(ops, geo, reverse, init=0, y=0, last=0, states=0, gy=0, gy_st=(0, 0), grads=(0,) * 8):
+    u, delta, A, B, Cm, skip, z, bias = ops
+    _, n_seq, T, rows, max_len, off = geo
     packed = off is not None
-    a = _lib.SsmScan()
-    a.dtype, a.n_seq, a.D, a.N, a.G, a.reverse = _DTYPES[u.dtype], n_seq, u.shape[-1], B.shape[-1], B.shape[-2], 1 if reverse else 0
-    a.T, a.rows, a.max_len, a.off = T, rows, max_len, _ptr(off)
-    a.u, a.delta, a.z, a.B, a.C = u.data_ptr(), delta.data_ptr(), _ptr(z), B.data_ptr(), Cm.data_ptr()
-    a.u_st, a.u_sb = _strides(u, packed)
-    a.delta_st, a.delta_sb = _strides(delta, packed)
-    if z is not None:
-        a.z_st, a.z_sb = _strides(z, packed)
-    a.B_st, a.B_sb = _strides(B, packed)
-    a.C_st, a.C_sb = _strides(Cm, packed)
-    a.A, a.skip, a.bias = A.data_ptr(), _ptr(skip), _ptr(bias)
-    return a
+    su, sd, sB, sC = _strides(u, packed), _strides(delta, packed), _strides(B, packed), _strides(Cm, packed)
+    sz = _strides(z, packed) if z is not None else (0, 0)
+    gu, gdelta, gA, gB, gC, gskip, gz, gbias = grads
+    return _SCAN.pack(_DTYPES[u.dtype], n_seq, u.shape[-1], B.shape[-1], B.shape[-2], reverse, T, rows, max_len, _ptr(off), u.data_ptr(),
+                      delta.data_ptr(), _ptr(z), B.data_ptr(), Cm.data_ptr(), su[0], su[1], sd[0], sd[1], sz[0], sz[1], sB[0], sB[1], sC[0], sC[1],
+                      gy_st[0], gy_st[1], A.data_ptr(), _ptr(skip), _ptr(bias), init, y, last, states, gy, gu, gdelta, gz, gB, gC, gA, gskip, gbias)
+
+
+def _scan_forward(handle, u, delta, A, B, Cm, skip, z, bias, init, geo, reverse, want_last, train=False):
+    ops = (u, delta, A, B, Cm, skip, z, bias)
+    y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
+    last = torch.empty(geo[1], u.shape[-1], A.shape[1], dtype=A.dtype, device=u.device) if want_last else None
+    states = None
+    if train:
+        n = handle.lib.rgp_ssm_scan_states_bytes(_scan_head(ops, geo, reverse) + _NO_WORK)
+        states = torch.empty(n, dtype=torch.uint8, device=u.device)
+    head = _scan_head(ops, geo, reverse, _ptr(init), y.data_ptr(), _ptr(last), _ptr(states))
+    work, tail = _new_work(handle, handle.lib.rgp_ssm_scan_workspace, head, 0)
+    _call(handle, handle.lib.rgp_ssm_scan_forward, head, tail)
+    return (y, last, states) if train else (y, last)
 
 
 class _ScanFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, handle, u, delta, A, B, Cm, skip, z, bias, init, geo, reverse, want_last, train):
-        y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
-        last = torch.empty(geo[1], u.shape[-1], A.shape[1], dtype=A.dtype, device=u.device) if want_last else None
-        a = _scan_args(u, delta, A, B, Cm, skip, z, bias, geo, reverse)
-        states = _work(handle, handle.lib.rgp_ssm_scan_states_bytes(C.byref(a))) if train else None
-        work = _work(handle, handle.lib.rgp_ssm_scan_workspace(C.byref(a), 0))
-        a.init, a.y, a.last, a.states, a.work, a.work_bytes = _ptr(init), y.data_ptr(), _ptr(last), _ptr(states), work.data_ptr(), work.numel()
-        _call(handle, handle.lib.rgp_ssm_scan_forward, a)
+    def forward(ctx, handle, u, delta, A, B, Cm, skip, z, bias, init, geo, reverse, want_last):
+        y, last, states = _scan_forward(handle, u, delta, A, B, Cm, skip, z, bias, init, geo, reverse, want_last, True)
         ctx.handle, ctx.geo, ctx.reverse = handle, geo, reverse
         ctx.save_for_backward(u, delta, A, B, Cm, skip, z, bias, states)
         ctx.set_materialize_grads(False)
@@ -278,22 +306,19 @@ class _ScanFn(torch.autograd.Function):
         return y, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gy, _):
+        _once()
         if gy is None:
-            return (None,) * 14
-        u, delta, A, B, Cm, skip, z, bias, states = ctx.saved_tensors
-        handle = ctx.handle
+            return (None,) * 13
+        saved = ctx.saved_tensors
+        ops, states, handle = saved[:8], saved[8], ctx.handle
         gy = _inner(gy, 1)
-        new = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)      # noqa: E731
-        gu, gdelta, gA, gB, gC, gskip, gz, gbias = (new(t) for t in (u, delta, A, B, Cm, skip, z, bias))
-        a = _scan_args(u, delta, A, B, Cm, skip, z, bias, ctx.geo, ctx.reverse)
-        a.gy_st, a.gy_sb = _strides(gy, ctx.geo[5] is not None)
-        work = _work(handle, handle.lib.rgp_ssm_scan_workspace(C.byref(a), 1))
-        a.states, a.gy, a.gu, a.gdelta, a.gz, a.gB, a.gC = states.data_ptr(), gy.data_ptr(), gu.data_ptr(), gdelta.data_ptr(), _ptr(gz), gB.data_ptr(), gC.data_ptr()
-        a.gA, a.gskip, a.gbias, a.work, a.work_bytes = gA.data_ptr(), _ptr(gskip), _ptr(gbias), work.data_ptr(), work.numel()
-        _call(handle, handle.lib.rgp_ssm_scan_backward, a)
-        return None, gu, gdelta, gA, gB, gC, gskip, gz, gbias, None, None, None, None, None
+        grads = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in ops]
+        head = _scan_head(ops, ctx.geo, ctx.reverse, states=states.data_ptr(), gy=gy.data_ptr(), gy_st=_strides(gy, ctx.geo[5] is not None),
+                          grads=[_ptr(t) for t in grads])
+        work, tail = _new_work(handle, handle.lib.rgp_ssm_scan_workspace, head, 1)
+        _call(handle, handle.lib.rgp_ssm_scan_backward, head, tail)
+        return (None, *grads, None, None, None, None)
 
 
 def _scan_check(u, delta, A, B, Cm, D, z, delta_bias, lead):
@@ -302,7 +327,7 @@ def _scan_check(u, delta, A, B, Cm, D, z, delta_bias, lead):
     for name, t in (('delta', delta), ('z', z)):
         if t is not None:
             _rows(name, t, u, lead)
-            if t.dim() != nd + 1 or t.shape[-1] != n:
+            if t.shape != u.shape:
                 _bad('%s has shape %s, %s expected' % (name, tuple(t.shape), tuple(u.shape)))
     if delta is None:
         _bad('delta is required')
@@ -335,8 +360,8 @@ def ssm_scan(handle, u, delta, A, B, Cm, D=None, z=None, delta_bias=None, seqs=N
     if init is not None:
         _no_grad_state('init', init)
         init = _param('init', init, (geo[1], u.shape[-1], A.shape[1]), u)
-    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ops)
-    y, last = _ScanFn.apply(handle, *ops, init, geo, bool(reverse), bool(return_state), train)
+    run = _ScanFn.apply if _wants_grad(*ops) else _scan_forward
+    y, last = run(handle, *ops, init, geo, bool(reverse), bool(return_state))
     return (y, last) if return_state else y
 
 
@@ -345,64 +370,59 @@ def ssm_scan_step(handle, u, delta, A, B, Cm, D, state, z=None, delta_bias=None)
     gradients."""
     if not isinstance(u, torch.Tensor) or u.dim() != 2:
         _bad('u must be (batch, D)')
+    geo = _geometry(handle, u, None, 'u', step=True)
     with torch.no_grad():
-        u3 = u.unsqueeze(0)
-        geo = _geometry(handle, u3, None, 'u')
-        ops = _scan_check(u, delta, A, B, Cm, D, z, delta_bias, (u.shape[0],))
-        _state('state', state, (u.shape[0], u.shape[1], A.shape[1]), _acc(u.dtype), u)
-        y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
-        a = _scan_args(*(t if i in (2, 5, 7) or t is None else t.unsqueeze(0) for i, t in enumerate(ops)), geo, False)
-        a.init = a.last = state.data_ptr()
-        a.y = y.data_ptr()
-        _call(handle, handle.lib.rgp_ssm_scan_step, a)
+        u, delta, A, B, Cm, skip, z, bias = _scan_check(u, delta, A, B, Cm, D, z, delta_bias, geo[0])
+    n, Dn = u.shape
+    N = A.shape[1]
+    _state('state', state, (n, Dn, N), A.dtype, u)
+    y, st = torch.empty(u.shape, dtype=u.dtype, device=u.device), state.data_ptr()
+    _call(handle, handle.lib.rgp_ssm_scan_step, _SCAN.pack(
+        _DTYPES[u.dtype], n, Dn, N, B.shape[-2], 0, 1, n, 1, 0, u.data_ptr(), delta.data_ptr(), _ptr(z), B.data_ptr(), Cm.data_ptr(), 0, u.stride(0), 0,
+        delta.stride(0), 0, 0 if z is None else z.stride(0), 0, B.stride(0), 0, Cm.stride(0), 0, 0, A.data_ptr(), _ptr(skip), _ptr(bias), st,
+        y.data_ptr(), st, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0))
     return y
 
 
 # ---------------------------------------------------------------------------------------------------------------------- norm
-def _rms_args(x, w, eps):
-    a = _lib.RmsNorm()
-    a.dtype, a.rows, a.C, a.eps = _DTYPES[x.dtype], x.shape[0], x.shape[1], eps
-    a.x, a.x_st, a.w = x.data_ptr(), x.stride(0), w.data_ptr()
-    return a
+def _rms_head(x, w, residual, eps, y=0, hid=0, rstd=0, gy=None, gh=None, gx=0, gw=0):
+    st = lambda t: 0 if t is None else t.stride(0)                           # noqa: E731
+    return _RMS.pack(_DTYPES[x.dtype], 0, x.shape[0], x.shape[1], eps, x.data_ptr(), _ptr(residual), x.stride(0), st(residual), st(gy), st(gh),
+                     w.data_ptr(), y, hid, rstd, _ptr(gy), _ptr(gh), gx, gw)
+
+
+def _rms_forward(handle, x, w, residual, eps, train=False):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    hid = torch.empty_like(y) if residual is not None else None
+    rstd = torch.empty(x.shape[0], dtype=w.dtype, device=x.device) if train else None
+    _call(handle, handle.lib.rgp_rms_norm_forward, _rms_head(x, w, residual, eps, y.data_ptr(), _ptr(hid), _ptr(rstd)))
+    return (y, hid, rstd) if train else (y, hid)
 
 
 class _RmsFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, handle, x, w, residual, eps, train):
-        a = _rms_args(x, w, eps)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        hid = torch.empty_like(y) if residual is not None else None
-        rstd = torch.empty(x.shape[0], dtype=w.dtype, device=x.device) if train else None
-        if residual is not None:
-            a.residual, a.residual_st, a.hid = residual.data_ptr(), residual.stride(0), hid.data_ptr()
-        a.y, a.rstd = y.data_ptr(), _ptr(rstd)
-        _call(handle, handle.lib.rgp_rms_norm_forward, a)
+    def forward(ctx, handle, x, w, residual, eps):
+        y, hid, rstd = _rms_forward(handle, x, w, residual, eps, True)
         ctx.handle, ctx.eps, ctx.two = handle, eps, residual is not None
         # 16-bit: the backward pass adds x and residual again, hid's rounding would show in the weight's gradient; 32 and 64 bits: hid is that sum
         again = residual is not None and x.element_size() == 2
         ctx.save_for_backward(x if again or residual is None else hid, residual if again else None, w, rstd)
         ctx.set_materialize_grads(False)
-        return (y, hid) if residual is not None else y
+        return y, hid
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gy, gh=None):
+    def backward(ctx, gy, gh):
+        _once()
         hid, residual, w, rstd = ctx.saved_tensors
         if gy is None:                                    # only the sum was used further on
-            return None, gh, None, gh if ctx.two else None, None, None
+            return None, gh, None, gh if ctx.two else None, None
         handle = ctx.handle
-        a = _rms_args(hid, w, ctx.eps)
-        gy = _inner(gy, 1)
+        gy, gh = _inner(gy, 1), None if gh is None else _inner(gh, 1)
         gx, gw = torch.empty(hid.shape, dtype=hid.dtype, device=hid.device), torch.empty_like(w)
-        work = _work(handle, handle.lib.rgp_rms_norm_workspace(C.byref(a), 1))
-        if residual is not None:
-            a.residual, a.residual_st = residual.data_ptr(), residual.stride(0)
-        if gh is not None:
-            gh = _inner(gh, 1)
-            a.ghid, a.ghid_st = gh.data_ptr(), gh.stride(0)
-        a.rstd, a.gy, a.gy_st, a.gx, a.gw, a.work, a.work_bytes = rstd.data_ptr(), gy.data_ptr(), gy.stride(0), gx.data_ptr(), gw.data_ptr(), work.data_ptr(), work.numel()
-        _call(handle, handle.lib.rgp_rms_norm_backward, a)
-        return None, gx, gw, gx if ctx.two else None, None, None
+        head = _rms_head(hid, w, residual, ctx.eps, rstd=rstd.data_ptr(), gy=gy, gh=gh, gx=gx.data_ptr(), gw=gw.data_ptr())
+        work, tail = _new_work(handle, handle.lib.rgp_rms_norm_workspace, head, 1)
+        _call(handle, handle.lib.rgp_rms_norm_backward, head, tail)
+        return None, gx, gw, gx if ctx.two else None, None
 
 
 def rms_norm(handle, x, weight, residual=None, eps=1e-6):
@@ -415,50 +435,50 @@ def rms_norm(handle, x, weight, residual=None, eps=1e-6):
     eps = float(eps)
     if not eps > 0.0 or math.isinf(eps):
         _bad('eps must be positive')
-    w = _param('weight', weight, (x.shape[-1],), x)
-    flat = lambda t: _inner(t.reshape(-1, t.shape[-1]), 1)                   # noqa: E731
+    w = _param('weight', weight, x.shape[-1:], x)
     if residual is not None:
         _rows('residual', residual, x, x.shape)
         if residual.dim() != x.dim():
             _bad('residual has shape %s, x %s' % (tuple(residual.shape), tuple(x.shape)))
-    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight))
-    r = _RmsFn.apply(handle, flat(x), w, None if residual is None else flat(residual), eps, train)
-    return r.view(x.shape) if residual is None else (r[0].view(x.shape), r[1].view(x.shape))
+    shape, two = x.shape, x.dim() == 2
+    x2 = _inner(x if two else x.reshape(-1, shape[-1]), 1)
+    r2 = None if residual is None else _inner(residual if two else residual.reshape(-1, shape[-1]), 1)
+    y, hid = (_RmsFn.apply if _wants_grad(x2, r2, w) else _rms_forward)(handle, x2, w, r2, eps)
+    if not two:
+        y, hid = y.view(shape), None if hid is None else hid.view(shape)
+    return y if residual is None else (y, hid)
 
 
 # ---------------------------------------------------------------------------------------------------------------------- gradient norm
-class _GradList(object):
-    """Checked pointer table of one call."""
+def _grad_list(handle, grads):
+    """(n, addresses, element counts, types) of one call's tensors, checked; the arrays live as long as the tuple."""
+    grads = list(grads)
+    n = len(grads)
+    for i, g in enumerate(grads):
+        if not isinstance(g, torch.Tensor) or g.dtype not in _DTYPES or g.device != handle.device or g.layout is not torch.strided:
+            _bad('gradient %d must be a float64, float32, bfloat16 or float16 tensor on %s' % (i, handle.device))
+        if not g.is_contiguous() and g.numel() and (_overlaps(g) or sum((m - 1) * s for m, s in zip(g.shape, g.stride())) + 1 != g.numel()):
+            _bad('gradient %d has gaps or repeats in memory: it cannot be clipped in place as one range' % i)
+    ptr, numel, dtype = [g.data_ptr() for g in grads], [g.numel() for g in grads], [_DTYPES[g.dtype] for g in grads]
+    end = 0
+    for p, k, d in sorted(t for t in zip(ptr, numel, dtype) if t[1]):
+        if p < end:
+            _bad('two gradients share memory: each element may be clipped once')
+        end = p + k * _BYTES[d]
+    return n, struct.pack('%dQ' % n, *ptr), struct.pack('%dq' % n, *numel), struct.pack('%di' % n, *dtype)
 
-    def __init__(self, handle, grads):
-        grads = list(grads)
-        n = len(grads)
-        spans = []
-        self.ptr, self.numel, self.dtype = (C.c_void_p * max(n, 1))(), (C.c_int64 * max(n, 1))(), (C.c_int32 * max(n, 1))()
-        for i, g in enumerate(grads):
-            if not isinstance(g, torch.Tensor) or g.device != handle.device or g.dtype not in _DTYPES or g.layout != torch.strided:
-                _bad('gradient %d must be a float64, float32, bfloat16 or float16 tensor on %s' % (i, handle.device))
-            k = g.numel()
-            if k and not g.is_contiguous() and (_overlaps(g) or sum((m - 1) * s for m, s in zip(g.shape, g.stride())) + 1 != k):
-                _bad('gradient %d has gaps or repeats in memory: it cannot be clipped in place as one range' % i)
-            p = g.data_ptr()
-            self.ptr[i], self.numel[i], self.dtype[i] = p, k, _DTYPES[g.dtype]
-            if k:
-                spans.append((p, p + k * g.element_size()))
-        spans.sort()
-        for (_, e), (s, _) in zip(spans, spans[1:]):
-            if s < e:
-                _bad('two gradients share memory: each element may be clipped once')
-        self.n = n
+
+_BYTES = {_lib.DT_F64: 8, _lib.DT_F32: 4, _lib.DT_BF16: 2, _lib.DT_F16: 2}
 
 
 def grad_sumsq(handle, grads):
     """Sum of the squares of all elements of ``grads`` as a float64 device scalar (a data-parallel caller adds the ranks' sums)."""
-    t = _GradList(handle, grads)
-    out = torch.empty((), dtype=torch.float64, device=handle.device)
-    work = _work(handle, handle.lib.rgp_grad_workspace(t.n, t.numel, t.dtype))
-    handle._check(handle.lib.rgp_grad_sumsq(handle.h, _stream(handle), t.n, t.ptr, t.numel, t.dtype, out.data_ptr(), work.data_ptr(), work.numel()))
-    return out
+    n, ptr, numel, dtype = _grad_list(handle, grads)
+    nbytes = handle.lib.rgp_grad_workspace(n, numel, dtype)
+    buf = torch.empty(1 + nbytes // 8, dtype=torch.float64, device=handle.device)
+    p = buf.data_ptr()
+    handle._check(handle.lib.rgp_grad_sumsq(handle.h, _stream(handle), n, ptr, numel, dtype, p, p + 8, nbytes))
+    return buf[0]
 
 
 def clip_grad_norm(handle, grads, max_norm, sumsq=None):
@@ -469,16 +489,13 @@ def clip_grad_norm(handle, grads, max_norm, sumsq=None):
     max_norm = float(max_norm)
     if not max_norm > 0.0:
         _bad('max_norm must be positive')
-    t = _GradList(handle, grads)
-    norm = torch.empty((), dtype=torch.float64, device=handle.device)
-    s = _stream(handle)
+    n, ptr, numel, dtype = _grad_list(handle, grads)
+    nbytes = 0
     if sumsq is None:
-        work = _work(handle, handle.lib.rgp_grad_workspace(t.n, t.numel, t.dtype))
-        handle._check(handle.lib.rgp_grad_sumsq(handle.h, s, t.n, t.ptr, t.numel, t.dtype, norm.data_ptr(), work.data_ptr(), work.numel()))
-        src = norm
-    else:
-        if not isinstance(sumsq, torch.Tensor) or sumsq.dtype != torch.float64 or sumsq.numel() != 1 or sumsq.device != handle.device:
-            _bad('sumsq must be one float64 value on %s' % handle.device)
-        src = sumsq
-    handle._check(handle.lib.rgp_grad_clip(handle.h, s, t.n, t.ptr, t.numel, t.dtype, src.data_ptr(), max_norm, norm.data_ptr()))
-    return norm
+        nbytes = handle.lib.rgp_grad_workspace(n, numel, dtype)
+    elif not isinstance(sumsq, torch.Tensor) or sumsq.dtype is not torch.float64 or sumsq.numel() != 1 or sumsq.device != handle.device:
+        _bad('sumsq must be one float64 value on %s' % handle.device)
+    buf = torch.empty(1 + nbytes // 8, dtype=torch.float64, device=handle.device)
+    p = buf.data_ptr()
+    handle._check(handle.lib.rgp_grad_clip(handle.h, _stream(handle), n, ptr, numel, dtype, _ptr(sumsq), max_norm, p, p + 8 if nbytes else 0, nbytes))
+    return buf[0]

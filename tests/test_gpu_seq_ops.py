@@ -372,6 +372,13 @@ def test_clip_below_the_threshold_and_without_a_finite_norm(h):
     assert float(seq_ops.clip_grad_norm(h, [y], 4.0, sumsq=total)) == 8.0 and torch.allclose(y, torch.full_like(y, 0.5), rtol=1e-6)
 
 
+def test_second_derivatives_are_refused(h):
+    from rgp_amd import seq_ops
+    x = torch.randn(3, 4, device='cuda', requires_grad=True)
+    with pytest.raises(RuntimeError, match='second derivatives'):
+        torch.autograd.grad(seq_ops.rms_norm(h, x, torch.ones(4, device='cuda')).sum(), x, create_graph=True)
+
+
 def test_library_refuses_what_python_would_not_send(h):
     """The C entries check by themselves: sizes, missing buffers, a work buffer that is too small."""
     from rgp_amd import _lib
@@ -389,4 +396,4 @@ def test_library_refuses_what_python_would_not_send(h):
     c.x = c.w = c.v = t.data_ptr()
     c.init = c.last = t.data_ptr()
     assert h.lib.rgp_ssm_conv_forward(h.h, None, C.byref(c)) == _lib.RGP_ERR_BAD_ARG
-    assert h.lib.rgp_grad_clip(h.h, None, 0, None, None, None, t.data_ptr(), 0.0, t.data_ptr()) == _lib.RGP_ERR_BAD_ARG
+    assert h.lib.rgp_grad_clip(h.h, None, 0, None, None, None, t.data_ptr(), 0.0, t.data_ptr() + 8, None, 0) == _lib.RGP_ERR_BAD_ARG
