@@ -17,6 +17,15 @@ template <typename A> static __device__ __forceinline__ A ssm_finite(A a) {
   return a < low ? low : a;
 }
 
+// Where channel c of a tile's row stands in LDS.  A thread writes V neighbouring channels, so at any one of its writes the wave's lanes are V
+// entries apart and would meet in the same banks; the place is c with its low bits exchanged by the number of the 128-byte line, which puts
+// those lanes side by side and leaves neighbouring channels in one line for the recurrence.
+template <int V, int BYTES>
+static __device__ __forceinline__ int ssm_place(int c) {
+  constexpr int SH = BYTES == 8 ? 4 : BYTES == 16 ? 3 : 2;
+  return V == 1 ? c : c ^ ((c >> SH) & (V - 1));
+}
+
 struct SsmDev {
   rgp_ssm_scan a;
   SeqGeo g;

@@ -284,10 +284,11 @@ static __global__ void __launch_bounds__(256) ssm_step_kernel(rgp_ssm_scan a, in
     if (whole) {
       s = *(const Quad*)st;
       Aq = *(const Quad*)Ar;
+      const SeqVec<T, R> b = *(const SeqVec<T, R>*)B, c = *(const SeqVec<T, R>*)C;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        Bq.v[r] = (A)B[r];
-        Cq.v[r] = (A)C[r];
+        Bq.v[r] = (A)b.e[r];
+        Cq.v[r] = (A)c.e[r];
       }
     } else {
 #pragma unroll
@@ -326,7 +327,8 @@ static hipError_t step_pick(const rgp_ssm_scan& a, hipStream_t s) {
   const int K = a.N <= 4 ? 1 : a.N <= 8 ? 2 : a.N <= 16 ? 4 : a.N <= 32 ? 8 : 16;
   const unsigned grid = (unsigned)(((int64_t)a.n_seq * a.D * K + 255) / 256);
   const int Dg = a.D / a.G;
-  const int whole = a.N == SSM_R * K && ((uintptr_t)a.last & 15) == 0 && ((uintptr_t)a.A & 15) == 0;
+  const int whole = a.N == SSM_R * K && ((uintptr_t)a.last & 15) == 0 && ((uintptr_t)a.A & 15) == 0 &&
+                    seq_aligned(a.B, 0, a.B_sb, (int)sizeof(T), SSM_R) && seq_aligned(a.C, 0, a.C_sb, (int)sizeof(T), SSM_R);
   switch (K) {
     case 1: hipLaunchKernelGGL((ssm_step_kernel<T, 1>), dim3(grid), dim3(256), 0, s, a, Dg, whole); break;
     case 2: hipLaunchKernelGGL((ssm_step_kernel<T, 2>), dim3(grid), dim3(256), 0, s, a, Dg, whole); break;

@@ -18,7 +18,7 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
   struct alignas(4 * sizeof(A)) Four { A x, y, z, w; };
   struct alignas(16) Quad { A v[R]; };
   __shared__ Four pl[TL][CH];                          // in: dt, u, gp, sigmoid(delta + bias); out: gu, gdelta, p
-  __shared__ A zf[MODE == 0 ? TL : 1][CH];              // gy silu'(z)
+  __shared__ A zf[MODE == 0 ? NI * V : 1][THREADS];     // gy silu'(z), each thread its own
   __shared__ Quad Bl[MODE == 0 ? TL : 1][K];
   __shared__ Quad Cl[TL][K];
   __shared__ A red[MODE == 0 ? WAVES : 1][MODE == 0 ? TL : 1][2 * NP];
@@ -31,7 +31,7 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
   const int ev = tid % NV, et = tid / NV;               // roles as in the forward kernel
   const bool here = ev * V < chn && et < TL;
   const int ech = ch0 + (ev * V < chn ? ev * V : 0);
-  const int ch = tid / K, k = tid % K;
+  const int ch = tid / K, k = tid % K, cp = ssm_place<V, sizeof(Four)>(ch);
   const bool live = ch < chn;
   if (!b.ok) {                                        // an empty block still owns a row of the partial sums
     if (MODE == 0) {
@@ -99,15 +99,16 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
           const A dt = seq_softplus((A)rd[i].e[j] + bias[j], p.w);
           const bool ok = tl < nt && ev * V < chn;             // all lanes' values are folded below
           p.x = ok ? dt : (A)0;
+          p.w = ok ? p.w : (A)0;
           p.y = MODE == 0 && ok ? (A)ru[i].e[j] : (A)0;
           A gp = (A)rg[i].e[j];
           if (a.z) {
             const A z = (A)rz[i].e[j], q = gp * seq_sigmoid(z);
-            if (MODE == 0) zf[tl][ev * V + j] = q + (gp - q) * (z * seq_sigmoid(z));
+            if (MODE == 0) zf[i * V + j][tid] = q + (gp - q) * (z * seq_sigmoid(z));
             gp = z * q;
           }
           p.z = ok ? gp : (A)0;
-          pl[tl][ev * V + j] = p;
+          pl[tl][ssm_place<V, sizeof(Four)>(ev * V + j)] = p;
         }
       }
     }
@@ -125,7 +126,7 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
     if (MODE == 1) {
 #pragma unroll
       for (int t = TL - 1; t >= 0; --t) {                         // steps behind the end change nothing
-        const Four p = pl[t][ch];
+        const Four p = pl[t][cp];
         const Quad C = Cl[t][k];
         sum += p.x;
 #pragma unroll
@@ -140,12 +141,12 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
 #pragma unroll
         for (int r = 0; r < R; ++r) s0[r] = live && k * R + r < N ? ckpt[((tt + tb) / CK) * ((int64_t)a.D * N) + r] : (A)0;
         // operands of a step are read from LDS while the step before is computed
-        Four p = pl[tb][ch];
+        Four p = pl[tb][cp];
         Quad B = Bl[tb][k], C;
 #pragma unroll
         for (int i = 0; i < CK; ++i) {
           const int tn = tb + (i + 1 < CK ? i + 1 : i);
-          const Four pn = pl[tn][ch];
+          const Four pn = pl[tn][cp];
           const Quad Bn = Bl[tn][k];
           const A w = p.x * p.y;
 #pragma unroll
@@ -160,7 +161,7 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
 #pragma unroll
         for (int i = CK - 1; i >= 0; --i) {
           const int t = tb + i, tn = t - (i ? 1 : 0);
-          const Four pn = pl[tn][ch];
+          const Four pn = pl[tn][cp];
           const Quad Bn = Bl[tn][k], Cn = Cl[tn][k];
           const A w = p.x * p.y;
           A g1 = (A)0, g2 = (A)0, yd = (A)0, vB[R], vC[R];
@@ -185,8 +186,8 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
           o.z = yd + skip * p.y;
           o.w = (A)0;
           gD += p.z * p.y;
-          gbias += t < nt ? o.y : (A)0;
-          if (k == 0) pl[t][ch] = o;
+          gbias += o.y;
+          if (k == 0) pl[t][cp] = o;
           // over the wave's channels: lane bit 5 selects gB / gC, bit 4 and bit 3 the state
           const bool b3 = (lane & 8) != 0;
           A f0 = seq_fold<true>(vB[0], vC[0]), f1 = seq_fold<true>(vB[1], vC[1]), f2 = seq_fold<true>(vB[2], vC[2]), f3 = seq_fold<true>(vB[3], vC[3]);
@@ -218,10 +219,10 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
           Vec ou, od, oz;
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            const Four p = pl[tl][ev * V + j];
+            const Four p = pl[tl][ssm_place<V, sizeof(Four)>(ev * V + j)];
             ou.e[j] = (T)p.x;
             od.e[j] = (T)p.y;
-            if (a.z) oz.e[j] = (T)(zf[tl][ev * V + j] * p.z);
+            if (a.z) oz.e[j] = (T)(zf[i * V + j][tid] * p.z);
           }
           const int64_t o = seq_row_index(d.g, b, tt + tl) * a.D + ech;
           *(Vec*)((T*)a.gu + o) = ou;

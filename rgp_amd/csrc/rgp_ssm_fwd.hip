@@ -14,7 +14,7 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
   constexpr int NI = RPI >= TL ? 1 : TL / RPI, NB = (TL * NP + THREADS - 1) / THREADS, CK = SSM_CK;
   struct alignas(2 * sizeof(A)) Pair { A dt, w; };
   struct alignas(16) Quad { A v[R]; };
-  __shared__ Pair pl[TL][CH];
+  __shared__ Pair pl[TL][CH + (V > 1 ? 4 : 0)];
   __shared__ Quad Bl[TL][K];
   __shared__ Quad Cl[MODE == 0 ? TL : 1][K];
   const rgp_ssm_scan& a = d.a;
@@ -50,7 +50,7 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
     skip[i] = MODE == 0 && a.skip ? ((const A*)a.skip)[ech + i] : (A)0;
   }
   // recurrence role: states k R .. k R + R - 1 of channel ch
-  const int ch = tid / K, k = tid % K;
+  const int ch = tid / K, k = tid % K, cp = ssm_place<V, sizeof(Pair)>(ch);
   const bool live = ch < chn;
   A Ar[R], s[R], sum = (A)0;
 #pragma unroll
@@ -103,7 +103,7 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
           Pair p;
           p.dt = tl < nt ? dt : (A)0;
           p.w = tl < nt ? dt * (A)ru[i].e[j] : (A)0;
-          pl[tl][ev * V + j] = p;
+          pl[tl][ssm_place<V, sizeof(Pair)>(ev * V + j)] = p;
         }
       }
     }
@@ -133,7 +133,7 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
 #pragma unroll
       for (int i = 0; i < CK; ++i) {
         const int t = tb + i;                                     // steps behind the end change nothing
-        const Pair p = pl[t][ch];
+        const Pair p = pl[t][cp];
         const Quad B = Bl[t][k];
         A acc = (A)0;
         if (MODE == 1) sum += p.dt;
@@ -145,7 +145,7 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
         }
         if (MODE == 0) {
           acc = seq_sum<K>(acc);
-          if (k == 0) pl[t][ch].dt = acc;
+          if (k == 0) pl[t][cp].dt = acc;
         }
       }
     }
@@ -158,7 +158,7 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
           Vec o;
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            A y = pl[tl][ev * V + j].dt + skip[j] * (A)cu[i].e[j];
+            A y = pl[tl][ssm_place<V, sizeof(Pair)>(ev * V + j)].dt + skip[j] * (A)cu[i].e[j];
             if (a.z) {
               const A z = (A)cz[i].e[j];
               y *= z * seq_sigmoid(z);
