@@ -4,16 +4,39 @@
 
 // ---- sums of partial results in a fixed order -----------------------------------------------------------------------------------------
 // A workgroup forms 64 outputs of one of up to five sums, 16 threads for each: thread q adds partials q, q + 16, ... in eight interleaved
-// sums (that many loads are in flight), then the 16 are added in LDS.  The order depends on the count of partials alone.
+// sums (that many loads are in flight), then the 16 are added in LDS; up to SEQ_FEW partials are added by one thread an output.  The order depends on the count of partials alone.
+#define SEQ_FEW 32
+static __host__ __device__ inline int64_t seq_sums_width(int64_t P) { return P <= SEQ_FEW ? 1024 : 64; }
+template <typename A>
+static __device__ __forceinline__ void seq_sums_store(const SeqSum& j, int64_t i, A v) {
+  const int64_t o = j.turn > 1 ? (i % (j.n / j.turn)) * j.turn + i / (j.n / j.turn) : i;
+  switch (j.dt) {
+    case RGP_F64: ((double*)j.out)[o] = (double)v; break;
+    case RGP_F32: ((float*)j.out)[o] = (float)v; break;
+    case RGP_BF16: ((__bf16*)j.out)[o] = (__bf16)(float)v; break;
+    default: ((_Float16*)j.out)[o] = (_Float16)(float)v; break;
+  }
+}
 template <typename A>
 static __global__ void __launch_bounds__(1024) seq_sums_kernel(SeqSums g) {
   __shared__ A sh[16][64];
   int k = 0;
   while (k + 1 < g.count && (int)blockIdx.x >= g.job[k + 1].block0) ++k;
   const SeqSum& j = g.job[k];
-  const int l = threadIdx.x & 63, q = threadIdx.x >> 6;
-  const int64_t i = (int64_t)((int)blockIdx.x - j.block0) * 64 + l;
   const A* const part = (const A*)j.part;
+  const int64_t o0 = (int64_t)((int)blockIdx.x - j.block0) * seq_sums_width(j.P);
+  if (j.P <= SEQ_FEW) {                                  // uniform over the workgroup
+    const int64_t i = o0 + threadIdx.x;
+    if (i < j.n) {
+      A v = (A)0;
+#pragma unroll 8
+      for (int64_t p = 0; p < j.P; ++p) v += part[p * j.stride + i];
+      seq_sums_store(j, i, v);
+    }
+    return;
+  }
+  const int l = threadIdx.x & 63, q = threadIdx.x >> 6;
+  const int64_t i = o0 + l;
   A v8[8] = {};
   if (i < j.n) {
     const A* p = part + q * j.stride + i;
@@ -32,20 +55,14 @@ static __global__ void __launch_bounds__(1024) seq_sums_kernel(SeqSums g) {
     A v = sh[0][l];
 #pragma unroll
     for (int r = 1; r < 16; ++r) v += sh[r][l];
-    const int64_t o = j.turn > 1 ? (i % (j.n / j.turn)) * j.turn + i / (j.n / j.turn) : i;
-    switch (j.dt) {
-      case RGP_F64: ((double*)j.out)[o] = (double)v; break;
-      case RGP_F32: ((float*)j.out)[o] = (float)v; break;
-      case RGP_BF16: ((__bf16*)j.out)[o] = (__bf16)(float)v; break;
-      default: ((_Float16*)j.out)[o] = (_Float16)(float)v; break;
-    }
+    seq_sums_store(j, i, v);
   }
 }
 void SeqSums::add(const void* part, int64_t P, int64_t stride, int64_t n, void* out, int dt, int turn) {
   if (!out || n < 1) return;
   SeqSum& j = job[count++];
   j.part = part; j.P = P; j.stride = stride; j.n = n; j.out = out; j.dt = dt; j.turn = turn; j.block0 = blocks;
-  blocks += (int)((n + 63) / 64);
+  blocks += (int)((n + seq_sums_width(P) - 1) / seq_sums_width(P));
 }
 rgp_status SeqSums::run(rgp_handle h, hipStream_t s, int acc) {
   if (!count) return RGP_OK;
