@@ -316,7 +316,9 @@ enum { RGP_F64 = 0, RGP_F32 = 1, RGP_BF16 = 2, RGP_F16 = 3 };
  * u, delta, z, gy [..][D]; B, C [..][G][N]; A [D][N]; skip, bias [D] (NULL = 0); init, last [n_seq][D][N] acc (NULL: zero / not wanted).
  * states: rgp_ssm_scan_states_bytes(a) bytes, written by the forward call when not NULL and read by the backward call.
  * Backward: gy = dL/dy -> gu, gdelta, gz [..][D], gB, gC [..][G][N] (dtype, contiguous), gA [D][N], gskip, gbias [D] (acc; the last
- * two, and gz, may be NULL where skip, bias, z are).  N <= 64.  work: rgp_ssm_scan_workspace(a, backward) bytes, 16-byte aligned. */
+ * two, and gz, may be NULL where skip, bias, z are).  N <= 64.  work: rgp_ssm_scan_workspace(a, backward) bytes, 16-byte aligned
+ * (backward, more than one workgroup of channels a group: their sums for gB and gC, 2 rows G N acc values for every 64 channels at
+ * N <= 16, 32 at N <= 32, 16 beyond). */
 typedef struct rgp_ssm_scan {
   int32_t dtype, n_seq, D, N, G, reverse;
   int64_t T, rows, max_len;
@@ -364,7 +366,7 @@ rgp_status rgp_ssm_conv_step(rgp_handle h, void* stream, const rgp_ssm_conv* a);
 /* Root-mean-square norm of x + residual over the last dimension, per row:
  *     hid = x + residual;  y = hid * r * w,  r = (mean(hid^2) + eps)^(-1/2)
  * x, residual (NULL = 0), y, hid [rows][C] dtype (row strides in elements; y, hid contiguous; hid NULL iff residual is), w [C] acc,
- * rstd [rows] acc (NULL: not wanted; the backward call reads it).  Backward: gy, ghid (NULL = 0) -> gx [rows][C] (the gradient of x and
+ * rstd [rows] acc (NULL: not wanted; the backward call reads it); rows < 2^24.  Backward: gy, ghid (NULL = 0) -> gx [rows][C] (the gradient of x and
  * of residual alike), gw [C] acc; x and residual are the forward call's (or x = hid and no residual: the same up to hid's rounding). */
 typedef struct rgp_rms_norm {
   int32_t dtype, reserved;

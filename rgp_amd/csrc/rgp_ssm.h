@@ -11,10 +11,11 @@
 #define SSM_CK_LG 3
 #define SSM_CK (1 << SSM_CK_LG)
 // A step behind the end of a block has dt = u = gp = 0 and changes nothing: its decay is exp(0 A) = 1.  For that A must be finite:
-// minus infinity (forget everything) is held as the lowest finite value, whose product with any dt of a real step still decays to 0.
+// minus infinity (forget everything) is held as a value whose product with the dt of any real step still decays to 0, likewise plus
+// infinity (2e38 log2 e is still finite in 32 bits).
 template <typename A> static __device__ __forceinline__ A ssm_finite(A a) {
-  const A low = sizeof(A) == 4 ? (A)-3.0e38f : (A)-1.0e308;
-  return a < low ? low : a;
+  const A most = sizeof(A) == 4 ? (A)2.0e38f : (A)1.0e308;
+  return a < -most ? -most : a > most ? most : a;
 }
 
 // Where channel c of a tile's row stands in LDS.  A thread writes V neighbouring channels, so at any one of its writes the wave's lanes are V

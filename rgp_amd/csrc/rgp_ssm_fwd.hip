@@ -57,8 +57,8 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
   for (int r = 0; r < R; ++r) {
     const bool ok = live && k * R + r < N;
     Ar[r] = ok ? ((const A*)a.A)[(int64_t)(ch0 + ch) * N + k * R + r] : (A)0;
-    if (sizeof(A) == 4) Ar[r] *= (A)1.44269504088896341;          // exp(dt A) = 2^(dt A log2 e)
     Ar[r] = ssm_finite(Ar[r]);
+    if (sizeof(A) == 4) Ar[r] *= (A)1.44269504088896341;          // exp(dt A) = 2^(dt A log2 e)
     s[r] = (A)0;
     if (MODE == 0 && ok) {
       if (d.part) s[r] = ((const A*)d.part)[(slot * a.D + ch0 + ch) * N + k * R + r];

@@ -37,13 +37,14 @@ class _TallLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, W, b):
         ctx.save_for_backward(x, W)
-        return torch.addmm(b, x, W.t())
+        ctx.bias = b is not None
+        return torch.addmm(b, x, W.t()) if b is not None else x.mm(W.t())
 
     @staticmethod
     def backward(ctx, g):
         x, W = ctx.saved_tensors
         g = g.contiguous()
-        return g.mm(W), _splitk_tn(g, x), g.sum(0)
+        return g.mm(W), _splitk_tn(g, x), g.sum(0) if ctx.bias else None
 
 
 def tall_linear(x, W, b):
@@ -166,9 +167,9 @@ class _SsmBlock(nn.Module):
     @staticmethod
     def _linear(x, W, b=None):
         W, b = W.to(x.dtype), None if b is None else b.to(x.dtype)
-        if b is not None and x.dim() == 3 and x.dtype == torch.float64 and x.shape[0] * x.shape[1] >= 1024:
-            return tall_linear(x, W, b)                                          # split-K weight gradients
-        return nn.functional.linear(x, W, b)
+        rows = x.reshape(-1, x.shape[-1])                                        # one plain product, never a batched one
+        tall = x.dtype == torch.float64 and rows.shape[0] >= 1024                # split-K weight gradients
+        return (_TallLinear.apply(rows, W, b) if tall else nn.functional.linear(rows, W, b)).view(*x.shape[:-1], W.shape[0])
 
     def _parts(self, handle, x):
         from . import seq_ops
@@ -198,6 +199,7 @@ class _SsmBlock(nn.Module):
         n = self._finish(handle, p, y, h)
         return (n, (conv, scan)) if return_state else n
 
+    @torch.no_grad()
     def step(self, handle, x, state):
         from . import seq_ops
         p, h, c, z = self._parts(handle, x)
@@ -300,6 +302,7 @@ class SeqEncoder(nn.Module):
         self._need_ssm()
         return [layer.initial_state(batch) for layer in self.layers]
 
+    @torch.no_grad()
     def step(self, x, state):
         """One observation of every sequence: x (batch, input_dim) -> (means, variances) of every layer, (batch, H) each; state is updated
         in place."""

@@ -58,8 +58,20 @@ def _new_work(handle, query, head, backward):
     return w, _WORK.pack(w.data_ptr(), n)
 
 
+def _new_like(t):
+    return None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _ptr(t):
     return 0 if t is None else t.data_ptr()
+
+
+def _wants_grad(*ts):
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _once():
@@ -92,6 +104,8 @@ class SeqTable(object):
         self.lengths, self.n_seq, self.rows, self.max_len = lengths, len(lengths), off[-1], max(lengths)
         self.device = handle.device
         self.off = torch.tensor(off, dtype=torch.int64).to(handle.device)
+        if self.device.type == 'cuda':                     # there for every stream from now on
+            torch.cuda.current_stream(self.device).synchronize()
 
 
 def _rows(name, t, like, lead):
@@ -168,7 +182,13 @@ def _state(name, t, shape, dtype, x):
         _bad('%s must be a contiguous %s tensor of shape %s on %s' % (name, dtype, tuple(shape), x.device))
     if t.requires_grad:
         _bad('%s is updated in place and takes no gradient' % name)
+    torch.autograd.graph.increment_version(t)       # a graph that saved the state notices the update
     return t
+
+
+def _no_step_grad(*ts):
+    if _wants_grad(*ts):
+        _bad('a single step takes no gradients: call it under torch.no_grad()')
 
 
 def _no_grad_state(name, t):
@@ -185,7 +205,7 @@ def _conv_head(x, w, bias, geo, reverse, init=0, v=0, last=0, gv=0, gv_st=(0, 0)
 
 
 def _conv_forward(handle, x, w, bias, init, geo, reverse, want_last):
-    v = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    v = _new_like(x)
     last = torch.empty(geo[1], w.shape[1] - 1, x.shape[-1], dtype=x.dtype, device=x.device) if want_last else None
     _call(handle, handle.lib.rgp_ssm_conv_forward, _conv_head(x, w, bias, geo, reverse, _ptr(init), v.data_ptr(), _ptr(last)))
     return v, last
@@ -210,8 +230,7 @@ class _ConvFn(torch.autograd.Function):
         x, w, bias, init = ctx.saved_tensors
         handle = ctx.handle
         gv = _inner(gv, 1)
-        gx, gw = torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty_like(w)
-        gb = torch.empty_like(bias) if bias is not None else None
+        gx, gw, gb = _new_like(x), _new_like(w), _new_like(bias)
         head = _conv_head(x, w, bias, ctx.geo, ctx.reverse, _ptr(init), 0, 0, gv.data_ptr(), _strides(gv, ctx.geo[5] is not None), gx.data_ptr(),
                           gw.data_ptr(), _ptr(gb))
         work, tail = _new_work(handle, handle.lib.rgp_ssm_conv_workspace, head, 1)
@@ -219,20 +238,13 @@ class _ConvFn(torch.autograd.Function):
         return None, gx, gw, gb, None, None, None, None
 
 
-def _wants_grad(*ts):
-    if torch.is_grad_enabled():
-        for t in ts:
-            if t is not None and t.requires_grad:
-                return True
-    return False
-
-
 def ssm_conv(handle, x, weight, bias=None, seqs=None, init=None, reverse=False, return_state=False):
     """silu(bias + causal convolution of x with one filter per channel): v_t uses x_{t-W+1} .. x_t of its own sequence.
 
     x: (T, batch, D), or packed (rows, D) with ``seqs``; weight (D, W), 2 <= W <= 8; bias (D,).  init: (n_seq, W - 1, D), the inputs before
     the first step, oldest first (zeros without it); return_state=True also returns them for the step behind the last one.  reverse=True
-    walks every sequence from its last step.  Gradients: x, weight, bias (states take none)."""
+    walks every sequence from its last step (init and the returned state are then those of that walk).  Gradients: x, weight, bias (states
+    take none)."""
     geo = _geometry(handle, x, seqs, 'x')
     D = x.shape[-1]
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not 2 <= weight.shape[1] <= 8:
@@ -251,7 +263,8 @@ def ssm_conv(handle, x, weight, bias=None, seqs=None, init=None, reverse=False, 
 
 
 def ssm_conv_step(handle, x, weight, bias, state):
-    """One step of ``ssm_conv``: x (batch, D), state (batch, W - 1, D) of x's type, updated in place.  No gradients."""
+    """One step of ``ssm_conv``: x (batch, D), state (batch, W - 1, D) of x's type, updated in place.  It takes no
+    gradients: operands that require them are refused outside torch.no_grad()."""
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         _bad('x must be (batch, D)')
     geo = _geometry(handle, x, None, 'x', step=True)
@@ -259,9 +272,10 @@ def ssm_conv_step(handle, x, weight, bias, state):
         _bad('weight must be (D, W) with 2 to 8 taps')
     D = x.shape[1]
     w, b = _param('weight', weight, (D, weight.shape[1]), x), _param('bias', bias, (D,), x, optional=True)
+    _no_step_grad(x, weight, bias)
     _state('state', state, (x.shape[0], weight.shape[1] - 1, D), x.dtype, x)
     x = _inner(x, 1)
-    v, st = torch.empty(x.shape, dtype=x.dtype, device=x.device), state.data_ptr()
+    v, st = _new_like(x), state.data_ptr()
     _call(handle, handle.lib.rgp_ssm_conv_step, _CONV.pack(_DTYPES[x.dtype], x.shape[0], D, w.shape[1], 0, 0, 1, x.shape[0], 1, 0, x.data_ptr(), 0,
                                                           x.stride(0), 0, 0, w.data_ptr(), _ptr(b), st, v.data_ptr(), st, 0, 0, 0, 0))
     return v
@@ -282,12 +296,13 @@ def _scan_head(ops, geo, reverse, init=0, y=0, last=0, states=0, gy=0, gy_st=(0,
 
 def _scan_forward(handle, u, delta, A, B, Cm, skip, z, bias, init, geo, reverse, want_last, train=False):
     ops = (u, delta, A, B, Cm, skip, z, bias)
-    y = torch.empty(u.shape, dtype=u.dtype, device=u.device)
+    y = _new_like(u)
     last = torch.empty(geo[1], u.shape[-1], A.shape[1], dtype=A.dtype, device=u.device) if want_last else None
     states = None
     if train:
-        n = handle.lib.rgp_ssm_scan_states_bytes(_scan_head(ops, geo, reverse) + _NO_WORK)
-        states = torch.empty(n, dtype=torch.uint8, device=u.device)
+        # a state of N every 8 steps of every sequence: (blocks of 8) D N values (rgp_ssm_scan_states_bytes)
+        blocks = (geo[3] >> 3) + geo[1] if geo[5] is not None else geo[1] * ((geo[2] + 7) >> 3)
+        states = torch.empty(blocks * A.numel(), dtype=A.dtype, device=u.device)
     head = _scan_head(ops, geo, reverse, _ptr(init), y.data_ptr(), _ptr(last), _ptr(states))
     work, tail = _new_work(handle, handle.lib.rgp_ssm_scan_workspace, head, 0)
     _call(handle, handle.lib.rgp_ssm_scan_forward, head, tail)
@@ -313,7 +328,7 @@ class _ScanFn(torch.autograd.Function):
         saved = ctx.saved_tensors
         ops, states, handle = saved[:8], saved[8], ctx.handle
         gy = _inner(gy, 1)
-        grads = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in ops]
+        grads = [_new_like(t) for t in ops]
         head = _scan_head(ops, ctx.geo, ctx.reverse, states=states.data_ptr(), gy=gy.data_ptr(), gy_st=_strides(gy, ctx.geo[5] is not None),
                           grads=[_ptr(t) for t in grads])
         work, tail = _new_work(handle, handle.lib.rgp_ssm_scan_workspace, head, 1)
@@ -366,17 +381,18 @@ def ssm_scan(handle, u, delta, A, B, Cm, D=None, z=None, delta_bias=None, seqs=N
 
 
 def ssm_scan_step(handle, u, delta, A, B, Cm, D, state, z=None, delta_bias=None):
-    """One step of ``ssm_scan``: u, delta, z (batch, Dn); B, C (batch, N) or (batch, G, N); state (batch, Dn, N), updated in place.  No
-    gradients."""
+    """One step of ``ssm_scan``: u, delta, z (batch, Dn); B, C (batch, N) or (batch, G, N); state (batch, Dn, N), updated in place.  It
+    takes no gradients: operands that require them are refused outside torch.no_grad()."""
     if not isinstance(u, torch.Tensor) or u.dim() != 2:
         _bad('u must be (batch, D)')
     geo = _geometry(handle, u, None, 'u', step=True)
+    _no_step_grad(u, delta, A, B, Cm, D, z, delta_bias)
     with torch.no_grad():
         u, delta, A, B, Cm, skip, z, bias = _scan_check(u, delta, A, B, Cm, D, z, delta_bias, geo[0])
     n, Dn = u.shape
     N = A.shape[1]
     _state('state', state, (n, Dn, N), A.dtype, u)
-    y, st = torch.empty(u.shape, dtype=u.dtype, device=u.device), state.data_ptr()
+    y, st = _new_like(u), state.data_ptr()
     _call(handle, handle.lib.rgp_ssm_scan_step, _SCAN.pack(
         _DTYPES[u.dtype], n, Dn, N, B.shape[-2], 0, 1, n, 1, 0, u.data_ptr(), delta.data_ptr(), _ptr(z), B.data_ptr(), Cm.data_ptr(), 0, u.stride(0), 0,
         delta.stride(0), 0, 0 if z is None else z.stride(0), 0, B.stride(0), 0, Cm.stride(0), 0, 0, A.data_ptr(), _ptr(skip), _ptr(bias), st,
@@ -392,8 +408,8 @@ def _rms_head(x, w, residual, eps, y=0, hid=0, rstd=0, gy=None, gh=None, gx=0, g
 
 
 def _rms_forward(handle, x, w, residual, eps, train=False):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    hid = torch.empty_like(y) if residual is not None else None
+    y = _new_like(x)
+    hid = _new_like(x) if residual is not None else None
     rstd = torch.empty(x.shape[0], dtype=w.dtype, device=x.device) if train else None
     _call(handle, handle.lib.rgp_rms_norm_forward, _rms_head(x, w, residual, eps, y.data_ptr(), _ptr(hid), _ptr(rstd)))
     return (y, hid, rstd) if train else (y, hid)
@@ -418,7 +434,7 @@ class _RmsFn(torch.autograd.Function):
             return None, gh, None, gh if ctx.two else None, None
         handle = ctx.handle
         gy, gh = _inner(gy, 1), None if gh is None else _inner(gh, 1)
-        gx, gw = torch.empty(hid.shape, dtype=hid.dtype, device=hid.device), torch.empty_like(w)
+        gx, gw = _new_like(hid), _new_like(w)
         head = _rms_head(hid, w, residual, ctx.eps, rstd=rstd.data_ptr(), gy=gy, gh=gh, gx=gx.data_ptr(), gw=gw.data_ptr())
         work, tail = _new_work(handle, handle.lib.rgp_rms_norm_workspace, head, 1)
         _call(handle, handle.lib.rgp_rms_norm_backward, head, tail)
@@ -452,7 +468,6 @@ def rms_norm(handle, x, weight, residual=None, eps=1e-6):
 # ---------------------------------------------------------------------------------------------------------------------- gradient norm
 def _grad_list(handle, grads):
     """(n, addresses, element counts, types) of one call's tensors, checked; the arrays live as long as the tuple."""
-    grads = list(grads)
     n = len(grads)
     for i, g in enumerate(grads):
         if not isinstance(g, torch.Tensor) or g.dtype not in _DTYPES or g.device != handle.device or g.layout is not torch.strided:
@@ -473,7 +488,7 @@ _BYTES = {_lib.DT_F64: 8, _lib.DT_F32: 4, _lib.DT_BF16: 2, _lib.DT_F16: 2}
 
 def grad_sumsq(handle, grads):
     """Sum of the squares of all elements of ``grads`` as a float64 device scalar (a data-parallel caller adds the ranks' sums)."""
-    n, ptr, numel, dtype = _grad_list(handle, grads)
+    n, ptr, numel, dtype = _grad_list(handle, list(grads))
     nbytes = handle.lib.rgp_grad_workspace(n, numel, dtype)
     buf = torch.empty(1 + nbytes // 8, dtype=torch.float64, device=handle.device)
     p = buf.data_ptr()
@@ -489,6 +504,7 @@ def clip_grad_norm(handle, grads, max_norm, sumsq=None):
     max_norm = float(max_norm)
     if not max_norm > 0.0:
         _bad('max_norm must be positive')
+    grads = list(grads)
     n, ptr, numel, dtype = _grad_list(handle, grads)
     nbytes = 0
     if sumsq is None:
@@ -497,5 +513,6 @@ def clip_grad_norm(handle, grads, max_norm, sumsq=None):
         _bad('sumsq must be one float64 value on %s' % handle.device)
     buf = torch.empty(1 + nbytes // 8, dtype=torch.float64, device=handle.device)
     p = buf.data_ptr()
+    torch.autograd.graph.increment_version(grads)
     handle._check(handle.lib.rgp_grad_clip(handle.h, _stream(handle), n, ptr, numel, dtype, _ptr(sumsq), max_norm, p, p + 8 if nbytes else 0, nbytes))
     return buf[0]

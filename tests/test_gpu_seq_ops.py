@@ -228,6 +228,68 @@ def test_scan_gradients_match_differences(h):
         assert abs(num - float((scan[g] * d).sum())) <= 1e-6 * max(1.0, abs(num)), (k, num)       # e^2 = 1e-10 of the third derivative, 1e-16 / e of rounding
 
 
+def test_broadcast_and_shared_operands(h):
+    """Operands with stride 0, one tensor as two operands, and gradients summed over what was broadcast."""
+    from rgp_amd import seq_ops
+    T, n, D, N = 19, 3, 8, 16
+    g = _gen(0)
+    u, delta = _randn(g, T, n, D).cuda().requires_grad_(True), _randn(g, T, 1, D).cuda().requires_grad_(True)
+    B, A = _randn(g, T, 1, 1, N).cuda().requires_grad_(True), -torch.rand(D, N, generator=g, dtype=F64).cuda()
+    gy = _randn(g, T, n, D).cuda()
+    Bx = B.expand(T, n, 2, N)
+    y = seq_ops.ssm_scan(h, u, delta.expand(T, n, D), A, Bx, Bx, z=u)
+    got = torch.autograd.grad(y, (u, delta, B), gy)
+    u2, d2, b2 = (t.detach().clone().requires_grad_(True) for t in (u, delta, B))
+    full = lambda t, *s: t.expand(*s).contiguous()                        # noqa: E731
+    y2 = seq_ops.ssm_scan(h, u2, full(d2, T, n, D), A, full(b2, T, n, 2, N), full(b2, T, n, 2, N), z=u2.clone())
+    want = torch.autograd.grad(y2, (u2, d2, b2), gy)
+    assert torch.equal(y, y2)
+    for a, b in zip(got, want):
+        torch.testing.assert_close(a, b, rtol=1e-12, atol=1e-12)
+
+
+def test_states_updated_in_place_are_noticed(h):
+    """A graph that saved a state refuses its backward pass once a step has changed it; steps refuse operands that want gradients."""
+    from rgp_amd import seq_ops
+    from rgp_amd._lib import RgpError
+    w = torch.randn(6, 4, device='cuda', requires_grad=True)
+    x, st = torch.randn(5, 2, 6, device='cuda'), torch.randn(2, 3, 6, device='cuda')
+    v = seq_ops.ssm_conv(h, x, w, init=st)
+    with pytest.raises(RgpError, match='no gradients'):
+        seq_ops.ssm_conv_step(h, x[0], w, None, st)
+    seq_ops.ssm_conv_step(h, x[0], w.detach(), None, st)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        v.sum().backward()
+
+
+def test_rows_beyond_2_31_elements(h):
+    """Packed rows whose last sequence lies behind 2^31 elements, forward and backward: it gives what it gives alone."""
+    from rgp_amd import seq_ops
+    D, N, tail = 2048, 2, 70
+    rows = (1 << 31) // D + 4000
+    g = torch.Generator(device='cuda').manual_seed(0)
+    f = lambda *s: torch.randn(*s, device='cuda', generator=g, dtype=F32).to(BF16)          # noqa: E731
+    big = {k: torch.zeros(rows, w, device='cuda', dtype=BF16) for k, w in (('x', D), ('u', D), ('delta', D), ('B', N), ('C', N), ('gy', D))}
+    for t in big.values():
+        t[-3 * tail:] = f(3 * tail, t.shape[1])
+    A, w, ws = -torch.rand(D, N, device='cuda') - 0.1, torch.randn(D, 4, device='cuda'), torch.rand(D, device='cuda')
+
+    def run(t, lengths):
+        s = seq_ops.SeqTable(h, lengths)
+        leaves = [t[k].detach().requires_grad_(True) for k in ('x', 'u', 'delta', 'B', 'C')]
+        x, u, delta, B, Cm = leaves
+        v = seq_ops.ssm_conv(h, x, w, seqs=s)
+        y = seq_ops.ssm_scan(h, u, delta, A, B, Cm, z=v, seqs=s)
+        n, hid = seq_ops.rms_norm(h, y, ws, residual=v)
+        return [o.detach()[-tail:].float() for o in (v, y, n, hid)] + [o[-tail:].float() for o in torch.autograd.grad((n, hid), leaves, (t['gy'], t['gy']))]
+    got = run(big, [rows - 3 * tail, 2 * tail, tail])
+    want = run({k: t[-tail:].clone() for k, t in big.items()}, [tail])
+    for a, b in zip(got, want):                                              # the same roundings except for the order of sums over channels
+        assert float((a - b).norm()) <= 1e-2 * float(b.norm())
+    del big
+    torch.cuda.empty_cache()
+
+
 def test_graph_capture_of_forward_and_backward(h):
     """Forward and backward in one captured region, replayed with new inputs and with eager work between the replays."""
     from rgp_amd import seq_ops

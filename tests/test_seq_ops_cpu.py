@@ -168,7 +168,12 @@ def test_size_queries_refuse_and_count():
     lib = _lib.load()
     a = _lib.SsmScan()
     a.dtype, a.n_seq, a.D, a.N, a.G, a.T, a.rows, a.max_len = _lib.DT_F32, 2, 6, 3, 2, 5, 10, 5
-    assert lib.rgp_ssm_scan_states_bytes(C.byref(a)) == 2 * 1 * 6 * 3 * 4          # one state every 16 steps of each sequence
+    assert lib.rgp_ssm_scan_states_bytes(C.byref(a)) == 2 * 1 * 6 * 3 * 4          # one state every 8 steps of each sequence
+    for T, rows, off in ((5, 10, 0), (8, 16, 0), (17, 34, 0), (0, 0, 1), (0, 7, 1), (0, 8, 1), (0, 1001, 1)):      # the count that seq_ops allocates by
+        b = _lib.SsmScan.from_buffer_copy(a)
+        b.T, b.rows, b.off = T, rows, off
+        blocks = (rows >> 3) + 2 if off else 2 * ((T + 7) >> 3)
+        assert lib.rgp_ssm_scan_states_bytes(C.byref(b)) == blocks * 6 * 3 * 4
     assert lib.rgp_ssm_scan_workspace(C.byref(a), 0) == 0 and lib.rgp_ssm_scan_workspace(C.byref(a), 1) > 0
     for f, v in (('dtype', 4), ('n_seq', 0), ('N', 65), ('N', 0), ('G', 4), ('rows', 9), ('T', 0)):
         b = _lib.SsmScan.from_buffer_copy(a)
