@@ -118,8 +118,27 @@ def _rows(name, t, like, lead):
         _bad('%s has shape %s, leading dimensions %s expected' % (name, tuple(t.shape), tuple(lead)))
 
 
+def _all_plain(x, acts, params):
+    """True for contiguous activations of x's type and parameters of its arithmetic type (or None), all on x's device: the common case, found
+    in one pass.  Anything else goes through the checks that name what is wrong."""
+    dt, dev = x.dtype, x.device
+    acc = torch.float64 if dt is torch.float64 else torch.float32
+    try:
+        for t in acts:
+            if t.dtype is not dt or t.device != dev or not t.is_contiguous():
+                return False
+        for t in params:
+            if t is not None and (t.dtype is not acc or t.device != dev or not t.is_contiguous()):
+                return False
+    except AttributeError:
+        return False
+    return True
+
+
 def _inner(t, dims):
     """The tensor with its last ``dims`` dimensions contiguous (a copy only where they are not)."""
+    if t.is_contiguous():
+        return t
     shape, stride, want = t.shape, t.stride(), 1
     for i in range(1, dims + 1):
         if stride[-i] != want and shape[-i] > 1:
@@ -282,19 +301,19 @@ def ssm_conv_step(handle, x, weight, bias, state):
 
 
 # ---------------------------------------------------------------------------------------------------------------------- scan
-def _scan_head(ops, geo, reverse, init=0, y=0, last=0, states=0, gy=0, gy_st=(0, 0), grads=(0,) * 8):
+def _scan_head(ops, geo, G, reverse, init=0, y=0, last=0, states=0, gy=0, gy_st=(0, 0), grads=(0,) * 8):
     u, delta, A, B, Cm, skip, z, bias = ops
     _, n_seq, T, rows, max_len, off = geo
     packed = off is not None
     su, sd, sB, sC = _strides(u, packed), _strides(delta, packed), _strides(B, packed), _strides(Cm, packed)
     sz = _strides(z, packed) if z is not None else (0, 0)
     gu, gdelta, gA, gB, gC, gskip, gz, gbias = grads
-    return _SCAN.pack(_DTYPES[u.dtype], n_seq, u.shape[-1], B.shape[-1], B.shape[-2], reverse, T, rows, max_len, _ptr(off), u.data_ptr(),
+    return _SCAN.pack(_DTYPES[u.dtype], n_seq, u.shape[-1], A.shape[1], G, reverse, T, rows, max_len, _ptr(off), u.data_ptr(),
                       delta.data_ptr(), _ptr(z), B.data_ptr(), Cm.data_ptr(), su[0], su[1], sd[0], sd[1], sz[0], sz[1], sB[0], sB[1], sC[0], sC[1],
                       gy_st[0], gy_st[1], A.data_ptr(), _ptr(skip), _ptr(bias), init, y, last, states, gy, gu, gdelta, gz, gB, gC, gA, gskip, gbias)
 
 
-def _scan_forward(handle, u, delta, A, B, Cm, skip, z, bias, init, geo, reverse, want_last, train=False):
+def _scan_forward(handle, u, delta, A, B, Cm, skip, z, bias, init, geo, G, reverse, want_last, train=False):
     ops = (u, delta, A, B, Cm, skip, z, bias)
     y = _new_like(u)
     last = torch.empty(geo[1], u.shape[-1], A.shape[1], dtype=A.dtype, device=u.device) if want_last else None
@@ -303,7 +322,7 @@ def _scan_forward(handle, u, delta, A, B, Cm, skip, z, bias, init, geo, reverse,
         # a state of N every 8 steps of every sequence: (blocks of 8) D N values (rgp_ssm_scan_states_bytes)
         blocks = (geo[3] >> 3) + geo[1] if geo[5] is not None else geo[1] * ((geo[2] + 7) >> 3)
         states = torch.empty(blocks * A.numel(), dtype=A.dtype, device=u.device)
-    head = _scan_head(ops, geo, reverse, _ptr(init), y.data_ptr(), _ptr(last), _ptr(states))
+    head = _scan_head(ops, geo, G, reverse, _ptr(init), y.data_ptr(), _ptr(last), _ptr(states))
     work, tail = _new_work(handle, handle.lib.rgp_ssm_scan_workspace, head, 0)
     _call(handle, handle.lib.rgp_ssm_scan_forward, head, tail)
     return (y, last, states) if train else (y, last)
@@ -311,9 +330,9 @@ def _scan_forward(handle, u, delta, A, B, Cm, skip, z, bias, init, geo, reverse,
 
 class _ScanFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, handle, u, delta, A, B, Cm, skip, z, bias, init, geo, reverse, want_last):
-        y, last, states = _scan_forward(handle, u, delta, A, B, Cm, skip, z, bias, init, geo, reverse, want_last, True)
-        ctx.handle, ctx.geo, ctx.reverse = handle, geo, reverse
+    def forward(ctx, handle, u, delta, A, B, Cm, skip, z, bias, init, geo, G, reverse, want_last):
+        y, last, states = _scan_forward(handle, u, delta, A, B, Cm, skip, z, bias, init, geo, G, reverse, want_last, True)
+        ctx.handle, ctx.geo, ctx.G, ctx.reverse = handle, geo, G, reverse
         ctx.save_for_backward(u, delta, A, B, Cm, skip, z, bias, states)
         ctx.set_materialize_grads(False)
         if want_last:
@@ -324,21 +343,28 @@ class _ScanFn(torch.autograd.Function):
     def backward(ctx, gy, _):
         _once()
         if gy is None:
-            return (None,) * 13
+            return (None,) * 14
         saved = ctx.saved_tensors
         ops, states, handle = saved[:8], saved[8], ctx.handle
         gy = _inner(gy, 1)
         grads = [_new_like(t) for t in ops]
-        head = _scan_head(ops, ctx.geo, ctx.reverse, states=states.data_ptr(), gy=gy.data_ptr(), gy_st=_strides(gy, ctx.geo[5] is not None),
+        head = _scan_head(ops, ctx.geo, ctx.G, ctx.reverse, states=states.data_ptr(), gy=gy.data_ptr(), gy_st=_strides(gy, ctx.geo[5] is not None),
                           grads=[_ptr(t) for t in grads])
         work, tail = _new_work(handle, handle.lib.rgp_ssm_scan_workspace, head, 1)
         _call(handle, handle.lib.rgp_ssm_scan_backward, head, tail)
-        return (None, *grads, None, None, None, None)
+        return (None, *grads, None, None, None, None, None)
 
 
 def _scan_check(u, delta, A, B, Cm, D, z, delta_bias, lead):
-    """Operands in the form the library takes: (.., D) activations with contiguous features, (.., G, N) maps, contiguous parameters."""
+    """Operands in the form the library takes: (.., D) activations with contiguous features, (.., N) or (.., G, N) maps, contiguous
+    parameters."""
     nd, n = len(lead), u.shape[-1]
+    if _all_plain(u, (u, delta, B, Cm) if z is None else (u, delta, B, Cm, z), (A, D, delta_bias)):      # then only the shapes are left to check
+        sh, sb, N = u.shape, B.shape, A.shape[-1]
+        G = 1 if len(sb) == nd + 1 else sb[-2] if len(sb) == nd + 2 else 0
+        if delta.shape == sh and (z is None or z.shape == sh) and Cm.shape == sb and sb[:nd] == lead and sb[-1] == N and G and not n % G and 1 <= N <= 64 \
+                and A.shape == (n, N) and (D is None or D.shape == (n,)) and (delta_bias is None or delta_bias.shape == (n,)):
+            return (u, delta, A, B, Cm, D, z, delta_bias), G
     for name, t in (('delta', delta), ('z', z)):
         if t is not None:
             _rows(name, t, u, lead)
@@ -349,18 +375,18 @@ def _scan_check(u, delta, A, B, Cm, D, z, delta_bias, lead):
     if not isinstance(A, torch.Tensor) or A.dim() != 2 or not 1 <= A.shape[1] <= 64:
         _bad('A must be (D, N) with 1 to 64 states')
     N = A.shape[1]
-    maps = []
+    maps, groups = [], []
     for name, t in (('B', B), ('C', Cm)):
         _rows(name, t, u, lead)
-        if t.dim() == nd + 1:
-            t = t.unsqueeze(-2)
-        if t.dim() != nd + 2 or t.shape[-1] != N or t.shape[-2] < 1 or n % t.shape[-2]:
+        G = 1 if t.dim() == nd + 1 else t.shape[-2] if t.dim() == nd + 2 else 0
+        if t.shape[-1] != N or G < 1 or n % G:
             _bad('%s has shape %s: (.., N) or (.., G, N) with N = %d and G a divisor of D = %d expected' % (name, tuple(t.shape), N, n))
-        maps.append(_inner(t, 2))
-    if maps[0].shape[-2] != maps[1].shape[-2]:
-        _bad('B has %d groups, C %d' % (maps[0].shape[-2], maps[1].shape[-2]))
+        groups.append(G)
+        maps.append(_inner(t, t.dim() - nd))
+    if groups[0] != groups[1]:
+        _bad('B has %d groups, C %d' % tuple(groups))
     return (_inner(u, 1), _inner(delta, 1), _param('A', A, (n, N), u), maps[0], maps[1], _param('D', D, (n,), u, optional=True),
-            None if z is None else _inner(z, 1), _param('delta_bias', delta_bias, (n,), u, optional=True))
+            None if z is None else _inner(z, 1), _param('delta_bias', delta_bias, (n,), u, optional=True)), groups[0]
 
 
 def ssm_scan(handle, u, delta, A, B, Cm, D=None, z=None, delta_bias=None, seqs=None, init=None, reverse=False, return_state=False):
@@ -371,12 +397,12 @@ def ssm_scan(handle, u, delta, A, B, Cm, D=None, z=None, delta_bias=None, seqs=N
     the state behind the last step.  reverse=True walks every sequence from its last step.  Gradients: u, delta, A, B, C, D, z, delta_bias
     (states take none)."""
     geo = _geometry(handle, u, seqs, 'u')
-    ops = _scan_check(u, delta, A, B, Cm, D, z, delta_bias, geo[0])
+    ops, G = _scan_check(u, delta, A, B, Cm, D, z, delta_bias, geo[0])
     if init is not None:
         _no_grad_state('init', init)
         init = _param('init', init, (geo[1], u.shape[-1], A.shape[1]), u)
     run = _ScanFn.apply if _wants_grad(*ops) else _scan_forward
-    y, last = run(handle, *ops, init, geo, bool(reverse), bool(return_state))
+    y, last = run(handle, *ops, init, geo, G, bool(reverse), bool(return_state))
     return (y, last) if return_state else y
 
 
@@ -387,14 +413,13 @@ def ssm_scan_step(handle, u, delta, A, B, Cm, D, state, z=None, delta_bias=None)
         _bad('u must be (batch, D)')
     geo = _geometry(handle, u, None, 'u', step=True)
     _no_step_grad(u, delta, A, B, Cm, D, z, delta_bias)
-    with torch.no_grad():
-        u, delta, A, B, Cm, skip, z, bias = _scan_check(u, delta, A, B, Cm, D, z, delta_bias, geo[0])
+    (u, delta, A, B, Cm, skip, z, bias), G = _scan_check(u, delta, A, B, Cm, D, z, delta_bias, geo[0])
     n, Dn = u.shape
     N = A.shape[1]
     _state('state', state, (n, Dn, N), A.dtype, u)
     y, st = _new_like(u), state.data_ptr()
     _call(handle, handle.lib.rgp_ssm_scan_step, _SCAN.pack(
-        _DTYPES[u.dtype], n, Dn, N, B.shape[-2], 0, 1, n, 1, 0, u.data_ptr(), delta.data_ptr(), _ptr(z), B.data_ptr(), Cm.data_ptr(), 0, u.stride(0), 0,
+        _DTYPES[u.dtype], n, Dn, N, G, 0, 1, n, 1, 0, u.data_ptr(), delta.data_ptr(), _ptr(z), B.data_ptr(), Cm.data_ptr(), 0, u.stride(0), 0,
         delta.stride(0), 0, 0 if z is None else z.stride(0), 0, B.stride(0), 0, Cm.stride(0), 0, 0, A.data_ptr(), _ptr(skip), _ptr(bias), st,
         y.data_ptr(), st, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0))
     return y
