@@ -144,8 +144,8 @@ static __device__ __forceinline__ A seq_sigmoid(A x) { return seq_rcp((A)1 + seq
 // ---- rows of sequences --------------------------------------------------------------------------------------------------------------
 // off == nullptr: n_seq sequences of T steps, step t of sequence s at base + s * sb + t * st; otherwise packed rows, step t of sequence s
 // at base + (off[s] + t) * st.  Sequences are cut into blocks of L = 2^lg steps that never cross a sequence; block j of sequence i is number
-// i * ceil(T / L) + j, or floor(off[i] / L) + i + j for packed rows: those numbers are increasing, distinct and below rows / L + n_seq
-// without a table of block counts (some stay empty).  Offsets are clamped to the rows there are, so a wrong table cannot make a kernel
+// j * n_seq + i (neighbours in number are neighbours in memory), or floor(off[i] / L) + i + j for packed rows: those numbers are increasing,
+// distinct and below rows / L + n_seq without a table of block counts (some stay empty).  Offsets are clamped to the rows there are, so a wrong table cannot make a kernel
 // touch memory outside its tensors.
 struct SeqGeo {
   const int64_t* off;
@@ -167,12 +167,12 @@ static __device__ __forceinline__ int64_t seq_off(const SeqGeo& g, int64_t i) {
 static __device__ __forceinline__ SeqBlock seq_find(const SeqGeo& g, uint32_t slot, int lg) {       // slot < 2^32, host-checked
   SeqBlock b;
   if (!g.off) {
-    const uint32_t per = (uint32_t)((g.T + ((int64_t)1 << lg) - 1) >> lg), q = slot / per;
-    b.seq = q;
-    b.j = slot - q * per;
+    const uint32_t q = slot / (uint32_t)g.n_seq;
+    b.seq = slot - q * (uint32_t)g.n_seq;
+    b.j = q;
     b.start = b.seq * g.T;
     b.len = g.T;
-    b.ok = b.seq < g.n_seq;
+    b.ok = (b.j << lg) < g.T;
     return b;
   }
   int lo = 0, hi = g.n_seq - 1;                         // the last i with floor(off[i] / L) + i <= slot
@@ -188,8 +188,9 @@ static __device__ __forceinline__ SeqBlock seq_find(const SeqGeo& g, uint32_t sl
   b.ok = b.j >= 0 && (b.j << lg) < b.len;
   return b;
 }
-static __device__ __forceinline__ int64_t seq_slot0(const SeqGeo& g, int64_t seq, int64_t start, int lg) {
-  return g.off ? (start >> lg) + seq : seq * ((g.T + ((int64_t)1 << lg) - 1) >> lg);
+// the number of block j of a sequence
+static __device__ __forceinline__ int64_t seq_slot(const SeqGeo& g, int64_t seq, int64_t start, int lg, int64_t j) {
+  return g.off ? (start >> lg) + seq + j : j * g.n_seq + seq;
 }
 struct SeqStride { int64_t st, sb; };
 template <typename T>

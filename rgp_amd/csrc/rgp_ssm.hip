@@ -2,6 +2,8 @@
 // blocks of the split, the sums over partial results, the scan's form for one step, and the short causal convolution.
 #include "rgp_ssm.h"
 
+#include <type_traits>
+
 // ---- sums of partial results in a fixed order -----------------------------------------------------------------------------------------
 // A workgroup forms 64 outputs of one of up to five sums, 16 threads for each: thread q adds partials q, q + 16, ... in eight interleaved
 // sums (that many loads are in flight), then the 16 are added in LDS; up to SEQ_FEW partials are added by one thread an output.  The order depends on the count of partials alone.
@@ -92,7 +94,7 @@ static __global__ void __launch_bounds__(Q == 1 ? 256 : Q * 64) ssm_join_kernel(
     const int64_t end = seq_off(d.g, seq + 1);
     len = end > start ? end - start : 0;
   }
-  const int64_t nb = (len + d.L - 1) >> d.lg, slot0 = seq_slot0(d.g, seq, start, d.lg);
+  const int64_t nb = (len + d.L - 1) >> d.lg, slot0 = seq_slot(d.g, seq, start, d.lg, 0), step = d.g.off ? 1 : d.g.n_seq;
   const int64_t each = (nb + Q - 1) / Q, j0 = q * each < nb ? q * each : nb, j1 = !ok ? j0 : (j0 + each < nb ? j0 + each : nb);
   const int64_t at0 = ok ? dn : 0, ch = at0 / a.N;
   const A Av = ssm_finite(((const A*)a.A)[at0]);
@@ -100,28 +102,38 @@ static __global__ void __launch_bounds__(Q == 1 ? 256 : Q * 64) ssm_join_kernel(
   const A* const sum = (const A*)d.sumdt + slot0 * a.D + ch;
   A P = (A)1, H = (A)0, s = (A)0;
   if (Q == 1) s = !back && a.init && ok ? ((const A*)a.init)[seq * DN + dn] : (A)0;
-  for (int pass = Q == 1 ? 1 : 0; pass < 2; ++pass) {
-    for (int64_t j = j0; j < j1; j += JOIN_U) {
-      A p[JOIN_U], e[JOIN_U];
+  const int64_t dp = (back ? -step : step) * DN, ds = (back ? -step : step) * a.D;
+  // up to n of the `left` blocks from pp / ps on: their sums are read together, then walked.  (The block that nothing follows has left no
+  // sums: what is read there goes unused.)
+  auto walk = [&](A* pp, const A* ps, int left, auto n, int pass) {
+    A p[n()], e[n()];
 #pragma unroll
-      for (int i = 0; i < JOIN_U; ++i) {                  // the block that nothing follows has left no sums: what is read there goes unused
-        const int64_t jj = j + i < j1 ? j + i : j, at = back ? nb - 1 - jj : jj;
-        p[i] = part[at * DN];
-        e[i] = seq_exp(Av * sum[at * a.D]);
-      }
+    for (int i = 0; i < n(); ++i) {
+      const int k = i < left ? i : 0;
+      p[i] = pp[k * dp];
+      e[i] = seq_exp(Av * ps[k * ds]);
+    }
 #pragma unroll
-      for (int i = 0; i < JOIN_U; ++i) {
-        if (j + i < j1) {
-          if (pass == 0) {
-            P *= e[i];
-            H = e[i] * H + p[i];
-          } else {
-            part[(back ? nb - 1 - (j + i) : j + i) * DN] = s;
-            s = e[i] * s + p[i];
-          }
+    for (int i = 0; i < n(); ++i) {
+      if (i < left) {
+        if (pass == 0) {
+          P *= e[i];
+          H = e[i] * H + p[i];
+        } else {
+          pp[i * dp] = s;
+          s = e[i] * s + p[i];
         }
       }
     }
+  };
+  for (int pass = Q == 1 ? 1 : 0; pass < 2; ++pass) {
+    A* pp = part + (back ? nb - 1 - j0 : j0) * step * DN;
+    const A* ps = sum + (back ? nb - 1 - j0 : j0) * step * a.D;
+    int left = (int)(j1 - j0);
+    for (; left >= JOIN_U; left -= JOIN_U, pp += JOIN_U * dp, ps += JOIN_U * ds) walk(pp, ps, JOIN_U, std::integral_constant<int, JOIN_U>(), pass);
+    if (left > 3) walk(pp, ps, left, std::integral_constant<int, JOIN_U>(), pass);
+    else if (left > 1) walk(pp, ps, left, std::integral_constant<int, 3>(), pass);
+    else if (left > 0) walk(pp, ps, left, std::integral_constant<int, 1>(), pass);
     if (pass == 0) {
       shP[q][l] = P;
       shH[q][l] = H;
@@ -190,7 +202,7 @@ static void scan_plan(const rgp_ssm_scan* a, bool back, ScanPlan& p) {
   d.lg = lg;
   d.L = (int64_t)1 << lg;
   const int64_t deep = (longest + d.L - 1) >> d.lg;
-  p.Q = deep <= 8 ? 1 : deep <= 128 ? 4 : 16;
+  p.Q = deep <= 8 || (double)a->n_seq * a->D * a->N >= 524288.0 ? 1 : deep <= 128 ? 4 : 16;      // one where the pairs alone fill the card
   d.nslot = seq_blocks(d.g, d.lg);
   const int64_t DN = (int64_t)a->D * a->N;
   p.part_bytes = p.split ? up256(d.nslot * DN * p.acc) : 0;
@@ -407,7 +419,7 @@ static __global__ void __launch_bounds__(256) conv_fwd_kernel(ConvDev d) {
   if (!b.ok) return;
   const int64_t t0 = b.j << d.lg;
   const int L = 1 << d.lg, nt = b.len - t0 < L ? (int)(b.len - t0) : L;
-  A w[W][V], bias[V], x[W][V];                     // x: the window, in the arithmetic type
+  A w[W][V], bias[V], x[W - 1 + CONV_FLY][V];      // x: the W - 1 rows before a batch of steps and the batch's, in the arithmetic type
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     bias[i] = a.bias ? ((const A*)a.bias)[c + i] : (A)0;
@@ -424,32 +436,30 @@ static __global__ void __launch_bounds__(256) conv_fwd_kernel(ConvDev d) {
   T* pv = (T*)a.v + seq_row_index(d.g, b, t0) * a.D + c;
   const int64_t sx = d.g.reverse ? -a.x_st : a.x_st, vrow = (d.g.off ? 1 : (int64_t)a.n_seq) * a.D, sv = d.g.reverse ? -vrow : vrow;
   for (int tb = 0; tb < nt; tb += CONV_FLY) {
-    Vec r[CONV_FLY];                               // this many rows are in flight at once; behind the end the last row again
 #pragma unroll
-    for (int k = 0; k < CONV_FLY; ++k) {
-      r[k] = *(const Vec*)px;
+    for (int k = 0; k < CONV_FLY; ++k) {           // behind the end the last row again
+      const Vec r = *(const Vec*)px;
       px += tb + k + 1 < nt ? sx : 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[W - 1 + k][i] = (A)r.e[i];
     }
 #pragma unroll
     for (int k = 0; k < CONV_FLY; ++k) {
-      if (tb + k < nt) {
-        Vec o;
+      Vec o;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          x[W - 1][i] = (A)r[k].e[i];
-          A p = bias[i];
+      for (int i = 0; i < V; ++i) {
+        A p = bias[i];
 #pragma unroll
-          for (int j = 0; j < W; ++j) p += w[j][i] * x[j][i];
-          o.e[i] = (T)(p * seq_sigmoid(p));
-        }
-        *(Vec*)pv = o;
-        pv += sv;
-#pragma unroll
-        for (int j = 0; j < W - 1; ++j)
-#pragma unroll
-          for (int i = 0; i < V; ++i) x[j][i] = x[j + 1][i];
+        for (int j = 0; j < W; ++j) p += w[j][i] * x[k + j][i];
+        o.e[i] = (T)(p * seq_sigmoid(p));
       }
+      if (tb + k < nt) *(Vec*)pv = o;
+      pv += sv;
     }
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[j][i] = x[j + CONV_FLY][i];
   }
 }
 // the W - 1 inputs before the step behind the last one
@@ -503,10 +513,12 @@ static __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvDev d) {
       const SeqBlock b = seq_find(d.g, d.lanes == 64 ? (uint32_t)__builtin_amdgcn_readfirstlane((int)run) : (uint32_t)run, d.lg);
       if (!b.ok) continue;
       const int64_t t0 = b.j << d.lg, L = (int64_t)1 << d.lg, t1 = t0 + L < b.len ? t0 + L : b.len;
-      A x[W][V], gp[W][V];
+      // x and gp: the W - 1 steps before a batch and the batch's.  Steps past the end are computed like the others, with gp = 0: branches
+      // around them would keep the windows from being renamed instead of moved.
+      A x[W - 1 + CONV_FLY][V], gp[W - 1 + CONV_FLY][V];
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const Vec r = conv_x<T, W, V>(d, b, t0 - (W - 1) + (j < W - 1 ? j : 0), c);
+      for (int j = 0; j < W - 1; ++j) {
+        const Vec r = conv_x<T, W, V>(d, b, t0 - (W - 1) + j, c);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           x[j][i] = (A)r.e[i];
@@ -520,54 +532,48 @@ static __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvDev d) {
       T* po = (T*)a.gx + seq_row_index(d.g, b, t0) * a.D + c;
       const int64_t orow = (d.g.off ? 1 : (int64_t)a.n_seq) * a.D;
       const int64_t sx = d.g.reverse ? -a.x_st : a.x_st, sg = d.g.reverse ? -a.gv_st : a.gv_st, so = d.g.reverse ? -orow : orow;
+      po -= (W - 1) * so;                                                // moves with gp's step, W - 1 steps ahead of gx's
       for (int kb = 0; kb < nt; kb += CONV_FLY) {
-        Vec rx[CONV_FLY], rg[CONV_FLY];
+        Vec rg[CONV_FLY];
 #pragma unroll
         for (int k = 0; k < CONV_FLY; ++k) {
-          rx[k] = *(const Vec*)px;                                       // behind the end the last row again
+          const Vec r = *(const Vec*)px;                                 // behind the end the last row again
           rg[k] = *(const Vec*)pg;
           px += kb + k + 1 < have ? sx : 0;
           pg += kb + k + 1 < have ? sg : 0;
+#pragma unroll
+          for (int i = 0; i < V; ++i) x[W - 1 + k][i] = (A)r.e[i];
         }
 #pragma unroll
         for (int k = 0; k < CONV_FLY; ++k) {
-          if (kb + k < nt) {
+          Vec o;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-              x[W - 1][i] = (A)rx[k].e[i];
-              A p = bias[i];
+          for (int i = 0; i < V; ++i) {
+            A p = bias[i];
 #pragma unroll
-              for (int j = 0; j < W; ++j) p += w[j][i] * x[j][i];
-              const A sg = seq_sigmoid(p);
-              const A q = kb + k < have ? (A)rg[k].e[i] * (sg + p * sg * ((A)1 - sg)) : (A)0;
-              gp[W - 1][i] = q;
-              if (kb + k < in) {
-                gb[i] += q;
+            for (int j = 0; j < W; ++j) p += w[j][i] * x[k + j][i];
+            const A sg_ = seq_sigmoid(p);
+            const A q = kb + k < have ? (A)rg[k].e[i] * (sg_ + p * sg_ * ((A)1 - sg_)) : (A)0;
+            gp[W - 1 + k][i] = q;
+            const A own = kb + k < in ? q : (A)0;                        // the W - 1 steps behind the run count in the next one
+            gb[i] += own;
 #pragma unroll
-                for (int j = 0; j < W; ++j) gw[j][i] += q * x[j][i];
-              }
-            }
-            if (kb + k >= W - 1) {
-              Vec o;
+            for (int j = 0; j < W; ++j) gw[j][i] += own * x[k + j][i];
+            A v = (A)0;
 #pragma unroll
-              for (int i = 0; i < V; ++i) {
-                A v = (A)0;
-#pragma unroll
-                for (int j = 0; j < W; ++j) v += w[W - 1 - j][i] * gp[j][i];      // gp[j] is j steps on, and its tap W - 1 - j reads this x
-                o.e[i] = (T)v;
-              }
-              *(Vec*)po = o;
-              po += so;
-            }
-#pragma unroll
-            for (int j = 0; j < W - 1; ++j)
-#pragma unroll
-              for (int i = 0; i < V; ++i) {
-                x[j][i] = x[j + 1][i];
-                gp[j][i] = gp[j + 1][i];
-              }
+            for (int j = 0; j < W; ++j) v += w[W - 1 - j][i] * gp[k + j][i];      // gp[k + j] is j steps on, and its tap W - 1 - j reads this x
+            o.e[i] = (T)v;
           }
+          if (kb + k >= W - 1 && kb + k < nt) *(Vec*)po = o;
+          po += so;
         }
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            x[j][i] = x[j + CONV_FLY][i];
+            gp[j][i] = gp[j + CONV_FLY][i];
+          }
       }
     }
   A* const part = (A*)d.part + (int64_t)blockIdx.x * (W + 1) * a.D;      // [W][D] taps, then [D] bias
@@ -633,8 +639,8 @@ static void conv_plan(const rgp_ssm_conv* a, bool wide, ConvDev& d, int64_t& nrb
   const int V = wide ? CONV_V(seq_dtype_bytes(a->dtype)) : 1;
   d.nvec = (a->D + V - 1) / V;
   d.same = d.nvec % 64 == 0;
-  // runs of 16 steps (the W - 1 rows before a run come from cache) unless that leaves fewer than four waves a SIMD
-  for (d.lg = 4; d.lg > 3 && seq_blocks(d.g, d.lg) * d.nvec < 262144; --d.lg) {}
+  // runs of 16 steps (the W - 1 rows before a run come from cache) unless that leaves fewer than two waves a SIMD
+  for (d.lg = 4; d.lg > 3 && seq_blocks(d.g, d.lg) * d.nvec < 131072; --d.lg) {}
   d.nrun = seq_blocks(d.g, d.lg);
   d.lanes = 1;
   while (d.lanes < 64 && d.lanes < d.nvec) d.lanes *= 2;

@@ -60,7 +60,8 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
     carry[r] = MODE == 0 && d.part && ok ? ((const A*)d.part)[(slot * a.D + ch0 + ch) * N + k * R + r] : (A)0;
     gA[r] = (A)0;
   }
-  const A* const ckpt = MODE == 0 ? (const A*)a.states + (seq_slot0(d.g, b.seq, b.start, SSM_CK_LG) * a.D + ch0 + ch) * N + k * R : nullptr;
+  const A* const ckpt = MODE == 0 ? (const A*)a.states + (seq_slot(d.g, b.seq, b.start, SSM_CK_LG, t0 >> SSM_CK_LG) * a.D + ch0 + ch) * N + k * R : nullptr;
+  const int64_t cks = (d.g.off ? 1 : (int64_t)d.g.n_seq) * a.D * N;
   const SeqStride su{a.u_st, a.u_sb}, sd{a.delta_st, a.delta_sb}, sz{a.z_st, a.z_sb}, sB{a.B_st, a.B_sb}, sC{a.C_st, a.C_sb}, sg{a.gy_st, a.gy_sb};
   auto decay = [&](A dt, int r) {
     return sizeof(A) == 4 ? (A)seq_exp2((float)(dt * (Ar[r] * (A)1.44269504088896341))) : seq_exp(dt * Ar[r]);
@@ -139,7 +140,7 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
         if (tb >= nt) continue;
         A s0[R], s[CK][R], e[CK][R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) s0[r] = live && k * R + r < N ? ckpt[((tt + tb) / CK) * ((int64_t)a.D * N) + r] : (A)0;
+        for (int r = 0; r < R; ++r) s0[r] = live && k * R + r < N ? ckpt[(int)((tt + tb - t0) >> SSM_CK_LG) * cks + r] : (A)0;
         // operands of a step are read from LDS while the step before is computed
         Four p = pl[tb][cp];
         Quad B = Bl[tb][k], C;

@@ -65,7 +65,9 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
       else if (a.init) s[r] = ((const A*)a.init)[(b.seq * a.D + ch0 + ch) * N + k * R + r];
     }
   }
-  A* const ckpt = MODE == 0 && a.states ? (A*)a.states + ((seq_slot0(d.g, b.seq, b.start, SSM_CK_LG)) * a.D + ch0 + ch) * N + k * R : nullptr;
+  // the states of the block: every CK steps, a stride of cks values apart
+  A* const ckpt = MODE == 0 && a.states ? (A*)a.states + (seq_slot(d.g, b.seq, b.start, SSM_CK_LG, t0 >> SSM_CK_LG) * a.D + ch0 + ch) * N + k * R : nullptr;
+  const int64_t cks = (d.g.off ? 1 : (int64_t)d.g.n_seq) * a.D * N;
   const SeqStride su{a.u_st, a.u_sb}, sd{a.delta_st, a.delta_sb}, sz{a.z_st, a.z_sb}, sB{a.B_st, a.B_sb}, sC{a.C_st, a.C_sb};
 
   Vec ru[NI], rd[NI], rz[NI];
@@ -120,7 +122,7 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
     if (tt + TL < t1) fetch(tt + TL);
     for (int tb = 0; tb < nt; tb += CK) {
       if (MODE == 0 && ckpt && live) {
-        A* const c = ckpt + (tt + tb) / CK * ((int64_t)a.D * N);
+        A* const c = ckpt + (int)((tt + tb - t0) >> SSM_CK_LG) * cks;
         if (N == NP) {
 #pragma unroll
           for (int r = 0; r < R; ++r) c[r] = s[r];
