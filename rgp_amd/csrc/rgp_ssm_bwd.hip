@@ -181,14 +181,17 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
           g1 = seq_sum<K>(g1);
           g2 = seq_sum<K>(g2);
           yd = seq_sum<K>(yd);
-          Four o;                                                 // the same in all K lanes
-          o.x = p.x * g1 + skip * p.z;
-          o.y = (p.y * g1 + g2) * p.w;
-          o.z = yd + skip * p.y;
-          o.w = (A)0;
+          // the same in all K lanes; lane k writes the k-th (every lane all of them where K < 4), without a branch around the store
+          const A o0 = p.x * g1 + skip * p.z, o1 = (p.y * g1 + g2) * p.w, o2 = yd + skip * p.y;
           gD += p.z * p.y;
-          gbias += o.y;
-          if (k == 0) pl[t][cp] = o;
+          gbias += o1;
+          if constexpr (K >= 4) {
+            ((A*)&pl[t][cp])[k & 3] = (k & 3) == 0 ? o0 : (k & 3) == 1 ? o1 : o2;
+          } else {
+            Four o;
+            o.x = o0; o.y = o1; o.z = o2; o.w = (A)0;
+            pl[t][cp] = o;
+          }
           // over the wave's channels: lane bit 5 selects gB / gC, bit 4 and bit 3 the state
           const bool b3 = (lane & 8) != 0;
           A f0 = seq_fold<true>(vB[0], vC[0]), f1 = seq_fold<true>(vB[1], vC[1]), f2 = seq_fold<true>(vB[2], vC[2]), f3 = seq_fold<true>(vB[3], vC[3]);
@@ -203,7 +206,7 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
             if constexpr (K <= 4) f += seq_xor4(f);
             if constexpr (K <= 2) f += seq_dpp<0x4E>(f);
             if constexpr (K == 1) f += seq_dpp<0xB1>(f);
-            if ((lane & 7) == k) f_to[b3] = f;
+            f_to[b3] = f;                                         // lanes that hold the same sum write it to the same place
           }
           p = pn;
           B = Bn;

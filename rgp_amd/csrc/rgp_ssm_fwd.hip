@@ -147,7 +147,7 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
         }
         if (MODE == 0) {
           acc = seq_sum<K>(acc);
-          if (k == 0) pl[t][cp].dt = acc;
+          pl[t][cp].dt = acc;                                     // all K lanes, the same value
         }
       }
     }
