@@ -182,20 +182,19 @@ static void scan_plan(const rgp_ssm_scan* a, bool back, ScanPlan& p) {
   if (p.K == 4 && (d.Dg + 15) / 16 * 16 < (d.Dg + 63) / 64 * 64) p.CH = 16;
   d.ncb = (d.Dg + p.CH - 1) / p.CH;
   const int64_t longest = a->off ? (a->max_len > 0 && a->max_len < a->rows ? a->max_len : a->rows) : a->T;
-  // Split over time.  In units of the time in which a SIMD with several waves walks one wave's step: unsplit, the whole work spread over
-  // 1024 SIMDs, but no less than the longest sequence at twice that time (a lone wave waits for its own results); split, about 1.65 times
-  // the work (the state's part of it is done twice), the two walks over one block, and the join.  Blocks of 64 steps, of 32 where that
-  // leaves most SIMDs idle, longer ones where the waves get many: shorter blocks balance ragged lengths, longer ones leave the join (and
-  // the sums of the backward pass) less to read.
+  // Split over time.  In units of the time in which a SIMD with several waves walks one wave's step (about 80 ns forward, 260 ns backward):
+  // unsplit, the whole work spread over 1024 SIMDs, but no less than the longest sequence at twice that time (a lone wave waits for its own
+  // results); split, the work, a walk over one block, the first walk (0.65 of the forward one, 0.3 of the backward one), and the join.
+  // Measured at 8 x 1024 x 1024 bf16, N = 32, backward: 445 us unsplit; 16 x 16 blocks of the same case at N = 16: 186 split.  Blocks of 64
+  // steps, of 32 where that leaves most SIMDs idle, longer ones where the waves get many: shorter blocks balance ragged lengths, longer ones
+  // leave the join (and the sums of the backward pass) less to read.
   const double waves = (double)a->G * d.ncb * (p.CH * p.K / 64.0), work = waves * a->rows / 1024.0, most = back ? 12288.0 : 24576.0;
   auto count = [&](int g) { return waves * ((double)(a->rows >> g) + a->n_seq); };
   int lg = count(6) < 1024.0 ? 5 : 6;
   while (lg < 20 && count(lg) > most) ++lg;
-  const double one = work > 2.0 * longest ? work : 2.0 * longest, two = 1.65 * (work + 2.0 * ((int64_t)1 << lg)) + 130.0;
+  const double one = work > 2.0 * longest ? work : 2.0 * longest, block = 2.0 * ((int64_t)1 << lg);
+  const double two = back ? 1.3 * (work + block) + 80.0 : 1.65 * (work + block) + 130.0;
   if (!(two < one)) lg = 0;
-#ifdef SSM_TUNE
-  if (getenv("SSM_LG")) lg = atoi(getenv("SSM_LG"));
-#endif
   p.split = lg > 0;
   if (!p.split)
     for (lg = 6; ((int64_t)1 << lg) < (a->off ? a->rows : a->T); ++lg) {}
