@@ -257,6 +257,18 @@ class _ConvFn(torch.autograd.Function):
         return None, gx, gw, gb, None, None, None, None
 
 
+def _conv_check(x, weight, bias):
+    """x, filters and bias in the form the library takes."""
+    D = x.shape[-1]
+    if _all_plain(x, (x,), (weight, bias)):
+        sw = weight.shape
+        if len(sw) == 2 and sw[0] == D and 2 <= sw[1] <= 8 and (bias is None or bias.shape == (D,)):
+            return x, weight, bias
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not 2 <= weight.shape[1] <= 8:
+        _bad('weight must be (D, W) with 2 to 8 taps')
+    return _inner(x, 1), _param('weight', weight, (D, weight.shape[1]), x), _param('bias', bias, (D,), x, optional=True)
+
+
 def ssm_conv(handle, x, weight, bias=None, seqs=None, init=None, reverse=False, return_state=False):
     """silu(bias + causal convolution of x with one filter per channel): v_t uses x_{t-W+1} .. x_t of its own sequence.
 
@@ -266,16 +278,12 @@ def ssm_conv(handle, x, weight, bias=None, seqs=None, init=None, reverse=False, 
     take none)."""
     geo = _geometry(handle, x, seqs, 'x')
     D = x.shape[-1]
-    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not 2 <= weight.shape[1] <= 8:
-        _bad('weight must be (D, W) with 2 to 8 taps')
-    w = _param('weight', weight, (D, weight.shape[1]), x)
-    b = _param('bias', bias, (D,), x, optional=True)
+    x, w, b = _conv_check(x, weight, bias)
     if init is not None:
         _no_grad_state('init', init)
         if init.shape != (geo[1], w.shape[1] - 1, D) or init.dtype is not x.dtype or init.device != x.device:
             _bad('init must be %s of shape %s on %s' % (x.dtype, (geo[1], w.shape[1] - 1, D), x.device))
         init = init.contiguous()
-    x = _inner(x, 1)
     run = _ConvFn.apply if _wants_grad(x, w, b) else _conv_forward
     v, last = run(handle, x, w, b, init, geo, bool(reverse), bool(return_state))
     return (v, last) if return_state else v
@@ -287,13 +295,10 @@ def ssm_conv_step(handle, x, weight, bias, state):
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         _bad('x must be (batch, D)')
     geo = _geometry(handle, x, None, 'x', step=True)
-    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not 2 <= weight.shape[1] <= 8:
-        _bad('weight must be (D, W) with 2 to 8 taps')
     D = x.shape[1]
-    w, b = _param('weight', weight, (D, weight.shape[1]), x), _param('bias', bias, (D,), x, optional=True)
-    _no_step_grad(x, weight, bias)
-    _state('state', state, (x.shape[0], weight.shape[1] - 1, D), x.dtype, x)
-    x = _inner(x, 1)
+    x, w, b = _conv_check(x, weight, bias)
+    _no_step_grad(x, w, b)
+    _state('state', state, (x.shape[0], w.shape[1] - 1, D), x.dtype, x)
     v, st = _new_like(x), state.data_ptr()
     _call(handle, handle.lib.rgp_ssm_conv_step, _CONV.pack(_DTYPES[x.dtype], x.shape[0], D, w.shape[1], 0, 0, 1, x.shape[0], 1, 0, x.data_ptr(), 0,
                                                           x.stride(0), 0, 0, w.data_ptr(), _ptr(b), st, v.data_ptr(), st, 0, 0, 0, 0))
@@ -476,14 +481,17 @@ def rms_norm(handle, x, weight, residual=None, eps=1e-6):
     eps = float(eps)
     if not eps > 0.0 or math.isinf(eps):
         _bad('eps must be positive')
-    w = _param('weight', weight, x.shape[-1:], x)
-    if residual is not None:
-        _rows('residual', residual, x, x.shape)
-        if residual.dim() != x.dim():
-            _bad('residual has shape %s, x %s' % (tuple(residual.shape), tuple(x.shape)))
     shape, two = x.shape, x.dim() == 2
-    x2 = _inner(x if two else x.reshape(-1, shape[-1]), 1)
-    r2 = None if residual is None else _inner(residual if two else residual.reshape(-1, shape[-1]), 1)
+    if two and _all_plain(x, (x,) if residual is None else (x, residual), (weight,)) and weight.shape == shape[1:] and (residual is None or residual.shape == shape):
+        x2, r2, w = x, residual, weight
+    else:
+        w = _param('weight', weight, shape[-1:], x)
+        if residual is not None:
+            _rows('residual', residual, x, shape)
+            if residual.dim() != x.dim():
+                _bad('residual has shape %s, x %s' % (tuple(residual.shape), tuple(shape)))
+        x2 = _inner(x if two else x.reshape(-1, shape[-1]), 1)
+        r2 = None if residual is None else _inner(residual if two else residual.reshape(-1, shape[-1]), 1)
     y, hid = (_RmsFn.apply if _wants_grad(x2, r2, w) else _rms_forward)(handle, x2, w, r2, eps)
     if not two:
         y, hid = y.view(shape), None if hid is None else hid.view(shape)
@@ -493,18 +501,24 @@ def rms_norm(handle, x, weight, residual=None, eps=1e-6):
 # ---------------------------------------------------------------------------------------------------------------------- gradient norm
 def _grad_list(handle, grads):
     """(n, addresses, element counts, types) of one call's tensors, checked; the arrays live as long as the tuple."""
-    n = len(grads)
-    for i, g in enumerate(grads):
-        if not isinstance(g, torch.Tensor) or g.dtype not in _DTYPES or g.device != handle.device or g.layout is not torch.strided:
-            _bad('gradient %d must be a float64, float32, bfloat16 or float16 tensor on %s' % (i, handle.device))
-        if not g.is_contiguous() and g.numel() and (_overlaps(g) or sum((m - 1) * s for m, s in zip(g.shape, g.stride())) + 1 != g.numel()):
-            _bad('gradient %d has gaps or repeats in memory: it cannot be clipped in place as one range' % i)
-    ptr, numel, dtype = [g.data_ptr() for g in grads], [g.numel() for g in grads], [_DTYPES[g.dtype] for g in grads]
+    n, dev = len(grads), handle.device
+    try:
+        plain = all([g.device == dev and g.is_contiguous() for g in grads])
+        dtype = [_DTYPES[g.dtype] for g in grads]
+    except (AttributeError, KeyError, RuntimeError):
+        plain = False
+    if not plain:
+        for i, g in enumerate(grads):
+            if not isinstance(g, torch.Tensor) or g.dtype not in _DTYPES or g.device != dev or g.layout is not torch.strided:
+                _bad('gradient %d must be a float64, float32, bfloat16 or float16 tensor on %s' % (i, dev))
+            if not g.is_contiguous() and g.numel() and (_overlaps(g) or sum((m - 1) * s for m, s in zip(g.shape, g.stride())) + 1 != g.numel()):
+                _bad('gradient %d has gaps or repeats in memory: it cannot be clipped in place as one range' % i)
+    ptr, numel = [g.data_ptr() for g in grads], [g.numel() for g in grads]
     end = 0
-    for p, k, d in sorted(t for t in zip(ptr, numel, dtype) if t[1]):
-        if p < end:
+    for p, k, d in sorted(zip(ptr, numel, dtype)):
+        if p < end and k:
             _bad('two gradients share memory: each element may be clipped once')
-        end = p + k * _BYTES[d]
+        end = max(end, p + k * _BYTES[d])
     return n, struct.pack('%dQ' % n, *ptr), struct.pack('%dq' % n, *numel), struct.pack('%di' % n, *dtype)
 
 
