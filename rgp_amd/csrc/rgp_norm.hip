@@ -271,7 +271,7 @@ static const char* rms_bad(const rgp_rms_norm* a) {
   if (!a) return "null arguments";
   if (a->dtype < 0 || a->dtype > 3) return "dtype must be RGP_F64, RGP_F32, RGP_BF16 or RGP_F16";
   if (a->rows < 0 || a->C < 1) return "empty rows";
-  if (!(a->eps > 0.0)) return "eps must be positive";
+  if (!(a->dtype == RGP_F64 ? a->eps > 0.0 : (float)a->eps > 0.0f)) return "eps must be positive in the arithmetic type";
   return nullptr;
 }
 extern "C" int64_t rgp_rms_norm_workspace(const rgp_rms_norm* a, int backward) {

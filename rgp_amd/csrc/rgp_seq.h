@@ -192,6 +192,7 @@ static __device__ __forceinline__ SeqBlock seq_find(const SeqGeo& g, uint32_t sl
 static __device__ __forceinline__ int64_t seq_slot(const SeqGeo& g, int64_t seq, int64_t start, int lg, int64_t j) {
   return g.off ? (start >> lg) + seq + j : j * g.n_seq + seq;
 }
+#define SEQ_MOST ((int64_t)1 << 40)            // rows: products of sizes stay below 2^63
 struct SeqStride { int64_t st, sb; };
 template <typename T>
 static __device__ __forceinline__ T* seq_row(T* base, const SeqGeo& g, const SeqBlock& b, SeqStride s, int64_t t) {
@@ -204,12 +205,13 @@ static __device__ __forceinline__ int64_t seq_row_index(const SeqGeo& g, const S
 }
 
 // out[i] = sum over p < P of part[p * stride + i], i < n, rounded to type dt; up to five such sums in one launch, each in a fixed order (no
-// atomics: results do not depend on timing).  turn > 1: the partials are [turn][n / turn], out is [n / turn][turn].
-struct SeqSum { const void* part; int64_t P, stride, n; void* out; int dt, turn, block0; };
+// atomics: results do not depend on timing).  turn > 1: the partials are [turn][n / turn], out is [n / turn][turn].  end: outputs from
+// end[0] * per on stay as they are (rows behind the last packed sequence, whose partials nobody wrote).
+struct SeqSum { const void* part; int64_t P, stride, n; void* out; int dt, turn, block0; const int64_t* end; int64_t per; };
 struct SeqSums {
   SeqSum job[5];
   int count = 0, blocks = 0;
-  void add(const void* part, int64_t P, int64_t stride, int64_t n, void* out, int dt, int turn = 1);
+  void add(const void* part, int64_t P, int64_t stride, int64_t n, void* out, int dt, int turn = 1, const int64_t* end = nullptr, int64_t per = 0);
   rgp_status run(rgp_handle h, hipStream_t s, int acc);
 };
 

@@ -27,9 +27,11 @@ static __global__ void __launch_bounds__(1024) seq_sums_kernel(SeqSums g) {
   const SeqSum& j = g.job[k];
   const A* const part = (const A*)j.part;
   const int64_t o0 = (int64_t)((int)blockIdx.x - j.block0) * seq_sums_width(j.P);
+  int64_t n = j.n;
+  if (j.end && j.end[0] * j.per < n) n = j.end[0] < 0 ? 0 : j.end[0] * j.per;
   if (j.P <= SEQ_FEW) {                                  // uniform over the workgroup
     const int64_t i = o0 + threadIdx.x;
-    if (i < j.n) {
+    if (i < n) {
       A v = (A)0;
 #pragma unroll 8
       for (int64_t p = 0; p < j.P; ++p) v += part[p * j.stride + i];
@@ -40,7 +42,7 @@ static __global__ void __launch_bounds__(1024) seq_sums_kernel(SeqSums g) {
   const int l = threadIdx.x & 63, q = threadIdx.x >> 6;
   const int64_t i = o0 + l;
   A v8[8] = {};
-  if (i < j.n) {
+  if (i < n) {
     const A* p = part + q * j.stride + i;
     int64_t left = j.P > q ? (j.P - q + 15) / 16 : 0;
     for (; left >= 8; left -= 8, p += 128 * j.stride) {
@@ -53,17 +55,17 @@ static __global__ void __launch_bounds__(1024) seq_sums_kernel(SeqSums g) {
   }
   sh[q][l] = ((v8[0] + v8[1]) + (v8[2] + v8[3])) + ((v8[4] + v8[5]) + (v8[6] + v8[7]));
   __syncthreads();
-  if (q == 0 && i < j.n) {
+  if (q == 0 && i < n) {
     A v = sh[0][l];
 #pragma unroll
     for (int r = 1; r < 16; ++r) v += sh[r][l];
     seq_sums_store(j, i, v);
   }
 }
-void SeqSums::add(const void* part, int64_t P, int64_t stride, int64_t n, void* out, int dt, int turn) {
+void SeqSums::add(const void* part, int64_t P, int64_t stride, int64_t n, void* out, int dt, int turn, const int64_t* end, int64_t per) {
   if (!out || n < 1) return;
   SeqSum& j = job[count++];
-  j.part = part; j.P = P; j.stride = stride; j.n = n; j.out = out; j.dt = dt; j.turn = turn; j.block0 = blocks;
+  j.part = part; j.P = P; j.stride = stride; j.n = n; j.out = out; j.dt = dt; j.turn = turn; j.block0 = blocks; j.end = end; j.per = per;
   blocks += (int)((n + seq_sums_width(P) - 1) / seq_sums_width(P));
 }
 rgp_status SeqSums::run(rgp_handle h, hipStream_t s, int acc) {
@@ -157,6 +159,7 @@ static const char* scan_bad(const rgp_ssm_scan* a) {
   if (a->dtype < 0 || a->dtype > 3) return "dtype must be RGP_F64, RGP_F32, RGP_BF16 or RGP_F16";
   if (a->n_seq < 1 || a->D < 1 || a->N < 1 || a->G < 1 || a->rows < 0 || a->T < 0) return "empty problem";
   if (a->N > 64) return "at most 64 states per channel";
+  if (a->rows > SEQ_MOST || a->T > SEQ_MOST) return "more than 2^40 rows";
   if (a->D % a->G) return "D must be a multiple of G";
   if (!a->off && (a->T < 1 || a->T * a->n_seq != a->rows)) return "rows must be T * n_seq, T >= 1";
   return nullptr;
@@ -273,9 +276,9 @@ static rgp_status scan_run(rgp_handle h, hipStream_t s, const rgp_ssm_scan* a, b
   sums.add(d.pD, d.nslot, 2 * (int64_t)a->D, a->D, a->gskip, acc);
   sums.add((char*)d.pD + (int64_t)a->D * p.acc, d.nslot, 2 * (int64_t)a->D, a->D, a->gbias, acc);
   if (d.ncb > 1) {
-    const int64_t n = a->rows * a->G * a->N;
-    sums.add(d.pBC, d.ncb, 2 * n, n, a->gB, a->dtype);
-    sums.add((char*)d.pBC + n * p.acc, d.ncb, 2 * n, n, a->gC, a->dtype);
+    const int64_t per = (int64_t)a->G * a->N, n = a->rows * per, *end = a->off ? a->off + a->n_seq : nullptr;
+    sums.add(d.pBC, d.ncb, 2 * n, n, a->gB, a->dtype, 1, end, per);
+    sums.add((char*)d.pBC + n * p.acc, d.ncb, 2 * n, n, a->gC, a->dtype, 1, end, per);
   }
   return sums.run(h, s, acc);
 }
@@ -330,7 +333,7 @@ static __global__ void __launch_bounds__(256) ssm_step_kernel(rgp_ssm_scan a, in
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      s.v[r] = seq_exp(dt * Aq.v[r]) * s.v[r] + w * Bq.v[r];
+      s.v[r] = seq_exp(dt * ssm_finite(Aq.v[r])) * s.v[r] + w * Bq.v[r];
       acc += s.v[r] * Cq.v[r];
     }
     if (whole) *(Quad*)st = s;
@@ -627,6 +630,7 @@ static const char* conv_bad(const rgp_ssm_conv* a) {
   if (a->dtype < 0 || a->dtype > 3) return "dtype must be RGP_F64, RGP_F32, RGP_BF16 or RGP_F16";
   if (a->n_seq < 1 || a->D < 1 || a->rows < 0 || a->T < 0) return "empty problem";
   if (a->W < 2 || a->W > 8) return "2 to 8 taps";
+  if (a->rows > SEQ_MOST || a->T > SEQ_MOST) return "more than 2^40 rows";
   if (!a->off && (a->T < 1 || a->T * a->n_seq != a->rows)) return "rows must be T * n_seq, T >= 1";
   return nullptr;
 }

@@ -459,3 +459,54 @@ def test_library_refuses_what_python_would_not_send(h):
     c.init = c.last = t.data_ptr()
     assert h.lib.rgp_ssm_conv_forward(h.h, None, C.byref(c)) == _lib.RGP_ERR_BAD_ARG
     assert h.lib.rgp_grad_clip(h.h, None, 0, None, None, None, t.data_ptr(), 0.0, t.data_ptr() + 8, None, 0) == _lib.RGP_ERR_BAD_ARG
+
+
+@pytest.mark.parametrize('D,reverse', [(130, False), (16, True)])
+def test_rows_behind_the_last_sequence_stay_as_they_are(h, monkeypatch, D, reverse):
+    """Packed rows may have capacity behind off[n_seq] (a table that is refilled between replays): nothing of it is read or written, also by
+    the sums over the channels' workgroups, and the other rows get the bits that a call without it gives."""
+    from rgp_amd import seq_ops
+    g, N, lengths, spare = _gen(11), 16, [70, 0, 5, 130], 77
+    rows = sum(lengths)
+    x, u, delta, z, gy, gv = [_randn(g, rows, D, dtype=F32).cuda() for _ in range(6)]
+    B, Cm = [_randn(g, rows, N, dtype=F32).cuda() for _ in range(2)]
+    A, w = -torch.exp(_randn(g, D, N)).float().cuda(), _randn(g, D, 4, dtype=F32).cuda()
+    A.requires_grad_(True), w.requires_grad_(True)
+
+    def run(pad):
+        seqs = seq_ops.SeqTable(h, lengths)
+        seqs.rows += pad
+        wide = lambda t: torch.cat([t, torch.full((pad,) + t.shape[1:], float('nan'), device='cuda')])       # noqa: E731
+        ops = [wide(t).requires_grad_(True) for t in (u, delta, B, Cm, z, x)]
+        y = seq_ops.ssm_scan(h, ops[0], ops[1], A, ops[2], ops[3], z=ops[4], seqs=seqs, reverse=reverse)
+        v = seq_ops.ssm_conv(h, ops[5], w, seqs=seqs, reverse=reverse)
+        out = [y, v] + list(torch.autograd.grad(y, ops[:5] + [A], wide(gy))) + list(torch.autograd.grad(v, [ops[5], w], wide(gv)))
+        return [t.detach() for t in out]
+
+    want = run(0)
+    monkeypatch.setattr(seq_ops, '_new_like', lambda t: None if t is None else torch.full_like(t, 7.0, memory_format=torch.contiguous_format, requires_grad=False))
+    got = run(spare)
+    for a, b in zip(want, got):
+        if b.shape[0] == rows + spare:
+            assert (b[rows:] == 7.0).all()
+            b = b[:rows]
+        assert torch.equal(a, b)
+
+
+def test_steps_with_infinite_decay(h):
+    """A = -inf forgets the state, also where a step's dt underflows to zero (then nothing decays), as over whole sequences."""
+    from rgp_amd import seq_ops
+    g, D, N = _gen(12), 6, 4
+    u, B, Cm = _randn(g, 2, D, dtype=F32).cuda(), _randn(g, 2, N, dtype=F32).cuda(), _randn(g, 2, N, dtype=F32).cuda()
+    A = torch.full((D, N), -float('inf'), device='cuda')
+    s0 = _randn(g, 2, D, N, dtype=F32).cuda()
+    for value in (0.5, -300.0):
+        delta = torch.full((2, D), value, device='cuda')
+        st = s0.clone()
+        y = seq_ops.ssm_scan_step(h, u, delta, A, B, Cm, None, st)
+        y1, last = seq_ops.ssm_scan(h, u[None], delta[None], A, B[None], Cm[None], init=s0, return_state=True)
+        assert torch.isfinite(st).all() and torch.isfinite(y).all()
+        if value < 0:
+            assert torch.equal(st, s0)
+        torch.testing.assert_close(st, last, rtol=1e-6, atol=1e-6)
+        torch.testing.assert_close(y, y1[0], rtol=1e-5, atol=1e-5)

@@ -197,3 +197,22 @@ def test_size_queries_refuse_and_count():
     assert C.sizeof(_lib.SsmScan) == 6 * 4 + 3 * 8 + 6 * 8 + 12 * 8 + 17 * 8 + 8
     assert C.sizeof(_lib.SsmConv) == 6 * 4 + 3 * 8 + 2 * 8 + 4 * 8 + 10 * 8 + 8
     assert C.sizeof(_lib.RmsNorm) == 2 * 4 + 2 * 8 + 8 + 2 * 8 + 4 * 8 + 9 * 8 + 8
+
+
+def test_sizes_beyond_the_library_are_refused():
+    from rgp_amd import _lib
+    lib = _lib.load()
+    a = _lib.SsmScan()
+    a.dtype, a.n_seq, a.D, a.N, a.G, a.off = _lib.DT_F32, 2, 6, 3, 2, 1
+    a.rows = 1 << 40
+    assert lib.rgp_ssm_scan_workspace(C.byref(a), 1) > 0
+    a.rows += 1
+    assert lib.rgp_ssm_scan_workspace(C.byref(a), 1) == -1
+    c = _lib.SsmConv()
+    c.dtype, c.n_seq, c.D, c.W, c.T, c.rows = _lib.DT_BF16, 1, 6, 4, (1 << 40) + 1, (1 << 40) + 1
+    assert lib.rgp_ssm_conv_workspace(C.byref(c), 1) == -1
+    r = _lib.RmsNorm()
+    r.dtype, r.rows, r.C, r.eps = _lib.DT_F64, 3, 7, 1e-60
+    assert lib.rgp_rms_norm_workspace(C.byref(r), 1) >= 7 * 8
+    r.dtype = _lib.DT_BF16                                  # zero in 32 bits: a row of zeros would have no norm
+    assert lib.rgp_rms_norm_workspace(C.byref(r), 1) == -1
