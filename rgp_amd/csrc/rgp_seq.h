@@ -105,37 +105,35 @@ static __device__ __forceinline__ float seq_rcp(float x) { return __builtin_amdg
 static __device__ __forceinline__ double seq_rcp(double x) { return 1.0 / x; }
 static __device__ __forceinline__ float seq_rsqrt(float x) { return 1.0f / sqrtf(x); }
 static __device__ __forceinline__ double seq_rsqrt(double x) { return 1.0 / sqrt(x); }
-// exp(-|x|) keeps its relative accuracy for large |x| (the argument is split in two before the exponent of 2 is taken)
+// exp(-|x|) keeps its relative accuracy for large |x| (the argument is split in two before the exponent of 2 is taken); a NaN counts as -200
 static __device__ __forceinline__ float seq_exp_neg(float x) {
-  const float a = -fabsf(x);
+  const float a = fmaxf(-fabsf(x), -200.0f);
   const float hi = a * 1.44269504088896341f;
   const float lo = fmaf(a, 1.44269504088896341f, -hi) + a * 1.92596299e-8f;       // log2(e) = 1.44269502... + 1.9259e-8
   const float e = __builtin_amdgcn_exp2f(hi);
-  return a < -200.0f ? 0.0f : fmaf(e, lo * 0.693147181f, e);
+  return fmaf(e, lo * 0.693147181f, e);
 }
 static __device__ __forceinline__ double seq_exp_neg(double x) { return exp(-fabs(x)); }
 
-// log(1 + e) for 0 <= e <= 1 as 2 atanh(e / (2 + e)): the odd series in s = e / (2 + e) <= 1/3, to 9^-8 / 17, keeps the RELATIVE accuracy
-// of small e, which the step size dt = softplus(x) needs (biases put it at 1e-3)
+// log(1 + e) for 0 <= e <= 1 as 2 atanh(s), s = e / (2 + e) <= 1/3: 2 s + 2 s q R(q) with q = s^2 keeps the RELATIVE accuracy of small e, which
+// the step size dt = softplus(x) needs (biases put it at 1e-3).  R is the cubic whose largest relative error in the result is smallest over
+// q <= 1/9 (4.5e-9, a thirteenth of a rounding; the series of atanh needs three terms more for that).
 static __device__ __forceinline__ float seq_log1p01(float e) {
   const float s = e * seq_rcp(2.0f + e), q = s * s;
-  float p = 1.0f / 15.0f;
-  p = fmaf(p, q, 1.0f / 13.0f);
-  p = fmaf(p, q, 1.0f / 11.0f);
-  p = fmaf(p, q, 1.0f / 9.0f);
-  p = fmaf(p, q, 1.0f / 7.0f);
-  p = fmaf(p, q, 1.0f / 5.0f);
-  p = fmaf(p, q, 1.0f / 3.0f);
+  float p = 0.14005993677f;
+  p = fmaf(p, q, 0.14000902572f);
+  p = fmaf(p, q, 0.20010763625f);
+  p = fmaf(p, q, 0.33333208143f);
   return fmaf(s * 2.0f * q, p, 2.0f * s);
 }
 static __device__ __forceinline__ double seq_log1p01(double e) { return log1p(e); }
 
-// softplus(x) and the sigmoid (its derivative); NaN passes through both
+// softplus(x) and the sigmoid (its derivative); NaN passes through the first, and with dt through everything that the second multiplies
 template <typename A>
 static __device__ __forceinline__ A seq_softplus(A x, A& sig) {
   const A e = seq_exp_neg(x), big = seq_rcp((A)1 + e);
   sig = x >= (A)0 ? big : e * big;
-  return (x > (A)0 ? x : (A)0) + seq_log1p01(e);
+  return (x < (A)0 ? (A)0 : x) + seq_log1p01(e);
 }
 // the sigmoid, off by at most |x| half steps relative to its value (what the argument of the exponential rounds by)
 template <typename A>

@@ -98,17 +98,15 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
         for (int j = 0; j < V; ++j) {
           Four p;
           const A dt = seq_softplus((A)rd[i].e[j] + bias[j], p.w);
-          const bool ok = tl < nt && ev * V < chn;             // all lanes' values are folded below
-          p.x = ok ? dt : (A)0;
-          p.w = ok ? p.w : (A)0;
-          p.y = MODE == 0 && ok ? (A)ru[i].e[j] : (A)0;
+          p.x = dt;
+          p.y = MODE == 0 ? (A)ru[i].e[j] : (A)0;
           A gp = (A)rg[i].e[j];
           if (a.z) {
             const A z = (A)rz[i].e[j], q = gp * seq_sigmoid(z);
             if (MODE == 0) zf[i * V + j][tid] = q + (gp - q) * (z * seq_sigmoid(z));
             gp = z * q;
           }
-          p.z = ok ? gp : (A)0;
+          p.z = gp;
           pl[tl][ssm_place<V, sizeof(Four)>(ev * V + j)] = p;
         }
       }
@@ -117,9 +115,26 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
     for (int i = 0; i < NB; ++i) {
       const int e = tid + i * THREADS, tl = e / NP, n = e % NP;
       if (TL * NP % THREADS == 0 || tl < TL) {
-        const bool ok = n < N && tl < nt;
-        if (MODE == 0) Bl[tl][n / R].v[n % R] = ok ? (A)rB[i] : (A)0;
-        Cl[tl][n / R].v[n % R] = ok ? (A)rC[i] : (A)0;
+        if (MODE == 0) Bl[tl][n / R].v[n % R] = (A)rB[i];
+        Cl[tl][n / R].v[n % R] = (A)rC[i];
+      }
+    }
+    if (nt < TL || N < NP || chn < CH) {                           // the same threads take back what is behind the end: all lanes' values are folded below
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int tl = et + i * RPI;
+        if (et < TL && (tl >= nt || ev * V >= chn)) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) pl[tl][ssm_place<V, sizeof(Four)>(ev * V + j)] = Four{(A)0, (A)0, (A)0, (A)0};
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int e = tid + i * THREADS, tl = e / NP, n = e % NP;
+        if ((TL * NP % THREADS == 0 || tl < TL) && (n >= N || tl >= nt)) {
+          if (MODE == 0) Bl[tl][n / R].v[n % R] = (A)0;
+          Cl[tl][n / R].v[n % R] = (A)0;
+        }
       }
     }
     __syncthreads();

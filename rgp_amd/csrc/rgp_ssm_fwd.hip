@@ -103,8 +103,8 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
           A sig;
           const A dt = seq_softplus((A)rd[i].e[j] + bias[j], sig);
           Pair p;
-          p.dt = tl < nt ? dt : (A)0;
-          p.w = tl < nt ? dt * (A)ru[i].e[j] : (A)0;
+          p.dt = dt;
+          p.w = dt * (A)ru[i].e[j];
           pl[tl][ssm_place<V, sizeof(Pair)>(ev * V + j)] = p;
         }
       }
@@ -113,9 +113,26 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
     for (int i = 0; i < NB; ++i) {
       const int e = tid + i * THREADS, tl = e / NP, n = e % NP;
       if (TL * NP % THREADS == 0 || tl < TL) {
-        const bool ok = n < N && tl < nt;
-        Bl[tl][n / R].v[n % R] = ok ? (A)rB[i] : (A)0;
-        if (MODE == 0) Cl[tl][n / R].v[n % R] = ok ? (A)rC[i] : (A)0;
+        Bl[tl][n / R].v[n % R] = (A)rB[i];
+        if (MODE == 0) Cl[tl][n / R].v[n % R] = (A)rC[i];
+      }
+    }
+    if (nt < TL || N < NP) {                                       // the same threads take back what is behind the end
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int tl = et + i * RPI;
+        if (et < TL && tl >= nt) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) pl[tl][ssm_place<V, sizeof(Pair)>(ev * V + j)] = Pair{(A)0, (A)0};
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int e = tid + i * THREADS, tl = e / NP, n = e % NP;
+        if ((TL * NP % THREADS == 0 || tl < TL) && (n >= N || tl >= nt)) {
+          Bl[tl][n / R].v[n % R] = (A)0;
+          if (MODE == 0) Cl[tl][n / R].v[n % R] = (A)0;
+        }
       }
     }
     __syncthreads();
