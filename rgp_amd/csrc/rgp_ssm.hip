@@ -385,10 +385,13 @@ extern "C" rgp_status rgp_ssm_scan_step(rgp_handle h, void* stream, const rgp_ss
 }
 
 // ---- short causal convolution ---------------------------------------------------------------------------------------------------------------
-// v_t = silu(bias + sum_j w_j x_{t-W+1+j}) reads x once and writes v once: bound by memory.  A thread holds V = 4 channels (2 in fp64) and walks a
-// run of CONV_RUN steps with the last W - 1 inputs in registers; the W - 1 rows before a run are read again (from cache).
+// v_t = silu(bias + sum_j w_j x_{t-W+1+j}) reads x once and writes v once: bound by memory.  A thread holds V = 2 channels (1 where alignment or
+// an odd width forbids pairs) and walks a run of 8 or 16 steps with the last W - 1 inputs in registers, CONV_FLY rows in flight; the W - 1 rows
+// before a run are read again (from cache).  Wider vectors have fewer waves to wait with: backward over 8191 x 1024 bf16 46 us with 8 channels
+// a thread, 31 with 4, 26 with 2; runs of 8 steps 36 (4 channels), of 32 29 (2 channels); 8 rows in flight change nothing.  Forward, 8 x 65536 x
+// 64 fp32: 50 us, 5.4 TB/s; the 16-bit forms reach 3 TB/s and are held up by the sigmoid and conversions.
 #define CONV_FLY 4
-#define CONV_V(bytes) ((bytes) == 8 ? 2 : 4)
+#define CONV_V 2
 struct ConvDev {
   rgp_ssm_conv a;
   SeqGeo g;
@@ -639,10 +642,10 @@ static void conv_plan(const rgp_ssm_conv* a, bool wide, ConvDev& d, int64_t& nrb
   d.a = *a;
   d.g = SeqGeo{a->off, a->T, a->rows, a->n_seq, a->reverse};
   d.wide = wide;
-  const int V = wide ? CONV_V(seq_dtype_bytes(a->dtype)) : 1;
+  const int V = wide ? CONV_V : 1;
   d.nvec = (a->D + V - 1) / V;
   d.same = d.nvec % 64 == 0;
-  // runs of 16 steps (the W - 1 rows before a run come from cache) unless that leaves fewer than two waves a SIMD
+  // runs of 16 steps unless that leaves fewer than two waves a SIMD
   for (d.lg = 4; d.lg > 3 && seq_blocks(d.g, d.lg) * d.nvec < 131072; --d.lg) {}
   d.nrun = seq_blocks(d.g, d.lg);
   d.lanes = 1;
@@ -678,7 +681,7 @@ static hipError_t conv_go(const ConvDev& d, int what, dim3 grid, hipStream_t s) 
 }
 template <typename T, int W>
 static hipError_t conv_wide(const ConvDev& d, int what, dim3 grid, hipStream_t s) {
-  return d.wide ? conv_go<T, W, CONV_V((int)sizeof(T))>(d, what, grid, s) : conv_go<T, W, 1>(d, what, grid, s);
+  return d.wide ? conv_go<T, W, CONV_V>(d, what, grid, s) : conv_go<T, W, 1>(d, what, grid, s);
 }
 template <typename T>
 static hipError_t conv_taps(const ConvDev& d, int what, dim3 grid, hipStream_t s) {
@@ -710,7 +713,7 @@ static rgp_status conv_run(rgp_handle h, hipStream_t s, const rgp_ssm_conv* a, i
   if (what == CONV_STEP && (!a->v || !a->last || a->init != a->last)) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "v and the state (init = last) are required");
   if (what == CONV_FWD && some && !a->v) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "v is required");
   if (what == CONV_FWD && a->last && a->last == a->init) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "last must not be init");
-  const int e = seq_dtype_bytes(a->dtype), V = CONV_V(e);
+  const int e = seq_dtype_bytes(a->dtype), V = CONV_V;
   const int64_t st = what == CONV_STEP ? 0 : a->x_st;
   bool wide = a->D % V == 0 && seq_aligned(a->x, st, a->x_sb, e, V);
   if (what == CONV_BWD) wide = wide && seq_aligned(a->gv, a->gv_st, a->gv_sb, e, V) && seq_aligned(a->gx, 0, 0, e, V);
