@@ -5,7 +5,6 @@
 
 struct NormDev {
   rgp_rms_norm a;
-  int wide;
   void* part;
 };
 
@@ -26,13 +25,13 @@ static __device__ __forceinline__ A row_sum(A v, A* sh) {
   }
 }
 
-// TPR threads a row, NE vectors of V elements each (V = 1 where alignment or an odd width forbids 16 bytes); rows of TPR * NE * V >= C
-// elements.  A workgroup takes every gridDim-th group of rows and keeps w; the next rows are loaded while these are normed.  hid is rounded
+// TPR threads a row, NE vectors of V elements each (16 bytes; V = 1 for rows shorter than that); rows of TPR * NE * V >= C elements.
+// WHOLE: C is a multiple of V, otherwise the row's last vector is moved back and its first elements belong to the one before.  A workgroup takes every gridDim-th group of rows and keeps w; the next rows are loaded while these are normed.  hid is rounded
 // to its type where it is written; the norm uses the sum before that rounding.
-template <typename T, int TPR, int NE, int V>
+template <typename T, int TPR, int NE, int V, bool WHOLE>
 static __global__ void __launch_bounds__(256) rms_fwd_kernel(NormDev d) {
   typedef typename SeqAcc<T>::type A;
-  typedef SeqVec<T, V> Vec;
+  typedef SeqAny<T, V> Vec;
   constexpr int RPB = 256 / TPR;
   __shared__ A sh[4];
   const rgp_rms_norm& a = d.a;
@@ -40,13 +39,15 @@ static __global__ void __launch_bounds__(256) rms_fwd_kernel(NormDev d) {
   A w[NE][V];
   int64_t col[NE];
   bool in[NE];
+  int own[NE];                                       // first element that this lane counts
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
     const int64_t c = (int64_t)(l + i * TPR) * V;
     in[i] = c < a.C;
-    col[i] = in[i] ? c : 0;
+    col[i] = !in[i] ? 0 : WHOLE || c + V <= a.C ? c : a.C - V;
+    own[i] = in[i] ? (int)(c - col[i]) : V;
 #pragma unroll
-    for (int j = 0; j < V; ++j) w[i][j] = in[i] ? ((const A*)a.w)[c + j] : (A)0;
+    for (int j = 0; j < V; ++j) w[i][j] = in[i] ? ((const A*)a.w)[col[i] + j] : (A)0;
   }
   Vec x[NE], r[NE];
   auto fetch = [&](int64_t row) {                    // rows behind the last one read the last one
@@ -67,7 +68,7 @@ static __global__ void __launch_bounds__(256) rms_fwd_kernel(NormDev d) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         h[i][j] = (A)x[i].e[j] + (a.residual ? (A)r[i].e[j] : (A)0);
-        q += in[i] ? h[i][j] * h[i][j] : (A)0;
+        q += (WHOLE ? in[i] : j >= own[i]) ? h[i][j] * h[i][j] : (A)0;
       }
     if (r0 + (int64_t)gridDim.x * RPB < a.rows) fetch(row + (int64_t)gridDim.x * RPB);
     q = row_sum<TPR>(q, sh);
@@ -94,7 +95,7 @@ static __global__ void __launch_bounds__(256) rms_fwd_kernel(NormDev d) {
 template <typename T, int V>
 static __global__ void __launch_bounds__(256) rms_fwd_long_kernel(NormDev d) {
   typedef typename SeqAcc<T>::type A;
-  typedef SeqVec<T, V> Vec;
+  typedef SeqAny<T, V> Vec;
   __shared__ A sh[4];
   const rgp_rms_norm& a = d.a;
   const int64_t row = blockIdx.x;
@@ -128,10 +129,10 @@ static __global__ void __launch_bounds__(256) rms_fwd_long_kernel(NormDev d) {
 // storage type: gw is a sum over many rows in 32 bits, and that rounding (2^-9 relative) would be its largest error by far.  A workgroup
 // takes every gridDim-th group of rows, sums gw in registers and adds its row groups through LDS; the workgroups' sums are added in a fixed
 // order afterwards.
-template <typename T, int TPR, int NE, int V>
-static __global__ void __launch_bounds__(256) rms_bwd_kernel(NormDev d) {
+template <typename T, int TPR, int NE, int V, bool WHOLE>
+static __global__ void __launch_bounds__(256, NE * V * sizeof(typename SeqAcc<T>::type) > 128 ? 1 : 2) rms_bwd_kernel(NormDev d) {
   typedef typename SeqAcc<T>::type A;
-  typedef SeqVec<T, V> Vec;
+  typedef SeqAny<T, V> Vec;
   constexpr int RPB = 256 / TPR;
   __shared__ A sh[4];
   __shared__ A acc[256 * V];
@@ -140,15 +141,17 @@ static __global__ void __launch_bounds__(256) rms_bwd_kernel(NormDev d) {
   A gw[NE][V], w[NE][V];
   int64_t col[NE];
   bool in[NE];
+  int own[NE];
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
     const int64_t c = (int64_t)(l + i * TPR) * V;
     in[i] = c < a.C;
-    col[i] = in[i] ? c : 0;
+    col[i] = !in[i] ? 0 : WHOLE || c + V <= a.C ? c : a.C - V;
+    own[i] = in[i] ? (int)(c - col[i]) : V;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       gw[i][j] = (A)0;
-      w[i][j] = in[i] ? ((const A*)a.w)[c + j] : (A)0;
+      w[i][j] = in[i] ? ((const A*)a.w)[col[i] + j] : (A)0;
     }
   }
   const A inv = (A)1 / (A)a.C;
@@ -171,7 +174,7 @@ static __global__ void __launch_bounds__(256) rms_bwd_kernel(NormDev d) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         hid[i][j] = (A)x[i].e[j] + (a.residual ? (A)r[i].e[j] : (A)0);
-        q += in[i] ? (A)g[i].e[j] * w[i][j] * hid[i][j] : (A)0;
+        q += (WHOLE ? in[i] : j >= own[i]) ? (A)g[i].e[j] * w[i][j] * hid[i][j] : (A)0;
       }
     q = row_sum<TPR>(q, sh) * inv * rs * rs;
 #pragma unroll
@@ -195,7 +198,8 @@ static __global__ void __launch_bounds__(256) rms_bwd_kernel(NormDev d) {
   for (int i = 0; i < NE; ++i) {
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < V; ++j) acc[threadIdx.x * V + j] = gw[i][j];
+    for (int j = 0; j < V; ++j)
+      if (WHOLE || j >= own[i]) acc[threadIdx.x * V + j - (WHOLE ? 0 : own[i])] = gw[i][j];       // what is left out lies behind the row's end
     __syncthreads();
     for (int e = threadIdx.x; e < TPR * V; e += 256) {
       A v = (A)0;
@@ -210,7 +214,7 @@ static __global__ void __launch_bounds__(256) rms_bwd_kernel(NormDev d) {
 template <typename T, int V>
 static __global__ void __launch_bounds__(256) rms_bwd_long_kernel(NormDev d) {
   typedef typename SeqAcc<T>::type A;
-  typedef SeqVec<T, V> Vec;
+  typedef SeqAny<T, V> Vec;
   __shared__ A sh[4];
   const rgp_rms_norm& a = d.a;
   A* const part = (A*)d.part + (int64_t)blockIdx.x * a.C;
@@ -247,8 +251,10 @@ static __global__ void __launch_bounds__(256) rms_bwd_long_kernel(NormDev d) {
 // Threads a row and vectors a thread: of the shapes that hold a row, the one that leaves the fewest lanes idle, and of those the one with the
 // fewest threads a row -- unless the rows are few, where more threads a row finish it sooner.
 struct RmsShape { int tpr, ne; };
-static RmsShape rms_shape(int64_t C, int V, int64_t rows) {
-  const int64_t nv = (C + V - 1) / V;
+static RmsShape rms_shape(const rgp_rms_norm* a) {
+  const int V = 16 / seq_dtype_bytes(a->dtype);
+  if (a->C < V) return RmsShape{8, 1};                                        // single elements, at most 7 of them
+  const int64_t nv = (a->C + V - 1) / V, rows = a->rows;
   static const int tprs[4] = {8, 16, 64, 256}, nes[5] = {1, 2, 3, 4, 8};
   RmsShape best{0, 0};
   for (int i = 0; i < 4; ++i)
@@ -261,12 +267,18 @@ static RmsShape rms_shape(int64_t C, int V, int64_t rows) {
     }
   return best;
 }
-static int64_t rms_blocks(const rgp_rms_norm* a, RmsShape s, int most) {
+static int64_t rms_blocks(const rgp_rms_norm* a, RmsShape s, int64_t most) {
   const int64_t rpb = s.tpr ? 256 / s.tpr : 1, want = (a->rows + rpb - 1) / rpb;
   return want < most ? (want < 1 ? 1 : want) : most;
 }
+// Backward: as many workgroups as are resident at once, two a CU (their sums of gw have to be joined, and a second round of a few is as long as
+// the first: 599 instead of 512 for 4793 x 7000 bf16 take 117 us instead of 83).  Short rows, of which a thread holds little, have room for
+// more, as long as each keeps eight groups of rows: 838860 x 40 takes 75 us with 2048, 116 with 512.
 #define RMS_FWD_BLOCKS 2048
-#define RMS_BWD_BLOCKS 512
+static int64_t rms_bwd_blocks(const rgp_rms_norm* a, RmsShape s) {
+  const int64_t eight = s.tpr == 8 && s.ne <= 2 ? rms_blocks(a, s, INT64_MAX) / 8 : 0;
+  return rms_blocks(a, s, eight < 512 ? 512 : eight > 2048 ? 2048 : eight);
+}
 static const char* rms_bad(const rgp_rms_norm* a) {
   if (!a) return "null arguments";
   if (a->dtype < 0 || a->dtype > 3) return "dtype must be RGP_F64, RGP_F32, RGP_BF16 or RGP_F16";
@@ -277,18 +289,23 @@ static const char* rms_bad(const rgp_rms_norm* a) {
 extern "C" int64_t rgp_rms_norm_workspace(const rgp_rms_norm* a, int backward) {
   if (rms_bad(a)) return -1;
   if (!backward) return 0;
-  const int64_t one = rms_blocks(a, rms_shape(a->C, 1, a->rows), RMS_BWD_BLOCKS);
-  const int64_t wide = rms_blocks(a, rms_shape(a->C, 16 / seq_dtype_bytes(a->dtype), a->rows), RMS_BWD_BLOCKS);
-  return (one > wide ? one : wide) * a->C * (a->dtype == RGP_F64 ? 8 : 4);
+  return rms_bwd_blocks(a, rms_shape(a)) * a->C * (a->dtype == RGP_F64 ? 8 : 4);
 }
 template <typename T, int TPR, int NE, int V>
 static hipError_t rms_go(const NormDev& d, bool back, int64_t blocks, hipStream_t s) {
-  if (back) hipLaunchKernelGGL((rms_bwd_kernel<T, TPR, NE, V>), dim3((unsigned)blocks), dim3(256), 0, s, d);
-  else hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, NE, V>), dim3((unsigned)blocks), dim3(256), 0, s, d);
+  const dim3 g((unsigned)blocks), t(256);
+  if (V == 1 || d.a.C % V == 0) {
+    if (back) hipLaunchKernelGGL((rms_bwd_kernel<T, TPR, NE, V, true>), g, t, 0, s, d);
+    else hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, NE, V, true>), g, t, 0, s, d);
+  } else if constexpr (V > 1) {
+    if (back) hipLaunchKernelGGL((rms_bwd_kernel<T, TPR, NE, V, false>), g, t, 0, s, d);
+    else hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, NE, V, false>), g, t, 0, s, d);
+  }
   return hipGetLastError();
 }
-template <typename T, int TPR, int V>
+template <typename T, int TPR>
 static hipError_t rms_ne(const NormDev& d, int ne, bool back, int64_t blocks, hipStream_t s) {
+  constexpr int V = 16 / (int)sizeof(T);
   switch (ne) {
     case 1: return rms_go<T, TPR, 1, V>(d, back, blocks, s);
     case 2: return rms_go<T, TPR, 2, V>(d, back, blocks, s);
@@ -300,21 +317,22 @@ static hipError_t rms_ne(const NormDev& d, int ne, bool back, int64_t blocks, hi
   }
 }
 template <typename T, int V>
-static hipError_t rms_shaped(const NormDev& d, RmsShape sh, bool back, int64_t blocks, hipStream_t s) {
-  switch (sh.tpr) {
-    case 8: return rms_ne<T, 8, V>(d, sh.ne, back, blocks, s);
-    case 16: return rms_ne<T, 16, V>(d, sh.ne, back, blocks, s);
-    case 64: return rms_ne<T, 64, V>(d, sh.ne, back, blocks, s);
-    case 256: return rms_ne<T, 256, V>(d, sh.ne, back, blocks, s);
-    default:
-      if (back) hipLaunchKernelGGL((rms_bwd_long_kernel<T, V>), dim3((unsigned)blocks), dim3(256), 0, s, d);
-      else hipLaunchKernelGGL((rms_fwd_long_kernel<T, V>), dim3((unsigned)d.a.rows), dim3(256), 0, s, d);
-      return hipGetLastError();
-  }
+static hipError_t rms_long(const NormDev& d, bool back, int64_t blocks, hipStream_t s) {
+  if (back) hipLaunchKernelGGL((rms_bwd_long_kernel<T, V>), dim3((unsigned)blocks), dim3(256), 0, s, d);
+  else hipLaunchKernelGGL((rms_fwd_long_kernel<T, V>), dim3((unsigned)d.a.rows), dim3(256), 0, s, d);
+  return hipGetLastError();
 }
 template <typename T>
 static hipError_t rms_pick(const NormDev& d, RmsShape sh, bool back, int64_t blocks, hipStream_t s) {
-  return d.wide ? rms_shaped<T, 16 / (int)sizeof(T)>(d, sh, back, blocks, s) : rms_shaped<T, 1>(d, sh, back, blocks, s);
+  constexpr int V = 16 / (int)sizeof(T);
+  if (d.a.C < V) return rms_go<T, 8, 1, 1>(d, back, blocks, s);                 // the shape of up to 8 single elements
+  switch (sh.tpr) {
+    case 8: return rms_ne<T, 8>(d, sh.ne, back, blocks, s);
+    case 16: return rms_ne<T, 16>(d, sh.ne, back, blocks, s);
+    case 64: return rms_ne<T, 64>(d, sh.ne, back, blocks, s);
+    case 256: return rms_ne<T, 256>(d, sh.ne, back, blocks, s);
+    default: return d.a.C % V == 0 ? rms_long<T, V>(d, back, blocks, s) : rms_long<T, 1>(d, back, blocks, s);
+  }
 }
 static rgp_status rms_run(rgp_handle h, hipStream_t s, const rgp_rms_norm* a, bool back) {
   const std::string name = back ? "rms norm backward: " : "rms norm: ";
@@ -323,14 +341,10 @@ static rgp_status rms_run(rgp_handle h, hipStream_t s, const rgp_rms_norm* a, bo
     return rgp_fail(h, RGP_ERR_BAD_ARG, name + "a required buffer is null");
   if (!back && a->rows > 0 && (a->residual != nullptr) != (a->hid != nullptr)) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "residual and hid go together");
   if (a->rows > 16777215) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "more than 2^24 - 1 rows");
-  const int e = seq_dtype_bytes(a->dtype), V = 16 / e;
   NormDev d{};
   d.a = *a;
-  d.wide = a->C % V == 0 && seq_aligned(a->x, a->x_st, 0, e) && (!a->residual || seq_aligned(a->residual, a->residual_st, 0, e));
-  if (back) d.wide = d.wide && seq_aligned(a->gy, a->gy_st, 0, e) && (!a->ghid || seq_aligned(a->ghid, a->ghid_st, 0, e)) && seq_aligned(a->gx, 0, 0, e);
-  else d.wide = d.wide && seq_aligned(a->y, 0, 0, e) && (!a->hid || seq_aligned(a->hid, 0, 0, e));
-  const RmsShape sh = rms_shape(a->C, d.wide ? V : 1, a->rows);
-  const int64_t blocks = rms_blocks(a, sh, back ? RMS_BWD_BLOCKS : RMS_FWD_BLOCKS);
+  const RmsShape sh = rms_shape(a);
+  const int64_t blocks = back ? rms_bwd_blocks(a, sh) : rms_blocks(a, sh, RMS_FWD_BLOCKS);
   if (back && (rgp_rms_norm_workspace(a, 1) > a->work_bytes || !a->work || ((uintptr_t)a->work & 15)))
     return rgp_fail(h, RGP_ERR_WORKSPACE, name + "work buffer too small or not 16-byte aligned");
   d.part = a->work;

@@ -240,11 +240,8 @@ static rgp_status scan_run(rgp_handle h, hipStream_t s, const rgp_ssm_scan* a, b
   SsmDev& d = p.d;
   if (p.bytes > a->work_bytes || (p.bytes && !a->work) || ((uintptr_t)a->work & 15))
     return rgp_fail(h, RGP_ERR_WORKSPACE, std::string(what) + "work buffer too small or not 16-byte aligned");
-  const int e = seq_dtype_bytes(a->dtype), V = 16 / e;
-  d.wide = d.Dg % V == 0 && seq_aligned(a->u, a->u_st, a->u_sb, e) && seq_aligned(a->delta, a->delta_st, a->delta_sb, e) &&
-           (!a->z || seq_aligned(a->z, a->z_st, a->z_sb, e));
-  if (back) d.wide = d.wide && seq_aligned(a->gy, a->gy_st, a->gy_sb, e) && seq_aligned(a->gu, 0, 0, e) && seq_aligned(a->gdelta, 0, 0, e) && (!a->z || seq_aligned(a->gz, 0, 0, e));
-  else d.wide = d.wide && seq_aligned(a->y, 0, 0, e);
+  const int V = 16 / seq_dtype_bytes(a->dtype), rest = d.Dg % p.CH;      // a workgroup's channels are one vector at least, or single elements
+  d.wide = rest == 0 || rest >= V;
   char* w = (char*)a->work;
   auto take = [&](int64_t bytes) { void* r = bytes ? (void*)w : nullptr; w += bytes; return r; };
   d.part = take(p.part_bytes);
@@ -359,7 +356,7 @@ static hipError_t step_pick(const rgp_ssm_scan& a, hipStream_t s) {
   const unsigned grid = (unsigned)(((int64_t)a.n_seq * a.D * K + 255) / 256);
   const int Dg = a.D / a.G;
   const int whole = a.N == SSM_R * K && ((uintptr_t)a.last & 15) == 0 && ((uintptr_t)a.A & 15) == 0 &&
-                    seq_aligned(a.B, 0, a.B_sb, (int)sizeof(T), SSM_R) && seq_aligned(a.C, 0, a.C_sb, (int)sizeof(T), SSM_R);
+                    seq_aligned(a.B, a.B_sb, (int)sizeof(T), SSM_R) && seq_aligned(a.C, a.C_sb, (int)sizeof(T), SSM_R);
   switch (K) {
     case 1: hipLaunchKernelGGL((ssm_step_kernel<T, 1>), dim3(grid), dim3(256), 0, s, a, Dg, whole); break;
     case 2: hipLaunchKernelGGL((ssm_step_kernel<T, 2>), dim3(grid), dim3(256), 0, s, a, Dg, whole); break;
@@ -385,8 +382,8 @@ extern "C" rgp_status rgp_ssm_scan_step(rgp_handle h, void* stream, const rgp_ss
 }
 
 // ---- short causal convolution ---------------------------------------------------------------------------------------------------------------
-// v_t = silu(bias + sum_j w_j x_{t-W+1+j}) reads x once and writes v once: bound by memory.  A thread holds V = 2 channels (1 where alignment or
-// an odd width forbids pairs) and walks a run of 8 or 16 steps with the last W - 1 inputs in registers, CONV_FLY rows in flight; the W - 1 rows
+// v_t = silu(bias + sum_j w_j x_{t-W+1+j}) reads x once and writes v once: bound by memory.  A thread holds V = 2 channels (1 where there
+// is only one, and in a step of an odd width) and walks a run of 8 or 16 steps with the last W - 1 inputs in registers, CONV_FLY rows in flight; the W - 1 rows
 // before a run are read again (from cache).  Wider vectors have fewer waves to wait with: backward over 8191 x 1024 bf16 46 us with 8 channels
 // a thread, 31 with 4, 26 with 2; runs of 8 steps 36 (4 channels), of 32 29 (2 channels); 8 rows in flight change nothing.  Forward, 8 x 65536 x
 // 64 fp32: 50 us, 5.4 TB/s; the 16-bit forms reach 3 TB/s and are held up by the sigmoid and conversions.
@@ -397,16 +394,20 @@ struct ConvDev {
   SeqGeo g;
   int64_t nrun, nvec;
   int lg;                          // a run has 2^lg steps
-  int wide, same, lanes;           // vector accesses; a wave's lanes are in one run; vectors side by side in a workgroup (backward)
+  int wide, same, lanes;           // pairs of channels; a wave's lanes are in one run; vectors side by side in a workgroup (backward)
   void* part;
 };
 
+// first channel of a vector: the last one of an odd width is moved back by one
+template <int V>
+static __device__ __forceinline__ int64_t conv_at(int64_t vec, int D) { return vec * V + V <= D ? vec * V : D - V; }
+
 // x at step t of the sequence, in walking order; before the first step the state
 template <typename T, int W, int V>
-static __device__ __forceinline__ SeqVec<T, V> conv_x(const ConvDev& d, const SeqBlock& b, int64_t t, int64_t c) {
+static __device__ __forceinline__ SeqAny<T, V> conv_x(const ConvDev& d, const SeqBlock& b, int64_t t, int64_t c) {
   const rgp_ssm_conv& a = d.a;
-  if (t >= 0) return *(const SeqVec<T, V>*)(seq_row((const T*)a.x, d.g, b, SeqStride{a.x_st, a.x_sb}, t) + c);
-  SeqVec<T, V> z;
+  if (t >= 0) return *(const SeqAny<T, V>*)(seq_row((const T*)a.x, d.g, b, SeqStride{a.x_st, a.x_sb}, t) + c);
+  SeqAny<T, V> z;
 #pragma unroll
   for (int i = 0; i < V; ++i) z.e[i] = a.init ? ((const T*)a.init)[(b.seq * (W - 1) + W - 1 + t) * a.D + c + i] : (T)0;
   return z;
@@ -415,10 +416,10 @@ static __device__ __forceinline__ SeqVec<T, V> conv_x(const ConvDev& d, const Se
 template <typename T, int W, int V>
 static __global__ void __launch_bounds__(256) conv_fwd_kernel(ConvDev d) {
   typedef typename SeqAcc<T>::type A;
-  typedef SeqVec<T, V> Vec;
+  typedef SeqAny<T, V> Vec;
   const rgp_ssm_conv& a = d.a;
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x, run = idx / (uint32_t)d.nvec;
-  const int64_t c = (int64_t)(idx - run * (uint32_t)d.nvec) * V;
+  const int64_t c = conv_at<V>(idx - run * (uint32_t)d.nvec, a.D);
   if (run >= d.nrun) return;
   const SeqBlock b = seq_find(d.g, d.same ? (uint32_t)__builtin_amdgcn_readfirstlane(run) : run, d.lg);
   if (!b.ok) return;
@@ -471,7 +472,7 @@ static __global__ void __launch_bounds__(256) conv_fwd_kernel(ConvDev d) {
 template <typename T, int W, int V>
 static __global__ void __launch_bounds__(256) conv_last_kernel(ConvDev d) {
   const rgp_ssm_conv& a = d.a;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x, seq = idx / d.nvec, c = (idx - seq * d.nvec) * V;
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x, seq = idx / d.nvec, c = conv_at<V>(idx - seq * d.nvec, a.D);
   if (seq >= a.n_seq) return;
   SeqBlock b;
   b.seq = seq;
@@ -484,7 +485,7 @@ static __global__ void __launch_bounds__(256) conv_last_kernel(ConvDev d) {
   }
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) {
-    const SeqVec<T, V> x = conv_x<T, W, V>(d, b, b.len - (W - 1) + j, c);
+    const SeqAny<T, V> x = conv_x<T, W, V>(d, b, b.len - (W - 1) + j, c);
 #pragma unroll
     for (int i = 0; i < V; ++i) ((T*)a.last)[(seq * (W - 1) + j) * a.D + c + i] = x.e[i];
   }
@@ -496,12 +497,13 @@ static __global__ void __launch_bounds__(256) conv_last_kernel(ConvDev d) {
 template <typename T, int W, int V>
 static __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvDev d) {
   typedef typename SeqAcc<T>::type A;
-  typedef SeqVec<T, V> Vec;
+  typedef SeqAny<T, V> Vec;
   __shared__ A sh[256 * V];
   const rgp_ssm_conv& a = d.a;
   const int lane = threadIdx.x % d.lanes, rl = threadIdx.x / d.lanes, nr = 256 / d.lanes;
-  const int64_t vec = (int64_t)blockIdx.y * d.lanes + lane, c = vec * V;
+  const int64_t vec = (int64_t)blockIdx.y * d.lanes + lane, c = conv_at<V>(vec, a.D);
   const bool live = vec < d.nvec;
+  const int twice = live ? (int)(vec * V - c) : 0;                       // channels that the vector before counts
   A w[W][V], bias[V], gw[W][V], gb[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -585,7 +587,8 @@ static __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvDev d) {
 #pragma unroll
   for (int j = 0; j <= W; ++j) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) sh[threadIdx.x * V + i] = j < W ? gw[j < W ? j : 0][i] : gb[i];
+    for (int i = 0; i < V; ++i)
+      if (i >= twice) sh[threadIdx.x * V + i - twice] = j < W ? gw[j < W ? j : 0][i] : gb[i];
     __syncthreads();
     for (int e = threadIdx.x; e < d.lanes * V; e += 256) {
       A v = (A)0;
@@ -600,7 +603,7 @@ static __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvDev d) {
 template <typename T, int W, int V>
 static __global__ void __launch_bounds__(256) conv_step_kernel(ConvDev d) {
   typedef typename SeqAcc<T>::type A;
-  typedef SeqVec<T, V> Vec;
+  typedef SeqAny<T, V> Vec;
   const rgp_ssm_conv& a = d.a;
   const uint32_t idx = blockIdx.x * 256u + threadIdx.x, seq = idx / (uint32_t)d.nvec;
   const int64_t c = (int64_t)(idx - seq * (uint32_t)d.nvec) * V;
@@ -659,14 +662,10 @@ static void conv_plan(const rgp_ssm_conv* a, bool wide, ConvDev& d, int64_t& nrb
 extern "C" int64_t rgp_ssm_conv_workspace(const rgp_ssm_conv* a, int backward) {
   if (conv_bad(a)) return -1;
   if (!backward) return 0;
-  int64_t most = 0;
-  for (int wide = 0; wide < 2; ++wide) {
-    ConvDev d;
-    int64_t nrb, nvb;
-    conv_plan(a, wide != 0, d, nrb, nvb);
-    most = nrb > most ? nrb : most;
-  }
-  return most * (a->W + 1) * a->D * (a->dtype == RGP_F64 ? 8 : 4);
+  ConvDev d;
+  int64_t nrb, nvb;
+  conv_plan(a, a->D >= CONV_V, d, nrb, nvb);
+  return nrb * (a->W + 1) * a->D * (a->dtype == RGP_F64 ? 8 : 4);
 }
 
 enum { CONV_FWD, CONV_LAST, CONV_BWD, CONV_STEP };
@@ -713,11 +712,7 @@ static rgp_status conv_run(rgp_handle h, hipStream_t s, const rgp_ssm_conv* a, i
   if (what == CONV_STEP && (!a->v || !a->last || a->init != a->last)) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "v and the state (init = last) are required");
   if (what == CONV_FWD && some && !a->v) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "v is required");
   if (what == CONV_FWD && a->last && a->last == a->init) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "last must not be init");
-  const int e = seq_dtype_bytes(a->dtype), V = CONV_V;
-  const int64_t st = what == CONV_STEP ? 0 : a->x_st;
-  bool wide = a->D % V == 0 && seq_aligned(a->x, st, a->x_sb, e, V);
-  if (what == CONV_BWD) wide = wide && seq_aligned(a->gv, a->gv_st, a->gv_sb, e, V) && seq_aligned(a->gx, 0, 0, e, V);
-  else wide = wide && seq_aligned(a->v, 0, 0, e, V) && (what != CONV_STEP || seq_aligned(a->last, 0, 0, e, V));
+  const bool wide = what == CONV_STEP ? a->D % CONV_V == 0 : a->D >= CONV_V;      // a step changes its state in place: no channel twice
   ConvDev d;
   int64_t nrb, nvb;
   conv_plan(a, wide, d, nrb, nvb);

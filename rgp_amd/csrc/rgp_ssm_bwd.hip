@@ -10,10 +10,10 @@
 #include "rgp_ssm.h"
 
 template <typename T, int K, int CH, int MODE, int V>
-static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2) ssm_bwd_kernel(SsmDev d) {
+static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K == 1 ? 1 : 2) ssm_bwd_kernel(SsmDev d) {
   typedef typename SeqAcc<T>::type A;
-  typedef SeqVec<T, V> Vec;
-  constexpr int THREADS = CH * K, NV = CH / V, RPI = THREADS / NV, CK = SSM_CK, TL = sizeof(T) == 8 ? 8 : sizeof(T) == 4 || K > 4 ? 16 : 32, SUB = TL / CK, NP = SSM_R * K, R = SSM_R, WAVES = THREADS / 64;
+  typedef SeqAny<T, V> Vec;
+  constexpr int THREADS = CH * K, NV = CH / V, RPI = THREADS / NV, CK = SSM_CK, TL = sizeof(T) == 8 ? 8 : sizeof(T) == 2 && CH * K == 256 && K == 4 ? 32 : 16, SUB = TL / CK, NP = SSM_R * K, R = SSM_R, WAVES = THREADS / 64;
   constexpr int NI = RPI >= TL ? 1 : TL / RPI, NB = (TL * NP + THREADS - 1) / THREADS;
   struct alignas(4 * sizeof(A)) Four { A x, y, z, w; };
   struct alignas(16) Quad { A v[R]; };
@@ -30,7 +30,7 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
   const int N = a.N, chn = d.Dg - c0 < CH ? d.Dg - c0 : CH, ch0 = grp * d.Dg + c0;
   const int ev = tid % NV, et = tid / NV;               // roles as in the forward kernel
   const bool here = ev * V < chn && et < TL;
-  const int ech = ch0 + (ev * V < chn ? ev * V : 0);
+  const int el = !here || ev * V + V <= chn ? ev * V : chn - V, ech = ch0 + (here ? el : 0);
   const int ch = tid / K, k = tid % K, cp = ssm_place<V, sizeof(Four)>(ch);
   const bool live = ch < chn;
   if (!b.ok) {                                        // an empty block still owns a row of the partial sums
@@ -107,7 +107,7 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
             gp = z * q;
           }
           p.z = gp;
-          pl[tl][ssm_place<V, sizeof(Four)>(ev * V + j)] = p;
+          pl[tl][ssm_place<V, sizeof(Four)>(el + j)] = p;
         }
       }
     }
@@ -123,9 +123,13 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int tl = et + i * RPI;
-        if (et < TL && (tl >= nt || ev * V >= chn)) {
+        if (et < TL) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) pl[tl][ssm_place<V, sizeof(Four)>(ev * V + j)] = Four{(A)0, (A)0, (A)0, (A)0};
+          for (int j = 0; j < V; ++j) {
+            const Four none{(A)0, (A)0, (A)0, (A)0};
+            if (tl >= nt) pl[tl][ssm_place<V, sizeof(Four)>(el + j)] = none;
+            if (ev * V + j >= chn) pl[tl][ssm_place<V, sizeof(Four)>(ev * V + j)] = none;
+          }
         }
       }
 #pragma unroll
@@ -238,7 +242,7 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K <= 2 ? 1 : 2
           Vec ou, od, oz;
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            const Four p = pl[tl][ssm_place<V, sizeof(Four)>(ev * V + j)];
+            const Four p = pl[tl][ssm_place<V, sizeof(Four)>(el + j)];
             ou.e[j] = (T)p.x;
             od.e[j] = (T)p.y;
             if (a.z) oz.e[j] = (T)(zf[i * V + j][tid] * p.z);

@@ -1,16 +1,22 @@
 // rgp_ssm_fwd.hip -- forward kernel of the selective state-space scan
 //     dt = softplus(delta + bias);  s[n] = exp(dt A[n]) s[n] + dt u B[n];  y = (sum_n C[n] s[n] + skip u) silu(z).
 // K lanes hold one channel's states, SSM_R each; a workgroup holds CH channels of one group of B / C and walks its block of time in tiles
-// of TL steps.  What is elementwise over (step, channel) -- softplus, silu, the loads and stores, 16 bytes a lane -- runs with the lanes
-// over the tile's elements (a vector of 16 bytes each, or single elements where alignment or an odd width forbids that); between them the recurrence reads (dt, dt u) and the rows of B and C from LDS and leaves y there.  The next
-// tile's loads are in flight while a tile is walked.
+// of TL steps.  What is elementwise over (step, channel) -- softplus, silu, the loads and stores -- runs with the lanes over the tile's
+// elements, a vector of V (16 bytes) each, the last one moved back to end with the channels; single elements where a workgroup has fewer
+// channels than a vector.  Between them the recurrence reads (dt, dt u) and the rows of B and C from LDS and leaves y there.  The next tile's
+// loads are in flight while a tile is walked.
+// Bound by the vector unit: a step of a wave (64 / K channels) takes 22.6 instructions in the recurrence, 4 of them exponentials at a quarter of
+// the rate, and 12 for the elements; the unit is busy 97 % of the kernel's time (SQ_ACTIVE_INST_VALU).  8191 x 1024 bf16, N = 16, training: 48 us,
+// and 33 for the walk that only sums the blocks (MODE 1).  8 x 65536 x 64 fp32: 174 us, 3.1 TB/s, and 123.  What else was tried: 8 states a lane
+// (fewer lane sums, but half the waves): 58 instead of 49 us.  Registers allow 4 waves a SIMD, which that takes (3: 188 instead of 174 us); with
+// one or two lanes a channel, tiles of 16 steps keep the element role in registers (8192 x 2000 fp32, N = 4: 64 us, with 32 steps 110).
 #include "rgp_ssm.h"
 
 template <typename T, int K, int CH, int MODE, int V>
-static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
+static __global__ void __launch_bounds__(CH* K, sizeof(T) < 8 && (K == 4 || K == 8) && CH * K == 256 && V > 1 ? 4 : 1) ssm_fwd_kernel(SsmDev d) {
   typedef typename SeqAcc<T>::type A;
-  typedef SeqVec<T, V> Vec;
-  constexpr int THREADS = CH * K, NV = CH / V, TL = sizeof(A) == 8 ? 16 : 32, NP = SSM_R * K, R = SSM_R, RPI = THREADS / NV;
+  typedef SeqAny<T, V> Vec;
+  constexpr int THREADS = CH * K, NV = CH / V, TL = sizeof(A) == 8 || K <= 2 ? 16 : 32, NP = SSM_R * K, R = SSM_R, RPI = THREADS / NV;
   constexpr int NI = RPI >= TL ? 1 : TL / RPI, NB = (TL * NP + THREADS - 1) / THREADS, CK = SSM_CK;
   struct alignas(2 * sizeof(A)) Pair { A dt, w; };
   struct alignas(16) Quad { A v[R]; };
@@ -42,7 +48,7 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
   // last row and the first channel there are, and count as zero.
   const int ev = tid % NV, et = tid / NV;
   const bool here = ev * V < chn && et < TL;
-  const int ech = ch0 + (ev * V < chn ? ev * V : 0);
+  const int el = !here || ev * V + V <= chn ? ev * V : chn - V, ech = ch0 + (here ? el : 0);       // first channel in the tile, in all
   A bias[V], skip[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -105,7 +111,7 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
           Pair p;
           p.dt = dt;
           p.w = dt * (A)ru[i].e[j];
-          pl[tl][ssm_place<V, sizeof(Pair)>(ev * V + j)] = p;
+          pl[tl][ssm_place<V, sizeof(Pair)>(el + j)] = p;
         }
       }
     }
@@ -123,7 +129,7 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
         const int tl = et + i * RPI;
         if (et < TL && tl >= nt) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) pl[tl][ssm_place<V, sizeof(Pair)>(ev * V + j)] = Pair{(A)0, (A)0};
+          for (int j = 0; j < V; ++j) pl[tl][ssm_place<V, sizeof(Pair)>(el + j)] = Pair{(A)0, (A)0};
         }
       }
 #pragma unroll
@@ -177,7 +183,7 @@ static __global__ void __launch_bounds__(CH* K) ssm_fwd_kernel(SsmDev d) {
           Vec o;
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            A y = pl[tl][ssm_place<V, sizeof(Pair)>(ev * V + j)].dt + skip[j] * (A)cu[i].e[j];
+            A y = pl[tl][ssm_place<V, sizeof(Pair)>(el + j)].dt + skip[j] * (A)cu[i].e[j];
             if (a.z) {
               const A z = (A)cz[i].e[j];
               y *= z * seq_sigmoid(z);

@@ -510,3 +510,41 @@ def test_steps_with_infinite_decay(h):
             assert torch.equal(st, s0)
         torch.testing.assert_close(st, last, rtol=1e-6, atol=1e-6)
         torch.testing.assert_close(y, y1[0], rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize('dtype', ALL, ids=str)
+@pytest.mark.parametrize('D', [2, 9, 65, 67, 79, 127])
+def test_widths_that_are_not_whole_vectors(h, dtype, D):
+    """Channels that end inside a 16-byte vector or with fewer than one vector in a tile (65), rows at any element's address: the moved-back
+    last vector counts no channel twice and writes nothing behind the row."""
+    p = Problem(dtype, D=D, N=16, T=37, n=2, W=4, seed=D)
+    want = p.reference()
+    p.compare(p.run(h), want)
+
+    def odd(t):
+        buf = torch.full((t.numel() + 1,), float('nan'), dtype=t.dtype, device=t.device)[1:].view(t.shape)
+        return buf.copy_(t).detach()
+    p.compare(p.run(h, odd), want)
+    q = Problem(dtype, D=D, N=5, lengths=[9, 0, 70], seed=D + 1, carry=True, z=False)
+    q.compare(q.run(h, odd), q.reference())
+
+
+@pytest.mark.parametrize('dtype', ALL, ids=str)
+@pytest.mark.parametrize('rows,C', [(70, 2), (700, 9), (4000, 15), (50, 33), (20000, 17), (300, 301), (11, 1027), (1300, 127), (6, 4099), (600, 8195)])
+def test_rms_norm_rows_that_are_not_whole_vectors(h, dtype, rows, C):
+    """Odd widths through every shape of the kernels, at an odd address, with no element of a neighbouring row touched."""
+    from rgp_amd import seq_ops
+    g = _gen(rows + C)
+    odd = lambda t: torch.full((rows, C + 1), float('nan'), dtype=dtype, device='cuda')[:, 1:].copy_(t)           # noqa: E731
+    x, r, gy, gh = (_randn(g, rows, C, dtype=dtype) for _ in range(4))
+    w = _randn(g, C, dtype=ref.acc_of(dtype))
+    lx, lr, lw = odd(x).requires_grad_(True), odd(r).requires_grad_(True), w.cuda().requires_grad_(True)
+    y, hid = seq_ops.rms_norm(h, lx, lw, residual=lr)
+    gx, gr, gw = torch.autograd.grad((y, hid), (lx, lr, lw), (odd(gy), odd(gh)))
+    d = lambda t: t.double()                                      # noqa: E731
+    want = ref.rms(d(x), d(r), d(w), 1e-6, d(gy), d(gh))
+    ops = C + rows + 64                                           # the additions over a row and over the rows
+    ref.check('y', y, *want['y'], ops=ops)
+    ref.check('hid', hid, *want['hid'], ops=ops)
+    ref.check('gx', gx, *want['gx'], ops=ops, acc=ref.acc_of(dtype))
+    ref.check('gw', gw, *want['gw'], ops=ops, acc=ref.acc_of(dtype))
