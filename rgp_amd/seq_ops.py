@@ -14,15 +14,25 @@ same bits every time.  Wrong arguments raise RgpError (RGP_ERR_BAD_ARG) before a
 
 A captured backward pass needs leaves that no eager graph holds at that time: take the gradients with torch.autograd.grad inside the
 captured region, on a forward pass of the same region.  There are no second derivatives: a backward pass with create_graph=True is refused."""
+import ctypes as C
 import math
-import struct
 
 import torch
 
 from . import _lib
+from . import _seq                            # csrc/rgp_torch.cpp: checks, allocation and autograd nodes around the C entries
 from ._lib import RgpError
 
-_DTYPES = {torch.float64: _lib.DT_F64, torch.float32: _lib.DT_F32, torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16}
+_DTYPES = (torch.float64, torch.float32, torch.bfloat16, torch.float16)
+
+
+def _bind():
+    lib = _lib.load()
+    _seq.bind(RgpError, {name: C.cast(getattr(lib, name), C.c_void_p).value for name in _lib.SYMBOLS if name.startswith(('rgp_ssm_', 'rgp_rms_', 'rgp_grad_'))
+                         or name == 'rgp_last_error'})
+
+
+_bind()
 
 
 def _bad(msg):
@@ -33,50 +43,15 @@ def _acc(dtype):
     return torch.float64 if dtype == torch.float64 else torch.float32
 
 
-def _stream(handle):
-    return torch._C._cuda_getCurrentRawStream(handle.device.index)
-
-
-# The argument structs of include/rgp_hip.h as one pack each (a ctypes struct costs several microseconds to fill, as much as a short kernel
-# runs); the last two fields, work and work_bytes, are packed apart because their size is asked for with the others.
-_SCAN, _CONV, _RMS = struct.Struct('@6i3q6Q12q16Q'), struct.Struct('@6i3q2Q4q9Q'), struct.Struct('@2i2qd2Q4q8Q')
-_WORK, _NO_WORK = struct.Struct('@Qq'), b'\0' * 16
-
-
-def _call(handle, fn, head, tail=_NO_WORK):
-    st = fn(handle.h, _stream(handle), head + tail)
-    if st != 0:
-        handle._check(st)
-
-
-def _new_work(handle, query, head, backward):
-    """The work buffer of a call and its fields of the struct."""
-    n = query(head + _NO_WORK, backward)
-    if n <= 0:
-        return None, _NO_WORK
-    w = torch.empty(n, dtype=torch.uint8, device=handle.device)
-    return w, _WORK.pack(w.data_ptr(), n)
-
-
-def _new_like(t):
-    return None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)
-
-
-def _ptr(t):
-    return 0 if t is None else t.data_ptr()
+def _again(r, what):
+    """The result of a call whose operands have been looked over (and made contiguous where that was all)."""
+    if r is None:
+        _bad('%s: operands that the library does not take' % what)
+    return r
 
 
 def _wants_grad(*ts):
-    if torch.is_grad_enabled():
-        for t in ts:
-            if t is not None and t.requires_grad:
-                return True
-    return False
-
-
-def _once():
-    if torch.is_grad_enabled():
-        raise RuntimeError('the sequence operators have no second derivatives (create_graph=True)')
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
 def _overlaps(t):
@@ -118,23 +93,6 @@ def _rows(name, t, like, lead):
         _bad('%s has shape %s, leading dimensions %s expected' % (name, tuple(t.shape), tuple(lead)))
 
 
-def _all_plain(x, acts, params):
-    """True for contiguous activations of x's type and parameters of its arithmetic type (or None), all on x's device: the common case, found
-    in one pass.  Anything else goes through the checks that name what is wrong."""
-    dt, dev = x.dtype, x.device
-    acc = torch.float64 if dt is torch.float64 else torch.float32
-    try:
-        for t in acts:
-            if t.dtype is not dt or t.device != dev or not t.is_contiguous():
-                return False
-        for t in params:
-            if t is not None and (t.dtype is not acc or t.device != dev or not t.is_contiguous()):
-                return False
-    except AttributeError:
-        return False
-    return True
-
-
 def _inner(t, dims):
     """The tensor with its last ``dims`` dimensions contiguous (a copy only where they are not)."""
     if t.is_contiguous():
@@ -148,7 +106,7 @@ def _inner(t, dims):
 
 
 def _geometry(handle, x, seqs, what, step=False):
-    """(lead, n_seq, T, rows, max_len, off) of a (T, batch, D) or packed (rows, D) activation."""
+    """(leading dimensions, sequences) of a (T, batch, D) or packed (rows, D) activation."""
     if not isinstance(x, torch.Tensor):
         _bad('%s must be a device tensor' % what)
     if x.dtype not in _DTYPES:
@@ -158,27 +116,21 @@ def _geometry(handle, x, seqs, what, step=False):
     if step:                                     # (batch, D): one row of every sequence
         if x.numel() == 0:
             _bad('%s is empty: shape %s' % (what, tuple(x.shape)))
-        return x.shape[:1], x.shape[0], 1, x.shape[0], 1, None
+        return x.shape[:1], x.shape[0]
     if seqs is None:
         if x.dim() != 3:
             _bad('%s must be (T, batch, features); packed rows need a SeqTable' % what)
         T, n = x.shape[0], x.shape[1]
         if T < 1 or n < 1 or x.shape[2] < 1:
             _bad('%s is empty: shape %s' % (what, tuple(x.shape)))
-        return x.shape[:2], n, T, T * n, T, None
+        return x.shape[:2], n
     if x.dim() != 2 or x.shape[1] < 1:
         _bad('%s must be packed rows (rows, features) with a SeqTable' % what)
     if seqs.device != x.device:
         _bad('the sequence table is on %s, %s on %s' % (seqs.device, what, x.device))
     if seqs.rows != x.shape[0]:
         _bad('%s has %d rows, the sequence table %d' % (what, x.shape[0], seqs.rows))
-    return x.shape[:1], seqs.n_seq, 0, seqs.rows, seqs.max_len, seqs.off
-
-
-def _strides(t, packed):
-    """Element strides of (step, sequence)."""
-    st = t.stride()
-    return (st[0], 0) if packed else (st[0], st[1])
+    return x.shape[:1], seqs.n_seq
 
 
 def _param(name, t, shape, x, optional=False):
@@ -201,8 +153,6 @@ def _state(name, t, shape, dtype, x):
         _bad('%s must be a contiguous %s tensor of shape %s on %s' % (name, dtype, tuple(shape), x.device))
     if t.requires_grad:
         _bad('%s is updated in place and takes no gradient' % name)
-    torch.autograd.graph.increment_version(t)       # a graph that saved the state notices the update
-    return t
 
 
 def _no_step_grad(*ts):
@@ -216,54 +166,9 @@ def _no_grad_state(name, t):
 
 
 # ---------------------------------------------------------------------------------------------------------------------- convolution
-def _conv_head(x, w, bias, geo, reverse, init=0, v=0, last=0, gv=0, gv_st=(0, 0), gx=0, gw=0, gb=0):
-    _, n_seq, T, rows, max_len, off = geo
-    st = _strides(x, off is not None)
-    return _CONV.pack(_DTYPES[x.dtype], n_seq, x.shape[-1], w.shape[1], reverse, 0, T, rows, max_len, _ptr(off), x.data_ptr(), st[0], st[1], gv_st[0],
-                      gv_st[1], w.data_ptr(), _ptr(bias), init, v, last, gv, gx, gw, gb)
-
-
-def _conv_forward(handle, x, w, bias, init, geo, reverse, want_last):
-    v = _new_like(x)
-    last = torch.empty(geo[1], w.shape[1] - 1, x.shape[-1], dtype=x.dtype, device=x.device) if want_last else None
-    _call(handle, handle.lib.rgp_ssm_conv_forward, _conv_head(x, w, bias, geo, reverse, _ptr(init), v.data_ptr(), _ptr(last)))
-    return v, last
-
-
-class _ConvFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, handle, x, w, bias, init, geo, reverse, want_last):
-        v, last = _conv_forward(handle, x, w, bias, init, geo, reverse, want_last)
-        ctx.handle, ctx.geo, ctx.reverse = handle, geo, reverse
-        ctx.save_for_backward(x, w, bias, init)
-        ctx.set_materialize_grads(False)
-        if want_last:
-            ctx.mark_non_differentiable(last)
-        return v, last
-
-    @staticmethod
-    def backward(ctx, gv, _):
-        _once()
-        if gv is None:
-            return (None,) * 8
-        x, w, bias, init = ctx.saved_tensors
-        handle = ctx.handle
-        gv = _inner(gv, 1)
-        gx, gw, gb = _new_like(x), _new_like(w), _new_like(bias)
-        head = _conv_head(x, w, bias, ctx.geo, ctx.reverse, _ptr(init), 0, 0, gv.data_ptr(), _strides(gv, ctx.geo[5] is not None), gx.data_ptr(),
-                          gw.data_ptr(), _ptr(gb))
-        work, tail = _new_work(handle, handle.lib.rgp_ssm_conv_workspace, head, 1)
-        _call(handle, handle.lib.rgp_ssm_conv_backward, head, tail)
-        return None, gx, gw, gb, None, None, None, None
-
-
 def _conv_check(x, weight, bias):
     """x, filters and bias in the form the library takes."""
     D = x.shape[-1]
-    if _all_plain(x, (x,), (weight, bias)):
-        sw = weight.shape
-        if len(sw) == 2 and sw[0] == D and 2 <= sw[1] <= 8 and (bias is None or bias.shape == (D,)):
-            return x, weight, bias
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not 2 <= weight.shape[1] <= 8:
         _bad('weight must be (D, W) with 2 to 8 taps')
     return _inner(x, 1), _param('weight', weight, (D, weight.shape[1]), x), _param('bias', bias, (D,), x, optional=True)
@@ -276,100 +181,40 @@ def ssm_conv(handle, x, weight, bias=None, seqs=None, init=None, reverse=False, 
     the first step, oldest first (zeros without it); return_state=True also returns them for the step behind the last one.  reverse=True
     walks every sequence from its last step (init and the returned state are then those of that walk).  Gradients: x, weight, bias (states
     take none)."""
-    geo = _geometry(handle, x, seqs, 'x')
-    D = x.shape[-1]
-    x, w, b = _conv_check(x, weight, bias)
-    if init is not None:
-        _no_grad_state('init', init)
-        if init.shape != (geo[1], w.shape[1] - 1, D) or init.dtype is not x.dtype or init.device != x.device:
-            _bad('init must be %s of shape %s on %s' % (x.dtype, (geo[1], w.shape[1] - 1, D), x.device))
-        init = init.contiguous()
-    run = _ConvFn.apply if _wants_grad(x, w, b) else _conv_forward
-    v, last = run(handle, x, w, b, init, geo, bool(reverse), bool(return_state))
-    return (v, last) if return_state else v
+    r = _seq.conv(handle, x, weight, bias, seqs, init, bool(reverse), bool(return_state))
+    if r is None:
+        _, n_seq = _geometry(handle, x, seqs, 'x')
+        x, w, b = _conv_check(x, weight, bias)
+        if init is not None:
+            _no_grad_state('init', init)
+            shape = (n_seq, w.shape[1] - 1, x.shape[-1])
+            if init.shape != shape or init.dtype is not x.dtype or init.device != x.device:
+                _bad('init must be %s of shape %s on %s' % (x.dtype, shape, x.device))
+            init = init.contiguous()
+        r = _again(_seq.conv(handle, x, w, b, seqs, init, bool(reverse), bool(return_state)), 'ssm_conv')
+    return r if return_state else r[0]
 
 
 def ssm_conv_step(handle, x, weight, bias, state):
     """One step of ``ssm_conv``: x (batch, D), state (batch, W - 1, D) of x's type, updated in place.  It takes no
     gradients: operands that require them are refused outside torch.no_grad()."""
-    if not isinstance(x, torch.Tensor) or x.dim() != 2:
-        _bad('x must be (batch, D)')
-    geo = _geometry(handle, x, None, 'x', step=True)
-    D = x.shape[1]
-    x, w, b = _conv_check(x, weight, bias)
-    _no_step_grad(x, w, b)
-    _state('state', state, (x.shape[0], w.shape[1] - 1, D), x.dtype, x)
-    v, st = _new_like(x), state.data_ptr()
-    _call(handle, handle.lib.rgp_ssm_conv_step, _CONV.pack(_DTYPES[x.dtype], x.shape[0], D, w.shape[1], 0, 0, 1, x.shape[0], 1, 0, x.data_ptr(), 0,
-                                                          x.stride(0), 0, 0, w.data_ptr(), _ptr(b), st, v.data_ptr(), st, 0, 0, 0, 0))
+    v = _seq.conv_step(handle, x, weight, bias, state)
+    if v is None:
+        if not isinstance(x, torch.Tensor) or x.dim() != 2:
+            _bad('x must be (batch, D)')
+        _geometry(handle, x, None, 'x', step=True)
+        x, w, b = _conv_check(x, weight, bias)
+        _no_step_grad(x, w, b)
+        _state('state', state, (x.shape[0], w.shape[1] - 1, x.shape[1]), x.dtype, x)
+        v = _again(_seq.conv_step(handle, x, w, b, state), 'ssm_conv_step')
     return v
 
 
 # ---------------------------------------------------------------------------------------------------------------------- scan
-def _scan_head(ops, geo, G, reverse, init=0, y=0, last=0, states=0, gy=0, gy_st=(0, 0), grads=(0,) * 8):
-    u, delta, A, B, Cm, skip, z, bias = ops
-    _, n_seq, T, rows, max_len, off = geo
-    packed = off is not None
-    su, sd, sB, sC = _strides(u, packed), _strides(delta, packed), _strides(B, packed), _strides(Cm, packed)
-    sz = _strides(z, packed) if z is not None else (0, 0)
-    gu, gdelta, gA, gB, gC, gskip, gz, gbias = grads
-    return _SCAN.pack(_DTYPES[u.dtype], n_seq, u.shape[-1], A.shape[1], G, reverse, T, rows, max_len, _ptr(off), u.data_ptr(),
-                      delta.data_ptr(), _ptr(z), B.data_ptr(), Cm.data_ptr(), su[0], su[1], sd[0], sd[1], sz[0], sz[1], sB[0], sB[1], sC[0], sC[1],
-                      gy_st[0], gy_st[1], A.data_ptr(), _ptr(skip), _ptr(bias), init, y, last, states, gy, gu, gdelta, gz, gB, gC, gA, gskip, gbias)
-
-
-def _scan_forward(handle, u, delta, A, B, Cm, skip, z, bias, init, geo, G, reverse, want_last, train=False):
-    ops = (u, delta, A, B, Cm, skip, z, bias)
-    y = _new_like(u)
-    last = torch.empty(geo[1], u.shape[-1], A.shape[1], dtype=A.dtype, device=u.device) if want_last else None
-    states = None
-    if train:
-        # a state of N every 8 steps of every sequence: (blocks of 8) D N values (rgp_ssm_scan_states_bytes)
-        blocks = (geo[3] >> 3) + geo[1] if geo[5] is not None else geo[1] * ((geo[2] + 7) >> 3)
-        states = torch.empty(blocks * A.numel(), dtype=A.dtype, device=u.device)
-    head = _scan_head(ops, geo, G, reverse, _ptr(init), y.data_ptr(), _ptr(last), _ptr(states))
-    work, tail = _new_work(handle, handle.lib.rgp_ssm_scan_workspace, head, 0)
-    _call(handle, handle.lib.rgp_ssm_scan_forward, head, tail)
-    return (y, last, states) if train else (y, last)
-
-
-class _ScanFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, handle, u, delta, A, B, Cm, skip, z, bias, init, geo, G, reverse, want_last):
-        y, last, states = _scan_forward(handle, u, delta, A, B, Cm, skip, z, bias, init, geo, G, reverse, want_last, True)
-        ctx.handle, ctx.geo, ctx.G, ctx.reverse = handle, geo, G, reverse
-        ctx.save_for_backward(u, delta, A, B, Cm, skip, z, bias, states)
-        ctx.set_materialize_grads(False)
-        if want_last:
-            ctx.mark_non_differentiable(last)
-        return y, last
-
-    @staticmethod
-    def backward(ctx, gy, _):
-        _once()
-        if gy is None:
-            return (None,) * 14
-        saved = ctx.saved_tensors
-        ops, states, handle = saved[:8], saved[8], ctx.handle
-        gy = _inner(gy, 1)
-        grads = [_new_like(t) for t in ops]
-        head = _scan_head(ops, ctx.geo, ctx.G, ctx.reverse, states=states.data_ptr(), gy=gy.data_ptr(), gy_st=_strides(gy, ctx.geo[5] is not None),
-                          grads=[_ptr(t) for t in grads])
-        work, tail = _new_work(handle, handle.lib.rgp_ssm_scan_workspace, head, 1)
-        _call(handle, handle.lib.rgp_ssm_scan_backward, head, tail)
-        return (None, *grads, None, None, None, None, None)
-
-
 def _scan_check(u, delta, A, B, Cm, D, z, delta_bias, lead):
     """Operands in the form the library takes: (.., D) activations with contiguous features, (.., N) or (.., G, N) maps, contiguous
     parameters."""
     nd, n = len(lead), u.shape[-1]
-    if _all_plain(u, (u, delta, B, Cm) if z is None else (u, delta, B, Cm, z), (A, D, delta_bias)):      # then only the shapes are left to check
-        sh, sb, N = u.shape, B.shape, A.shape[-1]
-        G = 1 if len(sb) == nd + 1 else sb[-2] if len(sb) == nd + 2 else 0
-        if delta.shape == sh and (z is None or z.shape == sh) and Cm.shape == sb and sb[:nd] == lead and sb[-1] == N and G and not n % G and 1 <= N <= 64 \
-                and A.shape == (n, N) and (D is None or D.shape == (n,)) and (delta_bias is None or delta_bias.shape == (n,)):
-            return (u, delta, A, B, Cm, D, z, delta_bias), G
     for name, t in (('delta', delta), ('z', z)):
         if t is not None:
             _rows(name, t, u, lead)
@@ -391,7 +236,7 @@ def _scan_check(u, delta, A, B, Cm, D, z, delta_bias, lead):
     if groups[0] != groups[1]:
         _bad('B has %d groups, C %d' % tuple(groups))
     return (_inner(u, 1), _inner(delta, 1), _param('A', A, (n, N), u), maps[0], maps[1], _param('D', D, (n,), u, optional=True),
-            None if z is None else _inner(z, 1), _param('delta_bias', delta_bias, (n,), u, optional=True)), groups[0]
+            None if z is None else _inner(z, 1), _param('delta_bias', delta_bias, (n,), u, optional=True))
 
 
 def ssm_scan(handle, u, delta, A, B, Cm, D=None, z=None, delta_bias=None, seqs=None, init=None, reverse=False, return_state=False):
@@ -401,138 +246,74 @@ def ssm_scan(handle, u, delta, A, B, Cm, D=None, z=None, delta_bias=None, seqs=N
     N <= 64; D, delta_bias (Dn,).  init: (n_seq, Dn, N), the state before the first step (zeros without it); return_state=True also returns
     the state behind the last step.  reverse=True walks every sequence from its last step.  Gradients: u, delta, A, B, C, D, z, delta_bias
     (states take none)."""
-    geo = _geometry(handle, u, seqs, 'u')
-    ops, G = _scan_check(u, delta, A, B, Cm, D, z, delta_bias, geo[0])
-    if init is not None:
-        _no_grad_state('init', init)
-        init = _param('init', init, (geo[1], u.shape[-1], A.shape[1]), u)
-    run = _ScanFn.apply if _wants_grad(*ops) else _scan_forward
-    y, last = run(handle, *ops, init, geo, G, bool(reverse), bool(return_state))
-    return (y, last) if return_state else y
+    r = _seq.scan(handle, u, delta, A, B, Cm, D, z, delta_bias, seqs, init, bool(reverse), bool(return_state))
+    if r is None:
+        lead, n_seq = _geometry(handle, u, seqs, 'u')
+        ops = _scan_check(u, delta, A, B, Cm, D, z, delta_bias, lead)
+        if init is not None:
+            _no_grad_state('init', init)
+            init = _param('init', init, (n_seq, u.shape[-1], A.shape[1]), u)
+        r = _again(_seq.scan(handle, *ops, seqs, init, bool(reverse), bool(return_state)), 'ssm_scan')
+    return r if return_state else r[0]
 
 
 def ssm_scan_step(handle, u, delta, A, B, Cm, D, state, z=None, delta_bias=None):
     """One step of ``ssm_scan``: u, delta, z (batch, Dn); B, C (batch, N) or (batch, G, N); state (batch, Dn, N), updated in place.  It
     takes no gradients: operands that require them are refused outside torch.no_grad()."""
-    if not isinstance(u, torch.Tensor) or u.dim() != 2:
-        _bad('u must be (batch, D)')
-    geo = _geometry(handle, u, None, 'u', step=True)
-    _no_step_grad(u, delta, A, B, Cm, D, z, delta_bias)
-    (u, delta, A, B, Cm, skip, z, bias), G = _scan_check(u, delta, A, B, Cm, D, z, delta_bias, geo[0])
-    n, Dn = u.shape
-    N = A.shape[1]
-    _state('state', state, (n, Dn, N), A.dtype, u)
-    y, st = _new_like(u), state.data_ptr()
-    _call(handle, handle.lib.rgp_ssm_scan_step, _SCAN.pack(
-        _DTYPES[u.dtype], n, Dn, N, G, 0, 1, n, 1, 0, u.data_ptr(), delta.data_ptr(), _ptr(z), B.data_ptr(), Cm.data_ptr(), 0, u.stride(0), 0,
-        delta.stride(0), 0, 0 if z is None else z.stride(0), 0, B.stride(0), 0, Cm.stride(0), 0, 0, A.data_ptr(), _ptr(skip), _ptr(bias), st,
-        y.data_ptr(), st, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0))
+    y = _seq.scan_step(handle, u, delta, A, B, Cm, D, z, delta_bias, state)
+    if y is None:
+        if not isinstance(u, torch.Tensor) or u.dim() != 2:
+            _bad('u must be (batch, D)')
+        lead, n = _geometry(handle, u, None, 'u', step=True)
+        _no_step_grad(u, delta, A, B, Cm, D, z, delta_bias)
+        ops = _scan_check(u, delta, A, B, Cm, D, z, delta_bias, lead)
+        _state('state', state, (n, u.shape[1], A.shape[1]), _acc(u.dtype), u)
+        y = _again(_seq.scan_step(handle, *ops, state), 'ssm_scan_step')
     return y
 
 
 # ---------------------------------------------------------------------------------------------------------------------- norm
-def _rms_head(x, w, residual, eps, y=0, hid=0, rstd=0, gy=None, gh=None, gx=0, gw=0):
-    st = lambda t: 0 if t is None else t.stride(0)                           # noqa: E731
-    return _RMS.pack(_DTYPES[x.dtype], 0, x.shape[0], x.shape[1], eps, x.data_ptr(), _ptr(residual), x.stride(0), st(residual), st(gy), st(gh),
-                     w.data_ptr(), y, hid, rstd, _ptr(gy), _ptr(gh), gx, gw)
-
-
-def _rms_forward(handle, x, w, residual, eps, train=False):
-    y = _new_like(x)
-    hid = _new_like(x) if residual is not None else None
-    rstd = torch.empty(x.shape[0], dtype=w.dtype, device=x.device) if train else None
-    _call(handle, handle.lib.rgp_rms_norm_forward, _rms_head(x, w, residual, eps, y.data_ptr(), _ptr(hid), _ptr(rstd)))
-    return (y, hid, rstd) if train else (y, hid)
-
-
-class _RmsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, handle, x, w, residual, eps):
-        y, hid, rstd = _rms_forward(handle, x, w, residual, eps, True)
-        ctx.handle, ctx.eps, ctx.two = handle, eps, residual is not None
-        # 16-bit: the backward pass adds x and residual again, hid's rounding would show in the weight's gradient; 32 and 64 bits: hid is that sum
-        again = residual is not None and x.element_size() == 2
-        ctx.save_for_backward(x if again or residual is None else hid, residual if again else None, w, rstd)
-        ctx.set_materialize_grads(False)
-        return y, hid
-
-    @staticmethod
-    def backward(ctx, gy, gh):
-        _once()
-        hid, residual, w, rstd = ctx.saved_tensors
-        if gy is None:                                    # only the sum was used further on
-            return None, gh, None, gh if ctx.two else None, None
-        handle = ctx.handle
-        gy, gh = _inner(gy, 1), None if gh is None else _inner(gh, 1)
-        gx, gw = _new_like(hid), _new_like(w)
-        head = _rms_head(hid, w, residual, ctx.eps, rstd=rstd.data_ptr(), gy=gy, gh=gh, gx=gx.data_ptr(), gw=gw.data_ptr())
-        work, tail = _new_work(handle, handle.lib.rgp_rms_norm_workspace, head, 1)
-        _call(handle, handle.lib.rgp_rms_norm_backward, head, tail)
-        return None, gx, gw, gx if ctx.two else None, None
-
-
 def rms_norm(handle, x, weight, residual=None, eps=1e-6):
     """weight * hid / sqrt(mean(hid^2) + eps) over the last dimension, hid = x + residual.  Returns the norm, or (norm, hid) where a residual
     is given.  x, residual: any leading shape; weight (C,).  Gradients: x, residual, weight."""
-    if not isinstance(x, torch.Tensor) or x.dtype not in _DTYPES or x.dim() < 1 or x.shape[-1] < 1:
-        _bad('x must be a device tensor of float64, float32, bfloat16 or float16 with a last dimension')
-    if x.device != handle.device:
-        _bad('x is on %s, the handle on %s' % (x.device, handle.device))
     eps = float(eps)
-    if not eps > 0.0 or math.isinf(eps):
-        _bad('eps must be positive')
-    shape, two = x.shape, x.dim() == 2
-    if two and _all_plain(x, (x,) if residual is None else (x, residual), (weight,)) and weight.shape == shape[1:] and (residual is None or residual.shape == shape):
-        x2, r2, w = x, residual, weight
-    else:
+    r = _seq.rms(handle, x, weight, residual, eps)
+    if r is None:
+        if not isinstance(x, torch.Tensor) or x.dtype not in _DTYPES or x.dim() < 1 or x.shape[-1] < 1:
+            _bad('x must be a device tensor of float64, float32, bfloat16 or float16 with a last dimension')
+        if x.device != handle.device:
+            _bad('x is on %s, the handle on %s' % (x.device, handle.device))
+        if not eps > 0.0 or math.isinf(eps):
+            _bad('eps must be positive')
+        shape = x.shape
         w = _param('weight', weight, shape[-1:], x)
+        rows = lambda t: _inner(t if t.dim() == 2 else t.reshape(-1, shape[-1]), 1)                          # noqa: E731
         if residual is not None:
             _rows('residual', residual, x, shape)
             if residual.dim() != x.dim():
                 _bad('residual has shape %s, x %s' % (tuple(residual.shape), tuple(shape)))
-        x2 = _inner(x if two else x.reshape(-1, shape[-1]), 1)
-        r2 = None if residual is None else _inner(residual if two else residual.reshape(-1, shape[-1]), 1)
-    y, hid = (_RmsFn.apply if _wants_grad(x2, r2, w) else _rms_forward)(handle, x2, w, r2, eps)
-    if not two:
-        y, hid = y.view(shape), None if hid is None else hid.view(shape)
-    return y if residual is None else (y, hid)
+            residual = rows(residual)
+        y, hid = _again(_seq.rms(handle, rows(x), w, residual, eps), 'rms_norm')
+        r = y.view(shape), None if hid is None else hid.view(shape)
+    return r[0] if residual is None else r
 
 
 # ---------------------------------------------------------------------------------------------------------------------- gradient norm
-def _grad_list(handle, grads):
-    """(n, addresses, element counts, types) of one call's tensors, checked; the arrays live as long as the tuple."""
-    n, dev = len(grads), handle.device
-    try:
-        plain = all([g.device == dev and g.is_contiguous() for g in grads])
-        dtype = [_DTYPES[g.dtype] for g in grads]
-    except (AttributeError, KeyError, RuntimeError):
-        plain = False
-    if not plain:
-        for i, g in enumerate(grads):
-            if not isinstance(g, torch.Tensor) or g.dtype not in _DTYPES or g.device != dev or g.layout is not torch.strided:
-                _bad('gradient %d must be a float64, float32, bfloat16 or float16 tensor on %s' % (i, dev))
-            if not g.is_contiguous() and g.numel() and (_overlaps(g) or sum((m - 1) * s for m, s in zip(g.shape, g.stride())) + 1 != g.numel()):
-                _bad('gradient %d has gaps or repeats in memory: it cannot be clipped in place as one range' % i)
-    ptr, numel = [g.data_ptr() for g in grads], [g.numel() for g in grads]
-    end = 0
-    for p, k, d in sorted(zip(ptr, numel, dtype)):
-        if p < end and k:
-            _bad('two gradients share memory: each element may be clipped once')
-        end = max(end, p + k * _BYTES[d])
-    return n, struct.pack('%dQ' % n, *ptr), struct.pack('%dq' % n, *numel), struct.pack('%di' % n, *dtype)
-
-
-_BYTES = {_lib.DT_F64: 8, _lib.DT_F32: 4, _lib.DT_BF16: 2, _lib.DT_F16: 2}
+def _bad_grads(handle, grads):
+    """Names what is wrong with a list of gradients."""
+    for i, g in enumerate(grads):
+        if not isinstance(g, torch.Tensor) or g.dtype not in _DTYPES or g.device != handle.device or g.layout is not torch.strided:
+            _bad('gradient %d must be a float64, float32, bfloat16 or float16 tensor on %s' % (i, handle.device))
+        if not g.is_contiguous() and g.numel() and (_overlaps(g) or sum((m - 1) * s for m, s in zip(g.shape, g.stride())) + 1 != g.numel()):
+            _bad('gradient %d has gaps or repeats in memory: it cannot be clipped in place as one range' % i)
+    _bad('two gradients share memory: each element may be clipped once')
 
 
 def grad_sumsq(handle, grads):
     """Sum of the squares of all elements of ``grads`` as a float64 device scalar (a data-parallel caller adds the ranks' sums)."""
-    n, ptr, numel, dtype = _grad_list(handle, list(grads))
-    nbytes = handle.lib.rgp_grad_workspace(n, numel, dtype)
-    buf = torch.empty(1 + nbytes // 8, dtype=torch.float64, device=handle.device)
-    p = buf.data_ptr()
-    handle._check(handle.lib.rgp_grad_sumsq(handle.h, _stream(handle), n, ptr, numel, dtype, p, p + 8, nbytes))
-    return buf[0]
+    grads = list(grads)
+    r = _seq.sumsq(handle, grads)
+    return _bad_grads(handle, grads) if r is None else r
 
 
 def clip_grad_norm(handle, grads, max_norm, sumsq=None):
@@ -544,14 +325,9 @@ def clip_grad_norm(handle, grads, max_norm, sumsq=None):
     if not max_norm > 0.0:
         _bad('max_norm must be positive')
     grads = list(grads)
-    n, ptr, numel, dtype = _grad_list(handle, grads)
-    nbytes = 0
-    if sumsq is None:
-        nbytes = handle.lib.rgp_grad_workspace(n, numel, dtype)
-    elif not isinstance(sumsq, torch.Tensor) or sumsq.dtype is not torch.float64 or sumsq.numel() != 1 or sumsq.device != handle.device:
-        _bad('sumsq must be one float64 value on %s' % handle.device)
-    buf = torch.empty(1 + nbytes // 8, dtype=torch.float64, device=handle.device)
-    p = buf.data_ptr()
-    torch.autograd.graph.increment_version(grads)
-    handle._check(handle.lib.rgp_grad_clip(handle.h, _stream(handle), n, ptr, numel, dtype, _ptr(sumsq), max_norm, p, p + 8 if nbytes else 0, nbytes))
-    return buf[0]
+    r = _seq.clip(handle, grads, max_norm, sumsq)
+    if r is None:
+        if sumsq is not None and (not isinstance(sumsq, torch.Tensor) or sumsq.dtype is not torch.float64 or sumsq.numel() != 1 or sumsq.device != handle.device):
+            _bad('sumsq must be one float64 value on %s' % handle.device)
+        _bad_grads(handle, grads)
+    return r
