@@ -161,7 +161,9 @@ def _no_step_grad(*ts):
 
 
 def _no_grad_state(name, t):
-    if t is not None and t.requires_grad:
+    if not isinstance(t, torch.Tensor):
+        _bad('%s must be a tensor' % name)
+    if t.requires_grad:
         _bad('%s takes no gradient: detach it' % name)
 
 

@@ -568,3 +568,78 @@ def test_rms_norm_rows_that_are_not_whole_vectors(h, dtype, rows, C):
     ref.check('hid', hid, *want['hid'], ops=ops)
     ref.check('gx', gx, *want['gx'], ops=ops, acc=ref.acc_of(dtype))
     ref.check('gw', gw, *want['gw'], ops=ops, acc=ref.acc_of(dtype))
+
+
+def test_graphs_keep_what_they_need_and_end_like_others(h):
+    """A backward pass twice without retain_graph is refused, with it gives the same bits; gradients of x and residual that accumulate into
+    leaves share no memory; a graph keeps its handle; a closed handle refuses."""
+    from rgp_amd import seq_ops
+    from rgp_amd._lib import RgpError
+    from rgp_amd.capi import Handle
+    g = _gen(21)
+    t = {k: _randn(g, *s, dtype=F32).cuda().requires_grad_(True) for k, s in
+         dict(u=(9, 2, 6), delta=(9, 2, 6), A=(6, 3), B=(9, 2, 3), C=(9, 2, 3), w=(6, 4), x=(5, 8), r=(5, 8), n=(8,)).items()}
+    other = Handle()
+    y = seq_ops.ssm_scan(other, t['u'], t['delta'], t['A'], t['B'], t['C'])
+    v = seq_ops.ssm_conv(other, t['u'], t['w'])
+    n, hid = seq_ops.rms_norm(other, t['x'], t['n'], residual=t['r'])
+    del other
+    for out, ins in ((y, 'u delta A B C'), (v, 'u w'), (n, 'x r n')):
+        ins = [t[k] for k in ins.split()]
+        one = torch.autograd.grad(out.sum(), ins, retain_graph=True)
+        two = torch.autograd.grad(out.sum(), ins)
+        assert all(torch.equal(a, b) for a, b in zip(one, two))
+        with pytest.raises(RuntimeError, match='second time'):
+            torch.autograd.grad(out.sum(), ins)
+    n, hid = seq_ops.rms_norm(h, t['x'], t['n'], residual=t['r'])
+    (n.sum() + 2 * hid.sum()).backward()
+    assert torch.equal(t['x'].grad, t['r'].grad) and t['x'].grad.data_ptr() != t['r'].grad.data_ptr()
+    before = t['r'].grad.clone()
+    t['x'].grad.zero_()
+    assert torch.equal(t['r'].grad, before)
+    n, hid = seq_ops.rms_norm(h, t['x'], t['n'], residual=t['x'])                # the same leaf twice
+    gx, = torch.autograd.grad(n.sum(), t['x'])
+    n2, _ = seq_ops.rms_norm(h, t['x'], t['n'], residual=t['x'].detach().clone().requires_grad_(True))
+    g2, = torch.autograd.grad(n2.sum(), t['x'])
+    torch.testing.assert_close(gx, 2 * g2)
+    closed = Handle()
+    closed.close()
+    with pytest.raises(RgpError):
+        seq_ops.rms_norm(closed, t['x'].detach(), t['n'].detach())
+
+
+def test_threads_with_streams_of_their_own_share_a_handle(h):
+    """Four threads at once on one handle, each on its own stream, forward and backward: everybody gets the bits that a lone caller gets."""
+    import threading
+    from rgp_amd import seq_ops
+    g = _gen(22)
+    inputs = [[_randn(g, 300, 3, n, dtype=F32).cuda() for n in (20, 20, 16, 16)] + [-torch.exp(_randn(g, 20, 16)).float().cuda(), _randn(g, 20, dtype=F32).cuda()]
+              for _ in range(4)]
+
+    def work(ops):
+        u, delta, B, Cm, A, w = [t.clone().requires_grad_(True) for t in ops]
+        y = seq_ops.ssm_scan(h, u, delta, A, B, Cm)
+        n, hid = seq_ops.rms_norm(h, y, w, residual=u)
+        grads = torch.autograd.grad(n.square().sum() + hid.sum(), (u, delta, A, B, Cm, w))
+        return [t.detach() for t in (y, n, hid) + grads]
+
+    want = [work(ops) for ops in inputs]
+    torch.cuda.synchronize()
+    got, failed = [None] * 4, []
+
+    def run(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got[i] = work(inputs[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                                      # noqa: BLE001
+            failed.append(e)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
