@@ -6,7 +6,8 @@
 
 // ---- sums of partial results in a fixed order -----------------------------------------------------------------------------------------
 // A workgroup forms 64 outputs of one of up to five sums, 16 threads for each: thread q adds partials q, q + 16, ... in eight interleaved
-// sums (that many loads are in flight), then the 16 are added in LDS; up to SEQ_FEW partials are added by one thread an output.  The order depends on the count of partials alone.
+// sums (that many loads are in flight), then the 16 are added in LDS; up to SEQ_FEW
+// partials are added by one thread an output.  The order depends on the count of partials alone.  4 to 9 us for all sums of a backward pass.
 #define SEQ_FEW 32
 static __host__ __device__ inline int64_t seq_sums_width(int64_t P) { return P <= SEQ_FEW ? 1024 : 64; }
 template <typename A>
@@ -80,7 +81,8 @@ rgp_status SeqSums::run(rgp_handle h, hipStream_t s, int acc) {
 // state by exp(A sum dt): the decays of a diagonal recurrence commute.  back: the same for the adjoint, from the last block to the first.
 // 64 lanes take neighbouring (channel, state) pairs of one sequence, Q threads a pair: each walks its part of the blocks twice, first for
 // what that stretch does as a whole, then with the state that enters it (Q = 1: once).  The walk waits for memory, JOIN_U blocks at a time;
-// with Q = 16 for 1024 blocks of 8 sequences it takes 21 us where one thread a pair took 479, but 98 instead of 15 for many short sequences.
+// with Q = 16 for 1024 blocks of 8 sequences x 64 channels it takes 14 us where one thread a pair took 479; for many short sequences Q = 1 takes
+// 14 us where Q = 16 took 98.
 #define JOIN_U 8
 template <typename A, int Q>
 static __global__ void __launch_bounds__(Q == 1 ? 256 : Q * 64) ssm_join_kernel(SsmDev d, int back) {
@@ -188,7 +190,7 @@ static void scan_plan(const rgp_ssm_scan* a, bool back, ScanPlan& p) {
   // Split over time.  In units of the time in which a SIMD with several waves walks one wave's step (about 80 ns forward, 260 ns backward):
   // unsplit, the whole work spread over 1024 SIMDs, but no less than the longest sequence at twice that time (a lone wave waits for its own
   // results); split, the work, a walk over one block, the first walk (0.65 of the forward one, 0.3 of the backward one), and the join.
-  // Measured at 8 x 1024 x 1024 bf16, N = 32, backward: 445 us unsplit; 16 x 16 blocks of the same case at N = 16: 186 split.  Blocks of 64
+  // Measured backward: 8 x 1024 x 1024 bf16, N = 32, 445 us unsplit; N = 16 in 16 blocks, 186 split.  Blocks of 64
   // steps, of 32 where that leaves most SIMDs idle, longer ones where the waves get many: shorter blocks balance ragged lengths, longer ones
   // leave the join (and the sums of the backward pass) less to read.
   const double waves = (double)a->G * d.ncb * (p.CH * p.K / 64.0), work = waves * a->rows / 1024.0, most = back ? 12288.0 : 24576.0;
@@ -287,7 +289,8 @@ extern "C" rgp_status rgp_ssm_scan_backward(rgp_handle h, void* stream, const rg
 }
 
 // ---- one step -----------------------------------------------------------------------------------------------------------------------------
-// Bound by reading and writing the state: K lanes a channel, 16 bytes of state a lane (32 in fp64), as in the kernels over time.
+// Bound by reading and writing the state: K lanes a channel, 16 bytes of state a lane (32 in fp64), as in the kernels over time.  256 x 2048
+// bf16, N = 16: 16.7 us for 67 MB of state and 8 MB beside it, 4.5 TB/s; one sequence of 40 channels 3.7 us, the launch.
 template <typename T, int K>
 static __global__ void __launch_bounds__(256) ssm_step_kernel(rgp_ssm_scan a, int Dg, int whole) {
   typedef typename SeqAcc<T>::type A;
@@ -491,7 +494,7 @@ static __global__ void __launch_bounds__(256) conv_last_kernel(ConvDev d) {
   }
 }
 
-// Backward: gp = gv silu'(pre), gx_t = sum_j w_j gp_{t+W-1-j}, gw_j = sum_t gp_t x_{t-W+1+j}, gbias = sum gp.  pre is formed again from x
+// Backward (8191 x 1024 bf16 26 us, 32 x 4096 x 64 fp32 30: waits for rows, the vector unit is busy half of the time): gp = gv silu'(pre), gx_t = sum_j w_j gp_{t+W-1-j}, gw_j = sum_t gp_t x_{t-W+1+j}, gbias = sum gp.  pre is formed again from x
 // (one more read would cost more than W multiply-adds).  A thread walks its runs and W - 1 steps behind each; the parameter sums of the
 // threads with the same channels go through LDS, then from all workgroups through `part`.
 template <typename T, int W, int V>
