@@ -27,9 +27,10 @@ static __device__ __forceinline__ A row_sum(A v, A* sh) {
   }
 }
 
-// TPR threads a row, NE vectors of V elements each (16 bytes; V = 1 for rows shorter than that); rows of TPR * NE * V >= C elements.
-// WHOLE: C is a multiple of V, otherwise the row's last vector is moved back and its first elements belong to the one before.  A workgroup takes every gridDim-th group of rows and keeps w; the next rows are loaded while these are normed.  hid is rounded
-// to its type where it is written; the norm uses the sum before that rounding.
+// TPR threads a row, NE vectors of V elements each (16 bytes; V = 1 for rows shorter than that); rows of TPR * NE * V >= C elements. WHOLE: C
+// is a multiple of V, otherwise the row's last vector is moved back and its first elements belong to the one before.  A workgroup takes every
+// gridDim-th group of rows and keeps w; the next rows are loaded while these are normed.  hid is rounded to its type where it is written; the
+// norm uses the sum before that rounding.
 template <typename T, int TPR, int NE, int V, bool WHOLE>
 static __global__ void __launch_bounds__(256) rms_fwd_kernel(NormDev d) {
   typedef typename SeqAcc<T>::type A;

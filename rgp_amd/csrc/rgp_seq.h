@@ -149,11 +149,11 @@ template <typename A>
 static __device__ __forceinline__ A seq_sigmoid(A x) { return seq_rcp((A)1 + seq_exp(-x)); }
 
 // ---- rows of sequences --------------------------------------------------------------------------------------------------------------
-// off == nullptr: n_seq sequences of T steps, step t of sequence s at base + s * sb + t * st; otherwise packed rows, step t of sequence s
-// at base + (off[s] + t) * st.  Sequences are cut into blocks of L = 2^lg steps that never cross a sequence; block j of sequence i is number
-// j * n_seq + i (neighbours in number are neighbours in memory), or floor(off[i] / L) + i + j for packed rows: those numbers are increasing,
-// distinct and below rows / L + n_seq without a table of block counts (some stay empty).  Offsets are clamped to the rows there are, so a wrong table cannot make a kernel
-// touch memory outside its tensors.
+// off == nullptr: n_seq sequences of T steps, step t of sequence s at base + s * sb + t * st; otherwise packed rows, step t of sequence s at
+// base + (off[s] + t) * st.  Sequences are cut into blocks of L = 2^lg steps that never cross a sequence; block j of sequence i is number j *
+// n_seq + i (neighbours in number are neighbours in memory), or floor(off[i] / L) + i + j for packed rows: those numbers are increasing,
+// distinct and below rows / L + n_seq without a table of block counts (some stay empty).  Offsets are clamped to the rows there are, so a wrong
+// table cannot make a kernel touch memory outside its tensors.
 struct SeqGeo {
   const int64_t* off;
   int64_t T, rows;

@@ -494,9 +494,10 @@ static __global__ void __launch_bounds__(256) conv_last_kernel(ConvDev d) {
   }
 }
 
-// Backward (8191 x 1024 bf16 26 us, 32 x 4096 x 64 fp32 30: waits for rows, the vector unit is busy half of the time): gp = gv silu'(pre), gx_t = sum_j w_j gp_{t+W-1-j}, gw_j = sum_t gp_t x_{t-W+1+j}, gbias = sum gp.  pre is formed again from x
-// (one more read would cost more than W multiply-adds).  A thread walks its runs and W - 1 steps behind each; the parameter sums of the
-// threads with the same channels go through LDS, then from all workgroups through `part`.
+// Backward (8191 x 1024 bf16 26 us, 32 x 4096 x 64 fp32 30: waits for rows, the vector unit is busy half of the time): gp = gv silu'(pre), gx_t
+// = sum_j w_j gp_{t+W-1-j}, gw_j = sum_t gp_t x_{t-W+1+j}, gbias = sum gp.  pre is formed again from x (one more read would cost more than W
+// multiply-adds).  A thread walks its runs and W - 1 steps behind each; the parameter sums of the threads with the same channels go through
+// LDS, then from all workgroups through `part`.
 template <typename T, int W, int V>
 static __global__ void __launch_bounds__(256) conv_bwd_kernel(ConvDev d) {
   typedef typename SeqAcc<T>::type A;

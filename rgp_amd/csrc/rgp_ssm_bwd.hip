@@ -3,22 +3,23 @@
 // the gradients are
 //     gu = dt sum_n lam B + skip gp;   gdelta = sigmoid(delta + bias) (u sum_n lam B + sum_n lam a s_{t-1} A);
 //     gB[n] = sum_d lam dt u;  gC[n] = sum_d gp s;  gA[n] = sum_t lam a s_{t-1} dt;  gskip = sum_t gp u;  gz = gy p silu'(z).
-// The work is laid out as in the forward pass.  A tile is walked in pieces of CK steps: each starts from a state that the
-// forward pass left there, keeps the piece's states and decays in registers, then walks back.  Running the recurrence backwards instead (s_{t-1} = (s_t - dt u B) / a) would
-// lose everything for small a.  The sums over channels in gB and gC fold 2 SSM_R values over the wave's channels with half-wave and
-// 16-lane register swaps, then over the waves through LDS; what crosses workgroups is written once and summed in a fixed order.
-// Bound by the vector unit: a step of a wave takes 86 instructions in the recurrence (13 for each of a lane's states, 17 for the sums over
-// channels, 6 for those over states) and about 28 for the elements, tiles and partial sums; SQ_ACTIVE_INST_VALU is 0.89 of the busy cycles.
-// 8191 x 1024 bf16, N = 16: 142 us, and 39 for the walk that only sums the blocks (MODE 1); 32 x 4096 x 64 fp32: 150 and 38; 8 x 512 x 40
-// fp64: 33 and 19.  Two waves a SIMD: a tile of 32 steps fits their LDS for 16-bit types with 4 lanes a channel, 16 steps elsewhere (with 2
-// lanes 64 instead of 71 us at 4096 x 1024, N = 8); fp64 and one lane a channel need the registers of two.
+// The work is laid out as in the forward pass.  A tile is walked in pieces of CK steps: each starts from a state that the forward pass left
+// there, keeps the piece's states and decays in registers, then walks back.  Running the recurrence backwards instead (s_{t-1} = (s_t - dt u B)
+// / a) would lose everything for small a.  The sums over channels in gB and gC fold 2 SSM_R values over the wave's channels with half-wave and
+// 16-lane register swaps, then over the waves through LDS; what crosses workgroups is written once and summed in a fixed order. Bound by the
+// vector unit: a step of a wave takes 86 instructions in the recurrence (13 for each of a lane's states, 17 for the sums over channels, 6 for
+// those over states) and about 28 for the elements, tiles and partial sums; SQ_ACTIVE_INST_VALU is 0.89 of the busy cycles. 8191 x 1024 bf16, N
+// = 16: 142 us, and 39 for the walk that only sums the blocks (MODE 1); 32 x 4096 x 64 fp32: 150 and 38; 8 x 512 x 40 fp64: 33 and 19.  Two
+// waves a SIMD: a tile of 32 steps fits their LDS for 16-bit types with 4 lanes a channel, 16 steps elsewhere (with 2 lanes 64 instead of 71 us
+// at 4096 x 1024, N = 8); fp64 and one lane a channel need the registers of two.
 #include "rgp_ssm.h"
 
 template <typename T, int K, int CH, int MODE, int V>
 static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K == 1 ? 1 : 2) ssm_bwd_kernel(SsmDev d) {
   typedef typename SeqAcc<T>::type A;
   typedef SeqAny<T, V> Vec;
-  constexpr int THREADS = CH * K, NV = CH / V, RPI = THREADS / NV, CK = SSM_CK, TL = sizeof(T) == 8 ? 8 : sizeof(T) == 2 && CH * K == 256 && K == 4 ? 32 : 16, SUB = TL / CK, NP = SSM_R * K, R = SSM_R, WAVES = THREADS / 64;
+  constexpr int THREADS = CH * K, NV = CH / V, RPI = THREADS / NV, CK = SSM_CK, NP = SSM_R * K, R = SSM_R, WAVES = THREADS / 64;
+  constexpr int TL = sizeof(T) == 8 ? 8 : sizeof(T) == 2 && CH * K == 256 && K == 4 ? 32 : 16, SUB = TL / CK;
   constexpr int NI = RPI >= TL ? 1 : TL / RPI, NB = (TL * NP + THREADS - 1) / THREADS;
   struct alignas(4 * sizeof(A)) Four { A x, y, z, w; };
   struct alignas(16) Quad { A v[R]; };

@@ -329,7 +329,8 @@ def clip_grad_norm(handle, grads, max_norm, sumsq=None):
     grads = list(grads)
     r = _seq.clip(handle, grads, max_norm, sumsq)
     if r is None:
-        if sumsq is not None and (not isinstance(sumsq, torch.Tensor) or sumsq.dtype is not torch.float64 or sumsq.numel() != 1 or sumsq.device != handle.device):
+        if sumsq is not None and (not isinstance(sumsq, torch.Tensor) or sumsq.dtype is not torch.float64 or sumsq.numel() != 1 or
+                                  sumsq.device != handle.device):
             _bad('sumsq must be one float64 value on %s' % handle.device)
         _bad_grads(handle, grads)
     return r
