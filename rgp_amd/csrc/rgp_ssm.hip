@@ -187,18 +187,23 @@ static void scan_plan(const rgp_ssm_scan* a, bool back, ScanPlan& p) {
   if (p.K == 4 && (d.Dg + 15) / 16 * 16 < (d.Dg + 63) / 64 * 64) p.CH = 16;
   d.ncb = (d.Dg + p.CH - 1) / p.CH;
   const int64_t longest = a->off ? (a->max_len > 0 && a->max_len < a->rows ? a->max_len : a->rows) : a->T;
-  // Split over time.  In units of the time in which a SIMD with several waves walks one wave's step (about 80 ns forward, 260 ns backward):
-  // unsplit, the whole work spread over 1024 SIMDs, but no less than the longest sequence at twice that time (a lone wave waits for its own
-  // results); split, the work, a walk over one block, the first walk (0.65 of the forward one, 0.3 of the backward one), and the join.
-  // Measured backward: 8 x 1024 x 1024 bf16, N = 32, 445 us unsplit; N = 16 in 16 blocks, 186 split.  Blocks of 64
-  // steps, of 32 where that leaves most SIMDs idle, longer ones where the waves get many: shorter blocks balance ragged lengths, longer ones
-  // leave the join (and the sums of the backward pass) less to read.
+  // Split over time.  In units of the time in which a SIMD with several waves walks one wave's step (about 80 ns forward, 260 ns backward, four
+  // times that in fp64): unsplit, the whole work spread over 1024 SIMDs, but no less than the longest sequence at twice that time (a lone wave
+  // waits for its own results); split, the work, a walk over one block, the first walk (0.65 of the forward one, 0.3 of the backward one), and
+  // the join.  Measured backward: 8 x 1024 x 1024 bf16, N = 32, 445 us unsplit; N = 16 in 16 blocks, 186 split.  Forward, 4 x 64 x 64 fp64: 37 us
+  // unsplit, 24 split.
+  // Blocks of 64 steps, longer ones where the waves get many (they leave the join and the sums of the backward pass less to read), shorter ones
+  // where that leaves SIMDs idle: training steps of 8 x 512 x 40 fp64 take 122 us of kernels with 32 steps a block, 96 with 16, 107 with 8; of 4 x
+  // 256 x 40 fp64 111, 81 and 72; of 8 x 4096 x 32 fp32 111 with 64 and 105 with 32 (backward alone; forward loses with them).
   const double waves = (double)a->G * d.ncb * (p.CH * p.K / 64.0), work = waves * a->rows / 1024.0, most = back ? 12288.0 : 24576.0;
   auto count = [&](int g) { return waves * ((double)(a->rows >> g) + a->n_seq); };
-  int lg = count(6) < 1024.0 ? 5 : 6;
+  const bool f64 = a->dtype == RGP_F64;
+  int lg = 6;
+  if (count(6) < (back || f64 ? 2048.0 : 1024.0)) lg = count(5) < (f64 ? 2048.0 : 1024.0) ? 4 : 5;
+  if (lg == 4 && count(4) < 512.0) lg = 3;
   while (lg < 20 && count(lg) > most) ++lg;
   const double one = work > 2.0 * longest ? work : 2.0 * longest, block = 2.0 * ((int64_t)1 << lg);
-  const double two = back ? 1.3 * (work + block) + 80.0 : 1.65 * (work + block) + 130.0;
+  const double two = back ? 1.3 * (work + block) + (f64 ? 25.0 : 80.0) : 1.65 * (work + block) + (f64 ? 40.0 : 130.0);
   if (!(two < one)) lg = 0;
   p.split = lg > 0;
   if (!p.split)

@@ -461,56 +461,55 @@ def test_library_refuses_what_python_would_not_send(h):
     assert h.lib.rgp_grad_clip(h.h, None, 0, None, None, None, t.data_ptr(), 0.0, t.data_ptr() + 8, None, 0) == _lib.RGP_ERR_BAD_ARG
 
 
-@pytest.mark.parametrize('D,reverse', [(130, 0), (16, 1)])
+@pytest.mark.parametrize('D,reverse', [(130, False), (16, True)])
 def test_rows_behind_the_last_sequence_stay_as_they_are(h, D, reverse):
     """Packed rows may have capacity behind off[n_seq] (a table that is refilled between replays): nothing of it is read or written, also by
-    the sums over the channels' workgroups, and the other rows get the bits that a call without it gives."""
+    the sums over the channels' workgroups, and the rows of the sequences are right."""
     from rgp_amd import _lib
-    g, N, lengths, spare = _gen(11), 16, [70, 0, 5, 130], 77
-    rows = sum(lengths)
-    acts = [_randn(g, rows, n, dtype=F32).cuda() for n in (D, D, D, D, N, N)]                    # u, delta, z, gy, B, C
-    x, gv = [_randn(g, rows, D, dtype=F32).cuda() for _ in range(2)]
-    A, w = -torch.exp(_randn(g, D, N)).float().cuda(), _randn(g, D, 4, dtype=F32).cuda()
+    N, spare = 16, 77
+    p = Problem(F32, D=D, N=N, lengths=[70, 0, 5, 130], skip=False, bias=False, reverse=reverse, seed=11)
+    rows, n = sum(p.lengths), len(p.lengths)
     off = torch.tensor([0, 70, 70, 75, 205], device='cuda')
+    A, w = p.par['A'].cuda(), p.par['w'].cuda()
     st = torch.cuda.current_stream().cuda_stream
 
-    def run(pad):
-        wide = lambda t: torch.cat([t, torch.full((pad,) + t.shape[1:], float('nan'), device='cuda')])       # noqa: E731
+    def run(behind):
+        acts = {k: torch.cat([t.cuda(), torch.full((spare,) + t.shape[1:], behind, device='cuda')]) for k, t in p.acts.items()}
         out = lambda *s: torch.full(s, 7.0, device='cuda')                                                   # noqa: E731
-        u, delta, z, gy, B, Cm = [wide(t) for t in acts]
-        o = dict(y=out(rows + pad, D), gu=out(rows + pad, D), gdelta=out(rows + pad, D), gz=out(rows + pad, D), gB=out(rows + pad, N), gC=out(rows + pad, N),
-                 gA=out(D, N))
+        scan = dict(y=out(rows + spare, D), gu=out(rows + spare, D), gdelta=out(rows + spare, D), gz=out(rows + spare, D), gB=out(rows + spare, 1, N),
+                    gC=out(rows + spare, 1, N), gA=out(D, N))
         a = _lib.SsmScan()
-        a.dtype, a.n_seq, a.D, a.N, a.G, a.reverse, a.rows, a.max_len, a.off = _lib.DT_F32, 4, D, N, 1, reverse, rows + pad, 130, off.data_ptr()
-        for k, t in dict(o, u=u, delta=delta, z=z, gy=gy, B=B, C=Cm, A=A).items():
+        a.dtype, a.n_seq, a.D, a.N, a.G, a.reverse, a.rows, a.max_len, a.off = _lib.DT_F32, n, D, N, 1, int(reverse), rows + spare, 130, off.data_ptr()
+        for k, t in dict(scan, A=A, **{k: acts[k] for k in ('u', 'delta', 'z', 'gy', 'B', 'C')}).items():
             setattr(a, k, t.data_ptr())
         a.u_st = a.delta_st = a.z_st = a.gy_st = D
         a.B_st = a.C_st = N
         states = torch.empty(h.lib.rgp_ssm_scan_states_bytes(C.byref(a)), dtype=torch.uint8, device='cuda')
         a.states = states.data_ptr()
         for back, fn in ((0, h.lib.rgp_ssm_scan_forward), (1, h.lib.rgp_ssm_scan_backward)):
-            work = torch.full((h.lib.rgp_ssm_scan_workspace(C.byref(a), back) // 4,), float('nan'), device='cuda')
+            work = torch.full((h.lib.rgp_ssm_scan_workspace(C.byref(a), back) // 4,), behind, device='cuda')
             a.work, a.work_bytes = work.data_ptr(), work.numel() * 4
             assert fn(h.h, st, C.byref(a)) == 0
-        x1, gv1 = wide(x), wide(gv)
-        p = dict(v=out(rows + pad, D), gx=out(rows + pad, D), gw=out(D, 4))
+        conv = dict(v=out(rows + spare, D), gx=out(rows + spare, D), gw=out(D, 4))
         c = _lib.SsmConv()
-        c.dtype, c.n_seq, c.D, c.W, c.reverse, c.rows, c.max_len, c.off = _lib.DT_F32, 4, D, 4, reverse, rows + pad, 130, off.data_ptr()
-        for k, t in dict(p, x=x1, gv=gv1, w=w).items():
+        c.dtype, c.n_seq, c.D, c.W, c.reverse, c.rows, c.max_len, c.off = _lib.DT_F32, n, D, 4, int(reverse), rows + spare, 130, off.data_ptr()
+        for k, t in dict(conv, x=acts['x'], gv=acts['gv'], w=w).items():
             setattr(c, k, t.data_ptr())
         c.x_st = c.gv_st = D
         assert h.lib.rgp_ssm_conv_forward(h.h, st, C.byref(c)) == 0
-        work = torch.full((h.lib.rgp_ssm_conv_workspace(C.byref(c), 1) // 4,), float('nan'), device='cuda')
+        work = torch.full((h.lib.rgp_ssm_conv_workspace(C.byref(c), 1) // 4,), behind, device='cuda')
         c.work, c.work_bytes = work.data_ptr(), work.numel() * 4
         assert h.lib.rgp_ssm_conv_backward(h.h, st, C.byref(c)) == 0
         torch.cuda.synchronize()
-        return list(o.values()) + list(p.values())
+        return conv, scan
 
-    for a, b in zip(run(0), run(spare)):
-        if b.shape[0] == rows + spare:
-            assert (b[rows:] == 7.0).all()
-            b = b[:rows]
-        assert torch.isfinite(b).all() and torch.equal(a, b)
+    got, other = run(float('nan')), run(3.0)
+    for g, o in zip(got, other):
+        for k in g:
+            assert torch.equal(g[k], o[k]), k
+            if g[k].shape[0] == rows + spare:
+                assert (g[k][rows:] == 7.0).all(), k
+    p.compare([{k: t[:rows] if t.shape[0] == rows + spare else t for k, t in g.items()} for g in got], p.reference())
 
 
 def test_steps_with_infinite_decay(h):
