@@ -3,7 +3,6 @@
 #pragma once
 #include "rgp_seq.h"
 
-#define SSM_R 4                      // states per lane
 
 // Steps between the states that a training forward pass leaves for the backward pass, and the steps whose states and decays the backward
 // kernel holds in registers.  At N = 16 their bytes per (row, channel) are 8 in 32 bits; 16 steps would halve that but need 64 registers
@@ -27,6 +26,8 @@ static __device__ __forceinline__ int ssm_place(int c) {
   return V == 1 ? c : c ^ ((c >> SH) & (V - 1));
 }
 
+struct SsmShape { int K, R, CH; };   // lanes a channel, states a lane, channels a workgroup
+
 struct SsmDev {
   rgp_ssm_scan a;
   SeqGeo g;
@@ -41,5 +42,5 @@ struct SsmDev {
 };
 
 // fwd: mode 0 = the whole operator, 1 = what a block adds to the state and its sum of dt; bwd likewise with the adjoint
-hipError_t ssm_fwd_launch(const SsmDev& d, int K, int CH, int mode, hipStream_t s);
-hipError_t ssm_bwd_launch(const SsmDev& d, int K, int CH, int mode, hipStream_t s);
+hipError_t ssm_fwd_launch(const SsmDev& d, SsmShape p, int mode, hipStream_t s);
+hipError_t ssm_bwd_launch(const SsmDev& d, SsmShape p, int mode, hipStream_t s);

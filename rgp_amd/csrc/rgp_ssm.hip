@@ -169,7 +169,8 @@ static const char* scan_bad(const rgp_ssm_scan* a) {
 
 struct ScanPlan {
   SsmDev d;
-  int K, CH, acc, Q;               // Q: threads that walk the blocks of one state in the join
+  SsmShape sh;
+  int acc, Q;                      // Q: threads that walk the blocks of one state in the join
   bool split;
   int64_t part_bytes, sum_bytes, pA_bytes, pD_bytes, pBC_bytes, bytes;
 };
@@ -182,10 +183,18 @@ static void scan_plan(const rgp_ssm_scan* a, bool back, ScanPlan& p) {
   d.g = SeqGeo{a->off, a->T, a->rows, a->n_seq, a->reverse};
   d.Dg = a->D / a->G;
   p.acc = a->dtype == RGP_F64 ? 8 : 4;
-  p.K = a->N <= 4 ? 1 : a->N <= 8 ? 2 : a->N <= 16 ? 4 : a->N <= 32 ? 8 : 16;
-  p.CH = p.K <= 4 ? 64 : 256 / p.K;
-  if (p.K == 4 && (d.Dg + 15) / 16 * 16 < (d.Dg + 63) / 64 * 64) p.CH = 16;
-  d.ncb = (d.Dg + p.CH - 1) / p.CH;
+  // States a lane: 4; 2 in fp64, where an exponential takes dozens of instructions: more lanes a channel shorten a step where the waves are few
+  // (training steps of 8 x 64 x 1000: 131 -> 105 us, 8 x 40 x 300: 83 -> 71) and the backward kernel gets two waves a SIMD (8191 x 512: N = 8 555 ->
+  // 463 us, N = 16 714 -> 708, N = 32 627 -> 653).
+  const bool f64 = a->dtype == RGP_F64;
+  SsmShape& h = p.sh;
+  h.R = f64 && a->N <= 32 ? 2 : 4;
+  h.K = f64 ? 2 : 1;
+  while (h.K * h.R < a->N) h.K *= 2;
+  h.CH = h.K <= 4 ? 64 : 256 / h.K;
+  const int few = 64 / h.K;                                         // channels of a single wave, where that leaves fewer lanes idle
+  if ((h.K == 4 || (f64 && h.K == 8)) && (d.Dg + few - 1) / few * few < (d.Dg + h.CH - 1) / h.CH * h.CH) h.CH = few;
+  d.ncb = (d.Dg + h.CH - 1) / h.CH;
   const int64_t longest = a->off ? (a->max_len > 0 && a->max_len < a->rows ? a->max_len : a->rows) : a->T;
   // Split over time.  In units of the time in which a SIMD with several waves walks one wave's step (about 80 ns forward, 260 ns backward, four
   // times that in fp64): unsplit, the whole work spread over 1024 SIMDs, but no less than the longest sequence at twice that time (a lone wave
@@ -195,9 +204,8 @@ static void scan_plan(const rgp_ssm_scan* a, bool back, ScanPlan& p) {
   // Blocks of 64 steps, longer ones where the waves get many (they leave the join and the sums of the backward pass less to read), shorter ones
   // where that leaves SIMDs idle: training steps of 8 x 512 x 40 fp64 take 122 us of kernels with 32 steps a block, 96 with 16, 107 with 8; of 4 x
   // 256 x 40 fp64 111, 81 and 72; of 8 x 4096 x 32 fp32 111 with 64 and 105 with 32 (backward alone; forward loses with them).
-  const double waves = (double)a->G * d.ncb * (p.CH * p.K / 64.0), work = waves * a->rows / 1024.0, most = back ? 12288.0 : 24576.0;
+  const double waves = (double)a->G * d.ncb * (h.CH * h.K / 64.0), work = waves * a->rows / 1024.0, most = back ? 12288.0 : 24576.0;
   auto count = [&](int g) { return waves * ((double)(a->rows >> g) + a->n_seq); };
-  const bool f64 = a->dtype == RGP_F64;
   int lg = 6;
   if (count(6) < (back || f64 ? 2048.0 : 1024.0)) lg = count(5) < (f64 ? 2048.0 : 1024.0) ? 4 : 5;
   if (lg == 4 && count(4) < 512.0) lg = 3;
@@ -247,7 +255,7 @@ static rgp_status scan_run(rgp_handle h, hipStream_t s, const rgp_ssm_scan* a, b
   SsmDev& d = p.d;
   if (p.bytes > a->work_bytes || (p.bytes && !a->work) || ((uintptr_t)a->work & 15))
     return rgp_fail(h, RGP_ERR_WORKSPACE, std::string(what) + "work buffer too small or not 16-byte aligned");
-  const int V = 16 / seq_dtype_bytes(a->dtype), rest = d.Dg % p.CH;      // a workgroup's channels are one vector at least, or single elements
+  const int V = 16 / seq_dtype_bytes(a->dtype), rest = d.Dg % p.sh.CH;      // a workgroup's channels are one vector at least, or single elements
   d.wide = rest == 0 || rest >= V;
   char* w = (char*)a->work;
   auto take = [&](int64_t bytes) { void* r = bytes ? (void*)w : nullptr; w += bytes; return r; };
@@ -258,19 +266,19 @@ static rgp_status scan_run(rgp_handle h, hipStream_t s, const rgp_ssm_scan* a, b
   d.pBC = take(p.pBC_bytes);
   const int64_t DN = (int64_t)a->D * a->N;
   const int64_t join = (int64_t)a->n_seq * (p.Q == 1 ? (DN + 255) / 256 : (DN + 63) / 64);
-  if ((double)d.nslot * p.CH * p.K > 4294967295.0 || (int64_t)a->G * d.ncb > 65535 || seq_blocks(d.g, SSM_CK_LG) > 4294967295 || (double)join * 1024 > 4294967295.0)
+  if ((double)d.nslot * p.sh.CH * p.sh.K > 4294967295.0 || (int64_t)a->G * d.ncb > 65535 || seq_blocks(d.g, SSM_CK_LG) > 4294967295 || (double)join * 1024 > 4294967295.0)
     return rgp_fail(h, RGP_ERR_BAD_ARG, std::string(what) + "more than 2^32 work items");
   hipError_t err = hipSuccess;
   if (d.nslot > 0) {
     if (p.split) {
-      err = back ? ssm_bwd_launch(d, p.K, p.CH, 1, s) : ssm_fwd_launch(d, p.K, p.CH, 1, s);
+      err = back ? ssm_bwd_launch(d, p.sh, 1, s) : ssm_fwd_launch(d, p.sh, 1, s);
       if (err == hipSuccess) {
         if (p.acc == 8) join_launch<double>(d, p.Q, (unsigned)join, back ? 1 : 0, s);
         else join_launch<float>(d, p.Q, (unsigned)join, back ? 1 : 0, s);
         err = hipGetLastError();
       }
     }
-    if (err == hipSuccess) err = back ? ssm_bwd_launch(d, p.K, p.CH, 0, s) : ssm_fwd_launch(d, p.K, p.CH, 0, s);
+    if (err == hipSuccess) err = back ? ssm_bwd_launch(d, p.sh, 0, s) : ssm_fwd_launch(d, p.sh, 0, s);
     if (err != hipSuccess) return rgp_fail(h, RGP_ERR_HIP, std::string(what) + hipGetErrorString(err));
   }
   if (!back) return RGP_OK;
@@ -296,10 +304,11 @@ extern "C" rgp_status rgp_ssm_scan_backward(rgp_handle h, void* stream, const rg
 // ---- one step -----------------------------------------------------------------------------------------------------------------------------
 // Bound by reading and writing the state: K lanes a channel, 16 bytes of state a lane (32 in fp64), as in the kernels over time.  256 x 2048
 // bf16, N = 16: 16.7 us for 67 MB of state and 8 MB beside it, 4.5 TB/s; one sequence of 40 channels 3.7 us, the launch.
+#define STEP_R 4                     // states a lane
 template <typename T, int K>
 static __global__ void __launch_bounds__(256) ssm_step_kernel(rgp_ssm_scan a, int Dg, int whole) {
   typedef typename SeqAcc<T>::type A;
-  constexpr int R = SSM_R;
+  constexpr int R = STEP_R;
   const uint32_t e = (blockIdx.x * 256u + threadIdx.x) / K;              // host-checked: below 2^32
   const int k = threadIdx.x % K, N = a.N;
   const bool live = e < (uint32_t)a.n_seq * (uint32_t)a.D;
@@ -363,8 +372,8 @@ static hipError_t step_pick(const rgp_ssm_scan& a, hipStream_t s) {
   const int K = a.N <= 4 ? 1 : a.N <= 8 ? 2 : a.N <= 16 ? 4 : a.N <= 32 ? 8 : 16;
   const unsigned grid = (unsigned)(((int64_t)a.n_seq * a.D * K + 255) / 256);
   const int Dg = a.D / a.G;
-  const int whole = a.N == SSM_R * K && ((uintptr_t)a.last & 15) == 0 && ((uintptr_t)a.A & 15) == 0 &&
-                    seq_aligned(a.B, a.B_sb, (int)sizeof(T), SSM_R) && seq_aligned(a.C, a.C_sb, (int)sizeof(T), SSM_R);
+  const int whole = a.N == STEP_R * K && ((uintptr_t)a.last & 15) == 0 && ((uintptr_t)a.A & 15) == 0 &&
+                    seq_aligned(a.B, a.B_sb, (int)sizeof(T), STEP_R) && seq_aligned(a.C, a.C_sb, (int)sizeof(T), STEP_R);
   switch (K) {
     case 1: hipLaunchKernelGGL((ssm_step_kernel<T, 1>), dim3(grid), dim3(256), 0, s, a, Dg, whole); break;
     case 2: hipLaunchKernelGGL((ssm_step_kernel<T, 2>), dim3(grid), dim3(256), 0, s, a, Dg, whole); break;

@@ -5,7 +5,7 @@
 //     gB[n] = sum_d lam dt u;  gC[n] = sum_d gp s;  gA[n] = sum_t lam a s_{t-1} dt;  gskip = sum_t gp u;  gz = gy p silu'(z).
 // The work is laid out as in the forward pass.  A tile is walked in pieces of CK steps: each starts from a state that the forward pass left
 // there, keeps the piece's states and decays in registers, then walks back.  Running the recurrence backwards instead (s_{t-1} = (s_t - dt u B)
-// / a) would lose everything for small a.  The sums over channels in gB and gC fold 2 SSM_R values over the wave's channels with half-wave and
+// / a) would lose everything for small a.  The sums over channels in gB and gC fold 2 R values over the wave's channels with half-wave and
 // 16-lane register swaps, then over the waves through LDS; what crosses workgroups is written once and summed in a fixed order. Bound by the
 // vector unit: a step of a wave takes 86 instructions in the recurrence (13 for each of a lane's states, 17 for the sums over channels, 6 for
 // those over states) and about 28 for the elements, tiles and partial sums; SQ_ACTIVE_INST_VALU is 0.89 of the busy cycles. 8191 x 1024 bf16, N
@@ -14,11 +14,11 @@
 // at 4096 x 1024, N = 8); fp64 and one lane a channel need the registers of two.
 #include "rgp_ssm.h"
 
-template <typename T, int K, int CH, int MODE, int V>
-static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K == 1 ? 1 : 2) ssm_bwd_kernel(SsmDev d) {
+template <typename T, int K, int R, int CH, int MODE, int V>
+static __global__ void __launch_bounds__(CH* K, (sizeof(T) == 8 && R == 4) || K == 1 ? 1 : 2) ssm_bwd_kernel(SsmDev d) {
   typedef typename SeqAcc<T>::type A;
   typedef SeqAny<T, V> Vec;
-  constexpr int THREADS = CH * K, NV = CH / V, RPI = THREADS / NV, CK = SSM_CK, NP = SSM_R * K, R = SSM_R, WAVES = THREADS / 64;
+  constexpr int THREADS = CH * K, NV = CH / V, RPI = THREADS / NV, CK = SSM_CK, NP = R * K, WAVES = THREADS / 64;
   constexpr int TL = sizeof(T) == 8 ? 8 : sizeof(T) == 2 && CH * K == 256 && K == 4 ? 32 : 16, SUB = TL / CK;
   constexpr int NI = RPI >= TL ? 1 : TL / RPI, NB = (TL * NP + THREADS - 1) / THREADS;
   struct alignas(4 * sizeof(A)) Four { A x, y, z, w; };
@@ -217,21 +217,29 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K == 1 ? 1 : 2
             o.x = o0; o.y = o1; o.z = o2; o.w = (A)0;
             pl[t][cp] = o;
           }
-          // over the wave's channels: lane bit 5 selects gB / gC, bit 4 and bit 3 the state
-          const bool b3 = (lane & 8) != 0;
-          A f0 = seq_fold<true>(vB[0], vC[0]), f1 = seq_fold<true>(vB[1], vC[1]), f2 = seq_fold<true>(vB[2], vC[2]), f3 = seq_fold<true>(vB[3], vC[3]);
-          f0 = seq_fold<false>(f0, f2);
-          f1 = seq_fold<false>(f1, f3);
-          A* const f_to = &red[wave][t][(lane >> 5) * NP + k * R + ((lane >> 4) & 1) * 2];
-          if constexpr (K == 16) {
-            f_to[0] = f0;
-            f_to[1] = f1;
-          } else {
-            A f = seq_fold8(f0, f1, b3);
+          // over the wave's channels: lane bit 5 selects gB / gC, bit 4 and (4 states a lane) bit 3 the state
+          A* const f_to = &red[wave][t][(lane >> 5) * NP + k * R + ((lane >> 4) & 1) * (R / 2)];
+          if constexpr (R == 2) {
+            A f = seq_fold<false>(seq_fold<true>(vB[0], vC[0]), seq_fold<true>(vB[1], vC[1]));
+            if constexpr (K <= 8) f += seq_dpp<0x128>(f);                  // row_ror:8
             if constexpr (K <= 4) f += seq_xor4(f);
             if constexpr (K <= 2) f += seq_dpp<0x4E>(f);
-            if constexpr (K == 1) f += seq_dpp<0xB1>(f);
-            f_to[b3] = f;                                         // lanes that hold the same sum write it to the same place
+            f_to[0] = f;                                           // lanes that hold the same sum write it to the same place
+          } else {
+            const bool b3 = (lane & 8) != 0;
+            A f0 = seq_fold<true>(vB[0], vC[0]), f1 = seq_fold<true>(vB[1], vC[1]), f2 = seq_fold<true>(vB[2], vC[2]), f3 = seq_fold<true>(vB[3], vC[3]);
+            f0 = seq_fold<false>(f0, f2);
+            f1 = seq_fold<false>(f1, f3);
+            if constexpr (K == 16) {
+              f_to[0] = f0;
+              f_to[1] = f1;
+            } else {
+              A f = seq_fold8(f0, f1, b3);
+              if constexpr (K <= 4) f += seq_xor4(f);
+              if constexpr (K <= 2) f += seq_dpp<0x4E>(f);
+              if constexpr (K == 1) f += seq_dpp<0xB1>(f);
+              f_to[b3] = f;
+            }
           }
           p = pn;
           B = Bn;
@@ -297,31 +305,40 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) == 8 || K == 1 ? 1 : 2
   }
 }
 
-template <typename T, int K, int CH>
+template <typename T, int K, int R, int CH>
 static hipError_t go(const SsmDev& d, int mode, hipStream_t s) {
   constexpr int V = 16 / (int)sizeof(T);
   const dim3 g((unsigned)d.nslot, (unsigned)(d.a.G * d.ncb)), t(CH * K);
-  if (mode == 0 && d.wide) hipLaunchKernelGGL((ssm_bwd_kernel<T, K, CH, 0, V>), g, t, 0, s, d);
-  else if (mode == 0) hipLaunchKernelGGL((ssm_bwd_kernel<T, K, CH, 0, 1>), g, t, 0, s, d);
-  else if (d.wide) hipLaunchKernelGGL((ssm_bwd_kernel<T, K, CH, 1, V>), g, t, 0, s, d);
-  else hipLaunchKernelGGL((ssm_bwd_kernel<T, K, CH, 1, 1>), g, t, 0, s, d);
+  if (mode == 0 && d.wide) hipLaunchKernelGGL((ssm_bwd_kernel<T, K, R, CH, 0, V>), g, t, 0, s, d);
+  else if (mode == 0) hipLaunchKernelGGL((ssm_bwd_kernel<T, K, R, CH, 0, 1>), g, t, 0, s, d);
+  else if (d.wide) hipLaunchKernelGGL((ssm_bwd_kernel<T, K, R, CH, 1, V>), g, t, 0, s, d);
+  else hipLaunchKernelGGL((ssm_bwd_kernel<T, K, R, CH, 1, 1>), g, t, 0, s, d);
   return hipGetLastError();
 }
 template <typename T>
-static hipError_t pick(const SsmDev& d, int K, int CH, int mode, hipStream_t s) {
-  switch (K) {
-    case 1: return go<T, 1, 64>(d, mode, s);
-    case 2: return go<T, 2, 64>(d, mode, s);
-    case 4: return CH == 16 ? go<T, 4, 16>(d, mode, s) : go<T, 4, 64>(d, mode, s);
-    case 8: return go<T, 8, 32>(d, mode, s);
-    default: return go<T, 16, 16>(d, mode, s);
+static hipError_t pick(const SsmDev& d, SsmShape p, int mode, hipStream_t s) {
+  if constexpr (sizeof(T) == 8) {
+    switch (p.K) {
+      case 2: return go<T, 2, 2, 64>(d, mode, s);
+      case 4: return p.CH == 16 ? go<T, 4, 2, 16>(d, mode, s) : go<T, 4, 2, 64>(d, mode, s);
+      case 8: return p.CH == 8 ? go<T, 8, 2, 8>(d, mode, s) : go<T, 8, 2, 32>(d, mode, s);
+      default: return p.R == 2 ? go<T, 16, 2, 16>(d, mode, s) : go<T, 16, 4, 16>(d, mode, s);
+    }
+  } else {
+    switch (p.K) {
+      case 1: return go<T, 1, 4, 64>(d, mode, s);
+      case 2: return go<T, 2, 4, 64>(d, mode, s);
+      case 4: return p.CH == 16 ? go<T, 4, 4, 16>(d, mode, s) : go<T, 4, 4, 64>(d, mode, s);
+      case 8: return go<T, 8, 4, 32>(d, mode, s);
+      default: return go<T, 16, 4, 16>(d, mode, s);
+    }
   }
 }
-hipError_t ssm_bwd_launch(const SsmDev& d, int K, int CH, int mode, hipStream_t s) {
+hipError_t ssm_bwd_launch(const SsmDev& d, SsmShape p, int mode, hipStream_t s) {
   switch (d.a.dtype) {
-    case RGP_F64: return pick<double>(d, K, CH, mode, s);
-    case RGP_F32: return pick<float>(d, K, CH, mode, s);
-    case RGP_BF16: return pick<__bf16>(d, K, CH, mode, s);
-    default: return pick<_Float16>(d, K, CH, mode, s);
+    case RGP_F64: return pick<double>(d, p, mode, s);
+    case RGP_F32: return pick<float>(d, p, mode, s);
+    case RGP_BF16: return pick<__bf16>(d, p, mode, s);
+    default: return pick<_Float16>(d, p, mode, s);
   }
 }

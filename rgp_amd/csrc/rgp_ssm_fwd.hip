@@ -1,6 +1,6 @@
 // rgp_ssm_fwd.hip -- forward kernel of the selective state-space scan
 //     dt = softplus(delta + bias);  s[n] = exp(dt A[n]) s[n] + dt u B[n];  y = (sum_n C[n] s[n] + skip u) silu(z).
-// K lanes hold one channel's states, SSM_R each; a workgroup holds CH channels of one group of B / C and walks its block of time in tiles
+// K lanes hold one channel's states, R each; a workgroup holds CH channels of one group of B / C and walks its block of time in tiles
 // of TL steps.  What is elementwise over (step, channel) -- softplus, silu, the loads and stores -- runs with the lanes over the tile's
 // elements, a vector of V (16 bytes) each, the last one moved back to end with the channels; single elements where a workgroup has fewer
 // channels than a vector.  Between them the recurrence reads (dt, dt u) and the rows of B and C from LDS and leaves y there.  The next tile's
@@ -12,11 +12,11 @@
 // one or two lanes a channel, tiles of 16 steps keep the element role in registers (8192 x 2000 fp32, N = 4: 64 us, with 32 steps 110).
 #include "rgp_ssm.h"
 
-template <typename T, int K, int CH, int MODE, int V>
+template <typename T, int K, int R, int CH, int MODE, int V>
 static __global__ void __launch_bounds__(CH* K, sizeof(T) < 8 && (K == 4 || K == 8) && CH * K == 256 && V > 1 ? 4 : 1) ssm_fwd_kernel(SsmDev d) {
   typedef typename SeqAcc<T>::type A;
   typedef SeqAny<T, V> Vec;
-  constexpr int THREADS = CH * K, NV = CH / V, TL = sizeof(A) == 8 || K <= 2 ? 16 : 32, NP = SSM_R * K, R = SSM_R, RPI = THREADS / NV;
+  constexpr int THREADS = CH * K, NV = CH / V, TL = sizeof(A) == 8 || K <= 2 ? 16 : 32, NP = R * K, RPI = THREADS / NV;
   constexpr int NI = RPI >= TL ? 1 : TL / RPI, NB = (TL * NP + THREADS - 1) / THREADS, CK = SSM_CK;
   struct alignas(2 * sizeof(A)) Pair { A dt, w; };
   struct alignas(16) Quad { A v[R]; };
@@ -208,31 +208,40 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) < 8 && (K == 4 || K ==
   }
 }
 
-template <typename T, int K, int CH>
+template <typename T, int K, int R, int CH>
 static hipError_t go(const SsmDev& d, int mode, hipStream_t s) {
   constexpr int V = 16 / (int)sizeof(T);
   const dim3 g((unsigned)d.nslot, (unsigned)(d.a.G * d.ncb)), t(CH * K);
-  if (mode == 0 && d.wide) hipLaunchKernelGGL((ssm_fwd_kernel<T, K, CH, 0, V>), g, t, 0, s, d);
-  else if (mode == 0) hipLaunchKernelGGL((ssm_fwd_kernel<T, K, CH, 0, 1>), g, t, 0, s, d);
-  else if (d.wide) hipLaunchKernelGGL((ssm_fwd_kernel<T, K, CH, 1, V>), g, t, 0, s, d);
-  else hipLaunchKernelGGL((ssm_fwd_kernel<T, K, CH, 1, 1>), g, t, 0, s, d);
+  if (mode == 0 && d.wide) hipLaunchKernelGGL((ssm_fwd_kernel<T, K, R, CH, 0, V>), g, t, 0, s, d);
+  else if (mode == 0) hipLaunchKernelGGL((ssm_fwd_kernel<T, K, R, CH, 0, 1>), g, t, 0, s, d);
+  else if (d.wide) hipLaunchKernelGGL((ssm_fwd_kernel<T, K, R, CH, 1, V>), g, t, 0, s, d);
+  else hipLaunchKernelGGL((ssm_fwd_kernel<T, K, R, CH, 1, 1>), g, t, 0, s, d);
   return hipGetLastError();
 }
 template <typename T>
-static hipError_t pick(const SsmDev& d, int K, int CH, int mode, hipStream_t s) {
-  switch (K) {
-    case 1: return go<T, 1, 64>(d, mode, s);
-    case 2: return go<T, 2, 64>(d, mode, s);
-    case 4: return CH == 16 ? go<T, 4, 16>(d, mode, s) : go<T, 4, 64>(d, mode, s);
-    case 8: return go<T, 8, 32>(d, mode, s);
-    default: return go<T, 16, 16>(d, mode, s);
+static hipError_t pick(const SsmDev& d, SsmShape p, int mode, hipStream_t s) {
+  if constexpr (sizeof(T) == 8) {
+    switch (p.K) {
+      case 2: return go<T, 2, 2, 64>(d, mode, s);
+      case 4: return p.CH == 16 ? go<T, 4, 2, 16>(d, mode, s) : go<T, 4, 2, 64>(d, mode, s);
+      case 8: return p.CH == 8 ? go<T, 8, 2, 8>(d, mode, s) : go<T, 8, 2, 32>(d, mode, s);
+      default: return p.R == 2 ? go<T, 16, 2, 16>(d, mode, s) : go<T, 16, 4, 16>(d, mode, s);
+    }
+  } else {
+    switch (p.K) {
+      case 1: return go<T, 1, 4, 64>(d, mode, s);
+      case 2: return go<T, 2, 4, 64>(d, mode, s);
+      case 4: return p.CH == 16 ? go<T, 4, 4, 16>(d, mode, s) : go<T, 4, 4, 64>(d, mode, s);
+      case 8: return go<T, 8, 4, 32>(d, mode, s);
+      default: return go<T, 16, 4, 16>(d, mode, s);
+    }
   }
 }
-hipError_t ssm_fwd_launch(const SsmDev& d, int K, int CH, int mode, hipStream_t s) {
+hipError_t ssm_fwd_launch(const SsmDev& d, SsmShape p, int mode, hipStream_t s) {
   switch (d.a.dtype) {
-    case RGP_F64: return pick<double>(d, K, CH, mode, s);
-    case RGP_F32: return pick<float>(d, K, CH, mode, s);
-    case RGP_BF16: return pick<__bf16>(d, K, CH, mode, s);
-    default: return pick<_Float16>(d, K, CH, mode, s);
+    case RGP_F64: return pick<double>(d, p, mode, s);
+    case RGP_F32: return pick<float>(d, p, mode, s);
+    case RGP_BF16: return pick<__bf16>(d, p, mode, s);
+    default: return pick<_Float16>(d, p, mode, s);
   }
 }
