@@ -34,12 +34,40 @@ struct SsmDev {
   int lg;                            // the time split has blocks of L = 2^lg steps
   int64_t L;
   int64_t nslot;                     // blocks
+  int join;                          // every block joins the sums of the blocks before it (behind it) by itself
   int Dg, ncb;                       // channels per group, channel blocks per group
   int wide;                          // every activation in 16-byte vectors: aligned, and Dg a multiple of a vector
   void* part;                        // state (forward) or adjoint (backward) that every block starts from [nslot][D][N]
   void* sumdt;                       // sum of dt over a block [nslot][D]
   void *pA, *pD, *pBC;               // partial sums of the backward pass: [nslot][D][N], [nslot][2][D], [ncb][rows][2][G][N]
 };
+
+// What enters block b: s (the initial state, or zero) through the sums that the first walk left of the blocks before it -- behind it for the
+// adjoint.  R states of one channel from n0 on; decay(sum of dt, r) is a block's.
+template <bool BACK, int R, typename A, typename F>
+static __device__ __forceinline__ void ssm_enter(const SsmDev& d, const SeqBlock& b, int ch, int n0, A (&s)[R], F decay) {
+  constexpr int U = 4;
+  const int64_t DN = (int64_t)d.a.D * d.a.N, last = ((b.len + d.L - 1) >> d.lg) - 1, step = (d.g.off ? 1 : (int64_t)d.g.n_seq) * (BACK ? -1 : 1);
+  const int64_t slot = seq_slot(d.g, b.seq, b.start, d.lg, BACK ? last : 0), dp = step * DN, dq = step * d.a.D;
+  const A* p = (const A*)d.part + slot * DN + (int64_t)ch * d.a.N + n0;
+  const A* q = (const A*)d.sumdt + slot * d.a.D + ch;
+  for (int left = (int)(BACK ? last - b.j : b.j); left > 0; left -= U, p += U * dp, q += U * dq) {
+    A h[U][R], t[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {                                  // read together
+      const int k = u < left ? u : 0;
+      t[u] = q[k * dq];
+#pragma unroll
+      for (int r = 0; r < R; ++r) h[u][r] = n0 + r < d.a.N ? p[k * dp + r] : (A)0;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u < left) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r] = decay(t[u], r) * s[r] + h[u][r];
+      }
+  }
+}
 
 // fwd: mode 0 = the whole operator, 1 = what a block adds to the state and its sum of dt; bwd likewise with the adjoint
 hipError_t ssm_fwd_launch(const SsmDev& d, SsmShape p, int mode, hipStream_t s);

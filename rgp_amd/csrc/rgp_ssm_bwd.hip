@@ -63,7 +63,7 @@ static __global__ void __launch_bounds__(CH* K, (sizeof(T) == 8 && R == 4) || K 
   for (int r = 0; r < R; ++r) {
     const bool ok = live && k * R + r < N;
     Ar[r] = ok ? ssm_finite(((const A*)a.A)[(int64_t)(ch0 + ch) * N + k * R + r]) : (A)0;
-    carry[r] = MODE == 0 && d.part && ok ? ((const A*)d.part)[(slot * a.D + ch0 + ch) * N + k * R + r] : (A)0;
+    carry[r] = MODE == 0 && d.part && !d.join && ok ? ((const A*)d.part)[(slot * a.D + ch0 + ch) * N + k * R + r] : (A)0;
     gA[r] = (A)0;
   }
   const A* const ckpt = MODE == 0 ? (const A*)a.states + (seq_slot(d.g, b.seq, b.start, SSM_CK_LG, t0 >> SSM_CK_LG) * a.D + ch0 + ch) * N + k * R : nullptr;
@@ -72,6 +72,7 @@ static __global__ void __launch_bounds__(CH* K, (sizeof(T) == 8 && R == 4) || K 
   auto decay = [&](A dt, int r) {
     return sizeof(A) == 4 ? (A)seq_exp2((float)(dt * (Ar[r] * (A)1.44269504088896341))) : seq_exp(dt * Ar[r]);
   };
+  if (MODE == 0 && d.join && live) ssm_enter<true>(d, b, ch0 + ch, k * R, carry, decay);
 
   Vec ru[NI], rd[NI], rz[NI], rg[NI];
   T rB[NB], rC[NB];

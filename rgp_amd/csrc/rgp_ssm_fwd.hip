@@ -67,10 +67,12 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) < 8 && (K == 4 || K ==
     if (sizeof(A) == 4) Ar[r] *= (A)1.44269504088896341;          // exp(dt A) = 2^(dt A log2 e)
     s[r] = (A)0;
     if (MODE == 0 && ok) {
-      if (d.part) s[r] = ((const A*)d.part)[(slot * a.D + ch0 + ch) * N + k * R + r];
+      if (d.part && !d.join) s[r] = ((const A*)d.part)[(slot * a.D + ch0 + ch) * N + k * R + r];
       else if (a.init) s[r] = ((const A*)a.init)[(b.seq * a.D + ch0 + ch) * N + k * R + r];
     }
   }
+  auto decay = [&](A dt, int r) { return sizeof(A) == 4 ? (A)seq_exp2((float)(dt * Ar[r])) : seq_exp(dt * Ar[r]); };
+  if (MODE == 0 && d.join && live) ssm_enter<false>(d, b, ch0 + ch, k * R, s, decay);
   // the states of the block: every CK steps, a stride of cks values apart
   A* const ckpt = MODE == 0 && a.states ? (A*)a.states + (seq_slot(d.g, b.seq, b.start, SSM_CK_LG, t0 >> SSM_CK_LG) * a.D + ch0 + ch) * N + k * R : nullptr;
   const int64_t cks = (d.g.off ? 1 : (int64_t)d.g.n_seq) * a.D * N;
@@ -164,8 +166,7 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) < 8 && (K == 4 || K ==
         if (MODE == 1) sum += p.dt;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const A e = sizeof(A) == 4 ? (A)seq_exp2((float)(p.dt * Ar[r])) : seq_exp(p.dt * Ar[r]);
-          s[r] = e * s[r] + p.w * B.v[r];
+          s[r] = decay(p.dt, r) * s[r] + p.w * B.v[r];
           if (MODE == 0) acc += s[r] * Cl[t][k].v[r];
         }
         if (MODE == 0) {

@@ -642,3 +642,15 @@ def test_threads_with_streams_of_their_own_share_a_handle(h):
     assert not failed, failed
     for a, b in zip(want, got):
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize('dtype', [F64, F32, BF16], ids=str)
+@pytest.mark.parametrize('T', [72, 96, 97, 104, 105, 200])
+def test_few_and_many_blocks_of_time(h, dtype, T):
+    """Lengths on both sides of where the blocks of the time split are joined by a launch of their own, states carried in, both directions; and
+    a packed batch whose longest sequence decides."""
+    for reverse in (False, True):
+        p = Problem(dtype, D=20, N=16, T=T, n=2, carry=True, reverse=reverse, seed=T)
+        p.compare(p.run(h), p.reference())
+    q = Problem(dtype, D=33, N=6, lengths=[T, 0, 1, T // 2, 9], carry=True, seed=T + 1)
+    q.compare(q.run(h), q.reference())
