@@ -258,12 +258,12 @@ static RmsShape rms_shape(const rgp_rms_norm* a) {
   const int V = 16 / seq_dtype_bytes(a->dtype);
   if (a->C < V) return RmsShape{8, 1};                                        // single elements, at most 7 of them
   const int64_t nv = (a->C + V - 1) / V, rows = a->rows;
-  static const int tprs[4] = {8, 16, 64, 256}, nes[5] = {1, 2, 3, 4, 8};
+  static const int tprs[5] = {8, 16, 32, 64, 256}, nes[5] = {1, 2, 3, 4, 8};
   RmsShape best{0, 0};
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 5; ++i)
     for (int j = 0; j < 5; ++j) {
       const int64_t hold = (int64_t)tprs[i] * nes[j];
-      if (hold < nv || (nes[j] == 8 && tprs[i] < 256)) continue;
+      if (hold < nv || (nes[j] == 8 && tprs[i] < 256) || (tprs[i] == 32 && nes[j] != 3)) continue;       // 32 threads fill the gap between 64 and 128
       const bool few = rows * tprs[i] <= 65536;                          // fewer threads than the card has lanes: the wider shape is free
       if (!best.tpr || hold < (int64_t)best.tpr * best.ne || (few && tprs[i] > best.tpr && hold <= 2 * (int64_t)best.tpr * best.ne))
         best = RmsShape{tprs[i], nes[j]};
@@ -332,6 +332,7 @@ static hipError_t rms_pick(const NormDev& d, RmsShape sh, bool back, int64_t blo
   switch (sh.tpr) {
     case 8: return rms_ne<T, 8>(d, sh.ne, back, blocks, s);
     case 16: return rms_ne<T, 16>(d, sh.ne, back, blocks, s);
+    case 32: return rms_go<T, 32, 3, V>(d, back, blocks, s);
     case 64: return rms_ne<T, 64>(d, sh.ne, back, blocks, s);
     case 256: return rms_ne<T, 256>(d, sh.ne, back, blocks, s);
     default: return d.a.C % V == 0 ? rms_long<T, V>(d, back, blocks, s) : rms_long<T, 1>(d, back, blocks, s);

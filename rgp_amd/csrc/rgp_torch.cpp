@@ -7,7 +7,9 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime_api.h>
 #include <torch/csrc/Device.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
@@ -184,8 +186,19 @@ struct OpNode : torch::autograd::Node {
   Geo geo;
   int reverse = 0;
   explicit OpNode(const Handle& h) : handle(h) { handle.keep(); }
-  static void once() {
+  // What a backward pass has to refuse.  The engine hands a gradient on to the stream on which the node that takes it was made: during a capture
+  // that must be the captured one.  A leaf that an eager graph still holds has its node on the eager stream, and an event from the capture to
+  // there ends the capture, and the process with it.
+  void begin() const {
     if (at::GradMode::is_enabled()) throw std::runtime_error("the sequence operators have no second derivatives (create_graph=True)");
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing((hipStream_t)handle.stream(), &capture) != hipSuccess || capture == hipStreamCaptureStatusNone) return;
+    const c10::Stream here = c10::impl::VirtualGuardImpl(handle.device.type()).getStream(handle.device);
+    for (const auto& e : next_edges()) {
+      const auto there = e.function ? e.function->stream() : std::nullopt;
+      if (there && *there != here)
+        throw std::runtime_error("a captured backward pass cannot reach a leaf that a graph made outside the capture still holds: drop that graph first");
+    }
   }
   void check(rgp_status st) const {
     if (st != RGP_OK) throw std::runtime_error("librgp_hip status " + std::to_string((int)st) + ": " + (handle.h ? lib.rgp_last_error(handle.h) : "the handle is closed"));
@@ -220,7 +233,7 @@ struct ConvNode : OpNode {
     x.reset_data(); w.reset_data(); b.reset_data(); init.reset_data();
   }
   variable_list apply(variable_list&& grads) override {
-    once();
+    begin();
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(3);
     if (!grads[0].defined()) return out;
@@ -328,7 +341,7 @@ struct ScanNode : OpNode {
     states.reset();
   }
   variable_list apply(variable_list&& grads) override {
-    once();
+    begin();
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(8);
     if (!grads[0].defined()) return out;
@@ -434,7 +447,7 @@ struct RmsNode : OpNode {
     x.reset_data(); residual.reset_data(); w.reset_data(); rstd.reset();
   }
   variable_list apply(variable_list&& grads) override {      // of y and, with a residual, of hid
-    once();
+    begin();
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(3);                            // x, weight, residual
     const Tensor ghid = two ? grads[1] : Tensor();

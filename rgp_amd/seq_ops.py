@@ -12,8 +12,9 @@ features; sequences of different lengths are packed rows (rows, features) with a
 stream of the handle's device, allocates through torch (so it can be captured into a graph together with its backward pass) and gives the
 same bits every time.  Wrong arguments raise RgpError (RGP_ERR_BAD_ARG) before anything is launched.
 
-A captured backward pass needs leaves that no eager graph holds at that time: take the gradients with torch.autograd.grad inside the
-captured region, on a forward pass of the same region.  There are no second derivatives: a backward pass with create_graph=True is refused."""
+A captured backward pass needs leaves that no eager graph holds at that time (it is refused): take the gradients with torch.autograd.grad
+inside the captured region, on a forward pass of the same region.  There are no second derivatives: a backward pass with create_graph=True is
+refused."""
 import ctypes as C
 import math
 

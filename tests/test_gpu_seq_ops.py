@@ -549,7 +549,7 @@ def test_widths_that_are_not_whole_vectors(h, dtype, D):
 
 
 @pytest.mark.parametrize('dtype', ALL, ids=str)
-@pytest.mark.parametrize('rows,C', [(70, 2), (700, 9), (4000, 15), (50, 33), (20000, 17), (300, 301), (11, 1027), (1300, 127), (6, 4099), (600, 8195)])
+@pytest.mark.parametrize('rows,C', [(70, 2), (700, 9), (4000, 15), (50, 33), (20000, 17), (300, 301), (11, 1027), (1300, 127), (6, 4099), (600, 8195), (90, 600), (41, 611), (60, 151)])
 def test_rms_norm_rows_that_are_not_whole_vectors(h, dtype, rows, C):
     """Odd widths through every shape of the kernels, at an odd address, with no element of a neighbouring row touched."""
     from rgp_amd import seq_ops
@@ -654,3 +654,64 @@ def test_few_and_many_blocks_of_time(h, dtype, T):
         p.compare(p.run(h), p.reference())
     q = Problem(dtype, D=33, N=6, lengths=[T, 0, 1, T // 2, 9], carry=True, seed=T + 1)
     q.compare(q.run(h), q.reference())
+
+
+def test_steps_in_a_graph(h):
+    """Single steps captured once and replayed: the states move on with every replay as with eager calls, with other work in between."""
+    from rgp_amd import seq_ops
+    g, n, D, N = _gen(31), 3, 24, 16
+    w, b, A, D0 = _randn(g, D, 4, dtype=F32).cuda(), _randn(g, D, dtype=F32).cuda(), -torch.exp(_randn(g, D, N)).float().cuda(), _randn(g, D, dtype=F32).cuda()
+    xs = [[_randn(g, n, k, dtype=BF16).cuda() for k in (D, D, N, N)] for _ in range(6)]
+    inp = [t.clone() for t in xs[0]]
+    cst, sst = torch.zeros(n, 3, D, device='cuda', dtype=BF16), torch.zeros(n, D, N, device='cuda')
+
+    def step(x, delta, B, Cm, c, s):
+        u = seq_ops.ssm_conv_step(h, x, w, b, c)
+        y = seq_ops.ssm_scan_step(h, u, delta, A, B, Cm, D0, s, delta_bias=b)
+        return seq_ops.rms_norm(h, y, D0, residual=u)[0]
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(*inp, cst, sst)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*inp, cst, sst)
+        cst.zero_(), sst.zero_()
+        ce, se = torch.zeros_like(cst), torch.zeros_like(sst)
+        for x in xs:
+            for t, v in zip(inp, x):
+                t.copy_(v)
+            graph.replay()
+            want = step(*x, ce, se)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and torch.equal(cst, ce) and torch.equal(sst, se)
+
+
+def test_captured_backward_refuses_leaves_of_an_eager_graph(h):
+    """While a graph made outside holds the leaf, the captured backward pass raises before anything crosses the streams; without it, it works."""
+    from rgp_amd import seq_ops
+    x, w = torch.randn(6, 8, device='cuda', requires_grad=True), torch.ones(8, device='cuda', requires_grad=True)
+    gy = torch.randn(6, 8, device='cuda')
+
+    def region():
+        return torch.autograd.grad(seq_ops.rms_norm(h, x, w), (x, w), gy)
+    region()
+    torch.cuda.synchronize()
+    eager = seq_ops.rms_norm(h, x, w)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match='outside the capture'):
+        with torch.cuda.graph(graph):
+            region()
+    torch.cuda.synchronize()
+    want = torch.autograd.grad(eager, (x, w), gy)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = region()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
