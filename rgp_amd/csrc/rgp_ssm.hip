@@ -82,7 +82,7 @@ rgp_status SeqSums::run(rgp_handle h, hipStream_t s, int acc) {
 // 64 lanes take neighbouring (channel, state) pairs of one sequence, Q threads a pair: each walks its part of the blocks twice, first for
 // what that stretch does as a whole, then with the state that enters it (Q = 1: once).  The walk waits for memory, JOIN_U blocks at a time;
 // with Q = 16 for 1024 blocks of 8 sequences x 64 channels it takes 14 us where one thread a pair took 479; for many short sequences Q = 1 takes
-// 14 us where Q = 16 took 98.
+// 14 us where Q = 16 took 98, and for 13 sequences x 1024 channels x 32 states 6.4 where Q = 4 took 16.
 #define JOIN_U 8
 template <typename A, int Q>
 static __global__ void __launch_bounds__(Q == 1 ? 256 : Q * 64) ssm_join_kernel(SsmDev d, int back) {
@@ -223,7 +223,7 @@ static void scan_plan(const rgp_ssm_scan* a, bool back, ScanPlan& p) {
   d.lg = lg;
   d.L = (int64_t)1 << lg;
   const int64_t deep = (longest + d.L - 1) >> d.lg;
-  p.Q = deep <= 8 || (double)a->n_seq * a->D * a->N >= 524288.0 ? 1 : deep <= 128 ? 4 : 16;      // one where the pairs alone fill the card
+  p.Q = deep <= 8 || (double)a->n_seq * a->D * a->N >= 131072.0 ? 1 : deep <= 128 ? 4 : 16;      // one where the pairs alone give two waves a SIMD
   d.nslot = seq_blocks(d.g, d.lg);
   d.join = p.split && deep <= JOIN_SELF;
   const int64_t DN = (int64_t)a->D * a->N;

@@ -20,7 +20,7 @@ static __global__ void __launch_bounds__(CH* K, (sizeof(T) == 8 && R == 4) || K 
   typedef typename SeqAcc<T>::type A;
   typedef SeqAny<T, V> Vec;
   constexpr int THREADS = CH * K, NV = CH / V, RPI = THREADS / NV, CK = SSM_CK, NP = R * K, WAVES = THREADS / 64;
-  constexpr int TL = sizeof(T) == 8 ? 8 : sizeof(T) == 2 && CH * K == 256 && K == 4 ? 32 : 16, SUB = TL / CK;
+  constexpr int TL = ssm_bwd_tile(sizeof(T), K, CH), SUB = TL / CK;
   constexpr int NI = RPI >= TL ? 1 : TL / RPI, NB = (TL * NP + THREADS - 1) / THREADS;
   struct alignas(4 * sizeof(A)) Four { A x, y, z, w; };
   struct alignas(16) Quad { A v[R]; };
@@ -309,7 +309,7 @@ static __global__ void __launch_bounds__(CH* K, (sizeof(T) == 8 && R == 4) || K 
 
 template <typename T, int K, int R, int CH>
 static hipError_t go(const SsmDev& d, int mode, hipStream_t s) {
-  constexpr int V = 16 / (int)sizeof(T);
+  constexpr int V = ssm_vec(sizeof(T), ssm_bwd_tile(sizeof(T), K, CH), K);
   const dim3 g((unsigned)d.nslot, (unsigned)(d.a.G * d.ncb)), t(CH * K);
   if (mode == 0 && d.wide) hipLaunchKernelGGL((ssm_bwd_kernel<T, K, R, CH, 0, V>), g, t, 0, s, d);
   else if (mode == 0) hipLaunchKernelGGL((ssm_bwd_kernel<T, K, R, CH, 0, 1>), g, t, 0, s, d);

@@ -16,7 +16,7 @@ template <typename T, int K, int R, int CH, int MODE, int V>
 static __global__ void __launch_bounds__(CH* K, sizeof(T) < 8 && (K == 4 || K == 8) && CH * K == 256 && V > 1 ? 4 : 1) ssm_fwd_kernel(SsmDev d) {
   typedef typename SeqAcc<T>::type A;
   typedef SeqAny<T, V> Vec;
-  constexpr int THREADS = CH * K, NV = CH / V, TL = sizeof(A) == 8 || K <= 2 ? 16 : 32, NP = R * K, RPI = THREADS / NV;
+  constexpr int THREADS = CH * K, NV = CH / V, TL = ssm_fwd_tile(sizeof(T), K), NP = R * K, RPI = THREADS / NV;
   constexpr int NI = RPI >= TL ? 1 : TL / RPI, NB = (TL * NP + THREADS - 1) / THREADS, CK = SSM_CK;
   struct alignas(2 * sizeof(A)) Pair { A dt, w; };
   struct alignas(16) Quad { A v[R]; };
@@ -211,7 +211,7 @@ static __global__ void __launch_bounds__(CH* K, sizeof(T) < 8 && (K == 4 || K ==
 
 template <typename T, int K, int R, int CH>
 static hipError_t go(const SsmDev& d, int mode, hipStream_t s) {
-  constexpr int V = 16 / (int)sizeof(T);
+  constexpr int V = ssm_vec(sizeof(T), ssm_fwd_tile(sizeof(T), K), K);
   const dim3 g((unsigned)d.nslot, (unsigned)(d.a.G * d.ncb)), t(CH * K);
   if (mode == 0 && d.wide) hipLaunchKernelGGL((ssm_fwd_kernel<T, K, R, CH, 0, V>), g, t, 0, s, d);
   else if (mode == 0) hipLaunchKernelGGL((ssm_fwd_kernel<T, K, R, CH, 0, 1>), g, t, 0, s, d);
