@@ -5,11 +5,13 @@
 #include <type_traits>
 
 // ---- sums of partial results in a fixed order -----------------------------------------------------------------------------------------
-// A workgroup forms 64 outputs of one of up to five sums, 16 threads for each: thread q adds partials q, q + 16, ... in eight interleaved
-// sums (that many loads are in flight), then the 16 are added in LDS; up to SEQ_FEW
-// partials are added by one thread an output.  The order depends on the count of partials alone.  4 to 9 us for all sums of a backward pass.
+// A workgroup forms W outputs of one of up to five sums, Q = 1024 / W threads for each: thread q adds partials q, q + Q, ... in eight
+// interleaved sums (that many loads are in flight), then the Q are added in LDS.  W = 64, 16 where there are many partials (2048 of 1024 outputs:
+// 9 us with 64), and up to SEQ_FEW partials are added by one thread an output.  The order depends on the count of partials alone.  4 to 6 us for
+// all sums of a backward pass.
 #define SEQ_FEW 32
-static __host__ __device__ inline int64_t seq_sums_width(int64_t P) { return P <= SEQ_FEW ? 1024 : 64; }
+#define SEQ_MANY 512
+static __host__ __device__ inline int64_t seq_sums_width(int64_t P) { return P <= SEQ_FEW ? 1024 : P <= SEQ_MANY ? 64 : 16; }
 template <typename A>
 static __device__ __forceinline__ void seq_sums_store(const SeqSum& j, int64_t i, A v) {
   const int64_t o = j.turn > 1 ? (i % (j.n / j.turn)) * j.turn + i / (j.n / j.turn) : i;
@@ -22,7 +24,7 @@ static __device__ __forceinline__ void seq_sums_store(const SeqSum& j, int64_t i
 }
 template <typename A>
 static __global__ void __launch_bounds__(1024) seq_sums_kernel(SeqSums g) {
-  __shared__ A sh[16][64];
+  __shared__ A sh[1024];
   int k = 0;
   while (k + 1 < g.count && (int)blockIdx.x >= g.job[k + 1].block0) ++k;
   const SeqSum& j = g.job[k];
@@ -40,26 +42,33 @@ static __global__ void __launch_bounds__(1024) seq_sums_kernel(SeqSums g) {
     }
     return;
   }
-  const int l = threadIdx.x & 63, q = threadIdx.x >> 6;
+  const int W = (int)seq_sums_width(j.P), Q = 1024 / W, G = W == 64 ? 4 : 8, l = threadIdx.x % W, q = threadIdx.x / W;       // Q = G G
   const int64_t i = o0 + l;
   A v8[8] = {};
   if (i < n) {
     const A* p = part + q * j.stride + i;
-    int64_t left = j.P > q ? (j.P - q + 15) / 16 : 0;
-    for (; left >= 8; left -= 8, p += 128 * j.stride) {
+    int64_t left = j.P > q ? (j.P - q + Q - 1) / Q : 0;
+    const int64_t step = Q * j.stride;
+    for (; left >= 8; left -= 8, p += 8 * step) {
 #pragma unroll
-      for (int u = 0; u < 8; ++u) v8[u] += p[u * 16 * j.stride];
+      for (int u = 0; u < 8; ++u) v8[u] += p[u * step];
     }
 #pragma unroll
     for (int u = 0; u < 7; ++u)
-      if (u < left) v8[u] += p[u * 16 * j.stride];
+      if (u < left) v8[u] += p[u * step];
   }
-  sh[q][l] = ((v8[0] + v8[1]) + (v8[2] + v8[3])) + ((v8[4] + v8[5]) + (v8[6] + v8[7]));
+  sh[threadIdx.x] = ((v8[0] + v8[1]) + (v8[2] + v8[3])) + ((v8[4] + v8[5]) + (v8[6] + v8[7]));
+  __syncthreads();
+  A v = (A)0;
+  if (q < G) {                                            // G groups of G threads' sums
+    v = sh[q * G * W + l];
+    for (int r = 1; r < G; ++r) v += sh[(q * G + r) * W + l];
+  }
+  __syncthreads();
+  if (q < G) sh[q * W + l] = v;
   __syncthreads();
   if (q == 0 && i < n) {
-    A v = sh[0][l];
-#pragma unroll
-    for (int r = 1; r < 16; ++r) v += sh[r][l];
+    for (int r = 1; r < G; ++r) v += sh[r * W + l];
     seq_sums_store(j, i, v);
   }
 }
