@@ -181,17 +181,16 @@ def _mlp():
     return DeepAutoreg_mlp([0, 3, 3], Y, U=U, U_win=2, nDims=[3, 2, 3], num_inducing=4, MLP_dims=[3, 2], inference_method='svi', mb_inf_tot_data_size=4, seed=3)
 
 
-def _same_step(a, b, lr, updates=1):
+def _same_step(a, b, lr, updates=1, n=None):
     """One step of two models from the same parameters: gradients to the order of their sums (kernels with atomic additions differ there from run
     to run, 1e-9 of the largest), parameters to what Adam makes of that.  Its update is lr m / (sqrt(v) + eps), eps = 1e-8, with both moments
     corrected for the step number.  One gradient enters m with a weight of at most 1 and sqrt(v) with a slope of at most 1, and |m| <= 8 sqrt(v)
     (Cauchy-Schwarz over the two weightings, 0.9 and 0.999), so a change dg of the gradient moves the update by at most (1 + 8) lr dg / eps
     wherever sqrt(v) is; plus 32 roundings of the parameter."""
     a.handle.sync(); b.handle.sync()
-    dg, dp = (a.grad_array - b.grad_array).abs(), (a.param_array - b.param_array).abs()
-    n = a.param_array.numel()
-    assert float(dg[:n].max()) <= 1e-9 * float(b.grad_array[:n].abs().max())
-    assert bool((dp <= updates * 9 * lr / 1e-8 * dg[:n] + 32 * 2.0 ** -53 * b.param_array.abs().max()).all())
+    dg, dp = (a.grad_array[:n] - b.grad_array[:n]).abs(), (a.param_array[:n] - b.param_array[:n]).abs()
+    assert float(dg.max()) <= 1e-9 * float(b.grad_array[:n].abs().max())
+    assert bool((dp <= updates * 9 * lr / 1e-8 * dg + 32 * 2.0 ** -53 * b.param_array[:n].abs().max()).all())
 
 
 @pytest.mark.parametrize('seqs', [slice(0, 4), [2, 0], [1, 1, 3], None])
@@ -275,4 +274,4 @@ def test_two_ranks_clip_like_one_process():
     for m in halves:
         m.handle.sync()
         assert abs(float(m.last_grad_norm) - float(one.last_grad_norm)) <= 1e-9 * float(one.last_grad_norm)
-        assert float((m.param_array[:m.n_global] - one.param_array[:one.n_global]).abs().max()) <= 1e-7
+        _same_step(m, one, 1e-2, n=one.n_global)
