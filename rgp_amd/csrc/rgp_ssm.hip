@@ -8,9 +8,10 @@
 // A workgroup forms W outputs of one of up to five sums, Q = 1024 / W threads for each: thread q adds partials q, q + Q, ... in eight
 // interleaved sums (that many loads are in flight), then the Q are added in LDS.  W = 64, 16 where there are many partials (2048 of 1024 outputs:
 // 9 us with 64), and up to SEQ_FEW partials are added by one thread an output.  The order depends on the count of partials alone.  4 to 6 us for
-// all sums of a backward pass.
+// all sums of a backward pass.  Beyond SEQ_HUGE partials (many short sequences) rows r, r + SEQ_MANY, ... are first added into row r.
 #define SEQ_FEW 32
 #define SEQ_MANY 512
+#define SEQ_HUGE 8192
 static __host__ __device__ inline int64_t seq_sums_width(int64_t P) { return P <= SEQ_FEW ? 1024 : P <= SEQ_MANY ? 64 : 16; }
 template <typename A>
 static __device__ __forceinline__ void seq_sums_store(const SeqSum& j, int64_t i, A v) {
@@ -72,14 +73,41 @@ static __global__ void __launch_bounds__(1024) seq_sums_kernel(SeqSums g) {
     seq_sums_store(j, i, v);
   }
 }
-void SeqSums::add(const void* part, int64_t P, int64_t stride, int64_t n, void* out, int dt, int turn, const int64_t* end, int64_t per) {
+template <typename A>
+static __global__ void __launch_bounds__(256) seq_gather_kernel(A* part, int64_t P, int64_t stride, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  A v8[8] = {};
+  int64_t r = blockIdx.y;                                 // this thread alone reads and writes column i of these rows
+  for (; r + 7 * SEQ_MANY < P; r += 8 * SEQ_MANY) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v8[u] += part[(r + u * SEQ_MANY) * stride + i];
+  }
+  for (; r < P; r += SEQ_MANY) v8[0] += part[r * stride + i];
+  part[blockIdx.y * stride + i] = ((v8[0] + v8[1]) + (v8[2] + v8[3])) + ((v8[4] + v8[5]) + (v8[6] + v8[7]));
+}
+void SeqSums::add(void* part, int64_t P, int64_t stride, int64_t n, void* out, int dt, int turn, const int64_t* end, int64_t per) {
   if (!out || n < 1) return;
   SeqSum& j = job[count++];
-  j.part = part; j.P = P; j.stride = stride; j.n = n; j.out = out; j.dt = dt; j.turn = turn; j.block0 = blocks; j.end = end; j.per = per;
-  blocks += (int)((n + seq_sums_width(P) - 1) / seq_sums_width(P));
+  j.part = part; j.P = P; j.stride = stride; j.n = n; j.out = out; j.dt = dt; j.turn = turn; j.end = end; j.per = per;
 }
 rgp_status SeqSums::run(rgp_handle h, hipStream_t s, int acc) {
   if (!count) return RGP_OK;
+  for (int k = 0; k < count; ++k) {
+    SeqSum& j = job[k];
+    if (j.P <= SEQ_HUGE) continue;
+    const dim3 g((unsigned)((j.n + 255) / 256), SEQ_MANY);
+    if (acc == RGP_F64) hipLaunchKernelGGL(seq_gather_kernel<double>, g, dim3(256), 0, s, (double*)j.part, j.P, j.stride, j.n);
+    else hipLaunchKernelGGL(seq_gather_kernel<float>, g, dim3(256), 0, s, (float*)j.part, j.P, j.stride, j.n);
+    const rgp_status st = seq_launched(h, "sum of partial results");
+    if (st) return st;
+    j.P = SEQ_MANY;
+  }
+  blocks = 0;
+  for (int k = 0; k < count; ++k) {
+    job[k].block0 = blocks;
+    blocks += (int)((job[k].n + seq_sums_width(job[k].P) - 1) / seq_sums_width(job[k].P));
+  }
   if (acc == RGP_F64) hipLaunchKernelGGL(seq_sums_kernel<double>, dim3(blocks), dim3(1024), 0, s, *this);
   else hipLaunchKernelGGL(seq_sums_kernel<float>, dim3(blocks), dim3(1024), 0, s, *this);
   return seq_launched(h, "sum of partial results");

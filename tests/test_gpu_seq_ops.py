@@ -715,3 +715,33 @@ def test_captured_backward_refuses_leaves_of_an_eager_graph(h):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize('dtype', [F64, F32], ids=str)
+def test_very_many_short_sequences(h, dtype):
+    """More blocks than the sums over them take at once (8192): gradients of the parameters are sums over all sequences."""
+    from rgp_amd import seq_ops
+    g, T, n, D, N = _gen(41), 2, 9001, 3, 2
+    acc = ref.acc_of(dtype)
+    acts = [_randn(g, T, n, k, dtype=dtype) for k in (D, D, N, N, D)]                            # u, delta, B, C, gy
+    par = [-torch.exp(_randn(g, D, N)).to(acc), _randn(g, D, dtype=acc), _randn(g, D, dtype=acc)]     # A, D, bias
+    leaves = [t.cuda().requires_grad_(True) for t in acts[:4] + par]
+    u, delta, B, Cm, A, skip, bias = leaves
+    y = seq_ops.ssm_scan(h, u, delta, A, B, Cm, D=skip, delta_bias=bias)
+    got = torch.autograd.grad(y, leaves, acts[4].cuda())
+    w = [t.double().requires_grad_(True) for t in acts[:4] + par]
+    u, delta, B, Cm, A, skip, bias = w
+    s, ys = torch.zeros(n, D, N, dtype=F64), []
+    for t in range(T):
+        dt = torch.nn.functional.softplus(delta[t] + bias)
+        s = torch.exp(dt[..., None] * A) * s + (dt * u[t])[..., None] * B[t][:, None]
+        ys.append((s * Cm[t][:, None]).sum(-1) + skip * u[t])
+    want = torch.autograd.grad(torch.stack(ys), w, acts[4].double())
+    # relative to the largest: rounding of the operands of each product (64 operations a term), and of adding T n terms of either sign, whose
+    # absolute values sum to at most T n times the largest term
+    half = torch.finfo(acc).eps / 2
+    for a, b in zip(got[:4], want[:4]):
+        assert float((a.cpu().double() - b).abs().max()) <= 64 * half * float(b.abs().max())
+    terms = T * n * 64 * half
+    for a, b in zip(got[4:], want[4:]):
+        assert float((a.cpu().double() - b).abs().max()) <= terms * max(1.0, float(b.abs().max()) / (T * n) ** 0.5)
