@@ -37,9 +37,14 @@ class Handle(object):
         self.h = h
 
     def close(self):
-        if getattr(self, 'h', None):
-            self.lib.rgp_destroy(self.h)
+        """Destroys the library's context.  Not while another thread is inside a call on it; graphs of the sequence
+        operators that are still alive refuse their backward pass from now on."""
+        h = getattr(self, 'h', None)
+        if h:
             self.h = None
+            context = C.c_void_p(h.value)
+            h.value = None                     # the place where those graphs look (csrc/rgp_torch.cpp)
+            self.lib.rgp_destroy(context)
 
     def __del__(self):
         try:

@@ -42,7 +42,7 @@ struct Entries {
 #undef ENTRY
 } lib;
 PyObject* rgp_error = nullptr;                      // rgp_amd._lib.RgpError
-PyObject *s_h, *s_value, *s_device, *s_off, *s_n_seq, *s_rows, *s_max_len;
+PyObject *s_h, *s_device, *s_off, *s_n_seq, *s_rows, *s_max_len;
 
 struct Failed { int code; std::string msg; };      // a status of the library
 
@@ -65,41 +65,59 @@ int64_t attr_int(PyObject* o, PyObject* name) {
   return v;
 }
 
+// Where a Handle's c_void_p holds the library's pointer; nullptr for None.
+void* const* cell_of(PyObject* p) {
+  if (p == Py_None) return nullptr;
+  Py_buffer b;
+  if (PyObject_GetBuffer(p, &b, PyBUF_SIMPLE) != 0) throw python_error();
+  void* const* at = b.len == sizeof(void*) ? (void* const*)b.buf : nullptr;
+  PyBuffer_Release(&b);
+  return at;
+}
+
 // A Handle: the library's pointer, its device, and the Python object, which a graph keeps alive.
 struct Handle {
-  rgp_handle h = nullptr;
+  rgp_handle h = nullptr;                           // for the length of a call
   at::Device device = at::kCPU;
-  std::shared_ptr<PyObject> owner;
-  explicit Handle(PyObject* o) {
+  PyObject* object;
+  explicit Handle(PyObject* o) : object(o) {
     PyObject* d = attr(o, s_device);
     if (THPDevice_Check(d)) device = ((THPDevice*)d)->device;
     Py_DECREF(d);
     PyObject* p = attr(o, s_h);
-    if (p != Py_None) {
-      PyObject* v = PyObject_GetAttr(p, s_value);
-      Py_DECREF(p);
-      if (!v) throw python_error();
-      h = v == Py_None ? nullptr : (rgp_handle)PyLong_AsVoidPtr(v);
-      Py_DECREF(v);
-    } else {
-      Py_DECREF(p);
-    }
-    object = o;
-  }
-  void keep() {                                     // for a node, which may outlive the call and end on any thread
-    Py_INCREF(object);
-    owner = std::shared_ptr<PyObject>(object, [](PyObject* q) {
-      if (!Py_IsInitialized()) return;
-      const PyGILState_STATE s = PyGILState_Ensure();
-      Py_DECREF(q);
-      PyGILState_Release(s);
-    });
+    std::shared_ptr<PyObject> hold(p, [](PyObject* q) { Py_DECREF(q); });
+    if (void* const* at = cell_of(p)) h = (rgp_handle)*at;
   }
   void* stream() const { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
   void check(rgp_status st) const {
     if (st != RGP_OK) throw Failed{(int)st, h ? lib.rgp_last_error(h) : "the handle is closed"};
   }
-  PyObject* object;
+};
+// What a graph, which may end on any thread, keeps of it.  close() clears the pointer in the c_void_p before it destroys the context, so a pass
+// that comes later finds none there; the place itself lives as long as the c_void_p.
+struct KeptHandle {
+  at::Device device;
+  std::shared_ptr<PyObject> owner;                  // the Handle and its c_void_p
+  void* const* cell = nullptr;
+  explicit KeptHandle(const Handle& from) : device(from.device) {
+    PyObject* p = attr(from.object, s_h);
+    PyObject* both = PyTuple_Pack(2, from.object, p);
+    Py_DECREF(p);
+    if (!both) throw python_error();
+    owner = std::shared_ptr<PyObject>(both, [](PyObject* q) {
+      if (!Py_IsInitialized()) return;
+      const PyGILState_STATE s = PyGILState_Ensure();
+      Py_DECREF(q);
+      PyGILState_Release(s);
+    });
+    cell = cell_of(PyTuple_GET_ITEM(both, 1));
+  }
+  rgp_handle get() const {
+    rgp_handle h = cell ? (rgp_handle)__atomic_load_n(cell, __ATOMIC_ACQUIRE) : nullptr;
+    if (!h) throw std::runtime_error("librgp_hip: the handle of this graph is closed");
+    return h;
+  }
+  void* stream() const { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
 };
 
 int type_code(at::ScalarType t) {
@@ -182,10 +200,10 @@ void put_stride(const Tensor& t, const Geo& g, int64_t& st, int64_t& sb) {
 
 // A node of the graph: what both passes need besides the saved operands.
 struct OpNode : torch::autograd::Node {
-  Handle handle;
+  KeptHandle handle;
   Geo geo;
   int reverse = 0;
-  explicit OpNode(const Handle& h) : handle(h) { handle.keep(); }
+  explicit OpNode(const Handle& h) : handle(h) {}
   // What a backward pass has to refuse.  The engine hands a gradient on to the stream on which the node that takes it was made: during a capture
   // that must be the captured one.  A leaf that an eager graph still holds has its node on the eager stream, and an event from the capture to
   // there ends the capture, and the process with it.
@@ -200,8 +218,8 @@ struct OpNode : torch::autograd::Node {
         throw std::runtime_error("a captured backward pass cannot reach a leaf that a graph made outside the capture still holds: drop that graph first");
     }
   }
-  void check(rgp_status st) const {
-    if (st != RGP_OK) throw std::runtime_error("librgp_hip status " + std::to_string((int)st) + ": " + (handle.h ? lib.rgp_last_error(handle.h) : "the handle is closed"));
+  static void check(rgp_handle h, rgp_status st) {
+    if (st != RGP_OK) throw std::runtime_error("librgp_hip status " + std::to_string((int)st) + ": " + lib.rgp_last_error(h));
   }
 };
 template <typename N>
@@ -244,7 +262,8 @@ struct ConvNode : OpNode {
     a.init = ptr(before); a.gv = gv.data_ptr(); a.gx = out[0].data_ptr(); a.gw = out[1].data_ptr(); a.gbias = ptr(out[2]);
     put_stride(gv, geo, a.gv_st, a.gv_sb);
     const Tensor work = work_of(c.x, lib.rgp_ssm_conv_workspace(&a, 1), a.work, a.work_bytes);
-    check(lib.rgp_ssm_conv_backward(handle.h, handle.stream(), &a));
+    const rgp_handle h = handle.get();
+    check(h, lib.rgp_ssm_conv_backward(h, handle.stream(), &a));
     return out;
   }
 };
@@ -355,7 +374,8 @@ struct ScanNode : OpNode {
     a.gskip = ptr(out[5]); a.gz = ptr(out[6]); a.gbias = ptr(out[7]);
     put_stride(gy, geo, a.gy_st, a.gy_sb);
     const Tensor work = work_of(s.u, lib.rgp_ssm_scan_workspace(&a, 1), a.work, a.work_bytes);
-    check(lib.rgp_ssm_scan_backward(handle.h, handle.stream(), &a));
+    const rgp_handle h = handle.get();
+    check(h, lib.rgp_ssm_scan_backward(h, handle.stream(), &a));
     return out;
   }
 };
@@ -463,7 +483,8 @@ struct RmsNode : OpNode {
     a.rstd = rstd.data_ptr(); a.gy = gy.data_ptr(); a.gy_st = gy.stride(0); a.ghid = ptr(gh); a.ghid_st = gh.defined() ? gh.stride(0) : 0;
     a.gx = out[0].data_ptr(); a.gw = out[1].data_ptr();
     const Tensor work = work_of(xs, lib.rgp_rms_norm_workspace(&a, 1), a.work, a.work_bytes);
-    check(lib.rgp_rms_norm_backward(handle.h, handle.stream(), &a));
+    const rgp_handle h = handle.get();
+    check(h, lib.rgp_rms_norm_backward(h, handle.stream(), &a));
     return out;
   }
 };
@@ -632,8 +653,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_seq", "The sequence operators on 
 }  // namespace
 
 PyMODINIT_FUNC PyInit__seq() {
-  const std::pair<PyObject**, const char*> names[] = {{&s_h, "h"}, {&s_value, "value"}, {&s_device, "device"}, {&s_off, "off"},
-                                                      {&s_n_seq, "n_seq"}, {&s_rows, "rows"}, {&s_max_len, "max_len"}};
+  const std::pair<PyObject**, const char*> names[] = {{&s_h, "h"}, {&s_device, "device"}, {&s_off, "off"}, {&s_n_seq, "n_seq"}, {&s_rows, "rows"},
+                                                      {&s_max_len, "max_len"}};
   for (const auto& n : names)
     if (!(*n.first = PyUnicode_InternFromString(n.second))) return nullptr;
   return PyModule_Create(&module);

@@ -1,0 +1,53 @@
+"""Calls of the sequence operators from places where they can be given what no kernel may see: a graph whose handle is gone, the framework's
+other ways to run a function, tensors whose memory does not hold their values."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F64, F32, BF16 = torch.float64, torch.float32, torch.bfloat16
+
+
+@pytest.fixture(scope='module')
+def h():
+    from rgp_amd.capi import Handle
+    return Handle()
+
+
+def _leaves(*names, seed=0, dtype=F32):
+    g = torch.Generator().manual_seed(seed)
+    shapes = dict(u=(9, 2, 6), delta=(9, 2, 6), A=(6, 3), B=(9, 2, 3), C=(9, 2, 3), w=(6, 4), x=(5, 8), r=(5, 8), n=(8,))
+    return [torch.randn(*shapes[k], generator=g, dtype=F64).to(dtype).cuda().requires_grad_(True) for k in names]
+
+
+def _three(h, ops):
+    """One result of each differentiable operator."""
+    from rgp_amd import seq_ops
+    u, delta, A, B, Cm, w, x, r, n = ops
+    return seq_ops.ssm_scan(h, u, delta, A, B, Cm), seq_ops.ssm_conv(h, u, w), seq_ops.rms_norm(h, x, n, residual=r)[0]
+
+
+ALL_LEAVES = ('u', 'delta', 'A', 'B', 'C', 'w', 'x', 'r', 'n')
+
+
+def test_backward_pass_after_the_handle_is_closed_is_refused(h):
+    """close() under graphs that are still alive: their backward passes raise, another handle's go on, and so do those of a handle that is only
+    out of scope."""
+    from rgp_amd.capi import Handle
+    ops = _leaves(*ALL_LEAVES)
+    other = Handle()
+    closed, mine = _three(other, ops), _three(h, ops)
+    other.close()
+    assert not other.h
+    for out in closed:
+        for _ in range(2):                                          # the refused pass takes nothing with it
+            with pytest.raises(RuntimeError, match='handle of this graph is closed'):
+                out.sum().backward(retain_graph=True)
+    assert all(t.grad is None for t in ops)
+    dropped = Handle()
+    still = _three(dropped, ops)
+    del dropped
+    for a, b in zip(mine, still):
+        for x, y in zip(torch.autograd.grad(a.sum(), ops, allow_unused=True), torch.autograd.grad(b.sum(), ops, allow_unused=True)):
+            assert (x is None and y is None) or torch.equal(x, y)
+    other.close()                                                   # once more is nothing
