@@ -12,6 +12,7 @@
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/Device.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -131,11 +132,19 @@ int type_code(at::ScalarType t) {
 }
 at::ScalarType acc_of(at::ScalarType t) { return t == at::kDouble ? at::kDouble : at::kFloat; }
 
+// Forward-mode derivatives: a tensor may carry its tangent beside its values, and no result here would get one.
+bool dual_level() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+thread_local bool duals = false;                    // a call made while there is a dual level
+void seen(const Tensor& t) {
+  if (duals && has_tangent(t)) throw Failed{RGP_ERR_BAD_ARG, "the sequence operators have no forward-mode derivatives: an operand carries a tangent"};
+}
 // None -> an undefined tensor; false: no tensor
 bool tensor(PyObject* o, Tensor& t, bool optional = false) {
   if (o == Py_None) return optional;
   if (!THPVariable_Check(o)) return false;
   t = THPVariable_Unpack(o);
+  seen(t);
   return t.layout() == at::kStrided;
 }
 bool like(const Tensor& t, const Tensor& x) { return t.scalar_type() == x.scalar_type() && t.device() == x.device(); }
@@ -207,8 +216,11 @@ struct OpNode : torch::autograd::Node {
   // What a backward pass has to refuse.  The engine hands a gradient on to the stream on which the node that takes it was made: during a capture
   // that must be the captured one.  A leaf that an eager graph still holds has its node on the eager stream, and an event from the capture to
   // there ends the capture, and the process with it.
-  void begin() const {
+  void begin(const variable_list& grads) const {
     if (at::GradMode::is_enabled()) throw std::runtime_error("the sequence operators have no second derivatives (create_graph=True)");
+    if (dual_level())
+      for (const Tensor& g : grads)
+        if (has_tangent(g)) throw std::runtime_error("the sequence operators have no second derivatives: a gradient carries a forward-mode tangent");
     hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing((hipStream_t)handle.stream(), &capture) != hipSuccess || capture == hipStreamCaptureStatusNone) return;
     const c10::Stream here = c10::impl::VirtualGuardImpl(handle.device.type()).getStream(handle.device);
@@ -251,7 +263,7 @@ struct ConvNode : OpNode {
     x.reset_data(); w.reset_data(); b.reset_data(); init.reset_data();
   }
   variable_list apply(variable_list&& grads) override {
-    begin();
+    begin(grads);
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(3);
     if (!grads[0].defined()) return out;
@@ -360,7 +372,7 @@ struct ScanNode : OpNode {
     states.reset();
   }
   variable_list apply(variable_list&& grads) override {
-    begin();
+    begin(grads);
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(8);
     if (!grads[0].defined()) return out;
@@ -467,7 +479,7 @@ struct RmsNode : OpNode {
     x.reset_data(); residual.reset_data(); w.reset_data(); rstd.reset();
   }
   variable_list apply(variable_list&& grads) override {      // of y and, with a residual, of hid
-    begin();
+    begin(grads);
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(3);                            // x, weight, residual
     const Tensor ghid = two ? grads[1] : Tensor();
@@ -534,6 +546,8 @@ bool grads_ok(const Handle& h, PyObject* list, Grads& g) {
   const Py_ssize_t n = PyList_GET_SIZE(list);
   std::vector<std::pair<char*, char*>> range(n);
   g.p.resize(n); g.n.resize(n); g.dt.resize(n);
+  for (Py_ssize_t i = 0; i < n; ++i)
+    if (THPVariable_Check(PyList_GET_ITEM(list, i))) seen(THPVariable_Unpack(PyList_GET_ITEM(list, i)));
   for (Py_ssize_t i = 0; i < n; ++i) {
     PyObject* o = PyList_GET_ITEM(list, i);
     if (!THPVariable_Check(o)) return false;
@@ -558,7 +572,7 @@ Tensor scalars(const Handle& h, int64_t bytes) {      // one result and the plac
 PyObject* sumsq(PyObject* const* o) {
   Handle h(o[0]);
   Grads g;
-  if (!h.device.is_cuda() || !grads_ok(h, o[1], g)) return nullptr;
+  if (!grads_ok(h, o[1], g) || !h.device.is_cuda()) return nullptr;
   const int n = (int)g.p.size();
   const int64_t bytes = lib.rgp_grad_workspace(n, g.n.data(), g.dt.data());
   Tensor buf = scalars(h, bytes);
@@ -576,7 +590,7 @@ PyObject* clip(PyObject* const* o) {
   Tensor sum;
   const double most = PyFloat_AsDouble(o[2]);
   if (most == -1.0 && PyErr_Occurred()) throw python_error();
-  if (!h.device.is_cuda() || !(most > 0.0) || !tensor(o[3], sum, true) || !grads_ok(h, o[1], g)) return nullptr;
+  if (!(most > 0.0) || !tensor(o[3], sum, true) || !grads_ok(h, o[1], g) || !h.device.is_cuda()) return nullptr;
   if (sum.defined() && (sum.scalar_type() != at::kDouble || sum.numel() != 1 || sum.device() != h.device)) return nullptr;
   const int n = (int)g.p.size();
   const int64_t bytes = sum.defined() ? 0 : lib.rgp_grad_workspace(n, g.n.data(), g.dt.data());
@@ -600,6 +614,7 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return nullptr;
   }
   try {
+    duals = dual_level();
     PyObject* r = F(args);
     if (r || PyErr_Occurred()) return r;
     Py_RETURN_NONE;

@@ -13,8 +13,8 @@ stream of the handle's device, allocates through torch (so it can be captured in
 same bits every time.  Wrong arguments raise RgpError (RGP_ERR_BAD_ARG) before anything is launched.
 
 A captured backward pass needs leaves that no eager graph holds at that time (it is refused): take the gradients with torch.autograd.grad
-inside the captured region, on a forward pass of the same region.  There are no second derivatives: a backward pass with create_graph=True is
-refused."""
+inside the captured region, on a forward pass of the same region.  There are no second derivatives (a backward pass with
+create_graph=True is refused) and no forward-mode ones (operands and gradients that carry a tangent are refused)."""
 import ctypes as C
 import math
 

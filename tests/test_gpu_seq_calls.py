@@ -51,3 +51,30 @@ def test_backward_pass_after_the_handle_is_closed_is_refused(h):
         for x, y in zip(torch.autograd.grad(a.sum(), ops, allow_unused=True), torch.autograd.grad(b.sum(), ops, allow_unused=True)):
             assert (x is None and y is None) or torch.equal(x, y)
     other.close()                                                   # once more is nothing
+
+
+def test_tangents_are_refused_in_both_directions(h):
+    """Forward-mode derivatives never come back as nothing: a dual operand, a dual gradient and a dual tensor to clip raise; inside a dual level
+    the operators work on tensors without tangents."""
+    import torch.autograd.forward_ad as fwad
+    from rgp_amd import seq_ops
+    from rgp_amd._lib import RgpError
+    ops = _leaves(*ALL_LEAVES)
+    plain = [t.detach() for t in _three(h, ops)]
+    with fwad.dual_level():
+        for i, t in enumerate(ops):
+            dual = list(ops)
+            dual[i] = fwad.make_dual(t.detach(), torch.ones_like(t))
+            with pytest.raises(RgpError, match='forward-mode'):
+                _three(h, dual)
+        outs = _three(h, ops)
+        assert all(torch.equal(a, b) for a, b in zip(outs, plain))
+        for out in outs:
+            with pytest.raises(RuntimeError, match='forward-mode tangent'):
+                torch.autograd.grad(out, ops, fwad.make_dual(torch.ones_like(out), torch.ones_like(out)), allow_unused=True, retain_graph=True)
+            torch.autograd.grad(out, ops, torch.ones_like(out), allow_unused=True)
+        g = torch.randn(40, device='cuda')
+        keep = g.clone()
+        with pytest.raises(RgpError, match='forward-mode'):
+            seq_ops.clip_grad_norm(h, [fwad.make_dual(g, g)], 1e-3)
+        assert torch.equal(g, keep)

@@ -1,0 +1,37 @@
+"""Calls of the sequence operators that are refused before the library is entered, whatever the device."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwad
+
+from test_seq_ops_cpu import H, _refused
+
+
+def _calls():
+    """{name: (function of its operands, operands)} for every entry point that takes tensors."""
+    from rgp_amd import seq_ops
+    z = torch.zeros
+    return {
+        'conv': (lambda x, w, b, init: seq_ops.ssm_conv(H, x, w, b, init=init), [z(5, 2, 6), z(6, 4), z(6), z(2, 3, 6)]),
+        'conv_step': (lambda x, w, b, st: seq_ops.ssm_conv_step(H, x, w, b, st), [z(2, 6), z(6, 4), z(6), z(2, 3, 6)]),
+        'scan': (lambda u, d, A, B, Cm, D, zz, b, init: seq_ops.ssm_scan(H, u, d, A, B, Cm, D=D, z=zz, delta_bias=b, init=init),
+                 [z(5, 2, 6), z(5, 2, 6), z(6, 3), z(5, 2, 3), z(5, 2, 3), z(6), z(5, 2, 6), z(6), z(2, 6, 3)]),
+        'scan_step': (lambda u, d, A, B, Cm, D, st, zz, b: seq_ops.ssm_scan_step(H, u, d, A, B, Cm, D, st, z=zz, delta_bias=b),
+                      [z(2, 6), z(2, 6), z(6, 3), z(2, 3), z(2, 3), z(6), z(2, 6, 3), z(2, 6), z(6)]),
+        'rms': (lambda x, w, r: seq_ops.rms_norm(H, x, w, residual=r), [z(3, 4), z(4), z(3, 4)]),
+        'rms of three dimensions': (lambda x, w, r: seq_ops.rms_norm(H, x, w, residual=r), [z(2, 3, 4), z(4), z(2, 3, 4)]),
+        'sumsq': (lambda a, b: seq_ops.grad_sumsq(H, [a, b]), [z(3), z(4)]),
+        'clip': (lambda a, b, s: seq_ops.clip_grad_norm(H, [a, b], 1.0, sumsq=s), [z(3), z(4), z(1, dtype=torch.float64)]),
+    }
+
+
+@pytest.mark.parametrize('name', list(_calls()))
+def test_operands_with_a_tangent_are_refused(name):
+    """Forward-mode derivatives: every operand that carries a tangent, one at a time; inside a dual level, tensors without one are as ever."""
+    f, ops = _calls()[name]
+    with fwad.dual_level():
+        for i, t in enumerate(ops):
+            with torch.no_grad():                                   # a step refuses gradients first
+                dual = list(ops)
+                dual[i] = fwad.make_dual(t, torch.ones_like(t))
+                _refused(lambda: f(*dual), 'forward-mode')
+        _refused(lambda: f(*ops), '^(?!.*forward-mode)')
