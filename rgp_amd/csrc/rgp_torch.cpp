@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
@@ -18,6 +19,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <array>
@@ -132,6 +134,11 @@ int type_code(at::ScalarType t) {
 }
 at::ScalarType acc_of(at::ScalarType t) { return t == at::kDouble ? at::kDouble : at::kFloat; }
 
+// While torch records a function (torch.jit.trace, make_fx), it would see the allocation of a result and nothing that fills it.
+bool recording() {
+  return torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value();
+}
+
 // Forward-mode derivatives: a tensor may carry its tangent beside its values, and no result here would get one.
 bool dual_level() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
 bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
@@ -218,6 +225,7 @@ struct OpNode : torch::autograd::Node {
   // there ends the capture, and the process with it.
   void begin(const variable_list& grads) const {
     if (at::GradMode::is_enabled()) throw std::runtime_error("the sequence operators have no second derivatives (create_graph=True)");
+    if (recording()) throw std::runtime_error("the sequence operators cannot be recorded: leave their backward passes out of make_fx");
     if (dual_level())
       for (const Tensor& g : grads)
         if (has_tangent(g)) throw std::runtime_error("the sequence operators have no second derivatives: a gradient carries a forward-mode tangent");
@@ -614,6 +622,7 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return nullptr;
   }
   try {
+    if (recording()) throw Failed{RGP_ERR_BAD_ARG, "the sequence operators cannot be recorded: leave them out of torch.jit.trace and make_fx"};
     duals = dual_level();
     PyObject* r = F(args);
     if (r || PyErr_Occurred()) return r;

@@ -78,3 +78,20 @@ def test_tangents_are_refused_in_both_directions(h):
         with pytest.raises(RgpError, match='forward-mode'):
             seq_ops.clip_grad_norm(h, [fwad.make_dual(g, g)], 1e-3)
         assert torch.equal(g, keep)
+
+
+def test_recording_a_function_is_refused(h):
+    """torch.jit.trace and make_fx raise, the latter for a backward pass too; afterwards the calls are as before."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from rgp_amd import seq_ops
+    from rgp_amd._lib import RgpError
+    ops = [t.detach() for t in _leaves(*ALL_LEAVES)]
+    plain = _three(h, ops)
+    for record in (lambda f, x: torch.jit.trace(f, x, check_trace=False), lambda f, x: make_fx(f)(x)):
+        with pytest.raises(RgpError, match='cannot be recorded'):
+            record(lambda x: seq_ops.rms_norm(h, x, ops[8]), ops[6])
+    leaf = ops[6].clone().requires_grad_(True)
+    out = seq_ops.rms_norm(h, leaf, ops[8])
+    with pytest.raises(RuntimeError, match='cannot be recorded'):
+        make_fx(lambda g: torch.autograd.grad(out, leaf, g, retain_graph=True)[0])(torch.ones_like(out))
+    assert all(torch.equal(a, b) for a, b in zip(_three(h, ops), plain))

@@ -35,3 +35,13 @@ def test_operands_with_a_tangent_are_refused(name):
                 dual[i] = fwad.make_dual(t, torch.ones_like(t))
                 _refused(lambda: f(*dual), 'forward-mode')
         _refused(lambda: f(*ops), '^(?!.*forward-mode)')
+
+
+@pytest.mark.parametrize('name', list(_calls()))
+def test_recording_a_function_is_refused(name):
+    """torch.jit.trace and make_fx see allocations only: a recorded function would return memory that nothing has written."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f, ops = _calls()[name]
+    with torch.no_grad():
+        _refused(lambda: torch.jit.trace(lambda x: f(x, *ops[1:]), ops[0], check_trace=False), 'cannot be recorded')
+        _refused(lambda: make_fx(lambda x: f(x, *ops[1:]))(ops[0]), 'cannot be recorded')
