@@ -146,13 +146,13 @@ thread_local bool duals = false;                    // a call made while there i
 void seen(const Tensor& t) {
   if (duals && has_tangent(t)) throw Failed{RGP_ERR_BAD_ARG, "the sequence operators have no forward-mode derivatives: an operand carries a tangent"};
 }
-// None -> an undefined tensor; false: no tensor
+// None -> an undefined tensor; false: no tensor, or one whose memory does not hold its values (a view of a conjugate with the negation pending)
 bool tensor(PyObject* o, Tensor& t, bool optional = false) {
   if (o == Py_None) return optional;
   if (!THPVariable_Check(o)) return false;
   t = THPVariable_Unpack(o);
   seen(t);
-  return t.layout() == at::kStrided;
+  return t.layout() == at::kStrided && !t.is_neg();
 }
 bool like(const Tensor& t, const Tensor& x) { return t.scalar_type() == x.scalar_type() && t.device() == x.device(); }
 bool inner(const Tensor& t, int dims) {              // the last dims dimensions contiguous
@@ -162,6 +162,10 @@ bool inner(const Tensor& t, int dims) {              // the last dims dimensions
     want *= t.size(-i);
   }
   return true;
+}
+Tensor rows_of(const Tensor& g) {                    // a gradient as the kernels read it
+  const Tensor t = g.is_neg() ? g.resolve_neg() : g;
+  return inner(t, 1) ? t : t.contiguous();
 }
 bool param(const Tensor& t, const Tensor& x, at::IntArrayRef shape) {
   return t.scalar_type() == acc_of(x.scalar_type()) && t.device() == x.device() && t.sizes() == shape && t.is_contiguous();
@@ -276,7 +280,7 @@ struct ConvNode : OpNode {
     variable_list out(3);
     if (!grads[0].defined()) return out;
     const ConvOps c{x.unpack(), w.unpack(), b.unpack()};
-    const Tensor before = init.unpack(), gv = inner(grads[0], 1) ? grads[0] : grads[0].contiguous();
+    const Tensor before = init.unpack(), gv = rows_of(grads[0]);
     rgp_ssm_conv a = conv_args(c, geo, reverse);
     out[0] = fresh(c.x); out[1] = fresh(c.w); out[2] = fresh(c.b);
     a.init = ptr(before); a.gv = gv.data_ptr(); a.gx = out[0].data_ptr(); a.gw = out[1].data_ptr(); a.gbias = ptr(out[2]);
@@ -385,7 +389,7 @@ struct ScanNode : OpNode {
     variable_list out(8);
     if (!grads[0].defined()) return out;
     const ScanOps s{u.unpack(), delta.unpack(), A.unpack(), B.unpack(), C.unpack(), skip.unpack(), z.unpack(), bias.unpack()};
-    const Tensor gy = inner(grads[0], 1) ? grads[0] : grads[0].contiguous();
+    const Tensor gy = rows_of(grads[0]);
     rgp_ssm_scan a = scan_args(s, geo, G, reverse);
     const Tensor* in[8] = {&s.u, &s.delta, &s.A, &s.B, &s.C, &s.skip, &s.z, &s.bias};
     for (int i = 0; i < 8; ++i) out[i] = fresh(*in[i]);
@@ -496,7 +500,7 @@ struct RmsNode : OpNode {
       return out;
     }
     const Tensor xs = x.unpack(of_hid ? shared_from_this() : nullptr), rs = residual.unpack(), ws = w.unpack();
-    const Tensor gy = inner(grads[0], 1) ? grads[0] : grads[0].contiguous(), gh = !ghid.defined() || inner(ghid, 1) ? ghid : ghid.contiguous();
+    const Tensor gy = rows_of(grads[0]), gh = ghid.defined() ? rows_of(ghid) : ghid;
     rgp_rms_norm a = rms_args(xs, rs, ws, eps);
     out[0] = fresh(xs); out[1] = fresh(ws);
     if (two) out[2] = out[0];
@@ -561,7 +565,7 @@ bool grads_ok(const Handle& h, PyObject* list, Grads& g) {
     if (!THPVariable_Check(o)) return false;
     const Tensor& t = THPVariable_Unpack(o);
     const int code = type_code(t.scalar_type());
-    if (code < 0 || !t.is_cuda() || t.device() != h.device || t.layout() != at::kStrided || !t.is_non_overlapping_and_dense()) return false;
+    if (code < 0 || !t.is_cuda() || t.device() != h.device || t.layout() != at::kStrided || t.is_neg() || !t.is_non_overlapping_and_dense()) return false;
     g.p[i] = t.data_ptr(); g.n[i] = t.numel(); g.dt[i] = code;
     range[i] = {(char*)g.p[i], (char*)g.p[i] + t.nbytes()};
   }

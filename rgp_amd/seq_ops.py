@@ -96,7 +96,8 @@ def _rows(name, t, like, lead):
 
 
 def _inner(t, dims):
-    """The tensor with its last ``dims`` dimensions contiguous (a copy only where they are not)."""
+    """The tensor with its last ``dims`` dimensions contiguous (a copy only where they are not, or where its memory holds the negated values)."""
+    t = t.resolve_neg()
     if t.is_contiguous():
         return t
     shape, stride, want = t.shape, t.stride(), 1
@@ -146,13 +147,15 @@ def _param(name, t, shape, x, optional=False):
         _bad('%s has shape %s, %s expected' % (name, tuple(t.shape), tuple(shape)))
     if t.dtype is not _acc(x.dtype):
         _bad('%s is %s: parameters and states are %s for %s activations' % (name, t.dtype, _acc(x.dtype), x.dtype))
-    return t if t.is_contiguous() else t.contiguous()
+    return t.resolve_neg().contiguous()
 
 
 def _state(name, t, shape, dtype, x):
     """A state that is updated in place."""
     if not isinstance(t, torch.Tensor) or t.device != x.device or t.shape != shape or t.dtype is not dtype or not t.is_contiguous():
         _bad('%s must be a contiguous %s tensor of shape %s on %s' % (name, dtype, tuple(shape), x.device))
+    if t.is_neg():
+        _bad('%s is updated in place: its memory must hold its values (resolve_neg)' % name)
     if t.requires_grad:
         _bad('%s is updated in place and takes no gradient' % name)
 
@@ -194,7 +197,7 @@ def ssm_conv(handle, x, weight, bias=None, seqs=None, init=None, reverse=False, 
             shape = (n_seq, w.shape[1] - 1, x.shape[-1])
             if init.shape != shape or init.dtype is not x.dtype or init.device != x.device:
                 _bad('init must be %s of shape %s on %s' % (x.dtype, shape, x.device))
-            init = init.contiguous()
+            init = init.resolve_neg().contiguous()
         r = _again(_seq.conv(handle, x, w, b, seqs, init, bool(reverse), bool(return_state)), 'ssm_conv')
     return r if return_state else r[0]
 
@@ -308,6 +311,8 @@ def _bad_grads(handle, grads):
     for i, g in enumerate(grads):
         if not isinstance(g, torch.Tensor) or g.dtype not in _DTYPES or g.device != handle.device or g.layout is not torch.strided:
             _bad('gradient %d must be a float64, float32, bfloat16 or float16 tensor on %s' % (i, handle.device))
+        if g.is_neg():
+            _bad('gradient %d is clipped in place: its memory must hold its values (resolve_neg)' % i)
         if not g.is_contiguous() and g.numel() and (_overlaps(g) or sum((m - 1) * s for m, s in zip(g.shape, g.stride())) + 1 != g.numel()):
             _bad('gradient %d has gaps or repeats in memory: it cannot be clipped in place as one range' % i)
     _bad('two gradients share memory: each element may be clipped once')
@@ -334,5 +339,7 @@ def clip_grad_norm(handle, grads, max_norm, sumsq=None):
         if sumsq is not None and (not isinstance(sumsq, torch.Tensor) or sumsq.dtype is not torch.float64 or sumsq.numel() != 1 or
                                   sumsq.device != handle.device):
             _bad('sumsq must be one float64 value on %s' % handle.device)
+        if sumsq is not None and sumsq.is_neg():
+            return clip_grad_norm(handle, grads, max_norm, sumsq.resolve_neg())
         _bad_grads(handle, grads)
     return r

@@ -95,3 +95,35 @@ def test_recording_a_function_is_refused(h):
     with pytest.raises(RuntimeError, match='cannot be recorded'):
         make_fx(lambda g: torch.autograd.grad(out, leaf, g, retain_graph=True)[0])(torch.ones_like(out))
     assert all(torch.equal(a, b) for a, b in zip(_three(h, ops), plain))
+
+
+@pytest.mark.parametrize('D', [1, 5])
+def test_operands_with_a_pending_negation(h, D):
+    """The imaginary part of a conjugate is a view whose memory holds the negated values (one feature: also one that looks contiguous): operands
+    and gradients of that kind count by their values."""
+    from rgp_amd import seq_ops
+    g = torch.Generator().manual_seed(D)
+    f = lambda *s: torch.randn(*s, generator=g).cuda()                                          # noqa: E731
+    ops = dict(u=f(7, 2, D), delta=f(7, 2, D), A=-f(D, 1).abs(), B=f(7, 2, 1), C=f(7, 2, 1), D=f(D), z=f(7, 2, D), bias=f(D), init=f(2, D, 1), w=f(D, 4),
+               cinit=f(2, 3, D), n=f(D), r=f(7, 2, D), gy=f(7, 2, D))
+
+    def negated(t):
+        v = torch.complex(torch.zeros_like(t), -t).conj().imag
+        assert v.is_neg()
+        return v
+
+    def run(t):
+        leaf = {k: v if k in ('init', 'cinit', 'gy') else v.detach().requires_grad_(True) for k, v in t.items()}
+        y = seq_ops.ssm_scan(h, leaf['u'], leaf['delta'], leaf['A'], leaf['B'], leaf['C'], D=leaf['D'], z=leaf['z'], delta_bias=leaf['bias'], init=leaf['init'])
+        v = seq_ops.ssm_conv(h, leaf['u'], leaf['w'], leaf['bias'], init=leaf['cinit'])
+        n, hid = seq_ops.rms_norm(h, leaf['u'], leaf['n'], residual=leaf['r'])
+        grads = torch.autograd.grad((y, v, n, hid), [leaf[k] for k in ('u', 'delta', 'A', 'B', 'C', 'D', 'z', 'bias', 'w', 'n', 'r')], [leaf['gy']] * 4)
+        return [y, v, n, hid] + list(grads)
+
+    want = run(ops)
+    for k in list(ops) + ['all']:
+        got = run({q: negated(t) if k in (q, 'all') else t for q, t in ops.items()})
+        assert all(torch.equal(a.detach(), b.detach()) for a, b in zip(got, want)), k
+    two = torch.full((D,), 2.0, device='cuda')
+    total = negated(torch.full((1,), 16.0, device='cuda', dtype=F64))
+    assert float(seq_ops.clip_grad_norm(h, [two], 2.0, sumsq=total)) == 4.0 and torch.allclose(two, torch.ones_like(two), rtol=1e-6)

@@ -45,3 +45,20 @@ def test_recording_a_function_is_refused(name):
     with torch.no_grad():
         _refused(lambda: torch.jit.trace(lambda x: f(x, *ops[1:]), ops[0], check_trace=False), 'cannot be recorded')
         _refused(lambda: make_fx(lambda x: f(x, *ops[1:]))(ops[0]), 'cannot be recorded')
+
+
+def _negated(t):
+    """The values of ``t`` as the imaginary part of a conjugate: memory that holds them negated."""
+    v = torch.complex(torch.zeros_like(t), -t).conj().imag
+    assert v.is_neg() and torch.equal(v, t)
+    return v
+
+
+def test_in_place_operands_with_a_pending_negation_are_refused():
+    from rgp_amd import seq_ops
+    z = lambda *s: torch._neg_view(torch.zeros(*s))                         # noqa: E731
+    _refused(lambda: seq_ops.ssm_conv_step(H, torch.zeros(2, 6), torch.zeros(6, 4), None, z(2, 3, 6)), 'resolve_neg')
+    _refused(lambda: seq_ops.ssm_scan_step(H, torch.zeros(2, 6), torch.zeros(2, 6), torch.zeros(6, 3), torch.zeros(2, 3), torch.zeros(2, 3), None, z(2, 6, 3)),
+             'resolve_neg')
+    _refused(lambda: seq_ops.clip_grad_norm(H, [z(5)], 1.0), 'gradient 0 is clipped in place')
+    _refused(lambda: seq_ops.clip_grad_norm(H, [_negated(torch.ones(1))], 1.0), 'gradient 0 is clipped in place')
