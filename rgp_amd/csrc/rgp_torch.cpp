@@ -167,6 +167,7 @@ Tensor rows_of(const Tensor& g) {                    // a gradient as the kernel
   const Tensor t = g.is_neg() ? g.resolve_neg() : g;
   return inner(t, 1) ? t : t.contiguous();
 }
+Tensor whole(const Tensor& t) { return t.defined() ? (t.is_neg() ? t.resolve_neg() : t).contiguous() : t; }
 bool param(const Tensor& t, const Tensor& x, at::IntArrayRef shape) {
   return t.scalar_type() == acc_of(x.scalar_type()) && t.device() == x.device() && t.sizes() == shape && t.is_contiguous();
 }
@@ -242,6 +243,11 @@ struct OpNode : torch::autograd::Node {
         throw std::runtime_error("a captured backward pass cannot reach a leaf that a graph made outside the capture still holds: drop that graph first");
     }
   }
+  // What a graph saved may come back through the user's hooks (torch.autograd.graph.saved_tensors_hooks): in another memory order, which the passes
+  // lay out again, or as something else, which the kernels must not be given.
+  static void came_back(bool ok) {
+    if (!ok) throw std::runtime_error("a saved operand of the sequence operators came back with another type, shape or device");
+  }
   static void check(rgp_handle h, rgp_status st) {
     if (st != RGP_OK) throw std::runtime_error("librgp_hip status " + std::to_string((int)st) + ": " + lib.rgp_last_error(h));
   }
@@ -279,8 +285,10 @@ struct ConvNode : OpNode {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(3);
     if (!grads[0].defined()) return out;
-    const ConvOps c{x.unpack(), w.unpack(), b.unpack()};
-    const Tensor before = init.unpack(), gv = rows_of(grads[0]);
+    const ConvOps c{rows_of(x.unpack()), whole(w.unpack()), whole(b.unpack())};
+    const Tensor before = whole(init.unpack()), gv = rows_of(grads[0]);
+    came_back(like(c.x, gv) && c.x.sizes() == gv.sizes() && conv_ok(c) &&
+              (!before.defined() || (like(before, gv) && before.sizes() == at::IntArrayRef({geo.n_seq, c.w.size(1) - 1, c.x.size(-1)}))));
     rgp_ssm_conv a = conv_args(c, geo, reverse);
     out[0] = fresh(c.x); out[1] = fresh(c.w); out[2] = fresh(c.b);
     a.init = ptr(before); a.gv = gv.data_ptr(); a.gx = out[0].data_ptr(); a.gw = out[1].data_ptr(); a.gbias = ptr(out[2]);
@@ -377,6 +385,7 @@ struct ScanNode : OpNode {
   SavedVariable u, delta, A, B, C, skip, z, bias;
   Tensor states;
   int G = 1;
+  int64_t N = 0;
   std::string name() const override { return "SsmScanBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -388,8 +397,12 @@ struct ScanNode : OpNode {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(8);
     if (!grads[0].defined()) return out;
-    const ScanOps s{u.unpack(), delta.unpack(), A.unpack(), B.unpack(), C.unpack(), skip.unpack(), z.unpack(), bias.unpack()};
-    const Tensor gy = rows_of(grads[0]);
+    const Tensor zs = z.unpack(), gy = rows_of(grads[0]);
+    ScanOps s{rows_of(u.unpack()), rows_of(delta.unpack()), whole(A.unpack()), B.unpack(), C.unpack(), whole(skip.unpack()), zs.defined() ? rows_of(zs) : zs, whole(bias.unpack())};
+    for (Tensor* t : {&s.B, &s.C})
+      if (t->is_neg() || t->dim() <= geo.dims || !inner(*t, (int)t->dim() - geo.dims)) *t = whole(*t);
+    int groups = 0;
+    came_back(like(s.u, gy) && s.u.sizes() == gy.sizes() && scan_ok(s, geo.dims, groups) && groups == G && s.A.size(1) == N);
     rgp_ssm_scan a = scan_args(s, geo, G, reverse);
     const Tensor* in[8] = {&s.u, &s.delta, &s.A, &s.B, &s.C, &s.skip, &s.z, &s.bias};
     for (int i = 0; i < 8; ++i) out[i] = fresh(*in[i]);
@@ -433,7 +446,7 @@ PyObject* scan(PyObject* const* o) {
   if (train) {
     auto node = new_node<ScanNode>(h);
     node->set_next_edges(torch::autograd::collect_next_edges(s.u, s.delta, s.A, s.B, s.C, s.skip, s.z, s.bias));
-    node->geo = g; node->reverse = reverse; node->G = G; node->states = states;
+    node->geo = g; node->reverse = reverse; node->G = G; node->N = N; node->states = states;
     node->u = SavedVariable(s.u, false); node->delta = SavedVariable(s.delta, false); node->A = SavedVariable(s.A, false);
     node->B = SavedVariable(s.B, false); node->C = SavedVariable(s.C, false); node->skip = SavedVariable(s.skip, false);
     node->z = SavedVariable(s.z, false); node->bias = SavedVariable(s.bias, false);
@@ -499,8 +512,9 @@ struct RmsNode : OpNode {
       out[0] = out[2] = ghid;
       return out;
     }
-    const Tensor xs = x.unpack(of_hid ? shared_from_this() : nullptr), rs = residual.unpack(), ws = w.unpack();
+    const Tensor xs = rows_of(x.unpack(of_hid ? shared_from_this() : nullptr)), rs0 = residual.unpack(), rs = rs0.defined() ? rows_of(rs0) : rs0, ws = whole(w.unpack());
     const Tensor gy = rows_of(grads[0]), gh = ghid.defined() ? rows_of(ghid) : ghid;
+    came_back(like(xs, gy) && xs.sizes() == gy.sizes() && param(ws, gy, {gy.size(1)}) && (!rs.defined() || (like(rs, gy) && rs.sizes() == gy.sizes())));
     rgp_rms_norm a = rms_args(xs, rs, ws, eps);
     out[0] = fresh(xs); out[1] = fresh(ws);
     if (two) out[2] = out[0];

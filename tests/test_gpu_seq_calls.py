@@ -127,3 +127,39 @@ def test_operands_with_a_pending_negation(h, D):
     two = torch.full((D,), 2.0, device='cuda')
     total = negated(torch.full((1,), 16.0, device='cuda', dtype=F64))
     assert float(seq_ops.clip_grad_norm(h, [two], 2.0, sumsq=total)) == 4.0 and torch.allclose(two, torch.ones_like(two), rtol=1e-6)
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16], ids=str)
+def test_saved_operands_that_come_back_through_hooks(h, dtype):
+    """torch.autograd.graph's hooks may keep saved operands elsewhere: on the host, in another memory order -- the gradients are the same bits; as
+    another type or shape they are refused."""
+    from rgp_amd import seq_ops
+    g = torch.Generator().manual_seed(4)
+    acc = F32
+    f = lambda *s, t=dtype: torch.randn(*s, generator=g).to(t).cuda()                                   # noqa: E731
+    ops = dict(u=f(9, 2, 6), delta=f(9, 2, 6), A=-f(6, 3, t=acc).abs(), B=f(9, 2, 2, 3), C=f(9, 2, 2, 3), D=f(6, t=acc), z=f(9, 2, 6), bias=f(6, t=acc), w=f(6, 4, t=acc),
+               n=f(6, t=acc), x=f(5, 6), r=f(5, 6))
+    leaf = {k: v.requires_grad_(True) for k, v in ops.items()}
+    cinit, init, gy = f(2, 3, 6), f(2, 6, 3, t=acc), f(9, 2, 6)
+
+    def forward():
+        y = seq_ops.ssm_scan(h, leaf['u'], leaf['delta'], leaf['A'], leaf['B'], leaf['C'], D=leaf['D'], z=leaf['z'], delta_bias=leaf['bias'], init=init)
+        return y, seq_ops.ssm_conv(h, leaf['u'], leaf['w'], leaf['bias'], init=cinit), seq_ops.rms_norm(h, leaf['x'], leaf['n'], residual=leaf['r'])[0]
+
+    def backward(outs):
+        return torch.autograd.grad(outs, list(leaf.values()), [gy, gy, gy[:5, 0].contiguous()])
+    want = backward(forward())
+    turned = lambda t: t.transpose(0, -1).contiguous().transpose(0, -1)                                 # noqa: E731
+    for pack, unpack in ((lambda t: t.cpu(), lambda t: t.cuda()), (lambda t: t, turned), (lambda t: t, lambda t: torch._neg_view(-t))):
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            outs = forward()
+        assert all(torch.equal(a, b) for a, b in zip(backward(outs), want))
+    with torch.autograd.graph.save_on_cpu():
+        outs = forward()
+    assert all(torch.equal(a, b) for a, b in zip(backward(outs), want))
+    for unpack in (lambda t: t.double(), lambda t: t[:1], lambda t: t[..., :2], lambda t: t.cpu()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            outs = forward()
+        for o in outs:
+            with pytest.raises(RuntimeError, match='came back'):
+                torch.autograd.grad(o.sum(), list(leaf.values()), allow_unused=True)
