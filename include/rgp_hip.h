@@ -87,6 +87,8 @@ typedef struct {
 /* ---- lifecycle --------------------------------------------------------------------------------------------- */
 rgp_status rgp_create(rgp_handle* out, int device, void* hip_stream);
 void       rgp_destroy(rgp_handle h);
+/* Message of the calling thread's last failed call on the handle, or, if it had none there, of the latest one of any thread.  Valid until the
+ * thread's next call of the library. */
 const char* rgp_last_error(rgp_handle h);
 int        rgp_abi_version(void);
 /* Blocks until the handle's stream is idle; returns RGP_ERR_NOT_PD / RGP_ERR_HIP if any step since the last call

@@ -2,6 +2,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <mutex>
 #include <string>
 #include <vector>
 
@@ -63,7 +64,9 @@ static inline int rgp_qp(int Q) { return (Q > 16 && Q <= 20) ? 20 : round_up(Q, 
 struct rgp_ctx {
   int device = 0;
   hipStream_t stream = nullptr;
-  std::string err;
+  std::string err;                   // the last failure's message, under err_lock; a thread's own is kept beside it (rgp_fail)
+  std::mutex err_lock;
+  uint64_t serial = 0;               // never given twice, as an address may be
   // workspace (grown on demand, never shrunk).  Layer steps alternate between two slots so that the M x M chain of one
   // layer (side streams) can overlap the psi passes of the next layer (main stream).
   char* ws = nullptr;

@@ -3,6 +3,8 @@
 #include <stdio.h>
 #include <stdlib.h>
 
+#include <atomic>
+
 #include "rgp_chain.h"
 #include "rgp_gemm.h"
 #include "rgp_psi.h"
@@ -38,8 +40,21 @@ static hipError_t static_scratch_lookup(int device, char** out) {
 // ==================================================================================================================
 // handle
 // ==================================================================================================================
+// Threads that share a handle may fail at the same time: each finds the message of its own failure, and one that had none a copy of the latest.
+static std::atomic<uint64_t> g_serial{0};
+struct LastError {
+  uint64_t serial = 0;
+  std::string own, latest;
+};
+static thread_local LastError t_error;
+
 rgp_status rgp_fail(rgp_handle h, rgp_status code, const std::string& msg) {
-  if (h) h->err = msg;
+  if (h) {
+    t_error.own = msg;
+    t_error.serial = h->serial;
+    std::lock_guard<std::mutex> lock(h->err_lock);
+    h->err = msg;
+  }
   return code;
 }
 
@@ -152,6 +167,7 @@ extern "C" void rgp_destroy(rgp_handle h);
 extern "C" rgp_status rgp_create(rgp_handle* out, int device, void* hip_stream) {
   if (!out) return RGP_ERR_BAD_ARG;
   rgp_ctx* h = new rgp_ctx();
+  h->serial = ++g_serial;
   h->device = device;
   h->stream = (hipStream_t)hip_stream;
   if (hipSetDevice(device) != hipSuccess) { delete h; return RGP_ERR_HIP; }
@@ -207,7 +223,13 @@ extern "C" void rgp_destroy(rgp_handle h) {
   delete h;
 }
 
-extern "C" const char* rgp_last_error(rgp_handle h) { return h ? h->err.c_str() : "null handle"; }
+extern "C" const char* rgp_last_error(rgp_handle h) {
+  if (!h) return "null handle";
+  if (t_error.serial == h->serial) return t_error.own.c_str();
+  std::lock_guard<std::mutex> lock(h->err_lock);
+  t_error.latest = h->err;
+  return t_error.latest.c_str();
+}
 
 extern "C" rgp_status rgp_sync_status(rgp_handle h, int* pivot) {
   if (!h) return RGP_ERR_BAD_ARG;

@@ -163,3 +163,49 @@ def test_saved_operands_that_come_back_through_hooks(h, dtype):
         for o in outs:
             with pytest.raises(RuntimeError, match='came back'):
                 torch.autograd.grad(o.sum(), list(leaf.values()), allow_unused=True)
+
+
+def test_threads_that_fail_at_once_read_their_own_messages(h):
+    """Refusals from several threads on one handle (the library is entered without the interpreter's lock): every thread finds the message of
+    its own call, and a thread without a failure a whole one."""
+    import ctypes as C
+    import threading
+    from rgp_amd import _lib
+    from rgp_amd.capi import Handle
+    other = Handle()
+    calls = []
+    for entry, struct in (('rgp_ssm_scan_forward', _lib.SsmScan), ('rgp_ssm_scan_step', _lib.SsmScan), ('rgp_ssm_conv_forward', _lib.SsmConv),
+                          ('rgp_ssm_conv_step', _lib.SsmConv), ('rgp_rms_norm_forward', _lib.RmsNorm), ('rgp_rms_norm_backward', _lib.RmsNorm)):
+        for dtype in (-1, 0):                                       # an unknown type, an empty problem
+            a = struct()
+            a.dtype = dtype
+            if struct is _lib.RmsNorm:
+                a.rows = -1 if dtype == 0 else 0
+            fn = getattr(h.lib, entry)
+            assert fn(other.h, None, C.byref(a)) == _lib.RGP_ERR_BAD_ARG
+            calls.append((fn, a, other.lib.rgp_last_error(other.h)))
+    assert len({m for _, _, m in calls}) == len(calls) and all(len(m) > 16 for _, _, m in calls)         # longer than a string holds in place
+    wrong, start = [], threading.Barrier(len(calls) + 1)
+
+    def run(fn, a, want):
+        start.wait()
+        for _ in range(2000):
+            if fn(h.h, None, C.byref(a)) != _lib.RGP_ERR_BAD_ARG or h.lib.rgp_last_error(h.h) != want:
+                wrong.append(want)
+
+    def read():
+        start.wait()
+        for _ in range(2000):
+            if h.lib.rgp_last_error(h.h) not in messages:
+                wrong.append(b'reader')
+    first = calls[0]
+    assert first[0](h.h, None, C.byref(first[1])) == _lib.RGP_ERR_BAD_ARG
+    messages = {m for _, _, m in calls}
+    threads = [threading.Thread(target=run, args=c) for c in calls] + [threading.Thread(target=read)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:3]
+    fresh = Handle()
+    assert fresh.lib.rgp_last_error(fresh.h) == b''                 # whatever address it has
