@@ -309,7 +309,9 @@ rgp_status rgp_rnn_scan_backward(rgp_handle h, const rgp_rnn_scan* a);
  *          ELEMENTS, features contiguous), outputs are contiguous [T][n_seq][features].  off != NULL: packed rows, sequence s is rows
  *          off[s] .. off[s+1] (device int64[n_seq + 1], increasing, off[0] = 0, off[n_seq] <= rows; lengths of 0 are allowed), step t
  *          at base + (off[s] + t) * st, outputs contiguous [rows][features]; rows behind off[n_seq] are neither read nor written.  max_len: the longest sequence (a hint for the split
- *          over time; any value is safe).  reverse != 0 walks every sequence from its last step to its first. */
+ *          over time; any value is safe).  reverse != 0 walks every sequence from its last step to its first.
+ *   Memory No output may share memory with an operand or another output; last and init of whole sequences are checked, and one and the
+ *          same only in the single-step forms. */
 enum { RGP_F64 = 0, RGP_F32 = 1, RGP_BF16 = 2, RGP_F16 = 3 };
 
 /* Selective state-space scan.  Per step, channel d < D, state n < N, group g = d / (D / G) of B and C:

@@ -247,6 +247,9 @@ static inline rgp_status seq_launched(rgp_handle h, const char* what) {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? RGP_OK : rgp_fail(h, RGP_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
 }
+static inline bool seq_overlap(const void* a, const void* b, int64_t bytes) {                // two buffers of that size
+  return a && b && (uintptr_t)a < (uintptr_t)b + bytes && (uintptr_t)b < (uintptr_t)a + bytes;
+}
 static inline int seq_dtype_bytes(int dt) { return dt == RGP_F64 ? 8 : dt == RGP_F32 ? 4 : 2; }
 static inline bool seq_aligned(const void* p, int64_t stride, int elem, int v) {        // for vectors of v elements
   return (uintptr_t)p % (v * elem) == 0 && stride % v == 0;

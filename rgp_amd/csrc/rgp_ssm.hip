@@ -290,6 +290,9 @@ static rgp_status scan_run(rgp_handle h, hipStream_t s, const rgp_ssm_scan* a, b
   const bool some = a->rows > 0;                       // without rows the activations may have no memory
   if (!a->A || (some && (!a->u || !a->delta || !a->B || !a->C))) return rgp_fail(h, RGP_ERR_BAD_ARG, std::string(what) + "u, delta, A, B and C are required");
   if (!back && some && !a->y) return rgp_fail(h, RGP_ERR_BAD_ARG, std::string(what) + "y is required");
+  // every block of time may read init while the last one writes last
+  if (!back && seq_overlap(a->last, a->init, (int64_t)a->n_seq * a->D * a->N * (a->dtype == RGP_F64 ? 8 : 4)))
+    return rgp_fail(h, RGP_ERR_BAD_ARG, std::string(what) + "last must not share memory with init");
   if (back && (!a->gA || (some && (!a->gy || !a->states || !a->gu || !a->gdelta || !a->gB || !a->gC || (a->z && !a->gz)))))
     return rgp_fail(h, RGP_ERR_BAD_ARG, std::string(what) + "gy, states and the gradients' buffers are required");
   ScanPlan p;
@@ -771,7 +774,8 @@ static rgp_status conv_run(rgp_handle h, hipStream_t s, const rgp_ssm_conv* a, i
   if (what == CONV_STEP && (a->off || a->T != 1)) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "one row per sequence (T = 1, no offsets)");
   if (what == CONV_STEP && (!a->v || !a->last || a->init != a->last)) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "v and the state (init = last) are required");
   if (what == CONV_FWD && some && !a->v) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "v is required");
-  if (what == CONV_FWD && a->last && a->last == a->init) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "last must not be init");
+  if (what == CONV_FWD && seq_overlap(a->last, a->init, (int64_t)a->n_seq * (a->W - 1) * a->D * seq_dtype_bytes(a->dtype)))
+    return rgp_fail(h, RGP_ERR_BAD_ARG, name + "last must not share memory with init");
   const bool wide = what == CONV_STEP ? a->D % CONV_V == 0 : a->D >= CONV_V;      // a step changes its state in place: no channel twice
   ConvDev d;
   int64_t nrb, nvb;

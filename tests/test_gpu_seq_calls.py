@@ -209,3 +209,55 @@ def test_threads_that_fail_at_once_read_their_own_messages(h):
     assert not wrong, wrong[:3]
     fresh = Handle()
     assert fresh.lib.rgp_last_error(fresh.h) == b''                 # whatever address it has
+
+
+def test_states_of_whole_sequences_must_not_share_memory(h):
+    """The C entries for whole sequences refuse a final state that overlaps the initial one (blocks of time run at once); buffers side by side
+    are taken, and give what two allocations give."""
+    import ctypes as C
+    from rgp_amd import _lib
+    T, n, D, N, W = 200, 2, 6, 3, 4
+    g = torch.Generator().manual_seed(5)
+    f = lambda *s: torch.randn(*s, generator=g).cuda()                                         # noqa: E731
+    x, delta, B, Cm, A, w = f(T, n, D), f(T, n, D), f(T, n, N), f(T, n, N), -f(D, N).abs(), f(D, W)
+    st = torch.cuda.current_stream().cuda_stream
+
+    def scan(buf, init, last):
+        a = _lib.SsmScan()
+        a.dtype, a.n_seq, a.D, a.N, a.G, a.T, a.rows, a.max_len = _lib.DT_F32, n, D, N, 1, T, T * n, T
+        y = torch.empty_like(x)
+        for k, t in dict(u=x, delta=delta, B=B, C=Cm, A=A, y=y).items():
+            setattr(a, k, t.data_ptr())
+        a.u_st = a.delta_st = n * D
+        a.u_sb = a.delta_sb = D
+        a.B_st = a.C_st = n * N
+        a.B_sb = a.C_sb = N
+        work = torch.empty(h.lib.rgp_ssm_scan_workspace(C.byref(a), 0), dtype=torch.uint8, device='cuda')
+        assert work.numel() > 0                                     # split over time: the case in which blocks read init while another writes last
+        a.work, a.work_bytes = work.data_ptr(), work.numel()
+        a.init, a.last = buf.data_ptr() + 4 * init, buf.data_ptr() + 4 * last
+        r = h.lib.rgp_ssm_scan_forward(h.h, st, C.byref(a))
+        torch.cuda.synchronize()
+        return r
+
+    def conv(buf, init, last):
+        c = _lib.SsmConv()
+        c.dtype, c.n_seq, c.D, c.W, c.T, c.rows, c.max_len = _lib.DT_F32, n, D, W, T, T * n, T
+        v = torch.empty_like(x)
+        for k, t in dict(x=x, w=w, v=v).items():
+            setattr(c, k, t.data_ptr())
+        c.x_st, c.x_sb = n * D, D
+        c.init, c.last = buf.data_ptr() + 4 * init, buf.data_ptr() + 4 * last
+        r = h.lib.rgp_ssm_conv_forward(h.h, st, C.byref(c))
+        torch.cuda.synchronize()
+        return r
+    for call, size in ((scan, n * D * N), (conv, n * (W - 1) * D)):
+        start = f(size)
+        for init, last in ((0, 0), (0, 1), (1, 0), (0, size - 1), (size - 1, 0)):
+            buf = torch.cat((start, start))
+            keep = buf.clone()
+            assert call(buf, init, last) == _lib.RGP_ERR_BAD_ARG and b'share memory' in h.lib.rgp_last_error(h.h)
+            assert torch.equal(buf, keep)
+        one, two = torch.cat((start, start)), torch.cat((start, start, start))
+        assert call(one, 0, size) == 0 and call(two, 0, 2 * size) == 0
+        assert torch.equal(one[size:], two[2 * size:]) and torch.equal(one[:size], start) and not torch.equal(one[size:], start)
