@@ -310,8 +310,9 @@ static rgp_status scan_run(rgp_handle h, hipStream_t s, const rgp_ssm_scan* a, b
   d.pD = take(p.pD_bytes);
   d.pBC = take(p.pBC_bytes);
   const int64_t DN = (int64_t)a->D * a->N;
-  const int64_t join = (int64_t)a->n_seq * (p.Q == 1 ? (DN + 255) / 256 : (DN + 63) / 64);
-  if ((double)d.nslot * p.sh.CH * p.sh.K > 4294967295.0 || (int64_t)a->G * d.ncb > 65535 || seq_blocks(d.g, SSM_CK_LG) > 4294967295 || (double)join * 1024 > 4294967295.0)
+  const int64_t join = p.split && !d.join ? (int64_t)a->n_seq * (p.Q == 1 ? (DN + 255) / 256 : (DN + 63) / 64) : 0;      // workgroups, where it is a launch
+  const double join_threads = (double)join * (p.Q == 1 ? 256 : p.Q * 64);
+  if ((double)d.nslot * p.sh.CH * p.sh.K > 4294967295.0 || (int64_t)a->G * d.ncb > 65535 || seq_blocks(d.g, SSM_CK_LG) > 4294967295 || join_threads > 4294967295.0)
     return rgp_fail(h, RGP_ERR_BAD_ARG, std::string(what) + "more than 2^32 work items");
   hipError_t err = hipSuccess;
   if (d.nslot > 0) {
