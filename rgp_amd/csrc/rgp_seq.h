@@ -214,10 +214,11 @@ static __device__ __forceinline__ int64_t seq_row_index(const SeqGeo& g, const S
 // out[i] = sum over p < P of part[p * stride + i], i < n, rounded to type dt; up to five such sums in one launch, each in a fixed order (no
 // atomics: results do not depend on timing).  turn > 1: the partials are [turn][n / turn], out is [n / turn][turn].  end: outputs from
 // end[0] * per on stay as they are (rows behind the last packed sequence, whose partials nobody wrote).
-struct SeqSum { void* part; int64_t P, stride, n; void* out; int dt, turn, block0; const int64_t* end; int64_t per; };
+struct SeqSum { void* part; int64_t P, stride, n; void* out; int dt, turn; int64_t block0; const int64_t* end; int64_t per; };
 struct SeqSums {
   SeqSum job[5];
-  int count = 0, blocks = 0;
+  int count = 0;
+  int64_t blocks = 0;              // workgroups' worth of outputs
   void add(void* part, int64_t P, int64_t stride, int64_t n, void* out, int dt, int turn = 1, const int64_t* end = nullptr, int64_t per = 0);
   rgp_status run(rgp_handle h, hipStream_t s, int acc);
 };

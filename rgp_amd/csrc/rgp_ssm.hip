@@ -12,6 +12,7 @@
 #define SEQ_FEW 32
 #define SEQ_MANY 512
 #define SEQ_HUGE 8192
+#define SEQ_SUMS_GRID 65536          // workgroups of a launch, which go on to further outputs (a launch holds fewer than 2^32 threads)
 static __host__ __device__ inline int64_t seq_sums_width(int64_t P) { return P <= SEQ_FEW ? 1024 : P <= SEQ_MANY ? 64 : 16; }
 template <typename A>
 static __device__ __forceinline__ void seq_sums_store(const SeqSum& j, int64_t i, A v) {
@@ -26,51 +27,54 @@ static __device__ __forceinline__ void seq_sums_store(const SeqSum& j, int64_t i
 template <typename A>
 static __global__ void __launch_bounds__(1024) seq_sums_kernel(SeqSums g) {
   __shared__ A sh[1024];
-  int k = 0;
-  while (k + 1 < g.count && (int)blockIdx.x >= g.job[k + 1].block0) ++k;
-  const SeqSum& j = g.job[k];
-  const A* const part = (const A*)j.part;
-  const int64_t o0 = (int64_t)((int)blockIdx.x - j.block0) * seq_sums_width(j.P);
-  int64_t n = j.n;
-  if (j.end && j.end[0] * j.per < n) n = j.end[0] < 0 ? 0 : j.end[0] * j.per;
-  if (j.P <= SEQ_FEW) {                                  // uniform over the workgroup
-    const int64_t i = o0 + threadIdx.x;
-    if (i < n) {
-      A v = (A)0;
+  for (int64_t at = blockIdx.x; at < g.blocks; at += gridDim.x) {
+    int k = 0;
+    while (k + 1 < g.count && at >= g.job[k + 1].block0) ++k;
+    const SeqSum& j = g.job[k];
+    const A* const part = (const A*)j.part;
+    const int64_t o0 = (at - j.block0) * seq_sums_width(j.P);
+    int64_t n = j.n;
+    if (j.end && j.end[0] * j.per < n) n = j.end[0] < 0 ? 0 : j.end[0] * j.per;
+    if (j.P <= SEQ_FEW) {                                  // uniform over the workgroup
+      const int64_t i = o0 + threadIdx.x;
+      if (i < n) {
+        A v = (A)0;
 #pragma unroll 8
-      for (int64_t p = 0; p < j.P; ++p) v += part[p * j.stride + i];
+        for (int64_t p = 0; p < j.P; ++p) v += part[p * j.stride + i];
+        seq_sums_store(j, i, v);
+      }
+      continue;
+    }
+    const int W = (int)seq_sums_width(j.P), Q = 1024 / W, G = W == 64 ? 4 : 8, l = threadIdx.x % W, q = threadIdx.x / W;       // Q = G G
+    const int64_t i = o0 + l;
+    A v8[8] = {};
+    if (i < n) {
+      const A* p = part + q * j.stride + i;
+      int64_t left = j.P > q ? (j.P - q + Q - 1) / Q : 0;
+      const int64_t step = Q * j.stride;
+      for (; left >= 8; left -= 8, p += 8 * step) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v8[u] += p[u * step];
+      }
+#pragma unroll
+      for (int u = 0; u < 7; ++u)
+        if (u < left) v8[u] += p[u * step];
+    }
+    __syncthreads();                                       // the outputs before these are out of sh
+    sh[threadIdx.x] = ((v8[0] + v8[1]) + (v8[2] + v8[3])) + ((v8[4] + v8[5]) + (v8[6] + v8[7]));
+    __syncthreads();
+    A v = (A)0;
+    if (q < G) {                                            // G groups of G threads' sums
+      v = sh[q * G * W + l];
+      for (int r = 1; r < G; ++r) v += sh[(q * G + r) * W + l];
+    }
+    __syncthreads();
+    if (q < G) sh[q * W + l] = v;
+    __syncthreads();
+    if (q == 0 && i < n) {
+      for (int r = 1; r < G; ++r) v += sh[r * W + l];
       seq_sums_store(j, i, v);
     }
-    return;
-  }
-  const int W = (int)seq_sums_width(j.P), Q = 1024 / W, G = W == 64 ? 4 : 8, l = threadIdx.x % W, q = threadIdx.x / W;       // Q = G G
-  const int64_t i = o0 + l;
-  A v8[8] = {};
-  if (i < n) {
-    const A* p = part + q * j.stride + i;
-    int64_t left = j.P > q ? (j.P - q + Q - 1) / Q : 0;
-    const int64_t step = Q * j.stride;
-    for (; left >= 8; left -= 8, p += 8 * step) {
-#pragma unroll
-      for (int u = 0; u < 8; ++u) v8[u] += p[u * step];
-    }
-#pragma unroll
-    for (int u = 0; u < 7; ++u)
-      if (u < left) v8[u] += p[u * step];
-  }
-  sh[threadIdx.x] = ((v8[0] + v8[1]) + (v8[2] + v8[3])) + ((v8[4] + v8[5]) + (v8[6] + v8[7]));
-  __syncthreads();
-  A v = (A)0;
-  if (q < G) {                                            // G groups of G threads' sums
-    v = sh[q * G * W + l];
-    for (int r = 1; r < G; ++r) v += sh[(q * G + r) * W + l];
-  }
-  __syncthreads();
-  if (q < G) sh[q * W + l] = v;
-  __syncthreads();
-  if (q == 0 && i < n) {
-    for (int r = 1; r < G; ++r) v += sh[r * W + l];
-    seq_sums_store(j, i, v);
   }
 }
 template <typename A>
@@ -106,10 +110,11 @@ rgp_status SeqSums::run(rgp_handle h, hipStream_t s, int acc) {
   blocks = 0;
   for (int k = 0; k < count; ++k) {
     job[k].block0 = blocks;
-    blocks += (int)((job[k].n + seq_sums_width(job[k].P) - 1) / seq_sums_width(job[k].P));
+    blocks += (job[k].n + seq_sums_width(job[k].P) - 1) / seq_sums_width(job[k].P);
   }
-  if (acc == RGP_F64) hipLaunchKernelGGL(seq_sums_kernel<double>, dim3(blocks), dim3(1024), 0, s, *this);
-  else hipLaunchKernelGGL(seq_sums_kernel<float>, dim3(blocks), dim3(1024), 0, s, *this);
+  const dim3 grid((unsigned)(blocks < SEQ_SUMS_GRID ? blocks : SEQ_SUMS_GRID));
+  if (acc == RGP_F64) hipLaunchKernelGGL(seq_sums_kernel<double>, grid, dim3(1024), 0, s, *this);
+  else hipLaunchKernelGGL(seq_sums_kernel<float>, grid, dim3(1024), 0, s, *this);
   return seq_launched(h, "sum of partial results");
 }
 

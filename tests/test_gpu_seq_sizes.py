@@ -4,6 +4,9 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
+import seq_batched
+import seq_reference as ref
+
 F64, F32, BF16, F16 = torch.float64, torch.float32, torch.bfloat16, torch.float16
 
 
@@ -35,4 +38,37 @@ def test_many_sequences_of_many_channels(h):
         small = run([t[:, s] for t in acts])
         assert torch.equal(big[0][s], small[0])
         assert all(torch.equal(a[:, s], b) for a, b in zip(big[1:], small[1:]))
+    torch.cuda.empty_cache()
+
+
+def _compare(h, acts, par, init, reverse=False, size=None, spare=0):
+    """Scan of (T, n, ..) activations forward and backward against the batched 64-bit form."""
+    from rgp_amd import seq_ops
+    names = [('gu', 'u'), ('gdelta', 'delta'), ('gB', 'B'), ('gC', 'Cm'), ('gz', 'z'), ('gA', 'A'), ('gD', 'D'), ('gbias', 'bias')]
+    leaf = {k: v.detach().requires_grad_(True) for k, v in list(acts.items()) + list(par.items()) if k != 'gy' and v is not None}
+    y, last = seq_ops.ssm_scan(h, leaf['u'], leaf['delta'], leaf['A'], leaf['B'], leaf['Cm'], D=leaf.get('D'), z=leaf.get('z'), delta_bias=leaf.get('bias'),
+                               init=init, reverse=reverse, return_state=True)
+    names = [(g, k) for g, k in names if k in leaf]
+    got = dict(zip([g for g, _ in names], torch.autograd.grad(y, [leaf[k] for _, k in names], acts['gy'])))
+    got.update(y=y, last=last)
+    T, n, Dn = acts['u'].shape
+    G, N = acts['B'].shape[2:]
+    want = seq_batched.scan_in_chunks(size or n, **acts, **par, init=init, reverse=reverse)
+    acc = ref.acc_of(acts['u'].dtype)
+    for k, t in got.items():                       # 8 roundings a step, the additions over states, channels and (parameters only) rows, 64 elementwise
+        ref.check(k, t, *want[k], ops=8 * T + N + Dn // G + 64 + (T * n if k in ('gA', 'gD', 'gbias') else 0), acc=acc)
+
+
+def _inputs(seed, T, n, D, N, G=1, dtype=F32, z=True, carry=True):
+    acc = ref.acc_of(dtype)
+    acts = dict(u=_randn(seed, T, n, D, dtype=dtype), delta=_randn(seed + 1, T, n, D, dtype=dtype), B=_randn(seed + 2, T, n, G, N, dtype=dtype),
+                Cm=_randn(seed + 3, T, n, G, N, dtype=dtype), z=_randn(seed + 4, T, n, D, dtype=dtype) if z else None, gy=_randn(seed + 5, T, n, D, dtype=dtype))
+    par = dict(A=-torch.exp(_randn(seed + 6, D, N)).to(acc), D=_randn(seed + 7, D).to(acc), bias=_randn(seed + 8, D).to(acc) - 2)
+    return acts, par, _randn(seed + 9, n, D, N).to(acc) if carry else None
+
+
+def test_more_sums_over_channels_than_a_launch_has_workgroups(h):
+    """gB and gC of 65544 rows, 64 states and 33 workgroups of channels: 131082 workgroups' worth of sums, twice what a launch takes at once."""
+    acts, par, init = _inputs(20, 8, 8193, 520, 64)
+    _compare(h, acts, par, init, size=1024)
     torch.cuda.empty_cache()
