@@ -370,7 +370,7 @@ rgp_status rgp_ssm_conv_step(rgp_handle h, void* stream, const rgp_ssm_conv* a);
 /* Root-mean-square norm of x + residual over the last dimension, per row:
  *     hid = x + residual;  y = hid * r * w,  r = (mean(hid^2) + eps)^(-1/2)
  * x, residual (NULL = 0), y, hid [rows][C] dtype (row strides in elements; y, hid contiguous; hid NULL iff residual is), w [C] acc,
- * rstd [rows] acc (NULL: not wanted; the backward call reads it); rows < 2^24.  Backward: gy, ghid (NULL = 0) -> gx [rows][C] (the gradient of x and
+ * rstd [rows] acc (NULL: not wanted; the backward call reads it); rows and C up to 2^40.  Backward: gy, ghid (NULL = 0) -> gx [rows][C] (the gradient of x and
  * of residual alike), gw [C] acc; x and residual are the forward call's (or x = hid and no residual: the same up to hid's rounding). */
 typedef struct rgp_rms_norm {
   int32_t dtype, reserved;

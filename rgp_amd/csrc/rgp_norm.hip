@@ -286,6 +286,7 @@ static const char* rms_bad(const rgp_rms_norm* a) {
   if (!a) return "null arguments";
   if (a->dtype < 0 || a->dtype > 3) return "dtype must be RGP_F64, RGP_F32, RGP_BF16 or RGP_F16";
   if (a->rows < 0 || a->C < 1) return "empty rows";
+  if (a->rows > SEQ_MOST || a->C > SEQ_MOST) return "more than 2^40 rows or columns";
   if (!(a->dtype == RGP_F64 ? a->eps > 0.0 : (float)a->eps > 0.0f)) return "eps must be positive in the arithmetic type";
   return nullptr;
 }
@@ -344,10 +345,11 @@ static rgp_status rms_run(rgp_handle h, hipStream_t s, const rgp_rms_norm* a, bo
   if (!a->w || (back && !a->gw) || (a->rows > 0 && (!a->x || (!back && !a->y) || (back && (!a->gy || !a->gx || !a->rstd)))))
     return rgp_fail(h, RGP_ERR_BAD_ARG, name + "a required buffer is null");
   if (!back && a->rows > 0 && (a->residual != nullptr) != (a->hid != nullptr)) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "residual and hid go together");
-  if (a->rows > 16777215) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "more than 2^24 - 1 rows");
   NormDev d{};
   d.a = *a;
   const RmsShape sh = rms_shape(a);
+  // a workgroup a row; more of such rows would fill over 500 GB
+  if (!back && !sh.tpr && a->rows > 16777215) return rgp_fail(h, RGP_ERR_BAD_ARG, name + "more than 2^24 - 1 rows of more than 32 KB");
   const int64_t blocks = back ? rms_bwd_blocks(a, sh) : rms_blocks(a, sh, RMS_FWD_BLOCKS);
   if (back && (rgp_rms_norm_workspace(a, 1) > a->work_bytes || !a->work || ((uintptr_t)a->work & 15)))
     return rgp_fail(h, RGP_ERR_WORKSPACE, name + "work buffer too small or not 16-byte aligned");

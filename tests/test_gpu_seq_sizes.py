@@ -72,3 +72,25 @@ def test_more_sums_over_channels_than_a_launch_has_workgroups(h):
     acts, par, init = _inputs(20, 8, 8193, 520, 64)
     _compare(h, acts, par, init, size=1024)
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize('rows,C', [((1 << 24) + 5, 2), ((1 << 24) + 5, 9), (5000, 16400)])
+def test_norms_of_many_rows(h, rows, C):
+    """More rows than 2^24: the values and gradients of the rows' own formula."""
+    from rgp_amd import seq_ops
+    x, r, gy, gh = (_randn(i, rows, C, dtype=BF16) for i in range(4))
+    w = _randn(5, C)
+    leaf = [t.detach().requires_grad_(True) for t in (x, r, w)]
+    y, hid = seq_ops.rms_norm(h, leaf[0], leaf[2], residual=leaf[1])
+    gx, gr, gw = torch.autograd.grad((y, hid), leaf, (gy, gh))
+    assert torch.equal(gx, gr)
+    gw64, gwm = torch.zeros(C, dtype=F64), torch.zeros(C, dtype=F64)
+    ops = C + 64                                                  # the additions over a row
+    for c in seq_batched.chunks(rows, max(1, (1 << 23) // C)):
+        want = ref.rms(x[c].double(), r[c].double(), w.double(), 1e-6, gy[c].double(), gh[c].double())
+        for k, t in (('y', y), ('hid', hid), ('gx', gx)):
+            ref.check(k, t[c], *(v.cpu() for v in want[k]), ops=ops, acc=F32)
+        gw64 += want['gw'][0].cpu()
+        gwm += want['gw'][1].cpu()
+    ref.check('gw', gw, gw64, gwm, ops=ops + rows, acc=F32)
+    torch.cuda.empty_cache()

@@ -62,3 +62,13 @@ def test_in_place_operands_with_a_pending_negation_are_refused():
              'resolve_neg')
     _refused(lambda: seq_ops.clip_grad_norm(H, [z(5)], 1.0), 'gradient 0 is clipped in place')
     _refused(lambda: seq_ops.clip_grad_norm(H, [_negated(torch.ones(1))], 1.0), 'gradient 0 is clipped in place')
+
+
+def test_the_norm_takes_as_many_rows_as_the_scan():
+    import ctypes as C
+    from rgp_amd import _lib
+    r = _lib.RmsNorm()
+    r.dtype, r.C, r.eps = _lib.DT_BF16, 40, 1e-6
+    for rows, ok in ((1 << 24, True), (1 << 40, True), ((1 << 40) + 1, False)):
+        r.rows = rows
+        assert (_lib.load().rgp_rms_norm_workspace(C.byref(r), 1) > 0) == ok
