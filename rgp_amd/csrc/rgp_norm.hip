@@ -461,13 +461,16 @@ static __global__ void __launch_bounds__(1024) grad_total_kernel(const double* p
 template <typename T>
 static __device__ __forceinline__ void grad_scale(T* p, int64_t n, double c) {
   typedef typename SeqAcc<T>::type A;
-  const A f = (A)c;
-  grad_walk(p, n, [&](T* q, int k, bool wide) {
-    SeqVec<T> v = seq_load((const T*)q, k, wide);
+  auto each = [&](auto f) {
+    grad_walk(p, n, [&](T* q, int k, bool wide) {
+      SeqVec<T> v = seq_load((const T*)q, k, wide);
 #pragma unroll
-    for (int i = 0; i < SeqVec<T>::V; ++i) v.e[i] = (T)((A)v.e[i] * f);
-    seq_store(q, v, k, wide);
-  });
+      for (int i = 0; i < SeqVec<T>::V; ++i) v.e[i] = (T)(A)((A)v.e[i] * f);
+      seq_store(q, v, k, wide);
+    });
+  };
+  if (sizeof(A) == 4 && c < 1.17549435082228751e-38) each(c);      // below the normal numbers of 32 bits the factor itself would be rounded away
+  else each((A)c);
 }
 // sum: nsum places to add (1: the sum itself).  Walks tensors and pieces from the last to the first: what the norm read last is still in the
 // memory-side cache.  The first workgroup of the launch that says so writes the norm.

@@ -94,3 +94,21 @@ def test_norms_of_many_rows(h, rows, C):
         gwm += want['gw'][1].cpu()
     ref.check('gw', gw, gw64, gwm, ops=ops + rows, acc=F32)
     torch.cuda.empty_cache()
+
+
+def test_clipping_by_a_factor_below_the_normal_numbers(h):
+    """Gradients near the end of the 32-bit range, and 32-bit gradients beside fp64 ones that are larger still: the factor is not one of 32 bits."""
+    from rgp_amd import seq_ops
+    for big, most in ((3e38, 1e-3), (1e39, 1.0), (1e70, 1e30)):
+        f32, b16 = (torch.linspace(lo, 3e38, n, device='cuda', dtype=F64).to(t) for lo, n, t in ((-3e38, 1003, F32), (1e36, 777, BF16)))
+        f64 = torch.full((33,), big, device='cuda', dtype=F64)
+        grads = [f32, b16, f64]
+        before = [t.double().clone() for t in grads]
+        norm = torch.sqrt(sum((t * t).sum() for t in before))
+        c = most / (float(norm) + 1e-6)
+        assert c < 2.0 ** -126
+        got = seq_ops.clip_grad_norm(h, grads, most)
+        assert abs(float(got) - float(norm)) <= 1e-12 * float(norm)
+        for t, b in zip(grads, before):              # the product's roundings, one in 32 bits and one to the type (half a step of the smallest numbers below the normal ones)
+            assert bool(((t.double() - b * c).abs() <= (ref.half(t.dtype) + ref.half(ref.acc_of(t.dtype)) + 1e-12) * (b * c).abs() +
+                         (2.0 ** -134 if t.dtype == BF16 else 2.0 ** -150)).all())
