@@ -72,7 +72,14 @@ class SeqTable(object):
     of whole numbers >= 0; it is checked here, once, and its offsets are kept on the handle's device."""
 
     def __init__(self, handle, lengths):
-        lengths = [int(v) for v in (lengths.tolist() if hasattr(lengths, 'tolist') else lengths)]
+        given = lengths.tolist() if hasattr(lengths, 'tolist') else lengths
+        try:
+            given = list(given)
+            lengths = [int(v) for v in given]
+        except (TypeError, ValueError, OverflowError):
+            lengths = None
+        if lengths is None or any(v != g for v, g in zip(lengths, given)):
+            _bad('the lengths of a sequence table must be a list of whole numbers, not %.200r' % (given,))
         if not lengths or min(lengths) < 0:
             _bad('a sequence table needs at least one length, none of them negative')
         off = [0]

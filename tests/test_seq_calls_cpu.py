@@ -72,3 +72,16 @@ def test_the_norm_takes_as_many_rows_as_the_scan():
     for rows, ok in ((1 << 24, True), (1 << 40, True), ((1 << 40) + 1, False)):
         r.rows = rows
         assert (_lib.load().rgp_rms_norm_workspace(C.byref(r), 1) > 0) == ok
+
+
+@pytest.mark.parametrize('lengths', [[2.7, 1], [3, 0.5], torch.tensor([1.5, 2.5]), [float('nan')], [float('inf'), 2], [[1, 2]], ['3'], [None], torch.tensor(3), 3])
+def test_lengths_that_are_not_whole_numbers_are_refused(lengths):
+    from rgp_amd import seq_ops
+    _refused(lambda: seq_ops.SeqTable(H, lengths), 'whole numbers')
+
+
+def test_whole_numbers_of_any_type_are_lengths():
+    import numpy as np
+    from rgp_amd import seq_ops
+    for lengths in ([3, 0, 2], (3, 0, 2), torch.tensor([3, 0, 2]), np.array([3, 0, 2]), [3.0, np.int64(0), torch.tensor(2)], iter([3, 0, 2])):
+        assert seq_ops.SeqTable(H, lengths).off.tolist() == [0, 3, 3, 5]
