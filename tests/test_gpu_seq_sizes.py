@@ -112,3 +112,108 @@ def test_clipping_by_a_factor_below_the_normal_numbers(h):
         for t, b in zip(grads, before):              # the product's roundings, one in 32 bits and one to the type (half a step of the smallest numbers below the normal ones)
             assert bool(((t.double() - b * c).abs() <= (ref.half(t.dtype) + ref.half(ref.acc_of(t.dtype)) + 1e-12) * (b * c).abs() +
                          (2.0 ** -134 if t.dtype == BF16 else 2.0 ** -150)).all())
+
+
+@pytest.mark.parametrize('reverse', [False, True])
+@pytest.mark.parametrize('dtype', [F64, F32, BF16], ids=str)
+def test_long_sequences_of_few_channels(h, dtype, reverse):
+    """512 blocks of 8 steps: the join with 16 threads a state, states carried in."""
+    acts, par, init = _inputs(30, 4096, 1, 8, 16, dtype=dtype)
+    _compare(h, acts, par, init, reverse=reverse)
+
+
+@pytest.mark.parametrize('dtype', [F64, F32, BF16], ids=str)
+def test_many_states_in_many_blocks(h, dtype):
+    """131072 states and 14 blocks of 64 steps (a ragged last one): the join with one thread a state, states carried in."""
+    acts, par, init = _inputs(40, 840, 4, 2048, 16, dtype=dtype)
+    _compare(h, acts, par, init, reverse=dtype == F32)
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize('dtype', [F16, BF16], ids=str)
+def test_packed_rows_of_many_channel_workgroups_with_rows_behind(h, dtype):
+    """33 workgroups of channels: gB and gC are sums of 33 partials, of which the rows behind the last sequence have none and stay as they are."""
+    import ctypes as C
+    from rgp_amd import _lib
+    D, N, spare, lengths, fill = 2112, 16, 9, [70, 0, 5, 130], 7.0
+    rows, n = sum(lengths), len(lengths)
+    off = torch.tensor([0, 70, 70, 75, 205], device='cuda')
+    code = _lib.DT_F16 if dtype == F16 else _lib.DT_BF16
+    acts, par, init = _inputs(50, rows, 1, D, N, dtype=dtype)
+    init = _randn(60, n, D, N)
+    behind = lambda t, v: torch.cat([t[:, 0], torch.full((spare,) + t.shape[2:], v, device='cuda', dtype=t.dtype)]).contiguous()      # noqa: E731
+    got = None
+    for v in (float('nan'), 3.0):
+        t = {k: behind(x, v) for k, x in acts.items()}
+        o = lambda *s, dt=dtype: torch.full(s, fill, device='cuda', dtype=dt)                                                       # noqa: E731
+        out = dict(y=o(rows + spare, D), gu=o(rows + spare, D), gdelta=o(rows + spare, D), gz=o(rows + spare, D), gB=o(rows + spare, 1, N), gC=o(rows + spare, 1, N),
+                   gA=o(D, N, dt=F32), gskip=o(D, dt=F32), gbias=o(D, dt=F32), last=o(n, D, N, dt=F32))
+        a = _lib.SsmScan()
+        a.dtype, a.n_seq, a.D, a.N, a.G, a.rows, a.max_len, a.off = code, n, D, N, 1, rows + spare, 130, off.data_ptr()
+        for k, x in dict(out, A=par['A'], skip=par['D'], bias=par['bias'], init=init, u=t['u'], delta=t['delta'], z=t['z'], gy=t['gy'], B=t['B'], C=t['Cm']).items():
+            setattr(a, k, x.data_ptr())
+        a.u_st = a.delta_st = a.z_st = a.gy_st = D
+        a.B_st = a.C_st = N
+        states = torch.empty(h.lib.rgp_ssm_scan_states_bytes(C.byref(a)), dtype=torch.uint8, device='cuda')
+        a.states = states.data_ptr()
+        for back, fn in ((0, h.lib.rgp_ssm_scan_forward), (1, h.lib.rgp_ssm_scan_backward)):
+            work = torch.full(((h.lib.rgp_ssm_scan_workspace(C.byref(a), back) + 3) // 4,), v, device='cuda')
+            a.work, a.work_bytes = work.data_ptr(), work.numel() * 4
+            assert fn(h.h, torch.cuda.current_stream().cuda_stream, C.byref(a)) == 0
+        torch.cuda.synchronize()
+        if got is not None:
+            assert all(torch.equal(got[k], out[k]) for k in out)
+        got = out
+    assert all(bool((got[k][rows:] == fill).all()) for k in ('y', 'gu', 'gdelta', 'gz', 'gB', 'gC'))
+    sums, start = {k: [0, 0] for k in ('gA', 'gD', 'gbias')}, 0
+    for i, L in enumerate(lengths):
+        cut = slice(start, start + L)
+        start += L
+        if L == 0:
+            assert torch.equal(got['last'][i], init[i])
+            continue
+        want = seq_batched.scan(**{k: x[cut] for k, x in acts.items()}, **par, init=init[i:i + 1])
+        ops = 8 * L + N + D + 64
+        for k in ('y', 'gu', 'gdelta', 'gz', 'gB', 'gC'):
+            ref.check(k, got[k][cut].unsqueeze(1), *want[k], ops=ops, acc=F32)
+        ref.check('last', got['last'][i:i + 1], *want['last'], ops=ops, acc=F32)
+        for k in sums:
+            sums[k] = [s + w for s, w in zip(sums[k], want[k])]
+    for k, t in (('gA', got['gA']), ('gD', got['gskip']), ('gbias', got['gbias'])):
+        ref.check(k, t, *sums[k], ops=8 * 130 + N + rows + 64, acc=F32)
+
+
+def test_clipping_of_many_large_tensors(h):
+    """130 MB of all types in 2000 pieces of 64 KB: more pieces than every workgroup adds for itself."""
+    from rgp_amd import seq_ops
+    sizes = [(20000003, F32), (9999999, BF16), (1500001, F64), (5000000, F16), (1, F64), (0, F32), (32769, F32)]
+    grads = [_randn(i, n).to(t) for i, (n, t) in enumerate(sizes)]
+    before = [t.double().clone() for t in grads]
+    norm = torch.sqrt(sum((t * t).sum() for t in before))
+    got = seq_ops.clip_grad_norm(h, grads, 2.5)
+    assert abs(float(got) - float(norm)) <= 1e-12 * float(norm)            # 4e7 additions of positive terms in pairs or chains of at most 1e4: below 1e4 half steps
+    c = 2.5 / (float(norm) + 1e-6)
+    for t, b in zip(grads, before):
+        acc, want = ref.acc_of(t.dtype), b * c
+        assert bool(((t.double() - want).abs() <= (ref.half(t.dtype) * 1.001 + 2 * ref.half(acc) + 1e-12) * want.abs() + (2.0 ** -25 if t.dtype == F16 else 0)).all())
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize('n', [20, 300, 3000, 9001])
+def test_sums_over_sequences(h, n):
+    """The gradient of D is a sum over sequences, by every way the sums have (one thread an output, 16 or 64, rows gathered first).  Where every
+    term and partial sum is a number of 32 bits -- multiples of 2^-8 up to 18002 -- it is exact; of positive terms it is off by the additions that
+    one of them passes: at most 20 in a chain, or 6 + 7 + 6 and 9 + 14 behind rows gathered by 6, and the 2 steps: below 32 half steps."""
+    from rgp_amd import seq_ops
+    T, D, N = 2, 70, 4
+    delta, B, Cm, A = _randn(1, T, n, D), _randn(2, T, n, N), _randn(3, T, n, N), -torch.ones(D, N, device='cuda')
+
+    def gD(u, gy):
+        skip = torch.ones(D, device='cuda', requires_grad=True)
+        y = seq_ops.ssm_scan(h, u, delta, A, B, Cm, D=skip)
+        g, = torch.autograd.grad(y, skip, gy)
+        return g.double(), (u.double() * gy.double()).sum((0, 1))
+    got, want = gD(*((torch.round(_randn(i, T, n, D) * 6).clamp(-16, 16) / 16) for i in (4, 5)))
+    assert torch.equal(got, want)
+    got, want = gD(*(0.5 + 0.5 * torch.rand(T, n, D, device='cuda', generator=torch.Generator(device='cuda').manual_seed(i)) for i in (6, 7)))
+    assert bool(((got - want).abs() <= 32 * 2.0 ** -24 * want).all())
