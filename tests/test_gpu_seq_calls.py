@@ -261,3 +261,44 @@ def test_states_of_whole_sequences_must_not_share_memory(h):
         one, two = torch.cat((start, start)), torch.cat((start, start, start))
         assert call(one, 0, size) == 0 and call(two, 0, 2 * size) == 0
         assert torch.equal(one[size:], two[2 * size:]) and torch.equal(one[:size], start) and not torch.equal(one[size:], start)
+
+
+@pytest.mark.parametrize('dtype', [F64, BF16], ids=str)
+@pytest.mark.parametrize('reentrant', [False, True])
+def test_checkpointed_regions(h, dtype, reentrant):
+    """torch.utils.checkpoint runs the region again in the backward pass: the same bits, whichever way it saves."""
+    from torch.utils.checkpoint import checkpoint
+    from rgp_amd import seq_ops
+    g = torch.Generator().manual_seed(6)
+    acc = F64 if dtype == F64 else F32
+    f = lambda *s, t=dtype: torch.randn(*s, generator=g, dtype=F64).to(t).cuda().requires_grad_(True)           # noqa: E731
+    x, delta, B, Cm, z = f(40, 2, 12), f(40, 2, 12), f(40, 2, 16), f(40, 2, 16), f(40, 2, 12)
+    A, w, b, n = f(12, 16, t=acc), f(12, 4, t=acc), f(12, t=acc), f(12, t=acc)
+
+    def region(x, delta, B, Cm, z, A, w, b, n):
+        v = seq_ops.ssm_conv(h, x, w, b)
+        y = seq_ops.ssm_scan(h, v, delta, -A.abs(), B, Cm, D=b, z=z, delta_bias=b)
+        return seq_ops.rms_norm(h, y, n, residual=x)
+    ops = (x, delta, B, Cm, z, A, w, b, n)
+    gy, gh = (torch.randn(40, 2, 12, generator=g, dtype=F64).to(dtype).cuda() for _ in range(2))
+    want = torch.autograd.grad(region(*ops), ops, (gy, gh))
+    outs = checkpoint(region, *ops, use_reentrant=reentrant)
+    torch.autograd.backward(outs, (gy, gh))
+    for t, e in zip(ops, want):
+        assert torch.equal(t.grad, e)
+
+
+def test_some_operands_without_gradients_and_other_modes(h):
+    """Each leaf alone gives the gradient that it has among all; inference mode and anomaly detection change nothing."""
+    ops = _leaves(*ALL_LEAVES)
+    outs = _three(h, ops)
+    want = torch.autograd.grad([o.square().sum() for o in outs], ops)
+    for i, e in enumerate(want):
+        one = [t.detach().requires_grad_(i == j) for j, t in enumerate(ops)]
+        loss = sum(o.square().sum() for o in _three(h, one))
+        assert torch.equal(torch.autograd.grad(loss, one[i])[0], e)
+    with torch.inference_mode():
+        assert all(torch.equal(a, b) for a, b in zip(_three(h, ops), outs))
+    with torch.autograd.detect_anomaly(check_nan=True):
+        got = torch.autograd.grad([o.square().sum() for o in _three(h, ops)], ops)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
