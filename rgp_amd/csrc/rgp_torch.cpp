@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
@@ -19,7 +20,6 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
-#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <array>
@@ -88,8 +88,9 @@ struct Handle {
     if (THPDevice_Check(d)) device = ((THPDevice*)d)->device;
     Py_DECREF(d);
     PyObject* p = attr(o, s_h);
-    std::shared_ptr<PyObject> hold(p, [](PyObject* q) { Py_DECREF(q); });
-    if (void* const* at = cell_of(p)) h = (rgp_handle)*at;
+    void* const* at = cell_of(p);
+    if (at) h = (rgp_handle)*at;
+    Py_DECREF(p);
   }
   void* stream() const { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
   void check(rgp_status st) const {
@@ -136,7 +137,8 @@ at::ScalarType acc_of(at::ScalarType t) { return t == at::kDouble ? at::kDouble 
 
 // While torch records a function (torch.jit.trace, make_fx), it would see the allocation of a result and nothing that fills it.
 bool recording() {
-  return torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value();
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  return c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::Tracer) || (Modes::any_modes_set() && Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value());
 }
 
 // Forward-mode derivatives: a tensor may carry its tangent beside its values, and no result here would get one.

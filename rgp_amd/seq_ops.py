@@ -104,7 +104,8 @@ def _rows(name, t, like, lead):
 
 def _inner(t, dims):
     """The tensor with its last ``dims`` dimensions contiguous (a copy only where they are not, or where its memory holds the negated values)."""
-    t = t.resolve_neg()
+    if t.is_neg():
+        t = t.resolve_neg()
     if t.is_contiguous():
         return t
     shape, stride, want = t.shape, t.stride(), 1
@@ -154,7 +155,7 @@ def _param(name, t, shape, x, optional=False):
         _bad('%s has shape %s, %s expected' % (name, tuple(t.shape), tuple(shape)))
     if t.dtype is not _acc(x.dtype):
         _bad('%s is %s: parameters and states are %s for %s activations' % (name, t.dtype, _acc(x.dtype), x.dtype))
-    return t.resolve_neg().contiguous()
+    return t if t.is_contiguous() and not t.is_neg() else t.resolve_neg().contiguous()
 
 
 def _state(name, t, shape, dtype, x):
