@@ -17,6 +17,10 @@ template <typename A> static __device__ __forceinline__ A ssm_finite(A a) {
   return a < -most ? -most : a > most ? most : a;
 }
 
+// What a block with decay e makes of the state s that enters it.  Where A is positive the product of many decays may be infinite: a state of zero
+// stays zero all the same.
+template <typename A> static __device__ __forceinline__ A ssm_through(A e, A s) { return s == (A)0 ? (A)0 : e * s; }
+
 // Where channel c of a tile's row stands in LDS.  A thread writes V neighbouring channels, so at any one of its writes the wave's lanes are V
 // entries apart and would meet in the same banks; the place is c with its low bits exchanged by the number of the 128-byte line, which puts
 // those lanes side by side and leaves neighbouring channels in one line for the recurrence.
@@ -70,7 +74,7 @@ static __device__ __forceinline__ void ssm_enter(const SsmDev& d, const SeqBlock
     for (int u = 0; u < U; ++u)
       if (u < left) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) s[r] = decay(t[u], r) * s[r] + h[u][r];
+        for (int r = 0; r < R; ++r) s[r] = ssm_through(decay(t[u], r), s[r]) + h[u][r];
       }
   }
 }

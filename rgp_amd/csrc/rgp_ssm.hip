@@ -164,10 +164,10 @@ static __global__ void __launch_bounds__(Q == 1 ? 256 : Q * 64) ssm_join_kernel(
       if (i < left) {
         if (pass == 0) {
           P *= e[i];
-          H = e[i] * H + p[i];
+          H = ssm_through(e[i], H) + p[i];
         } else {
           pp[i * dp] = s;
-          s = e[i] * s + p[i];
+          s = ssm_through(e[i], s) + p[i];
         }
       }
     }
@@ -185,7 +185,7 @@ static __global__ void __launch_bounds__(Q == 1 ? 256 : Q * 64) ssm_join_kernel(
       shH[q][l] = H;
       __syncthreads();                                    // also: every block's sums are read before the states replace them
       s = !back && a.init && ok ? ((const A*)a.init)[seq * DN + dn] : (A)0;
-      for (int r = 0; r < q; ++r) s = shP[r][l] * s + shH[r][l];
+      for (int r = 0; r < q; ++r) s = ssm_through(shP[r][l], s) + shH[r][l];
     }
   }
 }

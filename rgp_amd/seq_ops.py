@@ -260,7 +260,8 @@ def ssm_scan(handle, u, delta, A, B, Cm, D=None, z=None, delta_bias=None, seqs=N
     u, delta, z: (T, batch, Dn), or packed (rows, Dn) with ``seqs``; B, C: the same leading dimensions and (N,) or (G, N); A (Dn, N),
     N <= 64; D, delta_bias (Dn,).  init: (n_seq, Dn, N), the state before the first step (zeros without it); return_state=True also returns
     the state behind the last step.  reverse=True walks every sequence from its last step.  Gradients: u, delta, A, B, C, D, z, delta_bias
-    (states take none)."""
+    (states take none).  A is meant to be negative: long sequences are walked in blocks of time, and where A is positive and exp(sum of dt A)
+    over a block leaves the range of the arithmetic type, so does what the block makes of a state that is not zero."""
     r = _seq.scan(handle, u, delta, A, B, Cm, D, z, delta_bias, seqs, init, bool(reverse), bool(return_state))
     if r is None:
         lead, n_seq = _geometry(handle, u, seqs, 'u')

@@ -217,3 +217,32 @@ def test_sums_over_sequences(h, n):
     assert torch.equal(got, want)
     got, want = gD(*(0.5 + 0.5 * torch.rand(T, n, D, device='cuda', generator=torch.Generator(device='cuda').manual_seed(i)) for i in (6, 7)))
     assert bool(((got - want).abs() <= 32 * 2.0 ** -24 * want).all())
+
+
+@pytest.mark.parametrize('T', [60, 96, 200, 1500])
+@pytest.mark.parametrize('dtype', [F64, F32], ids=str)
+def test_growing_states_that_begin_late(h, dtype, T):
+    """A positive A: a block's decays multiply beyond the type's range, and what enters the blocks is zero -- inputs in the last three steps, gradients
+    of the first three -- so states and adjoints are finite wherever the steps one after the other make them so."""
+    acts, par, _ = _inputs(70, T, 2, 20, 16, dtype=dtype, carry=False)
+    acts['u'][:-3] = 0
+    acts['gy'][3:] = 0
+    acts['delta'].zero_()
+    par = dict(A=torch.full_like(par['A'], 20.0 if dtype == F32 else 160.0), D=par['D'], bias=torch.zeros_like(par['bias']))
+    _compare(h, acts, par, None)
+    _compare(h, {k: v.flip(0) for k, v in acts.items()}, par, None, reverse=True)
+
+
+def test_packed_sequences_without_rows_in_many_channels(h):
+    """No rows at all, three workgroups of channels: states are handed on and every gradient of a parameter is zero."""
+    from rgp_amd import seq_ops
+    D, N, seqs = 130, 16, seq_ops.SeqTable(h, [0, 0, 0])
+    e = lambda *s: torch.zeros(*s, device='cuda', requires_grad=True)                               # noqa: E731
+    A, skip, bias, w = (-_randn(1, D, N).abs()).requires_grad_(True), e(D), e(D), e(D, 4)
+    init, cinit = _randn(2, 3, D, N), _randn(3, 3, 3, D)
+    u, delta, B, Cm, z = e(0, D), e(0, D), e(0, 1, N), e(0, 1, N), e(0, D)
+    y, last = seq_ops.ssm_scan(h, u, delta, A, B, Cm, D=skip, z=z, delta_bias=bias, seqs=seqs, init=init, return_state=True)
+    v, clast = seq_ops.ssm_conv(h, u, w, bias, seqs=seqs, init=cinit, return_state=True)
+    assert y.shape == v.shape == (0, D) and torch.equal(last, init) and torch.equal(clast, cinit)
+    for g in torch.autograd.grad((y, v), (u, delta, A, B, Cm, skip, z, bias, w), (torch.zeros_like(y), torch.zeros_like(v))):
+        assert bool((g == 0).all())
