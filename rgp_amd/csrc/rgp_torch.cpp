@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/SavedTensorHooks.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
@@ -226,7 +227,8 @@ struct OpNode : torch::autograd::Node {
   KeptHandle handle;
   Geo geo;
   int reverse = 0;
-  explicit OpNode(const Handle& h) : handle(h) {}
+  bool hooked;                                       // the user's hooks have what the node saves
+  explicit OpNode(const Handle& h) : handle(h), hooked(at::SavedTensorDefaultHooks::get_hooks().has_value()) {}
   // What a backward pass has to refuse.  The engine hands a gradient on to the stream on which the node that takes it was made: during a capture
   // that must be the captured one.  A leaf that an eager graph still holds has its node on the eager stream, and an event from the capture to
   // there ends the capture, and the process with it.
@@ -246,7 +248,8 @@ struct OpNode : torch::autograd::Node {
     }
   }
   // What a graph saved may come back through the user's hooks (torch.autograd.graph.saved_tensors_hooks): in another memory order, which the passes
-  // lay out again, or as something else, which the kernels must not be given.
+  // lay out again, or as something else, which the kernels must not be given.  Asked only where there were hooks: the checks cost a small
+  // backward pass 2 to 3 us.
   static void came_back(bool ok) {
     if (!ok) throw std::runtime_error("a saved operand of the sequence operators came back with another type, shape or device");
   }
@@ -287,10 +290,15 @@ struct ConvNode : OpNode {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(3);
     if (!grads[0].defined()) return out;
-    const ConvOps c{rows_of(x.unpack()), whole(w.unpack()), whole(b.unpack())};
-    const Tensor before = whole(init.unpack()), gv = rows_of(grads[0]);
-    came_back(like(c.x, gv) && c.x.sizes() == gv.sizes() && conv_ok(c) &&
-              (!before.defined() || (like(before, gv) && before.sizes() == at::IntArrayRef({geo.n_seq, c.w.size(1) - 1, c.x.size(-1)}))));
+    ConvOps c{x.unpack(), w.unpack(), b.unpack()};
+    Tensor before = init.unpack();
+    const Tensor gv = rows_of(grads[0]);
+    if (hooked) {
+      c = ConvOps{rows_of(c.x), whole(c.w), whole(c.b)};
+      before = whole(before);
+      came_back(like(c.x, gv) && c.x.sizes() == gv.sizes() && conv_ok(c) &&
+                (!before.defined() || (like(before, gv) && before.sizes() == at::IntArrayRef({geo.n_seq, c.w.size(1) - 1, c.x.size(-1)}))));
+    }
     rgp_ssm_conv a = conv_args(c, geo, reverse);
     out[0] = fresh(c.x); out[1] = fresh(c.w); out[2] = fresh(c.b);
     a.init = ptr(before); a.gv = gv.data_ptr(); a.gx = out[0].data_ptr(); a.gw = out[1].data_ptr(); a.gbias = ptr(out[2]);
@@ -399,12 +407,16 @@ struct ScanNode : OpNode {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(8);
     if (!grads[0].defined()) return out;
-    const Tensor zs = z.unpack(), gy = rows_of(grads[0]);
-    ScanOps s{rows_of(u.unpack()), rows_of(delta.unpack()), whole(A.unpack()), B.unpack(), C.unpack(), whole(skip.unpack()), zs.defined() ? rows_of(zs) : zs, whole(bias.unpack())};
-    for (Tensor* t : {&s.B, &s.C})
-      if (t->is_neg() || t->dim() <= geo.dims || !inner(*t, (int)t->dim() - geo.dims)) *t = whole(*t);
-    int groups = 0;
-    came_back(like(s.u, gy) && s.u.sizes() == gy.sizes() && scan_ok(s, geo.dims, groups) && groups == G && s.A.size(1) == N);
+    ScanOps s{u.unpack(), delta.unpack(), A.unpack(), B.unpack(), C.unpack(), skip.unpack(), z.unpack(), bias.unpack()};
+    const Tensor gy = rows_of(grads[0]);
+    if (hooked) {
+      s.u = rows_of(s.u); s.delta = rows_of(s.delta); s.z = s.z.defined() ? rows_of(s.z) : s.z;
+      s.A = whole(s.A); s.skip = whole(s.skip); s.bias = whole(s.bias);
+      for (Tensor* t : {&s.B, &s.C})
+        if (t->is_neg() || t->dim() <= geo.dims || !inner(*t, (int)t->dim() - geo.dims)) *t = whole(*t);
+      int groups = 0;
+      came_back(like(s.u, gy) && s.u.sizes() == gy.sizes() && scan_ok(s, geo.dims, groups) && groups == G && s.A.size(1) == N);
+    }
     rgp_ssm_scan a = scan_args(s, geo, G, reverse);
     const Tensor* in[8] = {&s.u, &s.delta, &s.A, &s.B, &s.C, &s.skip, &s.z, &s.bias};
     for (int i = 0; i < 8; ++i) out[i] = fresh(*in[i]);
@@ -514,9 +526,12 @@ struct RmsNode : OpNode {
       out[0] = out[2] = ghid;
       return out;
     }
-    const Tensor xs = rows_of(x.unpack(of_hid ? shared_from_this() : nullptr)), rs0 = residual.unpack(), rs = rs0.defined() ? rows_of(rs0) : rs0, ws = whole(w.unpack());
+    Tensor xs = x.unpack(of_hid ? shared_from_this() : nullptr), rs = residual.unpack(), ws = w.unpack();
     const Tensor gy = rows_of(grads[0]), gh = ghid.defined() ? rows_of(ghid) : ghid;
-    came_back(like(xs, gy) && xs.sizes() == gy.sizes() && param(ws, gy, {gy.size(1)}) && (!rs.defined() || (like(rs, gy) && rs.sizes() == gy.sizes())));
+    if (hooked) {
+      xs = rows_of(xs); rs = rs.defined() ? rows_of(rs) : rs; ws = whole(ws);
+      came_back(like(xs, gy) && xs.sizes() == gy.sizes() && param(ws, gy, {gy.size(1)}) && (!rs.defined() || (like(rs, gy) && rs.sizes() == gy.sizes())));
+    }
     rgp_rms_norm a = rms_args(xs, rs, ws, eps);
     out[0] = fresh(xs); out[1] = fresh(ws);
     if (two) out[2] = out[0];
