@@ -418,9 +418,10 @@ static __global__ void __launch_bounds__(256) ssm_step_kernel(rgp_ssm_scan a, in
     ((T*)a.y)[row * a.D + ch] = (T)y;
   }
 }
+static int step_lanes(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }       // lanes a channel
 template <typename T>
 static hipError_t step_pick(const rgp_ssm_scan& a, hipStream_t s) {
-  const int K = a.N <= 4 ? 1 : a.N <= 8 ? 2 : a.N <= 16 ? 4 : a.N <= 32 ? 8 : 16;
+  const int K = step_lanes(a.N);
   const unsigned grid = (unsigned)(((int64_t)a.n_seq * a.D * K + 255) / 256);
   const int Dg = a.D / a.G;
   const int whole = a.N == STEP_R * K && ((uintptr_t)a.last & 15) == 0 && ((uintptr_t)a.A & 15) == 0 &&
@@ -440,7 +441,7 @@ extern "C" rgp_status rgp_ssm_scan_step(rgp_handle h, void* stream, const rgp_ss
     if (a->off || a->T != 1) return rgp_fail(h, RGP_ERR_BAD_ARG, "ssm scan step: one row per sequence (T = 1, no offsets)");
     if (!a->u || !a->delta || !a->B || !a->C || !a->A || !a->y || !a->last || a->init != a->last)
       return rgp_fail(h, RGP_ERR_BAD_ARG, "ssm scan step: u, delta, A, B, C, y and the state (init = last) are required");
-    if ((double)a->n_seq * a->D * 16 > 4294967295.0) return rgp_fail(h, RGP_ERR_BAD_ARG, "ssm scan step: more than 2^32 work items");
+    if ((double)a->n_seq * a->D * step_lanes(a->N) > 4294967295.0 - 255.0) return rgp_fail(h, RGP_ERR_BAD_ARG, "ssm scan step: more than 2^32 work items");
     const hipStream_t s = (hipStream_t)stream;
     const hipError_t e = a->dtype == RGP_F64 ? step_pick<double>(*a, s) : a->dtype == RGP_F32 ? step_pick<float>(*a, s)
                        : a->dtype == RGP_BF16 ? step_pick<__bf16>(*a, s) : step_pick<_Float16>(*a, s);

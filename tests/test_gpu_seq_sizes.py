@@ -246,3 +246,17 @@ def test_packed_sequences_without_rows_in_many_channels(h):
     assert y.shape == v.shape == (0, D) and torch.equal(last, init) and torch.equal(clast, cinit)
     for g in torch.autograd.grad((y, v), (u, delta, A, B, Cm, skip, z, bias, w), (torch.zeros_like(y), torch.zeros_like(v))):
         assert bool((g == 0).all())
+
+
+def test_a_step_of_very_many_sequences(h):
+    """131073 sequences of 2048 channels in one step: the first and the last ones give what they give alone, to the bit."""
+    from rgp_amd import seq_ops
+    n, D, N, k = 131073, 2048, 4, 40
+    ops = [_randn(i, n, w, dtype=BF16) for i, w in enumerate((D, D, N, N))]                       # u, delta, B, C
+    A, state = -torch.exp(_randn(7, D, N)), _randn(8, n, D, N)
+    parts = [(s, [t[s].clone() for t in ops], state[s].clone()) for s in (slice(0, k), slice(n - k, n))]
+    y = seq_ops.ssm_scan_step(h, ops[0], ops[1], A, ops[2], ops[3], None, state)
+    for s, (u, delta, B, Cm), st in parts:
+        assert torch.equal(y[s], seq_ops.ssm_scan_step(h, u, delta, A, B, Cm, None, st)) and torch.equal(state[s], st)
+    del ops, state, y
+    torch.cuda.empty_cache()
