@@ -1,8 +1,8 @@
 // rgp_norm.hip -- root-mean-square norm of x + residual and its gradient; global norm of many gradient tensors and their clipping.
 // All of it is bound by memory: every kernel reads its operands once, 16 bytes a lane, and keeps a row in registers between the sum of
 // squares and the product.  Norm of 16384 x 2048 bf16: forward 52 us, 5.2 TB/s, backward 72 us, 4.7 TB/s (a large copy reaches 5.07); rows of 300 or
-// 1001 elements the same to 6 %; 5 x 2048: 3 us, the launch.  Clipping of 400 M bf16 elements: 195 us for the norm (4.1 TB/s), 284 for the scaling
-// (5.6 TB/s, helped by what the norm left in the memory-side cache); 84 211 fp64 elements in 39 tensors: 4.5 + 5 us.
+// 1001 elements the same to 6 %; 5 x 2048: 3.6 us, the launch.  Clipping of 400 M bf16 elements: 193 us for the norm (4.1 TB/s), 283 for the scaling
+// (5.7 TB/s, helped by what the norm left in the memory-side cache); 84 211 fp64 elements in 39 tensors: 4.6 + 5.1 us.
 #include "rgp_seq.h"
 
 struct NormDev {

@@ -46,7 +46,7 @@ struct SsmDev {
   int64_t nslot;                     // blocks
   int join;                          // every block joins the sums of the blocks before it (behind it) by itself
   int Dg, ncb;                       // channels per group, channel blocks per group
-  int wide;                          // every activation in 16-byte vectors: aligned, and Dg a multiple of a vector
+  int wide;                          // activations in 16-byte vectors, at any element's address: no workgroup has fewer channels than a vector
   void* part;                        // state (forward) or adjoint (backward) that every block starts from [nslot][D][N]
   void* sumdt;                       // sum of dt over a block [nslot][D]
   void *pA, *pD, *pBC;               // partial sums of the backward pass: [nslot][D][N], [nslot][2][D], [ncb][rows][2][G][N]

@@ -7,7 +7,7 @@
 // ---- sums of partial results in a fixed order -----------------------------------------------------------------------------------------
 // A workgroup forms W outputs of one of up to five sums, Q = 1024 / W threads for each: thread q adds partials q, q + Q, ... in eight
 // interleaved sums (that many loads are in flight), then the Q are added in LDS.  W = 64, 16 where there are many partials (2048 of 1024 outputs:
-// 9 us with 64), and up to SEQ_FEW partials are added by one thread an output.  The order depends on the count of partials alone.  4 to 6 us for
+// 9 us with 64), and up to SEQ_FEW partials are added by one thread an output.  The order depends on the count of partials alone.  5 to 8 us for
 // all sums of a backward pass.  Beyond SEQ_HUGE partials (many short sequences) rows r, r + SEQ_MANY, ... are first added into row r.
 #define SEQ_FEW 32
 #define SEQ_MANY 512
@@ -305,7 +305,9 @@ static rgp_status scan_run(rgp_handle h, hipStream_t s, const rgp_ssm_scan* a, b
   SsmDev& d = p.d;
   if (p.bytes > a->work_bytes || (p.bytes && !a->work) || ((uintptr_t)a->work & 15))
     return rgp_fail(h, RGP_ERR_WORKSPACE, std::string(what) + "work buffer too small or not 16-byte aligned");
-  const int V = 16 / seq_dtype_bytes(a->dtype), rest = d.Dg % p.sh.CH;      // a workgroup's channels are one vector at least, or single elements
+  // Vectors need as many channels as they have elements in every workgroup; where the last one has fewer, all take the kernels of single elements
+  // (training steps of 512 x 16 x 1025 bf16 take 382 us, x 1032 332, x 1024 237; of 4096 x 32 x 65 fp32 525, x 68 505, x 64 279).
+  const int V = 16 / seq_dtype_bytes(a->dtype), rest = d.Dg % p.sh.CH;
   d.wide = rest == 0 || rest >= V;
   char* w = (char*)a->work;
   auto take = [&](int64_t bytes) { void* r = bytes ? (void*)w : nullptr; w += bytes; return r; };
@@ -354,7 +356,7 @@ extern "C" rgp_status rgp_ssm_scan_backward(rgp_handle h, void* stream, const rg
 
 // ---- one step -----------------------------------------------------------------------------------------------------------------------------
 // Bound by reading and writing the state: K lanes a channel, 16 bytes of state a lane (32 in fp64), as in the kernels over time.  256 x 2048
-// bf16, N = 16: 16.7 us for 67 MB of state and 8 MB beside it, 4.5 TB/s; one sequence of 40 channels 3.7 us, the launch.
+// bf16, N = 16: 17.8 us for 67 MB of state and 8 MB beside it, 4.2 TB/s; one sequence of 40 channels 3.8 us, the launch.
 #define STEP_R 4                     // states a lane
 template <typename T, int K>
 static __global__ void __launch_bounds__(256) ssm_step_kernel(rgp_ssm_scan a, int Dg, int whole) {
@@ -455,7 +457,8 @@ extern "C" rgp_status rgp_ssm_scan_step(rgp_handle h, void* stream, const rgp_ss
 // is only one, and in a step of an odd width) and walks a run of 8 or 16 steps with the last W - 1 inputs in registers, CONV_FLY rows in flight; the W - 1 rows
 // before a run are read again (from cache).  Wider vectors have fewer waves to wait with: backward over 8191 x 1024 bf16 46 us with 8 channels
 // a thread, 31 with 4, 26 with 2; runs of 8 steps 36 (4 channels), of 32 29 (2 channels); 8 rows in flight change nothing.  Forward, 8 x 65536 x
-// 64 fp32: 50 us, 5.4 TB/s; the 16-bit forms reach 3 TB/s and are held up by the sigmoid and conversions.
+// 64 fp32: 49 us, 5.5 TB/s; in 16 bits a thread's two channels make accesses of 4 bytes, and 8191 x 1024 takes 11 us, 3.0 TB/s: the waves wait
+// 0.63 of their cycles (SQ_WAIT_ANY), the vector unit issues 0.58 of the time.
 #define CONV_FLY 4
 #define CONV_V 2
 struct ConvDev {
@@ -560,7 +563,8 @@ static __global__ void __launch_bounds__(256) conv_last_kernel(ConvDev d) {
   }
 }
 
-// Backward (8191 x 1024 bf16 26 us, 32 x 4096 x 64 fp32 30: waits for rows, the vector unit is busy half of the time): gp = gv silu'(pre), gx_t
+// Backward (8191 x 1024 bf16 26 us, 1.9 TB/s, 32 x 4096 x 64 fp32 30, 3.3 TB/s: the waves wait 0.66 of their cycles, the vector unit issues 0.55 of
+// the time): gp = gv silu'(pre), gx_t
 // = sum_j w_j gp_{t+W-1-j}, gw_j = sum_t gp_t x_{t-W+1+j}, gbias = sum gp.  pre is formed again from x (one more read would cost more than W
 // multiply-adds).  A thread walks its runs and W - 1 steps behind each; the parameter sums of the threads with the same channels go through
 // LDS, then from all workgroups through `part`.

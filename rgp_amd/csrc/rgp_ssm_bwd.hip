@@ -10,9 +10,11 @@
 //
 // Bound by the vector unit: a step of a wave takes 86 instructions in the recurrence (13 for each of a lane's states, 17 for the sums over
 // channels, 6 for those over states) and about 28 for the elements, tiles and partial sums; SQ_ACTIVE_INST_VALU is 0.88 of the busy cycles.
-// 8191 x 1024 bf16, N = 16: 143 us, and 39 for the walk that only sums the blocks (MODE 1); 32 x 4096 x 64 fp32: 150 and 38; 8 x 512 x 40
-// fp64 in blocks of 16 steps: 23 and 13.  Two waves a SIMD: a tile of 32 steps fits their LDS for 16-bit types with 4 lanes a channel, 16 steps
-// elsewhere (with 2 lanes 64 instead of 71 us at 4096 x 1024, N = 8); one lane a channel, and 4 states a lane in fp64, need the registers of two.
+// 8191 x 1024 bf16, N = 16: 139 us, and 39 for the walk that only sums the blocks (MODE 1); 32 x 4096 x 64 fp32: 148 and 38; 8 x 512 x 40
+// fp64 in blocks of 16 steps: 21 and 11.  fp64 that fills the card (32 x 4096 x 64: 429 and 186) is bound the same way, by 172 and 85 instructions a
+// step of a wave with 8 channels (issue ratios 0.80 and 0.89).  Two waves a SIMD: a tile of 32 steps fits their LDS for 16-bit types with 4 lanes a
+// channel, 16 steps elsewhere (with 2 lanes 64 instead of 71 us at 4096 x 1024, N = 8); one lane a channel, and 4 states a lane in fp64, need the
+// registers of two.
 #include "rgp_ssm.h"
 
 template <typename T, int K, int R, int CH, int MODE, int V>

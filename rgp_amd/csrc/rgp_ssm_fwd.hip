@@ -6,8 +6,9 @@
 // channels than a vector.  Between them the recurrence reads (dt, dt u) and the rows of B and C from LDS and leaves y there.  The next tile's
 // loads are in flight while a tile is walked.
 // Bound by the vector unit: a step of a wave (64 / K channels) takes 22.6 instructions in the recurrence, 4 of them exponentials at a quarter of
-// the rate, and 12 for the elements; the unit is busy 97 % of the kernel's time (SQ_ACTIVE_INST_VALU).  8191 x 1024 bf16, N = 16, training: 48 us,
-// and 33 for the walk that only sums the blocks (MODE 1).  8 x 65536 x 64 fp32: 174 us, 3.1 TB/s, and 123.  What else was tried: 8 states a lane
+// the rate, and 12 for the elements; the unit is busy 96 % of the kernel's time (SQ_ACTIVE_INST_VALU).  8191 x 1024 bf16, N = 16, training: 49 us,
+// and 33 for the walk that only sums the blocks (MODE 1).  8 x 65536 x 64 fp32: 170 us, 3.5 TB/s, and 119.  32 x 4096 x 64 fp64: 200 and 154, the unit
+// busy all the time, 99 and 74 instructions a step of a wave with 8 channels.  What else was tried: 8 states a lane
 // (fewer lane sums, but half the waves): 58 instead of 49 us.  Registers allow 4 waves a SIMD, which that takes (3: 188 instead of 174 us); with
 // one or two lanes a channel, tiles of 16 steps keep the element role in registers (8192 x 2000 fp32, N = 4: 64 us, with 32 steps 110).
 #include "rgp_ssm.h"

@@ -879,7 +879,8 @@ class DeepAutoreg_rnn(_EncoderParamsMixin, DeepAutoreg):
     """autoreg.DeepAutoreg_rnn (model.py:284-629): q(X) of every hidden layer is produced by a recurrent encoder from the
     raw sequences (equal lengths, stacked to (T, batch, D_y + D_u) as at model.py:429), so the latents are NOT free
     parameters; the trainable parameters are the GP globals and the encoder weights.  The GP layers run through
-    librgp_hip.so exactly as in DeepAutoreg (latents with one row per raw time step); the encoder is PyTorch-ROCm fp64.
+    librgp_hip.so exactly as in DeepAutoreg (latents with one row per raw time step); the encoder's products and heads are PyTorch-ROCm fp64, its
+    time loops device scans of the library (rnn_encoder.py).
 
     rnn_type 'ssm' (no counterpart in the reference): the encoder layers are state-space blocks (rnn_encoder.MeanVarSSM), which parallelise
     over time and can go on from a state one observation at a time (``online_state`` / ``encode_online``).  rnn_compute_dtype (such encoders
