@@ -15,7 +15,8 @@ same bits every time.  Wrong arguments raise RgpError (RGP_ERR_BAD_ARG) before a
 A captured backward pass needs leaves that no eager graph holds at that time (it is refused): take the gradients with torch.autograd.grad
 inside the captured region, on a forward pass of the same region.  There are no second derivatives (a backward pass with
 create_graph=True is refused) and no forward-mode ones (operands and gradients that carry a tangent are refused).  A
-function that torch records (torch.jit.trace, make_fx) cannot hold these operators: refused too."""
+function that torch records (torch.jit.trace, make_fx) cannot hold these operators: refused too.  So is the backward pass of a graph whose handle
+has been closed in between."""
 import ctypes as C
 import math
 
