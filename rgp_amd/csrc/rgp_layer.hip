@@ -226,8 +226,12 @@ extern "C" void rgp_destroy(rgp_handle h) {
 extern "C" const char* rgp_last_error(rgp_handle h) {
   if (!h) return "null handle";
   if (t_error.serial == h->serial) return t_error.own.c_str();
-  std::lock_guard<std::mutex> lock(h->err_lock);
-  t_error.latest = h->err;
+  try {
+    std::lock_guard<std::mutex> lock(h->err_lock);
+    t_error.latest = h->err;
+  } catch (...) {                                        // nothing crosses the C boundary
+    return "no memory for the message";
+  }
   return t_error.latest.c_str();
 }
 
