@@ -19,7 +19,7 @@ struct alignas(W * sizeof(T)) SeqVec {
 };
 
 // The same at any address that an element may have: global memory takes 16-byte accesses at element boundaries at 94 % or more of the rate of
-// aligned ones (measured on rows of 301 and 2047 two-byte elements), so odd widths and strides need no path of their own.  Where a row is not
+// aligned ones (measured on rows of 301 and 2047 two-byte elements), so odd widths and strides need no path of their own (less than a vector does). Where a row is not
 // whole vectors the last one is moved back to end with the row: two lanes then write the same values to the elements they share, and only one
 // of them may count these in a sum.
 template <typename T, int W>

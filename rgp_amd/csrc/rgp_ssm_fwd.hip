@@ -2,8 +2,8 @@
 //     dt = softplus(delta + bias);  s[n] = exp(dt A[n]) s[n] + dt u B[n];  y = (sum_n C[n] s[n] + skip u) silu(z).
 // K lanes hold one channel's states, R each; a workgroup holds CH channels of one group of B / C and walks its block of time in tiles
 // of TL steps.  What is elementwise over (step, channel) -- softplus, silu, the loads and stores -- runs with the lanes over the tile's
-// elements, a vector of V (16 bytes) each, the last one moved back to end with the channels; single elements where a workgroup has fewer
-// channels than a vector.  Between them the recurrence reads (dt, dt u) and the rows of B and C from LDS and leaves y there.  The next tile's
+// elements, a vector of V (16 bytes) each, the last one moved back to end with the channels; single elements, in every workgroup, where the last
+// one has fewer channels than a vector.  Between them the recurrence reads (dt, dt u) and the rows of B and C from LDS and leaves y there.  The next tile's
 // loads are in flight while a tile is walked.
 // Bound by the vector unit: a step of a wave (64 / K channels) takes 22.6 instructions in the recurrence, 4 of them exponentials at a quarter of
 // the rate, and 12 for the elements; the unit is busy 96 % of the kernel's time (SQ_ACTIVE_INST_VALU).  8191 x 1024 bf16, N = 16, training: 49 us,
